@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <mutex>
 
 #include "../../include/gqa_attn.h"
@@ -31,7 +32,9 @@ using gqa::TensorRef;
 // 14: gqa_split_flat_launch, gqa_paged_split_flat_launch (flat splits).
 // 15: gqa_fwd_short_launch, gqa_paged_fwd_short_launch (the single pass of
 // short calls).
-constexpr int kAbiVersion = 15;
+// 16: changed scores (gqa_scored_launch, gqa_paged_scored_launch), norms and
+// rotation, document spans, block tables (gqa_abi_ops.hip).
+constexpr int kAbiVersion = 16;
 
 int check_dims(int B, int Hq, int Hkv, int Sq, int Skv, int D, int dtype) {
   if (B < 0 || Hq <= 0 || Hkv <= 0 || Sq < 0 || Skv < 0) return GQA_E_SHAPE;
@@ -98,6 +101,12 @@ const char* gqa_strerror(int code) {
     case GQA_E_FLAT:
       return "flat split: slots must be in [1, GQA_MAX_SPLITS] and the call one the LDS-DMA first pass takes with "
              "at most 32 packed rows per kv head (16 at head_dim 64)";
+    case GQA_E_SCORE:
+      return "changed scores: softcap / scale must be 0 or in [GQA_MIN_RAW_SOFTCAP, GQA_MAX_RAW_SOFTCAP], the scale "
+             "positive, prefix_lens with causal, spans over contiguous K/V with seq_q <= seq_kv in the single pass";
+    case GQA_E_ROPE:
+      return "rotation: rotary_dim must be a multiple of 16 up to head_dim, axes in [1, 4] and every pair's below it, "
+             "max_positions positive, eps not negative";
     default: break;
   }
   if (code > 0) return hipGetErrorString(static_cast<hipError_t>(code));
@@ -125,7 +134,7 @@ int fwd_impl(const void* q, const int64_t q_stride[4], const void* k, const int6
              const int64_t v_stride[4], void* o, const int64_t o_stride[4], float* lse, int batch, int num_heads,
              int num_kv_heads, int seq_q, int seq_kv, int head_dim, float scale_log2, int causal, int dtype,
              void* stream, int n_split = 0, float* part_ws = nullptr, int* part_cnt = nullptr,
-             bool short_form = false) {
+             bool short_form = false, const gqa::ScoreMod* mod = nullptr) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, dtype);
   if (rc) return rc;
   const int G = num_heads / num_kv_heads, rows = short_form ? gqa::kShortRows : gqa::kFwdRows;
@@ -158,7 +167,7 @@ int fwd_impl(const void* q, const int64_t q_stride[4], const void* k, const int6
   // The scheduling counters follow the split blocks' counters.
   p.sched = part_cnt != nullptr ? part_cnt + (size_t)batch * num_kv_heads * n_split : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return to_code(short_form ? gqa::launch_short(p, dtype, st) : gqa::launch_fwd(p, dtype, st));
+  return to_code(short_form ? gqa::launch_short(p, dtype, st, mod) : gqa::launch_fwd(p, dtype, st, mod));
 }
 
 // Variable query lengths: q_start and q_len both NULL (uniform seq_q) or
@@ -180,7 +189,8 @@ int paged_fwd_impl(const void* q, const int64_t q_stride[4], const void* k_cache
                    const int* q_len, int block_size, int max_seq_len, void* o, const int64_t o_stride[4],
                    float* lse, float* workspace, int kv_splits, int batch, int num_heads, int num_kv_heads,
                    int seq_q, int head_dim, float scale_log2, int causal, int dtype, void* stream,
-                   int n_split = 0, float* part_ws = nullptr, int* part_cnt = nullptr, bool short_form = false);
+                   int n_split = 0, float* part_ws = nullptr, int* part_cnt = nullptr, bool short_form = false,
+                   const gqa::ScoreMod* mod = nullptr);
 
 }  // namespace
 
@@ -246,10 +256,14 @@ int gqa_paged_fwd_short_launch(const void* q, const int64_t q_stride[4], const v
                         nullptr, true);
 }
 
-int gqa_split_first_launch(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
+}  // extern "C"
+
+namespace {
+
+int split_first_impl(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
                            const void* v, const int64_t v_stride[4], float* workspace, int splits, int batch,
                            int num_heads, int num_kv_heads, int seq_q, int seq_kv, int head_dim,
-                           float scale_log2, int causal, int dtype, void* stream) {
+                           float scale_log2, int causal, int dtype, void* stream, const gqa::ScoreMod* mod = nullptr) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, dtype);
   if (rc) return rc;
   if (splits < 1 || splits > GQA_MAX_SPLITS) return GQA_E_SPLITS;
@@ -276,16 +290,31 @@ int gqa_split_first_launch(const void* q, const int64_t q_stride[4], const void*
   p.counters = nullptr;
   p.o = TensorRef{nullptr, 0, 0, 0};
   p.lse = nullptr;
-  return to_code(gqa::launch_split_first(p, dtype, static_cast<hipStream_t>(stream)));
+  return to_code(gqa::launch_split_first(p, dtype, static_cast<hipStream_t>(stream), mod));
 }
 
-int gqa_paged_split_first_launch(const void* q, const int64_t q_stride[4], const void* k_cache,
+}  // namespace
+
+extern "C" {
+
+int gqa_split_first_launch(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
+                           const void* v, const int64_t v_stride[4], float* workspace, int splits, int batch,
+                           int num_heads, int num_kv_heads, int seq_q, int seq_kv, int head_dim,
+                           float scale_log2, int causal, int dtype, void* stream) {
+  return split_first_impl(q, q_stride, k, k_stride, v, v_stride, workspace, splits, batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream);
+}
+
+}  // extern "C"
+
+namespace {
+
+int paged_split_first_impl(const void* q, const int64_t q_stride[4], const void* k_cache,
                                  const int64_t k_cache_stride[4], const void* v_cache,
                                  const int64_t v_cache_stride[4], const int* block_table, int table_stride,
                                  const int* seq_lens, const int* q_start, const int* q_len, int block_size,
                                  int max_seq_len, float* workspace, int splits, int batch, int num_heads,
                                  int num_kv_heads, int seq_q, int head_dim, float scale_log2, int causal, int dtype,
-                                 void* stream) {
+                                 void* stream, const gqa::ScoreMod* mod = nullptr) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, max_seq_len, head_dim, dtype);
   if (rc) return rc;
   if (block_size < 1 || block_size > GQA_MAX_BLOCK_SIZE || (block_size & (block_size - 1)) != 0)
@@ -334,7 +363,21 @@ int gqa_paged_split_first_launch(const void* q, const int64_t q_stride[4], const
   p.rotate = p.k.ss == head_dim && p.v.ss == head_dim;
   p.q_start = q_start;
   p.q_len = q_len;
-  return to_code(gqa::launch_paged_split_first(p, dtype, static_cast<hipStream_t>(stream)));
+  return to_code(gqa::launch_paged_split_first(p, dtype, static_cast<hipStream_t>(stream), mod));
+}
+
+}  // namespace
+
+extern "C" {
+
+int gqa_paged_split_first_launch(const void* q, const int64_t q_stride[4], const void* k_cache,
+                                 const int64_t k_cache_stride[4], const void* v_cache,
+                                 const int64_t v_cache_stride[4], const int* block_table, int table_stride,
+                                 const int* seq_lens, const int* q_start, const int* q_len, int block_size,
+                                 int max_seq_len, float* workspace, int splits, int batch, int num_heads,
+                                 int num_kv_heads, int seq_q, int head_dim, float scale_log2, int causal, int dtype,
+                                 void* stream) {
+  return paged_split_first_impl(q, q_stride, k_cache, k_cache_stride, v_cache, v_cache_stride, block_table, table_stride, seq_lens, q_start, q_len, block_size, max_seq_len, workspace, splits, batch, num_heads, num_kv_heads, seq_q, head_dim, scale_log2, causal, dtype, stream);
 }
 
 int gqa_paged_fwd_launch(const void* q, const int64_t q_stride[4], const void* k_cache,
@@ -471,7 +514,7 @@ int reduce_impl(const float* workspace, int splits, void* o, const int64_t o_str
 // it (acc, m, l, plan), first pass, then the combine unless the first pass
 // writes o.
 int flat_impl(gqa::SplitParams& p, float* workspace, void* o, const int64_t o_stride[4], float* lse, int dtype,
-              void* stream) {
+              void* stream, const gqa::ScoreMod* mod) {
   const size_t rows = ((size_t)p.slots + p.dm.B) * p.dm.Hq * p.dm.Sq;
   p.ws_acc = workspace;
   p.ws_m = workspace + rows * p.dm.D;
@@ -481,7 +524,7 @@ int flat_impl(gqa::SplitParams& p, float* workspace, void* o, const int64_t o_st
   p.lse = lse;
   if (!gqa::decode_kernel_fits(p)) return GQA_E_FLAT;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int rc = to_code(gqa::launch_decode_first(p, dtype, st));
+  const int rc = to_code(gqa::launch_decode_first(p, dtype, st, mod));
   if (rc || p.direct) return rc;
   gqa::ReduceParams r{};
   r.ws_acc = p.ws_acc;
@@ -554,10 +597,14 @@ size_t gqa_split_flat_workspace_bytes(int batch, int num_heads, int seq_q, int h
   return rows * ((size_t)head_dim + 2) * sizeof(float) + (size_t)batch * 2 * sizeof(int);
 }
 
-int gqa_split_flat_launch(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
+}  // extern "C"
+
+namespace {
+
+int split_flat_impl(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
                           const void* v, const int64_t v_stride[4], void* o, const int64_t o_stride[4], float* lse,
                           float* workspace, int slots, int batch, int num_heads, int num_kv_heads, int seq_q,
-                          int seq_kv, int head_dim, float scale_log2, int causal, int dtype, void* stream) {
+                          int seq_kv, int head_dim, float scale_log2, int causal, int dtype, void* stream, const gqa::ScoreMod* mod = nullptr) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, dtype);
   if (rc) return rc;
   if (slots < 1 || slots > GQA_MAX_SPLITS || seq_kv < 1) return GQA_E_FLAT;
@@ -581,16 +628,31 @@ int gqa_split_flat_launch(const void* q, const int64_t q_stride[4], const void* 
   p.rotate = p.k.ss == head_dim && p.v.ss == head_dim;
   // One slot per sequence: each is one piece, written to o by the first pass.
   p.direct = slots == batch;
-  return flat_impl(p, workspace, o, o_stride, lse, dtype, stream);
+  return flat_impl(p, workspace, o, o_stride, lse, dtype, stream, mod);
 }
 
-int gqa_paged_split_flat_launch(const void* q, const int64_t q_stride[4], const void* k_cache,
+}  // namespace
+
+extern "C" {
+
+int gqa_split_flat_launch(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
+                          const void* v, const int64_t v_stride[4], void* o, const int64_t o_stride[4], float* lse,
+                          float* workspace, int slots, int batch, int num_heads, int num_kv_heads, int seq_q,
+                          int seq_kv, int head_dim, float scale_log2, int causal, int dtype, void* stream) {
+  return split_flat_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, slots, batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream);
+}
+
+}  // extern "C"
+
+namespace {
+
+int paged_split_flat_impl(const void* q, const int64_t q_stride[4], const void* k_cache,
                                 const int64_t k_cache_stride[4], const void* v_cache,
                                 const int64_t v_cache_stride[4], const int* block_table, int table_stride,
                                 const int* seq_lens, const int* q_start, const int* q_len, int block_size,
                                 int max_seq_len, void* o, const int64_t o_stride[4], float* lse, float* workspace,
                                 int slots, int batch, int num_heads, int num_kv_heads, int seq_q, int head_dim,
-                                float scale_log2, int causal, int dtype, void* stream) {
+                                float scale_log2, int causal, int dtype, void* stream, const gqa::ScoreMod* mod = nullptr) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, max_seq_len, head_dim, dtype);
   if (rc) return rc;
   if (block_size < 1 || block_size > GQA_MAX_BLOCK_SIZE || (block_size & (block_size - 1)) != 0)
@@ -623,7 +685,21 @@ int gqa_paged_split_flat_launch(const void* q, const int64_t q_stride[4], const 
   p.rotate = p.k.ss == head_dim && p.v.ss == head_dim;
   p.q_start = q_start;
   p.q_len = q_len;
-  return flat_impl(p, workspace, o, o_stride, lse, dtype, stream);
+  return flat_impl(p, workspace, o, o_stride, lse, dtype, stream, mod);
+}
+
+}  // namespace
+
+extern "C" {
+
+int gqa_paged_split_flat_launch(const void* q, const int64_t q_stride[4], const void* k_cache,
+                                const int64_t k_cache_stride[4], const void* v_cache,
+                                const int64_t v_cache_stride[4], const int* block_table, int table_stride,
+                                const int* seq_lens, const int* q_start, const int* q_len, int block_size,
+                                int max_seq_len, void* o, const int64_t o_stride[4], float* lse, float* workspace,
+                                int slots, int batch, int num_heads, int num_kv_heads, int seq_q, int head_dim,
+                                float scale_log2, int causal, int dtype, void* stream) {
+  return paged_split_flat_impl(q, q_stride, k_cache, k_cache_stride, v_cache, v_cache_stride, block_table, table_stride, seq_lens, q_start, q_len, block_size, max_seq_len, o, o_stride, lse, workspace, slots, batch, num_heads, num_kv_heads, seq_q, head_dim, scale_log2, causal, dtype, stream);
 }
 
 int gqa_split_reduce_launch(const float* workspace, int splits, void* o, const int64_t o_stride[4], int batch,
@@ -639,11 +715,15 @@ int gqa_split_reduce_lse_launch(const float* workspace, int splits, void* o, con
   return reduce_impl(workspace, splits, o, o_stride, lse, batch, num_heads, seq_q, head_dim, dtype, stream);
 }
 
-int gqa_fwd_chunks_launch(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
+}  // extern "C"
+
+namespace {
+
+int fwd_chunks_impl(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
                           const void* v, const int64_t v_stride[4], void* o, const int64_t o_stride[4], float* lse,
                           float* workspace, int* counters, int kv_splits, int batch, int num_heads,
                           int num_kv_heads, int seq_q, int seq_kv, int head_dim, float scale_log2, int causal,
-                          int dtype, void* stream) {
+                          int dtype, void* stream, const gqa::ScoreMod* mod = nullptr) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, dtype);
   if (rc) return rc;
   const int G = num_heads / num_kv_heads;
@@ -675,9 +755,21 @@ int gqa_fwd_chunks_launch(const void* q, const int64_t q_stride[4], const void* 
   p.ws_acc = workspace;
   p.ws_m = workspace + rows * head_dim;
   p.ws_l = p.ws_m + rows;
-  rc = to_code(gqa::launch_fwd(p, dtype, static_cast<hipStream_t>(stream)));
+  rc = to_code(gqa::launch_fwd(p, dtype, static_cast<hipStream_t>(stream), mod));
   if (rc) return rc;
   return reduce_impl(workspace, kv_splits, o, o_stride, lse, batch, num_heads, seq_q, head_dim, dtype, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int gqa_fwd_chunks_launch(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
+                          const void* v, const int64_t v_stride[4], void* o, const int64_t o_stride[4], float* lse,
+                          float* workspace, int* counters, int kv_splits, int batch, int num_heads,
+                          int num_kv_heads, int seq_q, int seq_kv, int head_dim, float scale_log2, int causal,
+                          int dtype, void* stream) {
+  return fwd_chunks_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, counters, kv_splits, batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream);
 }
 
 int gqa_split_reduce_varlen_launch(const float* workspace, int splits, void* o, const int64_t o_stride[4],
@@ -735,7 +827,7 @@ int paged_fwd_impl(const void* q, const int64_t q_stride[4], const void* k_cache
                    const int* q_len, int block_size, int max_seq_len, void* o, const int64_t o_stride[4],
                    float* lse, float* workspace, int kv_splits, int batch, int num_heads, int num_kv_heads,
                    int seq_q, int head_dim, float scale_log2, int causal, int dtype, void* stream,
-                   int n_split, float* part_ws, int* part_cnt, bool short_form) {
+                   int n_split, float* part_ws, int* part_cnt, bool short_form, const gqa::ScoreMod* mod) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, max_seq_len, head_dim, dtype);
   if (rc) return rc;
   const int G = num_heads / num_kv_heads, block_rows = short_form ? gqa::kShortRows : gqa::kFwdRows;
@@ -791,8 +883,8 @@ int paged_fwd_impl(const void* q, const int64_t q_stride[4], const void* k_cache
   p.block_shift = shift;
   p.q_start = q_start;
   p.q_len = q_len;
-  if (short_form) return to_code(gqa::launch_short(p, dtype, static_cast<hipStream_t>(stream)));
-  if (kv_splits == 0) return to_code(gqa::launch_paged_fwd(p, dtype, static_cast<hipStream_t>(stream)));
+  if (short_form) return to_code(gqa::launch_short(p, dtype, static_cast<hipStream_t>(stream), mod));
+  if (kv_splits == 0) return to_code(gqa::launch_paged_fwd(p, dtype, static_cast<hipStream_t>(stream), mod));
   // Key chunks: chunk c of every query block covers key tiles [c * ct,
   // (c + 1) * ct) of the longest sequence's range; the partials go to the
   // split-KV workspace layout and the split combine writes o (and lse),
@@ -805,7 +897,7 @@ int paged_fwd_impl(const void* q, const int64_t q_stride[4], const void* k_cache
   p.ws_acc = workspace;
   p.ws_m = workspace + rows * head_dim;
   p.ws_l = p.ws_m + rows;
-  rc = to_code(gqa::launch_paged_fwd(p, dtype, static_cast<hipStream_t>(stream)));
+  rc = to_code(gqa::launch_paged_fwd(p, dtype, static_cast<hipStream_t>(stream), mod));
   if (rc) return rc;
   return reduce_impl(workspace, kv_splits, o, o_stride, lse, batch, num_heads, seq_q, head_dim, dtype, stream,
                      q_start, q_len);
@@ -872,6 +964,121 @@ int gqa_split_noalloc_launch(const void* q, const int64_t q_stride[4], const voi
                               seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream);
   if (rc) return rc;
   return reduce_impl(ws, splits, o, o_stride, lse, batch, num_heads, seq_q, head_dim, dtype, stream);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Changed scores
+// ---------------------------------------------------------------------------
+namespace {
+
+// The kernels' parameters of `score`; scale = scale_log2 / log2(e).
+int score_mod(const gqa_score* score, float scale_log2, int causal, bool paged, int seq_q, int seq_kv,
+              gqa::ScoreMod& m) {
+  constexpr float kLog2e = 1.44269504088896340736f;
+  if (score == nullptr) return GQA_E_NULL;
+  m = gqa::ScoreMod{};
+  const float scale = scale_log2 / kLog2e;
+  if (!(scale > 0.f) || !std::isfinite(scale)) return GQA_E_SCORE;
+  if (score->softcap != 0.f) {
+    if (!(score->softcap > 0.f)) return GQA_E_SCORE;
+    m.cap = score->softcap / scale;
+    if (!(m.cap >= GQA_MIN_RAW_SOFTCAP && m.cap <= GQA_MAX_RAW_SOFTCAP)) return GQA_E_SCORE;
+    m.cap_exp = 2.f * kLog2e / m.cap;
+  }
+  if (((reinterpret_cast<uintptr_t>(score->alibi_slopes) | reinterpret_cast<uintptr_t>(score->prefix_lens) |
+        reinterpret_cast<uintptr_t>(score->span_lo) | reinterpret_cast<uintptr_t>(score->span_hi)) &
+       3u) != 0)
+    return GQA_E_STRIDE;
+  if (score->prefix_lens != nullptr && !causal) return GQA_E_SCORE;
+  if ((score->span_lo == nullptr) != (score->span_hi == nullptr)) return GQA_E_NULL;
+  if (score->span_lo != nullptr && (paged || seq_q > seq_kv)) return GQA_E_SCORE;
+  m.slopes = score->alibi_slopes;
+  m.inv_scale = 1.f / scale;
+  m.prefix = score->prefix_lens;
+  m.span_lo = score->span_lo;
+  m.span_hi = score->span_hi;
+  return GQA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gqa_scored_launch(int form, const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
+                      const void* v, const int64_t v_stride[4], void* o, const int64_t o_stride[4], float* lse,
+                      float* workspace, int* counters, int parts, int batch, int num_heads, int num_kv_heads,
+                      int seq_q, int seq_kv, int head_dim, float scale_log2, int causal, int dtype,
+                      const gqa_score* score, void* stream) {
+  gqa::ScoreMod m;
+  int rc = score_mod(score, scale_log2, causal, false, seq_q, seq_kv, m);
+  if (rc) return rc;
+  if ((reinterpret_cast<uintptr_t>(lse) & 3u) != 0) return GQA_E_STRIDE;
+  if (m.span_lo != nullptr && (form == GQA_FORM_SPLIT || form == GQA_FORM_FLAT)) return GQA_E_SCORE;
+  switch (form) {
+    case GQA_FORM_SPLIT:
+      if (batch > 0 && seq_q > 0 && (rc = check_tensor(o, o_stride))) return rc;
+      rc = split_first_impl(q, q_stride, k, k_stride, v, v_stride, workspace, parts, batch, num_heads, num_kv_heads,
+                            seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream, &m);
+      return rc ? rc
+                : reduce_impl(workspace, parts, o, o_stride, lse, batch, num_heads, seq_q, head_dim, dtype, stream);
+    case GQA_FORM_SINGLE:
+      return fwd_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, batch, num_heads, num_kv_heads, seq_q,
+                      seq_kv, head_dim, scale_log2, causal, dtype, stream, parts, workspace, counters, false, &m);
+    case GQA_FORM_CHUNKS:
+      return fwd_chunks_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, counters, parts,
+                             batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype,
+                             stream, &m);
+    case GQA_FORM_FLAT:
+      return split_flat_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, parts, batch,
+                             num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream, &m);
+    case GQA_FORM_SHORT:
+      return fwd_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, batch, num_heads, num_kv_heads, seq_q,
+                      seq_kv, head_dim, scale_log2, causal, dtype, stream, 0, nullptr, nullptr, true, &m);
+    default: return GQA_E_SCORE;
+  }
+}
+
+int gqa_paged_scored_launch(int form, const void* q, const int64_t q_stride[4], const void* k_cache,
+                            const int64_t k_cache_stride[4], const void* v_cache, const int64_t v_cache_stride[4],
+                            const int* block_table, int table_stride, const int* seq_lens, const int* q_start,
+                            const int* q_len, int block_size, int max_seq_len, void* o, const int64_t o_stride[4],
+                            float* lse, float* workspace, int* counters, int parts, int batch, int num_heads,
+                            int num_kv_heads, int seq_q, int head_dim, float scale_log2, int causal, int dtype,
+                            const gqa_score* score, void* stream) {
+  gqa::ScoreMod m;
+  int rc = score_mod(score, scale_log2, causal, true, seq_q, max_seq_len, m);
+  if (rc) return rc;
+  if ((reinterpret_cast<uintptr_t>(lse) & 3u) != 0) return GQA_E_STRIDE;
+  switch (form) {
+    case GQA_FORM_SPLIT:
+      if (batch > 0 && seq_q > 0 && (rc = check_tensor(o, o_stride))) return rc;
+      rc = paged_split_first_impl(q, q_stride, k_cache, k_cache_stride, v_cache, v_cache_stride, block_table,
+                                  table_stride, seq_lens, q_start, q_len, block_size, max_seq_len, workspace, parts,
+                                  batch, num_heads, num_kv_heads, seq_q, head_dim, scale_log2, causal, dtype, stream,
+                                  &m);
+      return rc ? rc
+                : reduce_impl(workspace, parts, o, o_stride, lse, batch, num_heads, seq_q, head_dim, dtype, stream,
+                              q_start, q_len);
+    case GQA_FORM_FLAT:
+      return paged_split_flat_impl(q, q_stride, k_cache, k_cache_stride, v_cache, v_cache_stride, block_table,
+                                   table_stride, seq_lens, q_start, q_len, block_size, max_seq_len, o, o_stride, lse,
+                                   workspace, parts, batch, num_heads, num_kv_heads, seq_q, head_dim, scale_log2,
+                                   causal, dtype, stream, &m);
+    case GQA_FORM_SINGLE:
+    case GQA_FORM_CHUNKS:
+    case GQA_FORM_SHORT: {
+      if (form == GQA_FORM_CHUNKS && (parts < 1 || parts > GQA_MAX_SPLITS)) return GQA_E_SPLITS;
+      const bool single = form == GQA_FORM_SINGLE;
+      return paged_fwd_impl(q, q_stride, k_cache, k_cache_stride, v_cache, v_cache_stride, block_table, table_stride,
+                            seq_lens, q_start, q_len, block_size, max_seq_len, o, o_stride, lse, workspace,
+                            form == GQA_FORM_CHUNKS ? parts : 0, batch, num_heads, num_kv_heads, seq_q, head_dim,
+                            scale_log2, causal, dtype, stream, single ? parts : 0, single ? workspace : nullptr,
+                            single ? counters : nullptr, form == GQA_FORM_SHORT, &m);
+    }
+    default: return GQA_E_SCORE;
+  }
 }
 
 }  // extern "C"

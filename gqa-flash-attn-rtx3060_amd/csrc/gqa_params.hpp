@@ -160,6 +160,20 @@ struct ReduceParams {
   FastDiv div_sq, div_hq, div_total;  // set by the launcher (div_total: B * units)
 };
 
+// Changed scores (gqa_score.hpp): what a kernel does to s = q . k before the
+// softmax, in units of the raw product (scores divided by the score scale).
+struct ScoreMod {
+  float cap;           // softcap / scale: s <- cap tanh(s / cap); 0: none
+  float cap_exp;       // 2 log2(e) / cap
+  const float* slopes; // (Hq): s <- s - slope |p - j| / scale; nullptr: none
+  float inv_scale;
+  const int* prefix;   // (B): keys below prefix[b] are visible to every row (causal only); nullptr: none
+  // (B, Skv): the keys [span_lo, span_hi) of the document of each position;
+  // nullptr: one document.  Contiguous K/V with Sq <= Skv only.
+  const int* span_lo;
+  const int* span_hi;
+};
+
 // Packed query rows per single-pass workgroup (8 waves x 32 rows).
 constexpr int kFwdRows = 256;
 constexpr int kFwdThreads = 512;
@@ -211,6 +225,73 @@ struct CacheWriteParams {
   int elem_bytes;
 };
 
+struct FwdModParams : FwdParams {
+  ScoreMod mod;
+};
+struct SplitModParams : SplitParams {
+  ScoreMod mod;
+};
+
+// Per-head norm and rotation of queries and keys (gqa_rope.hip); with kc.ptr
+// set, K and V go to their slots of a paged cache.
+struct RopeParams {
+  TensorRef q, k, v, qo, ko;  // (b, h, s) strides; k, v, ko may have no pointer
+  TensorRef kc, vc;           // caches as CacheWriteParams
+  const void* wq;             // (D) norm weights, or nullptr: no norm
+  const void* wk;
+  const float* table;         // (max_pos, R / 2) pairs (cos, sin), or nullptr: no rotation
+  const void* pos;            // (axes, B * S) int32 or int64
+  const int64_t* slots;       // (B * S), negative: not stored
+  int64_t n_tokens;           // B * S
+  int S, Hq, Hkv, D, R, max_pos;
+  int axes, pos64, interleaved, w32, block_shift;
+  uint32_t pair_axis[4];      // 2 bits a pair
+  float eps;
+  int parts;                  // waves a token's heads are dealt to (set by the launcher)
+  FastDiv div_parts;
+};
+
+// The spans of documents, runs of equal ids (gqa_tables.hip).
+struct SpanParams {
+  const int* ids;
+  int64_t stride;  // between rows
+  int* lo;
+  int* hi;
+  int B, S;
+};
+
+// Block tables and slots of a step (gqa_tables.hip).
+struct TablesParams {
+  int* tables;  // pool: (n_rows, width), rows `stride` apart
+  int64_t stride;
+  int* lens;  // pool: (n_rows)
+  const int* rows;  // (B), or nullptr: row b
+  const int* new_lens;  // (B)
+  const int* free_blocks;
+  int* free_count;
+  int n_rows, width, n_free, B, n_tokens, block_shift, update;
+  // Outputs.
+  int* seq_lens;     // (B)
+  int* query_start;  // (B)
+  int* query_lens;   // (B)
+  int64_t* slots;    // (n_tokens)
+  int* positions;    // (n_tokens)
+  int* batch_tables; // (B, width)
+  int* new_free;     // (1)
+  int* refused;      // (1)
+  int* scratch;      // n_rows + 2 B + 1 ints: owners of the pool rows; old lengths, blocks taken before, free blocks
+};
+struct ReleaseParams {
+  const int* tables;
+  int64_t stride;
+  int* lens;
+  const int* rows;  // (B)
+  int* free_blocks;
+  int* free_count;
+  int n_rows, width, n_free, B, block_shift;
+  int* scratch;  // n_rows ints
+};
+
 // Compute units of the current device (0 if unknown), cached per device.
 inline int device_cu_count() {
   static int cached[64] = {};
@@ -223,21 +304,32 @@ inline int device_cu_count() {
   return n;
 }
 
-hipError_t launch_fwd(const FwdParams& p, int dtype, hipStream_t stream);
-hipError_t launch_paged_fwd(const FwdParams& p, int dtype, hipStream_t stream);
+// `mod`: changed scores, or nullptr.
+hipError_t launch_fwd(const FwdParams& p, int dtype, hipStream_t stream, const ScoreMod* mod = nullptr);
+hipError_t launch_paged_fwd(const FwdParams& p, int dtype, hipStream_t stream, const ScoreMod* mod = nullptr);
+// (gqa_fwd_mod.hip: both, with changed scores.)
+hipError_t launch_fwd_mod(const FwdParams& p, int dtype, hipStream_t stream, const ScoreMod& mod);
 // Single pass of short calls (gqa_short.hip): contiguous, or paged when
 // p.block_table is set; no split blocks, no key chunks.
-hipError_t launch_short(const FwdParams& p, int dtype, hipStream_t stream);
-hipError_t launch_split_first(const SplitParams& p, int dtype, hipStream_t stream);  // fused if p.counters
-hipError_t launch_paged_split_first(const SplitParams& p, int dtype, hipStream_t stream);
+hipError_t launch_short(const FwdParams& p, int dtype, hipStream_t stream, const ScoreMod* mod = nullptr);
+// Fused if p.counters (not with changed scores).
+hipError_t launch_split_first(const SplitParams& p, int dtype, hipStream_t stream, const ScoreMod* mod = nullptr);
+hipError_t launch_paged_split_first(const SplitParams& p, int dtype, hipStream_t stream,
+                                    const ScoreMod* mod = nullptr);
 hipError_t launch_paged_cache_write(const CacheWriteParams& p, hipStream_t stream);
 hipError_t launch_split_reduce(const ReduceParams& p, int dtype, hipStream_t stream);
+hipError_t launch_rope(const RopeParams& p, int dtype, hipStream_t stream);
+hipError_t launch_spans(const SpanParams& p, hipStream_t stream);
+hipError_t launch_tables(const TablesParams& p, hipStream_t stream);
+hipError_t launch_release(const ReleaseParams& p, hipStream_t stream);
 // Keys of one tile step of the decode-shaped first pass, the unit of a flat
 // split.
 constexpr int decode_unit(int head_dim) { return head_dim == 64 ? 128 : 64; }
 // Decode-shaped first pass (gqa_decode.hip): whether it takes these rows,
 // pages, strides and workspace offsets.
 bool decode_kernel_fits(const SplitParams& p);
-hipError_t launch_decode_first(const SplitParams& p, int dtype, hipStream_t stream);  // fused if p.counters
+hipError_t launch_decode_first(const SplitParams& p, int dtype, hipStream_t stream,
+                               const ScoreMod* mod = nullptr);  // fused if p.counters
+hipError_t launch_decode_first_mod(const SplitParams& p, int dtype, hipStream_t stream, const ScoreMod& mod);
 
 }  // namespace gqa

@@ -28,11 +28,14 @@
 #include "gqa_fwd_parts.hpp"
 #include "gqa_lds.hpp"
 #include "gqa_params.hpp"
+#include "gqa_score.hpp"
 
 namespace gqa {
 
-template <int DT, int D, int PG>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void gqa_short_kernel(FwdParams p) {
+// P: FwdModParams for changed scores (gqa_score.hpp).
+template <int DT, int D, int PG, typename P = FwdParams>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void gqa_short_kernel(P p) {
+  constexpr bool MOD = kHasMod<P>;
   using E = Elem<DT>;
   using T = typename E::T;
   using ST = FwdStage<D>;
@@ -85,10 +88,21 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // Tiles of the block (its last visible key); loads end with them, so a
   // tile past an odd count reads zeros and is masked.
   const int pos_hi = min(pos_lo + p.block_m, sq) - 1;
-  const int kv_end = dm.causal ? max(min(skv, pos_hi + (skv - sq) + 1), 0) : skv;
-  const int ntiles = (kv_end + ST::kKeys - 1) / ST::kKeys;
+  int kv_end = dm.causal ? max(min(skv, pos_hi + (skv - sq) + 1), 0) : skv;
+  [[maybe_unused]] RowSpan span;
+  [[maybe_unused]] float slope = 0.f;  // changed scores: this lane's row's, in raw units
+  if constexpr (MOD) {
+    span = row_span(p.mod, dm, b, skv, sq, pos_lo, pos_hi, pos, valid, lane, hh);
+    slope = row_slope(p.mod, head);
+    kv_end = span.end;
+  }
+  // Tiles tb + 2 j + grp (changed scores: from the first that a row sees).
+  const int tb = MOD ? span.beg / ST::kKeys : 0;
+  const int ntiles = (kv_end + ST::kKeys - 1) / ST::kKeys - tb;
   const int steps = (ntiles + 1) >> 1;
-  const int rows_ld = min(skv, ntiles * ST::kKeys);
+  // (Changed scores: up to the last row that the block sees, so that no padding
+  // behind a document is multiplied with its probabilities of zero.)
+  const int rows_ld = MOD ? kv_end : min(skv, ntiles * ST::kKeys);
 
   const uint32_t kssb = (uint32_t)(2 * p.k.ss), vssb = (uint32_t)(2 * p.v.ss);
   const char* kbh = static_cast<const char*>(p.k.ptr) + 2 * ((PAGED ? 0 : (int64_t)b * p.k.sb) + (int64_t)kvh * p.k.sh);
@@ -103,14 +117,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const uint32_t voff = (uint32_t)(lrow * vssb) + 16u * (uint32_t)((lane % CPR) ^ ST::sv(lrow));
   using Blocks = FwdTileBlocks<D, PG>;
   auto ids = [&](int j) __attribute__((always_inline)) -> Blocks {  // block(s) of this group's tile j
-    return tile_blocks<D, PG>(table_row, p.block_shift, rows_ld, 2 * j + grp, gw);
+    return tile_blocks<D, PG>(table_row, p.block_shift, rows_ld, tb + 2 * j + grp, gw);
   };
   auto issue_k = [&](char* stage, int j, const Blocks& blk) __attribute__((always_inline)) {
-    issue_fwd_tile<D, PG>(stage + grp * TB, kbh, rk, kssb, koff, p.k.sb, p.block_shift, rows_ld, 2 * j + grp, blk, true,
+    issue_fwd_tile<D, PG>(stage + grp * TB, kbh, rk, kssb, koff, p.k.sb, p.block_shift, rows_ld, tb + 2 * j + grp, blk, true,
                           gw, lane);
   };
   auto issue_v = [&](char* stage, int j, const Blocks& blk) __attribute__((always_inline)) {
-    issue_fwd_tile<D, PG>(stage + grp * TB, vbh, rv, vssb, voff, p.v.sb, p.block_shift, rows_ld, 2 * j + grp, blk,
+    issue_fwd_tile<D, PG>(stage + grp * TB, vbh, rv, vssb, voff, p.v.sb, p.block_shift, rows_ld, tb + 2 * j + grp, blk,
                           false, gw, lane);
   };
 
@@ -262,9 +276,17 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     issue_v(PAR == 0 ? lds0_v1 : lds0_v0, j + 1, id_v);
     id_v = id_k;
     id_k = ids(j + 3);
-    const int key0 = (2 * j + grp) * ST::kKeys;
-    const bool need_mask = (key0 + ST::kKeys > skv) || (dm.causal && key0 + ST::kKeys - 1 > qpos_lo);
-    if (need_mask) mask_tile(sc, vis - key0);
+    const int key0 = (tb + 2 * j + grp) * ST::kKeys;
+    if constexpr (MOD) {
+      if (p.mod.cap > 0.f) cap_scores<16>(sc, p.mod);
+      if (p.mod.slopes != nullptr)
+        bias_scores<16>(sc, slope, key0 + span.rel0, key0 + ST::kKeys - 1 <= qpos_lo,
+                        [](int e) { return 32 * (e >> 4) + key_of(e & 15, 0); });
+      if (key0 + ST::kKeys > span.full_hi || key0 < span.full_lo) mask_tile_span(sc, span.vis - key0, span.lo - key0);
+    } else {
+      const bool need_mask = (key0 + ST::kKeys > skv) || (dm.causal && key0 + ST::kKeys - 1 > qpos_lo);
+      if (need_mask) mask_tile(sc, vis - key0);
+    }
     float rs0 = 0.f, rs1 = 0.f;
     bool keep = false;
     if constexpr (!FIRST) keep = __builtin_amdgcn_ballot_w64(m_run == -__builtin_inff()) == 0;
@@ -301,6 +323,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
 
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * ST::NI));  // K(0) and Q
+  if constexpr (MOD) pin(slope);  // (loaded before them)
   phase_barrier();
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks)
@@ -369,7 +392,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const float a0 = fast_exp2((m0 - mu) * c), a1 = fast_exp2((m1 - mu) * c);
   const float l0 = grp == 0 ? l_run : l_o, l1 = grp == 0 ? l_o : l_run;
   const float l_tot = xhalf_sum(__builtin_fmaf(l0, a0, l1 * a1));
-  const float inv = skv == 0 ? 0.f : 1.0f / l_tot;  // (a sequence without keys: zero rows)
+  const float inv = (MOD ? l_tot == 0.f : skv == 0) ? 0.f : 1.0f / l_tot;  // (a sequence without keys: zero rows)
   if (p.lse != nullptr && valid && grp == 0 && hh == 0) {
     const int64_t li = varlen ? (tok0 + pos) * dm.Hq + head : ((int64_t)b * dm.Hq + head) * dm.Sq + pos;
     p.lse[li] = (mm * c + __log2f(l_tot)) * kLn2;
@@ -410,31 +433,37 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
 }
 
-template <int DT, int D, int PG>
-static hipError_t launch_short_t(FwdParams p, hipStream_t stream) {
+template <int DT, int D, int PG, typename P> static hipError_t launch_short_t(P p, hipStream_t stream) {
   const int64_t total = (int64_t)p.n_mblk * p.dm.Hkv * p.dm.B;
   if (total <= 0) return hipSuccess;
   set_item_order(p, p.n_mblk, PG > 0 || D == 64 || total > device_cu_count(), kDealPairs(D));
   p.div_hkv = make_fast_div((uint32_t)p.dm.Hkv);
   p.bm_mul = (65536u + (uint32_t)p.block_m - 1) / (uint32_t)p.block_m;
-  hipLaunchKernelGGL((gqa_short_kernel<DT, D, PG>), dim3((unsigned)total), dim3(kFwdThreads), 0, stream, p);
+  hipLaunchKernelGGL((gqa_short_kernel<DT, D, PG, P>), dim3((unsigned)total), dim3(kFwdThreads), 0, stream, p);
   return hipGetLastError();
 }
 
-template <int PG>
-static hipError_t launch_short_pg(const FwdParams& p, int dtype, hipStream_t stream) {
+template <int PG, typename P> static hipError_t launch_short_pg(const P& p, int dtype, hipStream_t stream) {
   if (dtype == 0)
     return p.dm.D == 128 ? launch_short_t<0, 128, PG>(p, stream) : launch_short_t<0, 64, PG>(p, stream);
   return p.dm.D == 128 ? launch_short_t<1, 128, PG>(p, stream) : launch_short_t<1, 64, PG>(p, stream);
 }
 
-// p.block_m = kShortRows / G, p.n_mblk accordingly; paged as launch_paged_fwd.
-hipError_t launch_short(const FwdParams& p, int dtype, hipStream_t stream) {
+template <typename P> static hipError_t launch_short_p(const P& p, int dtype, hipStream_t stream) {
   if (p.block_table == nullptr) return launch_short_pg<0>(p, dtype, stream);
   if ((1 << p.block_shift) < 512 / p.dm.D) return hipErrorInvalidValue;
   if (p.block_shift >= 6) return launch_short_pg<1>(p, dtype, stream);
   const bool medium = p.block_shift >= 4 && (p.dm.D != 64 || (2 * p.k.ss) % 64 == 0);
   return medium ? launch_short_pg<3>(p, dtype, stream) : launch_short_pg<2>(p, dtype, stream);
+}
+
+// p.block_m = kShortRows / G, p.n_mblk accordingly; paged as launch_paged_fwd.
+hipError_t launch_short(const FwdParams& p, int dtype, hipStream_t stream, const ScoreMod* mod) {
+  if (mod == nullptr) return launch_short_p(p, dtype, stream);
+  FwdModParams m;
+  static_cast<FwdParams&>(m) = p;
+  m.mod = *mod;
+  return launch_short_p(m, dtype, stream);
 }
 
 }  // namespace gqa

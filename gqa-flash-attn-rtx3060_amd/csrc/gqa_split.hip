@@ -34,6 +34,7 @@
 
 #include "gqa_common.hpp"
 #include "gqa_params.hpp"
+#include "gqa_score.hpp"
 
 namespace gqa {
 
@@ -145,9 +146,11 @@ __device__ inline void combine_rows(const SplitParams& p, int b, int kvh, int rb
 }
 
 // KV: 0 contiguous K/V, 1 paged cache with pages of >= 64 keys, 2 paged
-// cache with smaller pages.
-template <int DT, int D, int KV>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void gqa_split_first_kernel(SplitParams p) {
+// cache with smaller pages.  P: SplitModParams for changed scores
+// (gqa_score.hpp).
+template <int DT, int D, int KV, typename P = SplitParams>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void gqa_split_first_kernel(P p) {
+  constexpr bool MOD = kHasMod<P>;
   using E = Elem<DT>;
   using T = typename E::T;
   using ST = SubTile<D>;
@@ -210,7 +213,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   int c1 = min(c0 + p.chunk, skv);
   const int pos_lo = (32 * rb) / dm.G;
   const int pos_hi = min(sq - 1, (32 * rb + 31) / dm.G);
-  if (dm.causal) c1 = min(c1, pos_hi + (skv - sq) + 1);
+  [[maybe_unused]] int prefix = 0;  // changed scores: every row sees the keys below it
+  [[maybe_unused]] float slope = 0.f;
+  if constexpr (MOD) {
+    prefix = seq_prefix(p.mod, b, skv);
+    slope = row_slope(p.mod, head);
+    if (dm.causal) c1 = min(c1, max(pos_hi + (skv - sq) + 1, prefix));
+  } else {
+    if (dm.causal) c1 = min(c1, pos_hi + (skv - sq) + 1);
+  }
   const int ntiles = c1 > c0 ? (c1 - c0 + kSplitTileKeys - 1) / kSplitTileKeys : 0;
   const int qpos_lo = pos_lo + (skv - sq);
 
@@ -298,12 +309,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int kb0 = key0 + 32 * wave;  // this wave's 32 keys
     if (kb0 >= c1) continue;           // wave-uniform: nothing visible here
     f32x16 sc = qk_block<DT, D>(mytile, qreg, mb, lane);
-    const bool need_mask = (kb0 + 32 > c1) || (dm.causal && kb0 + 31 > qpos_lo);
+    if constexpr (MOD) {
+      f32x16 s1[1] = {sc};
+      if (p.mod.cap > 0.f) cap_scores<16>(s1, p.mod);
+      if (p.mod.slopes != nullptr)
+        bias_scores<16>(s1, slope, kb0 + 8 * hh - qpos, kb0 + 31 <= qpos_lo, [](int e) { return key_of(e, 0); });
+      sc = s1[0];
+    }
+    // The last keys that this row, and every row of the block, sees.
+    const int seen = MOD ? max(qpos, prefix - 1) : qpos, seen_lo = MOD ? max(qpos_lo, prefix - 1) : qpos_lo;
+    const bool need_mask = (kb0 + 32 > c1) || (dm.causal && kb0 + 31 > seen_lo);
     if (need_mask) {
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
         const int key = kb0 + key_of(v, hh);
-        if (key >= c1 || (dm.causal && key > qpos)) sc[v] = -__builtin_inff();
+        if (key >= c1 || (dm.causal && key > seen)) sc[v] = -__builtin_inff();
       }
     }
     float mx = sc[0];
@@ -387,7 +407,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       // otherwise: the chunk's largest score contributes exp2(0) = 1 to l),
       // which the combine turns into a zero row.
       if (db == 0 && hh == 0) {
-        store_coherent(p.ws_m + row, skv == 0 ? 0.f : mstar * c);
+        if constexpr (MOD) store_coherent(p.ws_m + row, mstar == -__builtin_inff() ? kEmptyRef : mstar * c);
+        else store_coherent(p.ws_m + row, skv == 0 ? 0.f : mstar * c);
         store_coherent(p.ws_l + row, lsum);
       }
     }
@@ -536,11 +557,10 @@ __global__ __launch_bounds__(256) void gqa_split_reduce_kernel(ReduceParams p) {
   }
 }
 
-template <int DT, int D, int KV>
-static hipError_t launch_split_first_t(const SplitParams& p, hipStream_t stream) {
+template <int DT, int D, int KV, typename P> static hipError_t launch_split_first_t(const P& p, hipStream_t stream) {
   const int64_t total = (int64_t)p.dm.B * p.dm.Hkv * p.n_rblk * p.splits;
   if (total <= 0) return hipSuccess;
-  hipLaunchKernelGGL((gqa_split_first_kernel<DT, D, KV>), dim3((unsigned)total), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((gqa_split_first_kernel<DT, D, KV, P>), dim3((unsigned)total), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -558,24 +578,33 @@ static hipError_t launch_split_reduce_t(ReduceParams p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t launch_split_first(const SplitParams& p, int dtype, hipStream_t stream) {
-  if (decode_kernel_fits(p)) return launch_decode_first(p, dtype, stream);
-  if (dtype == 0)
-    return p.dm.D == 128 ? launch_split_first_t<0, 128, 0>(p, stream) : launch_split_first_t<0, 64, 0>(p, stream);
-  return p.dm.D == 128 ? launch_split_first_t<1, 128, 0>(p, stream) : launch_split_first_t<1, 64, 0>(p, stream);
-}
-
-template <int KV>
-static hipError_t launch_paged_t(const SplitParams& p, int dtype, hipStream_t stream) {
+template <int KV, typename P> static hipError_t launch_split_kv(const P& p, int dtype, hipStream_t stream) {
   if (dtype == 0)
     return p.dm.D == 128 ? launch_split_first_t<0, 128, KV>(p, stream) : launch_split_first_t<0, 64, KV>(p, stream);
   return p.dm.D == 128 ? launch_split_first_t<1, 128, KV>(p, stream) : launch_split_first_t<1, 64, KV>(p, stream);
 }
 
+static SplitModParams with_mod(const SplitParams& p, const ScoreMod& mod) {
+  SplitModParams m;
+  static_cast<SplitParams&>(m) = p;
+  m.mod = mod;
+  return m;
+}
+
+hipError_t launch_split_first(const SplitParams& p, int dtype, hipStream_t stream, const ScoreMod* mod) {
+  if (mod != nullptr && p.counters != nullptr) return hipErrorInvalidValue;
+  if (decode_kernel_fits(p)) return launch_decode_first(p, dtype, stream, mod);
+  return mod != nullptr ? launch_split_kv<0>(with_mod(p, *mod), dtype, stream) : launch_split_kv<0>(p, dtype, stream);
+}
+
 // Requires p.chunk to be a multiple of 64 (sub-tiles start 64-aligned).
-hipError_t launch_paged_split_first(const SplitParams& p, int dtype, hipStream_t stream) {
-  if (decode_kernel_fits(p)) return launch_decode_first(p, dtype, stream);
-  return p.block_shift >= 6 ? launch_paged_t<1>(p, dtype, stream) : launch_paged_t<2>(p, dtype, stream);
+hipError_t launch_paged_split_first(const SplitParams& p, int dtype, hipStream_t stream, const ScoreMod* mod) {
+  if (decode_kernel_fits(p)) return launch_decode_first(p, dtype, stream, mod);
+  if (mod != nullptr) {
+    const SplitModParams m = with_mod(p, *mod);
+    return p.block_shift >= 6 ? launch_split_kv<1>(m, dtype, stream) : launch_split_kv<2>(m, dtype, stream);
+  }
+  return p.block_shift >= 6 ? launch_split_kv<1>(p, dtype, stream) : launch_split_kv<2>(p, dtype, stream);
 }
 
 hipError_t launch_split_reduce(const ReduceParams& p, int dtype, hipStream_t stream) {

@@ -22,13 +22,32 @@ GQA_PAGED_CHUNK_PAGES = 2048
 GQA_NOALLOC_SCRATCH_BYTES = 16 << 20
 GQA_E_SCRATCH = -9
 GQA_E_FLAT = -10
-ABI_VERSION = 15
+GQA_E_SCORE = -11
+GQA_E_ROPE = -12
+GQA_MIN_RAW_SOFTCAP = 1e-2
+GQA_MAX_RAW_SOFTCAP = 1e8
+ABI_VERSION = 16
 
 _i64x4 = ctypes.c_int64 * 4
 _i64x3 = ctypes.c_int64 * 3
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
+
+
+class Score(ctypes.Structure):
+    """gqa_score of include/gqa_attn.h: what changes the scores of a call."""
+
+    _fields_ = [("softcap", _f), ("alibi_slopes", _p), ("prefix_lens", _p), ("span_lo", _p), ("span_hi", _p)]
+
+
+class Rope(ctypes.Structure):
+    """gqa_rope of include/gqa_attn.h: norms and rotation of a call."""
+
+    _fields_ = [("table", _p), ("max_positions", _i), ("rotary_dim", _i), ("interleaved", _i), ("positions", _p),
+                ("positions64", _i), ("axes", _i), ("pair_axis", ctypes.c_uint32 * 4), ("q_weight", _p),
+                ("k_weight", _p), ("weights32", _i), ("eps", _f)]
+
 
 # (name, restype, argtypes) for every entry point of include/gqa_attn.h.
 SIGNATURES = {
@@ -122,6 +141,35 @@ SIGNATURES = {
         _i,
         [_p, _i64x4, _p, _i64x4, _p, _i64x4, _p, _i, _p, _p, _p, _i, _i, _p, _i64x4, _p, _p, _i,
          _i, _i, _i, _i, _i, _f, _i, _i, _p],
+    ),
+    "gqa_scored_launch": (
+        _i,
+        [_i, _p, _i64x4, _p, _i64x4, _p, _i64x4, _p, _i64x4, _p, _p, _p, _i,
+         _i, _i, _i, _i, _i, _i, _f, _i, _i, ctypes.POINTER(Score), _p],
+    ),
+    "gqa_paged_scored_launch": (
+        _i,
+        [_i, _p, _i64x4, _p, _i64x4, _p, _i64x4, _p, _i, _p, _p, _p, _i, _i, _p, _i64x4, _p, _p, _p, _i,
+         _i, _i, _i, _i, _i, _f, _i, _i, ctypes.POINTER(Score), _p],
+    ),
+    "gqa_qk_norm_rope_launch": (
+        _i,
+        [_p, _i64x4, _p, _i64x4, _p, _i64x4, _p, _i64x4, ctypes.POINTER(Rope), _i, _i, _i, _i, _i, _i, _p],
+    ),
+    "gqa_qk_norm_rope_write_launch": (
+        _i,
+        [_p, _i64x3, _p, _i64x3, _p, _i64x3, _p, _i64x3, _p, _i64x4, _p, _i64x4, _p, ctypes.POINTER(Rope),
+         _i, _i, _i, _i, _i, _i, _p],
+    ),
+    "gqa_document_spans_launch": (_i, [_p, ctypes.c_int64, _p, _p, _i, _i, _p]),
+    "gqa_extend_tables_scratch_bytes": (ctypes.c_size_t, [_i, _i]),
+    "gqa_extend_tables_launch": (
+        _i,
+        [_p, ctypes.c_int64, _i, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i] + [_p] * 10,
+    ),
+    "gqa_release_blocks_launch": (
+        _i,
+        [_p, ctypes.c_int64, _i, _p, _i, _p, _i, _p, _p, _i, _i, _p, _p],
     ),
     "gqa_split_noalloc_launch": (
         _i,

@@ -18,7 +18,8 @@ import torch
 
 from . import _lib
 from .gqa_split import (_counter_buffer, _counters, _decode_host, _workspace_buffer, _workspaces, decode_forward,
-                        flat_forward, stream_handle)
+                        flat_forward, flat_workspace_bytes, stream_handle, workspace_bytes)
+from .scores import check_score, refuse_grad, scored_launch, workspace
 
 __all__ = ["gqa_flash_attn", "Route", "choose_plan", "choose_route"]
 
@@ -753,7 +754,8 @@ def _kernel_ready(t: torch.Tensor) -> torch.Tensor:
     return t if _is_kernel_ready(t) else t.clone(memory_format=torch.contiguous_format)
 
 
-def gqa_flash_attn(q, k, v, causal=True, *, return_lse=False):
+def gqa_flash_attn(q, k, v, causal=True, *, return_lse=False, softcap=None, alibi_slopes=None, prefix_lens=None,
+                   documents=None):
     """GQA flash attention.
 
     Args:
@@ -771,11 +773,27 @@ def gqa_flash_attn(q, k, v, causal=True, *, return_lse=False):
                 ranges merge exactly with it (context-parallel / ring
                 attention, prefix-cache composition).
 
+        Changed scores (keyword-only, not in the reference; any of them
+        together), for a query at position p = i + seq_kv - seq_q and key j:
+
+        softcap: s <- softcap tanh(s / softcap) on the scaled scores.
+        alibi_slopes: float32 (num_heads,); s <- s - slope |p - j|.
+        prefix_lens: int32 (batch,); keys below prefix_lens[b] are visible to
+                every query of sequence b, in both directions (needs causal).
+        documents: ``document_spans(ids)``; queries see the keys of their own
+                document only (needs seq_q <= seq_kv).
+
+        With one of them a row that sees no key gives zeros and LSE -inf
+        (without: NaN, as the reference), and inputs that need a gradient are
+        refused.  V must be finite at hidden keys that share a 64-key tile with
+        a visible one.
+
     Returns:
         (batch, num_heads, seq_q, head_dim), same dtype as q; with
         return_lse=True the pair (o, lse).
     """
-    host = _lib._host
+    changed = softcap or alibi_slopes is not None or prefix_lens is not None or documents is not None
+    host = _lib._host if not changed else None
     if host is not None:
         # A planned shape with every check passed, natively; else None.
         out = host.flash_attn(q, k, v, bool(causal), bool(return_lse), _workspaces, _counters)
@@ -793,6 +811,12 @@ def gqa_flash_attn(q, k, v, causal=True, *, return_lse=False):
     dev = q.get_device()  # device index (an int: no torch.device objects on this path)
     assert k.get_device() == dev and v.get_device() == dev, "q, k, v must be on one device"
 
+    if changed:
+        refuse_grad("gqa_flash_attn with changed scores", q, k, v, alibi_slopes)
+        score = check_score(softcap, alibi_slopes, prefix_lens, documents, batch=batch, num_heads=num_heads,
+                            seq_q=seq_q, seq_kv=seq_kv, causal=bool(causal), scale=head_dim ** -0.5, device=q.device)
+        with torch.cuda.device(dev):
+            return _scored(q, k, v, causal, return_lse, dev, score, documents is not None)
     host = _decode_host()
     route = _plan_cached(batch, num_heads, num_kv_heads, seq_q, seq_kv, _cu_count(dev), bool(causal), head_dim)
     if host is not None and batch > 0 and seq_q > 0:
@@ -842,6 +866,49 @@ def _launch(route, q_in, k, v, causal, return_lse, dev):
     if route.kind == "short":
         return short_forward(q, k, v, o, causal, return_lse)
     return single_pass_forward(q, k, v, o, causal, route.fwd_split, return_lse)
+
+
+def _scored(q_in, k, v, causal, return_lse, dev, score, spans):
+    """gqa_flash_attn with changed scores: the same routes, through
+    gqa_scored_launch."""
+    batch, num_heads, seq_q, head_dim = q_in.shape
+    _, num_kv_heads, seq_kv, _ = k.shape
+    q, k, v = _kernel_ready(q_in), _kernel_ready(k), _kernel_ready(v)
+    o = torch.empty_like(q_in)
+    if not _is_kernel_ready(o):
+        o = torch.empty_like(q_in, memory_format=torch.contiguous_format)
+    lse = torch.empty(batch, num_heads, seq_q, dtype=torch.float32, device=q.device) if return_lse else None
+    cu = _cu_count(dev)
+    shape = (batch, num_heads, num_kv_heads, seq_q, seq_kv, cu, bool(causal), head_dim)
+    if spans:  # (the single pass alone has a first visible key)
+        route = Route("single")
+    else:
+        route = _plan_cached(*shape)
+        if route.kind != "single" and (seq_kv + 192) * max(k.stride(2), v.stride(2)) >= 1 << 30:
+            route = _route_cached(*shape)  # as _launch
+    stream = stream_handle(q.device)
+
+    def launch(route):
+        lib, ws, cnt, parts = _lib.load(), None, None, route.splits
+        if route.kind in ("split", "chunks"):
+            ws = workspace(workspace_bytes(batch, num_heads, seq_q, head_dim, parts), q.device)
+        elif route.kind == "flat":
+            ws = workspace(flat_workspace_bytes(batch, num_heads, seq_q, head_dim, parts), q.device)
+        elif route.kind == "single":
+            parts = route.fwd_split
+            if parts:
+                ws = workspace(lib.gqa_fwd_split_workspace_bytes(batch, num_kv_heads, head_dim, parts), q.device)
+        if route.kind in ("single", "chunks"):
+            cnt = _counter_buffer(q.device, stream, lib.gqa_fwd_split_counters_count(
+                batch, num_kv_heads, parts if route.kind == "single" else 0))
+        return scored_launch(_KIND_IDS[route.kind], parts, q, k, v, o, lse, ws, cnt, causal,
+                             (head_dim ** -0.5) * LOG2E, _DTYPES[q.dtype], score, stream)
+
+    rc = launch(route)
+    if rc == _lib.GQA_E_FLAT:
+        rc = launch(_route_cached(*shape))
+    _lib.check(rc)
+    return o if lse is None else (o, lse)
 
 
 def single_pass_forward(q, k, v, o, causal, fwd_split=0, return_lse=False):

@@ -31,6 +31,7 @@ of block ``block_table[b, j // block_size]``.  A slot index is
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 import threading
@@ -44,6 +45,10 @@ from .dispatch import (_KIND_IDS, FWD_ROWS, SPLIT_MIN_KV, _fwd_block_tiles, choo
                        flat_piece_steps, flat_steps, fwd_split_makespan, use_short)
 from .gqa_split import (_counter_buffer, _counters, _decode_host, _workspace_buffer, _workspaces,
                         flat_workspace_bytes, stream_handle, workspace_bytes)
+from .rotary import qk_norm_rope, qk_norm_rope_write
+from .scores import check_score, refuse_grad
+from .scores import workspace as own_workspace
+from .tables import BlockPool, StepTables, extend_block_tables, release_blocks
 
 __all__ = [
     "paged_attention",
@@ -54,6 +59,10 @@ __all__ = [
     "paged_kv_chunks",
     "paged_single_plan",
     "PagedKVCache",
+    "BlockPool",
+    "StepTables",
+    "extend_block_tables",
+    "release_blocks",
     "PagedAttentionMetadata",
     "GQAPagedAttention",
 ]
@@ -361,7 +370,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
                     splits: Optional[int] = None, return_lse: bool = False,
                     out: Optional[torch.Tensor] = None, route: Optional[str] = None,
                     query_start: Optional[torch.Tensor] = None, query_lens: Optional[torch.Tensor] = None,
-                    max_query_len: Optional[int] = None):
+                    max_query_len: Optional[int] = None, softcap: Optional[float] = None,
+                    alibi_slopes: Optional[torch.Tensor] = None, prefix_lens: Optional[torch.Tensor] = None):
     """GQA attention of q over K/V held in a paged cache.
 
     Args:
@@ -404,13 +414,17 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
             int) bounds query_lens; causal alignment per sequence uses its own
             query length; o (and out) are (num_tokens, num_heads, head_dim),
             lse (num_tokens, num_heads).
+        softcap, alibi_slopes, prefix_lens: changed scores, as
+            ``gqa_flash_attn`` takes them (p = i + seq_lens[b] - the sequence's
+            query length).
 
     Returns:
         o (batch, num_heads, seq_q, head_dim), or (o, lse).
     """
     varlen = query_start is not None
+    changed = bool(softcap) or alibi_slopes is not None or prefix_lens is not None
     default_route = route is None and splits is None and (not varlen or query_lens is not None)
-    native = _lib._host if default_route else None
+    native = _lib._host if default_route and not changed else None
     if native is not None:
         # A planned shape with every check passed, natively; else None.
         res = native.paged_attn(q, k_cache, v_cache, block_table, seq_lens, bool(causal),
@@ -480,7 +494,12 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
     dtype = _DTYPES[q.dtype]
     stream = stream_handle(qdev)
     plan_key = None
-    if default_route and batch > 0 and seq_q > 0:
+    score = None
+    if changed:
+        refuse_grad("paged_attention with changed scores", q, k_cache, v_cache, alibi_slopes)
+        score = check_score(softcap, alibi_slopes, prefix_lens, None, batch=batch, num_heads=num_heads, seq_q=seq_q,
+                            seq_kv=max_seq_len, causal=bool(causal), scale=scale, device=qdev)
+    if default_route and not changed and batch > 0 and seq_q > 0:
         plan_key = [1, batch, num_heads, num_kv_heads, seq_q, max_seq_len, head_dim, int(bool(causal)), dev, block_size,
                     int(interleaved), int(varlen)]
     kv_chunks = fwd_split = 0
@@ -517,6 +536,15 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
             return res
     lse = torch.empty(lse_shape, dtype=torch.float32, device=qdev) if return_lse else None
     counters = None
+    if score is not None:
+        with torch.cuda.device(qdev):
+            return _paged_scored("flat" if flat else route, flat_slots if flat else n_parts, q, k_cache, v_cache,
+                                 block_table, table_stride, seq_lens, query_start if varlen else None,
+                                 query_lens if varlen else None, block_size, max_seq_len, out, lse, batch, seq_q,
+                                 scale * LOG2E, causal, dtype, score,
+                                 lambda: splits if splits is not None else paged_splits(
+                                     batch, num_heads, num_kv_heads, seq_q, max_seq_len, _cu_count(dev), block_size,
+                                     head_dim, interleaved))
     if flat:
         workspace = _workspace_buffer(qdev, stream, flat_workspace_bytes(batch, num_heads, seq_q, head_dim, flat_slots))
         if host is not None:
@@ -605,6 +633,38 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
     else:
         _lib.check(lib.gqa_split_reduce_lse_launch(workspace.data_ptr(), splits, out.data_ptr(), ost,
                                                    lse_p, batch, num_heads, seq_q, head_dim, dtype, stream))
+    return out if lse is None else (out, lse)
+
+
+def _paged_scored(kind, parts, q, k_cache, v_cache, block_table, table_stride, seq_lens, query_start, query_lens,
+                  block_size, max_seq_len, out, lse, batch, seq_q, scale_log2, causal, dtype, score, fixed_splits):
+    """paged_attention's launch with changed scores (gqa_paged_scored_launch);
+    ``fixed_splits``: the split count where the flat split is refused."""
+    lib, dev, varlen = _lib.load(), q.device, query_start is not None
+    num_heads, head_dim, num_kv_heads = q.shape[1], q.shape[-1], k_cache.shape[2]
+    stream = stream_handle(dev)
+
+    def launch(kind, parts):
+        ws = cnt = None
+        if kind in ("split", "chunks"):
+            ws = own_workspace(workspace_bytes(batch, num_heads, seq_q, head_dim, parts), dev)
+        elif kind == "flat":
+            ws = own_workspace(flat_workspace_bytes(batch, num_heads, seq_q, head_dim, parts), dev)
+        elif kind == "single" and parts:
+            ws = own_workspace(lib.gqa_fwd_split_workspace_bytes(batch, num_kv_heads, head_dim, parts), dev)
+            cnt = _counter_buffer(dev, stream, lib.gqa_fwd_split_counters_count(batch, num_kv_heads, parts))
+        return lib.gqa_paged_scored_launch(
+            _KIND_IDS[kind], q.data_ptr(), _row_strides(q, varlen), k_cache.data_ptr(), _lib.strides(k_cache),
+            v_cache.data_ptr(), _lib.strides(v_cache), block_table.data_ptr(), table_stride, seq_lens.data_ptr(),
+            query_start.data_ptr() if varlen else None, query_lens.data_ptr() if varlen else None, block_size,
+            max_seq_len, out.data_ptr(), _row_strides(out, varlen), None if lse is None else lse.data_ptr(),
+            None if ws is None else ws.data_ptr(), None if cnt is None else cnt.data_ptr(), parts, batch, num_heads,
+            num_kv_heads, seq_q, head_dim, scale_log2, int(bool(causal)), dtype, ctypes.byref(score), stream)
+
+    rc = launch(kind, parts)
+    if rc == _lib.GQA_E_FLAT:
+        rc = launch("split", fixed_splits())
+    _lib.check(rc)
     return out if lse is None else (out, lse)
 
 
@@ -809,6 +869,10 @@ class PagedAttentionMetadata:
     query_lens: new tokens of each sequence (host ints) for a mixed batch
         (prefill chunks and decode steps together); overrides query_len.
     max_seq_len: an upper bound of seq_lens (default: the tables' capacity).
+    positions: the tokens' positions, for a layer with rotation (as
+        ``qk_norm_rope_write`` takes them).
+    prefix_lens: int32 (num_seqs,), keys that every query of a sequence sees
+        (as ``paged_attention``).
     """
     slot_mapping: torch.Tensor
     block_tables: torch.Tensor
@@ -816,6 +880,8 @@ class PagedAttentionMetadata:
     query_len: int = 1
     max_seq_len: Optional[int] = None
     query_lens: Optional[Sequence[int]] = None
+    positions: Optional[torch.Tensor] = None
+    prefix_lens: Optional[torch.Tensor] = None
 
 
 class GQAPagedAttention(torch.nn.Module):
@@ -833,10 +899,19 @@ class GQAPagedAttention(torch.nn.Module):
     whose query block suits the split-KV pass (decode-like) and one for the
     rest (prefill chunks).  Returns (num_tokens, num_heads * head_size),
     written in place when ``output`` is given.
+
+    softcap, alibi_slopes: changed scores (``paged_attention``).  rotary (a
+    ``RotaryTable``), q_norm_weight, k_norm_weight, norm_eps: queries and keys are
+    normed per head and rotated in the pass that stores K and V
+    (``qk_norm_rope_write``, at ``attn_metadata.positions``); the caller's query
+    is not changed.
     """
 
     def __init__(self, num_heads: int, head_size: int, scale: Optional[float] = None,
-                 num_kv_heads: Optional[int] = None, causal: bool = True):
+                 num_kv_heads: Optional[int] = None, causal: bool = True, softcap: Optional[float] = None,
+                 alibi_slopes: Optional[torch.Tensor] = None, rotary=None,
+                 q_norm_weight: Optional[torch.Tensor] = None, k_norm_weight: Optional[torch.Tensor] = None,
+                 norm_eps: float = 1e-6):
         super().__init__()
         self.num_heads = num_heads
         self.head_size = head_size
@@ -845,6 +920,12 @@ class GQAPagedAttention(torch.nn.Module):
         assert head_size in (64, 128), f"unsupported head_size {head_size}"
         self.scale = head_size ** -0.5 if scale is None else float(scale)
         self.causal = causal
+        self.softcap, self.alibi_slopes = softcap, alibi_slopes
+        self.rotary, self.norm_eps = rotary, norm_eps
+        self.q_norm_weight, self.k_norm_weight = q_norm_weight, k_norm_weight
+
+    def _normed(self) -> bool:
+        return self.rotary is not None or self.q_norm_weight is not None or self.k_norm_weight is not None
 
     def forward(self, query, key, value, kv_cache, attn_metadata: PagedAttentionMetadata, output=None):
         md = attn_metadata
@@ -857,7 +938,9 @@ class GQAPagedAttention(torch.nn.Module):
             assert num_tokens == batch * md.query_len, "num_tokens must equal num_seqs * query_len"
         else:
             assert len(md.query_lens) == batch and sum(md.query_lens) == num_tokens
-        if key is not None:
+        if self._normed():
+            query = self._norm_rope(query, key, value, k_cache, v_cache, md)
+        elif key is not None:
             write_kv(key.view(num_tokens, Hkv, D), value.view(num_tokens, Hkv, D), k_cache, v_cache,
                      md.slot_mapping)
         if output is None:
@@ -867,7 +950,8 @@ class GQAPagedAttention(torch.nn.Module):
             q4 = query.view(batch, sq, H, D).permute(0, 2, 1, 3)
             o4 = output.view(batch, sq, H, D).permute(0, 2, 1, 3)
             paged_attention(q4, k_cache, v_cache, md.block_tables, md.seq_lens, self.causal,
-                            max_seq_len=md.max_seq_len, scale=self.scale, out=o4)
+                            max_seq_len=md.max_seq_len, scale=self.scale, out=o4, softcap=self.softcap,
+                            alibi_slopes=self.alibi_slopes, prefix_lens=md.prefix_lens)
             return output
         # Mixed batch: token-major views, one launch per kernel route over
         # that route's sequences only (a launch spreads its sequences' work
@@ -903,10 +987,28 @@ class GQAPagedAttention(torch.nn.Module):
             off += 3 * n
             if idx[-1] - idx[0] + 1 == n:
                 tables, lens = md.block_tables[idx[0]:idx[-1] + 1], md.seq_lens[idx[0]:idx[-1] + 1]
+                prefix = None if md.prefix_lens is None else md.prefix_lens[idx[0]:idx[-1] + 1]
             else:
                 tables, lens = md.block_tables.index_select(0, sel), md.seq_lens.index_select(0, sel)
+                prefix = None if md.prefix_lens is None else md.prefix_lens.index_select(0, sel)
             max_q = max(md.query_lens[b] for b in idx)
             # (paged_attention routes the longest query block as `kind`.)
             paged_attention(q3, k_cache, v_cache, tables, lens, self.causal, max_seq_len=max_seq_len,
-                            scale=self.scale, out=o3, query_start=qs, query_lens=ql, max_query_len=max_q)
+                            scale=self.scale, out=o3, query_start=qs, query_lens=ql, max_query_len=max_q,
+                            softcap=self.softcap, alibi_slopes=self.alibi_slopes, prefix_lens=prefix)
         return output
+
+    def _norm_rope(self, query, key, value, k_cache, v_cache, md):
+        """Normed and rotated queries (a new tensor); keys and values, if given,
+        go to the cache."""
+        T, H, Hkv, D = query.shape[0], self.num_heads, self.num_kv_heads, self.head_size
+        q = query.view(T, H, D)
+        if key is None:
+            if self.rotary is None and self.q_norm_weight is None:
+                return query
+            out, _ = qk_norm_rope(q, None, md.positions, self.rotary, q_weight=self.q_norm_weight, eps=self.norm_eps)
+        else:
+            out = qk_norm_rope_write(q, key.view(T, Hkv, D), value.view(T, Hkv, D), md.positions, self.rotary, k_cache,
+                                     v_cache, md.slot_mapping, q_weight=self.q_norm_weight,
+                                     k_weight=self.k_norm_weight, eps=self.norm_eps)
+        return out.reshape(T, H * D)

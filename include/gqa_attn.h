@@ -54,6 +54,8 @@ extern "C" {
                                  GQA_NOALLOC_SCRATCH_BYTES */
 #define GQA_E_FLAT (-10)      /* flat split: slots out of [1, GQA_MAX_SPLITS], no keys, or a call
                                  the LDS-DMA first pass does not take (see gqa_split_flat_launch) */
+#define GQA_E_SCORE (-11)     /* changed scores: see gqa_scored_launch */
+#define GQA_E_ROPE (-12)      /* rotation: see gqa_rope */
 
 #define GQA_MAX_SPLITS 1024
 #define GQA_MAX_BLOCK_SIZE 65536
@@ -451,6 +453,64 @@ int gqa_paged_fwd_split_launch(const void* q, const int64_t q_stride[4],
                                int seq_q, int head_dim,
                                float scale_log2, int causal, int dtype, void* stream);
 
+/* Attention with changed scores (no counterpart in the reference): for query
+ * row i of a sequence with S_kv keys, at position p = i + S_kv - S_q, and key j
+ *   s = scale q_i . k_j;  softcap > 0: s <- softcap tanh(s / softcap);
+ *   alibi_slopes: s <- s - alibi_slopes[head] |p - j|;
+ * key j is visible if it lies in [0, S_kv), and (causal) j <= p or, with
+ * prefix_lens, j < prefix_lens[b], and, with spans, span_lo[b, p] <= j <
+ * span_hi[b, p].  A row without visible keys gives zeros and LSE -inf.
+ * softcap 0 and NULL pointers leave a change out; the pointers are device
+ * arrays, 4-byte aligned, contiguous.  V rows of hidden keys must be finite
+ * (they are multiplied with a probability of zero), K rows may hold anything.
+ * GQA_E_SCORE: softcap / scale outside its range, scale_log2 not positive,
+ * prefix_lens without causal, spans with paged caches, with seq_q > seq_kv or
+ * with the split and flat forms, or an unknown form. */
+#define GQA_MIN_RAW_SOFTCAP 1e-2f
+#define GQA_MAX_RAW_SOFTCAP 1e8f
+typedef struct gqa_score {
+  float softcap;
+  const float* alibi_slopes; /* (num_heads) */
+  const int* prefix_lens;    /* (batch) */
+  const int* span_lo;        /* (batch, seq_kv) */
+  const int* span_hi;        /* (batch, seq_kv) */
+} gqa_score;
+
+/* form: the launch whose work decomposition (and meaning of workspace, counters
+ * and parts) the call takes: gqa_split_launch (parts: splits),
+ * gqa_fwd_split_launch (n_split), gqa_fwd_chunks_launch (kv_splits),
+ * gqa_split_flat_launch (slots), gqa_fwd_short_launch (0), or their paged
+ * counterparts, whose other arguments and errors hold. */
+#define GQA_FORM_SPLIT 0
+#define GQA_FORM_SINGLE 1
+#define GQA_FORM_CHUNKS 2
+#define GQA_FORM_FLAT 3
+#define GQA_FORM_SHORT 4
+int gqa_scored_launch(int form,
+                      const void* q, const int64_t q_stride[4],
+                      const void* k, const int64_t k_stride[4],
+                      const void* v, const int64_t v_stride[4],
+                      void* o, const int64_t o_stride[4], float* lse,
+                      float* workspace, int* counters, int parts,
+                      int batch, int num_heads, int num_kv_heads,
+                      int seq_q, int seq_kv, int head_dim,
+                      float scale_log2, int causal, int dtype,
+                      const gqa_score* score, void* stream);
+
+int gqa_paged_scored_launch(int form,
+                            const void* q, const int64_t q_stride[4],
+                            const void* k_cache, const int64_t k_cache_stride[4],
+                            const void* v_cache, const int64_t v_cache_stride[4],
+                            const int* block_table, int table_stride,
+                            const int* seq_lens, const int* q_start, const int* q_len,
+                            int block_size, int max_seq_len,
+                            void* o, const int64_t o_stride[4], float* lse,
+                            float* workspace, int* counters, int parts,
+                            int batch, int num_heads, int num_kv_heads,
+                            int seq_q, int head_dim,
+                            float scale_log2, int causal, int dtype,
+                            const gqa_score* score, void* stream);
+
 /* gqa_split_reduce_launch for variable query lengths (q_start, q_len as
  * above, non-NULL; o token-major); lse may be NULL or receives (tokens,
  * num_heads). */
@@ -473,6 +533,100 @@ int gqa_paged_cache_write_launch(const void* k, const int64_t k_stride[3],
                                  const int64_t* slot_mapping, int num_tokens,
                                  int num_kv_heads, int head_dim, int block_size,
                                  int dtype, void* stream);
+
+/* Per-head RMS norm and rotation of queries and keys (no counterpart in the
+ * reference), in fp32 and rounded once:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight   (weight NULL: y = x)
+ *   pair i = (a, b), i < rotary_dim / 2, turned by the angle of row
+ *   positions[axis(i), token] of `table`: (a cos - b sin, b cos + a sin).
+ * table: (max_positions, rotary_dim / 2) pairs of floats (cos, sin), 16-byte
+ * aligned, or NULL: no rotation.  Pairs are dimensions (i, i + rotary_dim / 2),
+ * or (2 i, 2 i + 1) with interleaved != 0.  positions: (axes, tokens) int32, or
+ * int64 with positions64 != 0; a negative position is taken as 0, one past the
+ * table gives NaN.  axes <= 4; axis(i) is 2 bits, pair_axis[i / 16] >> 2 (i %
+ * 16).  Weights: (head_dim) of the tensors' dtype, or float with weights32;
+ * 16-byte aligned. */
+typedef struct gqa_rope {
+  const float* table;
+  int max_positions;
+  int rotary_dim; /* a multiple of 16 up to head_dim */
+  int interleaved;
+  const void* positions;
+  int positions64;
+  int axes;
+  uint32_t pair_axis[4];
+  const void* q_weight;
+  const void* k_weight;
+  int weights32;
+  float eps;
+} gqa_rope;
+
+/* q, k: (batch, heads, seq, head_dim) with element strides (last 1, rows
+ * 16-byte aligned); q_out and k_out likewise, and may be q and k.  k and k_out
+ * NULL: queries alone.  Token (b, s) is token b * seq + s of the positions. */
+int gqa_qk_norm_rope_launch(const void* q, const int64_t q_stride[4],
+                            const void* k, const int64_t k_stride[4],
+                            void* q_out, const int64_t q_out_stride[4],
+                            void* k_out, const int64_t k_out_stride[4],
+                            const gqa_rope* rope,
+                            int batch, int num_heads, int num_kv_heads, int seq,
+                            int head_dim, int dtype, void* stream);
+
+/* The same for token-major q, k, v (num_tokens, heads, head_dim), with k (normed,
+ * rotated) and v (as it is) stored at their slots of paged caches as
+ * gqa_paged_cache_write_launch stores them. */
+int gqa_qk_norm_rope_write_launch(const void* q, const int64_t q_stride[3],
+                                  const void* k, const int64_t k_stride[3],
+                                  const void* v, const int64_t v_stride[3],
+                                  void* q_out, const int64_t q_out_stride[3],
+                                  void* k_cache, const int64_t k_cache_stride[4],
+                                  void* v_cache, const int64_t v_cache_stride[4],
+                                  const int64_t* slot_mapping, const gqa_rope* rope,
+                                  int num_tokens, int num_heads, int num_kv_heads,
+                                  int head_dim, int block_size, int dtype,
+                                  void* stream);
+
+/* lo, hi (batch, seq) <- the first token, and the first behind the last, of each
+ * token's document: a run of equal ids in its row of ids (batch, seq; int32, rows
+ * row_stride apart).  Tokens of negative ids (padding): [0, 0). */
+int gqa_document_spans_launch(const int* ids, int64_t row_stride, int* lo, int* hi,
+                              int batch, int seq, void* stream);
+
+/* One step of a batch over a pool of paged sequences, on the device: request b
+ * appends query_lens[b] tokens to the sequence of pool row rows[b] (NULL: row
+ * b), whose keys so far are pool_lens[row] and whose pages block_tables[row, :]
+ * (rows table_stride apart, table_width entries).  New pages come from the top
+ * of the free list (free_blocks[0 .. *free_count)), request by request, and are
+ * entered in block_tables; with update != 0, pool_lens and *free_count move on
+ * too.  Outputs: seq_lens (batch) keys after the step; query_start (batch);
+ * query_lens_out (batch), 0 for a refused request; slot_mapping and positions
+ * (num_tokens): the tokens in request order, slot -1 and position 0 for tokens of
+ * refused requests and behind the last; batch_tables (batch, table_width), 0
+ * behind a request's pages; new_free_count (1); refused (1).
+ * A request is refused, and its sequence stays as it was, if its row is outside
+ * the pool or another request's before it, its tokens pass num_tokens, its pages
+ * the table's width, or the blocks that it and the requests before it need the
+ * free list.  A negative row is an empty place, not counted in refused.
+ * scratch: gqa_extend_tables_scratch_bytes bytes.  Calls that share a pool or a
+ * scratch are ordered on one stream. */
+size_t gqa_extend_tables_scratch_bytes(int pool_rows, int batch);
+int gqa_extend_tables_launch(int* block_tables, int64_t table_stride, int table_width,
+                             int* pool_lens, int pool_rows, const int* rows,
+                             const int* query_lens, const int* free_blocks,
+                             int* free_count, int num_blocks, int block_size,
+                             int update, int batch, int num_tokens,
+                             int* seq_lens, int* query_start, int* query_lens_out,
+                             int64_t* slot_mapping, int* positions,
+                             int* batch_tables, int* new_free_count, int* refused,
+                             int* scratch, void* stream);
+
+/* The blocks of the sequences in rows (batch) go back on top of the free list,
+ * their lengths become 0.  Rows outside the pool, and a row's second mention,
+ * are passed over.  scratch: as above. */
+int gqa_release_blocks_launch(const int* block_tables, int64_t table_stride, int table_width,
+                              int* pool_lens, int pool_rows, const int* rows, int batch,
+                              int* free_blocks, int* free_count, int num_blocks,
+                              int block_size, int* scratch, void* stream);
 
 #ifdef __cplusplus
 }
