@@ -974,18 +974,27 @@ int gqa_split_noalloc_launch(const void* q, const int64_t q_stride[4], const voi
 namespace {
 
 // The kernels' parameters of `score`; scale = scale_log2 / log2(e).
-int score_mod(const gqa_score* score, float scale_log2, int causal, bool paged, int seq_q, int seq_kv,
+// scale_log2 becomes the kernel's Dims::c.
+int score_mod(const gqa_score* score, float& scale_log2, int causal, bool paged, int seq_q, int seq_kv,
               gqa::ScoreMod& m) {
   constexpr float kLog2e = 1.44269504088896340736f;
   if (score == nullptr) return GQA_E_NULL;
   m = gqa::ScoreMod{};
   const float scale = scale_log2 / kLog2e;
   if (!(scale > 0.f) || !std::isfinite(scale)) return GQA_E_SCORE;
+  m.unit = 1.f / scale;
   if (score->softcap != 0.f) {
     if (!(score->softcap > 0.f)) return GQA_E_SCORE;
-    m.cap = score->softcap / scale;
-    if (!(m.cap >= GQA_MIN_RAW_SOFTCAP && m.cap <= GQA_MAX_RAW_SOFTCAP)) return GQA_E_SCORE;
-    m.cap_exp = 2.f * kLog2e / m.cap;
+    const float cap = score->softcap / scale;
+    if (!(cap >= GQA_MIN_RAW_SOFTCAP && cap <= GQA_MAX_RAW_SOFTCAP)) return GQA_E_SCORE;
+    if (score->softcap <= gqa::kUsualCap) {
+      m.cap_exp = 2.f * kLog2e / cap;
+      m.shift2 = score->softcap * kLog2e;
+      m.unit = 0.5f / score->softcap;
+      scale_log2 = 2.f * score->softcap * kLog2e;
+    } else {
+      gqa::set_wide_cap(m, cap);
+    }
   }
   if (((reinterpret_cast<uintptr_t>(score->alibi_slopes) | reinterpret_cast<uintptr_t>(score->prefix_lens) |
         reinterpret_cast<uintptr_t>(score->span_lo) | reinterpret_cast<uintptr_t>(score->span_hi)) &
@@ -995,7 +1004,6 @@ int score_mod(const gqa_score* score, float scale_log2, int causal, bool paged, 
   if ((score->span_lo == nullptr) != (score->span_hi == nullptr)) return GQA_E_NULL;
   if (score->span_lo != nullptr && (paged || seq_q > seq_kv)) return GQA_E_SCORE;
   m.slopes = score->alibi_slopes;
-  m.inv_scale = 1.f / scale;
   m.prefix = score->prefix_lens;
   m.span_lo = score->span_lo;
   m.span_hi = score->span_hi;

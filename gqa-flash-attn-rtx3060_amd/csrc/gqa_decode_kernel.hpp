@@ -609,10 +609,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int j = 0; j < NMB * NKS; ++j) sc[j % NMB] = E::mfma(opk[j], qreg[j / NMB], sc[j % NMB]);
     }
     const int key0 = c0 + tile_rel(it) * 64;
+    [[maybe_unused]] float row_t = 0.f;  // changed scores: added to every score of the lane
+    const auto at = [&](float x) __attribute__((always_inline)) {
+      if constexpr (MOD) return x + row_t;
+      else return x;
+    };
     if constexpr (MOD) {
-      if (p.mod.cap > 0.f) cap_scores<16>(sc, p.mod);
+      cap_scores<16>(sc, p.mod);
       if (p.mod.slopes != nullptr)
-        bias_scores<16>(sc, slope, key0 + 32 * kh * NMB + 8 * hh - qpos, key0 + 63 <= qpos_lo,
+        row_t = bias_scores<16>(sc, slope, key0 + 32 * kh * NMB + 8 * hh - qpos, key0 + 63 <= qpos_lo,
                         [](int e) { return 32 * (e >> 4) + key_of(e & 15, 0); });
     }
     const bool need_mask = (key0 + 64 > c1) || (dm.causal && key0 + 63 > seen_lo);
@@ -640,17 +645,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       m1[10] = vmax3(sc[NMB - 1][14], sc[NMB - 1][15], sc[NMB - 1][15]);
       const float n0 = vmax3(m1[0], m1[1], m1[2]), n1 = vmax3(m1[3], m1[4], m1[5]);
       const float n2 = vmax3(m1[6], m1[7], m1[8]), n3 = vmax3(m1[9], m1[10], m1[10]);
-      mx = xhalf_max(vmax3(vmax3(n0, n1, n2), n3, n3));
+      mx = xhalf_max(at(vmax3(vmax3(n0, n1, n2), n3, n3)));
     } else {
       float m1[5];
 #pragma unroll
       for (int k = 0; k < 5; ++k) m1[k] = vmax3(sc[0][3 * k], sc[0][3 * k + 1], sc[0][3 * k + 2]);
-      mx = xhalf_max(vmax3(vmax3(m1[0], m1[1], m1[2]), vmax3(m1[3], m1[4], sc[0][15]), sc[0][15]));
+      mx = xhalf_max(at(vmax3(vmax3(m1[0], m1[1], m1[2]), vmax3(m1[3], m1[4], sc[0][15]), sc[0][15])));
     }
     const float m_new = fmaxf(m_run, mx);
     const float m_use = (m_new == -__builtin_inff()) ? 0.f : m_new;
     const float alpha = fast_exp2((m_run - m_use) * c);
-    const float nmc = -m_use * c;
+    const float nmc = MOD ? (row_t - m_use) * c : -m_use * c;
     u32x4 pk[NMB][2];
     float rs = 0.f;
 #pragma unroll
@@ -753,7 +758,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const float l_tot = xhalf_sum(l_run);
   if (FLAT && p.direct) {
     if (valid && kh == 0)
-      store_rows_direct<DT>(p, b, head, pos, varlen, tok0, skv, m_run * c,
+      store_rows_direct<DT>(p, b, head, pos, varlen, tok0, skv, log2_ref(p, m_run, c),
                             MOD && l_tot == 0.f ? __builtin_inff() : l_tot, db0 == 0 && hh == 0,
                             [&](auto put) {
 #pragma unroll
@@ -781,7 +786,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // combine turns into a zero row.  One wave per row half stores them.
     if (db0 == 0 && hh == 0) {
       float m_out = skv == 0 ? 0.f : m_run * c;
-      if constexpr (MOD) m_out = m_run == -__builtin_inff() ? kEmptyRef : m_run * c;
+      if constexpr (MOD) m_out = m_run == -__builtin_inff() ? kEmptyRef : log2_ref(p, m_run, c);
       store_coherent(p.ws_m + row, m_out);
       store_coherent(p.ws_l + row, l_tot);
     }
@@ -1114,10 +1119,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int kb = 0; kb < NKB; ++kb) sc[kb] = E::mfma16(opk[kb * NKS + ks], qreg[ks], sc[kb]);
     }
     const int key0 = c0 + tile_rel(it) * TK;
+    [[maybe_unused]] float row_t = 0.f;  // changed scores: added to every score of the lane
+    const auto at = [&](float x) __attribute__((always_inline)) {
+      if constexpr (MOD) return x + row_t;
+      else return x;
+    };
     if constexpr (MOD) {
-      if (p.mod.cap > 0.f) cap_scores<4>(sc, p.mod);
+      cap_scores<4>(sc, p.mod);
       if (p.mod.slopes != nullptr)
-        bias_scores<4>(sc, slope, key0 + 4 * lg - qpos, key0 + TK - 1 <= qpos_lo,
+        row_t = bias_scores<4>(sc, slope, key0 + 4 * lg - qpos, key0 + TK - 1 <= qpos_lo,
                        [](int e) { return 16 * (e >> 2) + (e & 3); });
     }
     const bool need_mask = (key0 + TK > c1) || (dm.causal && key0 + TK - 1 > seen_lo);
@@ -1138,7 +1148,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const float t0 = vmax3(sc[0][0], sc[0][1], sc[0][2]), t1 = vmax3(sc[0][3], sc[1][0], sc[1][1]);
       const float t2 = vmax3(sc[1][2], sc[1][3], sc[2][0]), t3 = vmax3(sc[2][1], sc[2][2], sc[2][3]);
       const float t4 = vmax3(sc[3][0], sc[3][1], sc[3][2]);
-      mx = xhalf_max(xquad_max(fmaxf(vmax3(t0, t1, t2), vmax3(t3, t4, sc[3][3]))));
+      mx = xhalf_max(xquad_max(at(fmaxf(vmax3(t0, t1, t2), vmax3(t3, t4, sc[3][3])))));
     } else {
       float tb[NKB];
 #pragma unroll
@@ -1147,12 +1157,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int w = NKB / 2; w >= 1; w /= 2)
 #pragma unroll
         for (int kb = 0; kb < w; ++kb) tb[kb] = fmaxf(tb[kb], tb[kb + w]);
-      mx = xhalf_max(xquad_max(tb[0]));
+      mx = xhalf_max(xquad_max(at(tb[0])));
     }
     const float m_new = fmaxf(m_run, mx);
     const float m_use = (m_new == -__builtin_inff()) ? 0.f : m_new;
     const float alpha = fast_exp2((m_run - m_use) * c);
-    const float nmc = -m_use * c;
+    const float nmc = MOD ? (row_t - m_use) * c : -m_use * c;
     float pv[NKB][4];
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb)
@@ -1220,7 +1230,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const float l_tot = xhalf_sum(xquad_sum(l_run));
   if (FLAT && p.direct) {
     if (valid)
-      store_rows_direct<DT>(p, b, head, pos, varlen, tok0, skv, m_run * c,
+      store_rows_direct<DT>(p, b, head, pos, varlen, tok0, skv, log2_ref(p, m_run, c),
                             MOD && l_tot == 0.f ? __builtin_inff() : l_tot, wave == 0 && lg == 0,
                             [&](auto put) {
 #pragma unroll
@@ -1236,7 +1246,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       store_coherent4(rw, (uint32_t)((row * D + (D / 4) * wave + 16 * db + 4 * lg) * 4), 0, acc[db]);
     if (wave == 0 && lg == 0) {
       float m_out = skv == 0 ? 0.f : m_run * c;
-      if constexpr (MOD) m_out = m_run == -__builtin_inff() ? kEmptyRef : m_run * c;
+      if constexpr (MOD) m_out = m_run == -__builtin_inff() ? kEmptyRef : log2_ref(p, m_run, c);
       store_coherent(p.ws_m + row, m_out);
       store_coherent(p.ws_l + row, l_tot);
     }

@@ -66,7 +66,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(D == 64 && 
   using ST = FwdStage<D>;
   constexpr int CPR = ST::CPR;
   constexpr bool PAGED = PG != 0;
-  constexpr bool PERSIST = PG == 0 && D == 128;
+  constexpr bool PERSIST = PG == 0 && D == 128 && !MOD;
   using TileBlocks = FwdTileBlocks<D, PG>;
   constexpr int NDB = D / 32;  // 32-wide d blocks of O^T
   constexpr int NKS = D / 16;  // k-steps of S^T
@@ -337,20 +337,27 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(D == 64 && 
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) qreg[ks] = *reinterpret_cast<const u32x4*>(qrow + 16 * ks + 8 * hh);
   };
+  // The tt-th tile to be taken.
+  bool back = false;
+  if constexpr (MOD) back = p.mod.slopes != nullptr && dm.causal;
+  auto tile_of = [&](const Item& x, int tt) __attribute__((always_inline)) -> int {
+    if constexpr (MOD) return tile_at(x.tb, x.ntiles, tt, back);
+    else return x.tb + tt;
+  };
   auto prologue_kv = [&](const Item& x) __attribute__((always_inline)) -> TileBlocks {
-    TileBlocks bn = tile_block(x, x.tb);
+    TileBlocks bn = tile_block(x, tile_of(x, 0));
     if (grp == 0) {
-      issue_k(x, lds1_k0, x.tb, bn);
+      issue_k(x, lds1_k0, tile_of(x, 0), bn);
     } else {
-      issue_v(x, lds0_v1, x.tb, bn);
+      issue_v(x, lds0_v1, tile_of(x, 0), bn);
     }
-    bn = tile_block(x, x.tb + 1);
+    bn = tile_block(x, tile_of(x, 1));
     if (grp == 0) {
-      issue_k(x, lds1_k1, x.tb + 1, bn);
+      issue_k(x, lds1_k1, tile_of(x, 1), bn);
     } else {
-      issue_v(x, lds0_v2, x.tb + 1, bn);
+      issue_v(x, lds0_v2, tile_of(x, 1), bn);
     }
-    bn = tile_block(x, x.tb + 2);
+    bn = tile_block(x, tile_of(x, 2));
     return bn;
   };
   TileBlocks blk_next = prologue_kv(it);
@@ -430,18 +437,18 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(D == 64 && 
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
-    const int ta = it.tb + tt;  // absolute tile index
     if (grp == 0) {
-      issue_k(it, kstage(std::integral_constant<int, (S3 + 2) % 3>{}), ta + 2, blk_next);
+      issue_k(it, kstage(std::integral_constant<int, (S3 + 2) % 3>{}), tile_of(it, tt + 2), blk_next);
     } else {
-      issue_v(it, vstage(s3), ta + 2, blk_next);
+      issue_v(it, vstage(s3), tile_of(it, tt + 2), blk_next);
     }
-    blk_next = tile_block(it, ta + 3);
-    const int key0 = ta * ST::kKeys;
+    blk_next = tile_block(it, tile_of(it, tt + 3));
+    const int key0 = tile_of(it, tt) * ST::kKeys;
+    [[maybe_unused]] float row_t = 0.f;  // changed scores: added to every score of the lane
     if constexpr (MOD) {
-      if (p.mod.cap > 0.f) cap_scores<16>(sc, p.mod);
+      cap_scores<16>(sc, p.mod);
       if (p.mod.slopes != nullptr)
-        bias_scores<16>(sc, slope, key0 + it.span.rel0, key0 + ST::kKeys - 1 <= it.qpos_lo,
+        row_t = bias_scores<16>(sc, slope, key0 + it.span.rel0, key0 + ST::kKeys - 1 <= it.qpos_lo,
                         [](int e) { return 32 * (e >> 4) + key_of(e & 15, 0); });
       if (key0 + ST::kKeys > it.span.full_hi || key0 < it.span.full_lo)
         mask_tile_span(sc, it.span.vis - key0, it.span.lo - key0);
@@ -456,7 +463,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(D == 64 && 
     bool keep = false;
     if constexpr (!FIRST) keep = __builtin_amdgcn_ballot_w64(m_run == -__builtin_inff()) == 0;
     if (keep) {
-      const float nmc = -m_run * c;
+      const float nmc = MOD ? (row_t - m_run) * c : -m_run * c;
       rs0 = softmax_exp<DT>(sc[0], nmc, c, pk[0]);
       rs1 = softmax_exp<DT>(sc[1], nmc, c, pk[1]);
       keep = __builtin_amdgcn_ballot_w64(!(rs0 + rs1 <= kRescaleSum)) == 0;
@@ -465,9 +472,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(D == 64 && 
       float nmc;
       if constexpr (FIRST) {
         f32x16 none[1] = {f32x16{}};
-        nmc = softmax_rebase<1>(sc, m_run, l_run, none, c);
+        if constexpr (MOD) nmc = softmax_rebase_at<1>(sc, row_t, m_run, l_run, none, c);
+        else nmc = softmax_rebase<1>(sc, m_run, l_run, none, c);
       } else {
-        nmc = softmax_rebase<NDB>(sc, m_run, l_run, acc, c);
+        if constexpr (MOD) nmc = softmax_rebase_at<NDB>(sc, row_t, m_run, l_run, acc, c);
+        else nmc = softmax_rebase<NDB>(sc, m_run, l_run, acc, c);
       }
       rs0 = softmax_exp<DT>(sc[0], nmc, c, pk[0]);
       rs1 = softmax_exp<DT>(sc[1], nmc, c, pk[1]);
@@ -661,7 +670,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(D == 64 && 
             *reinterpret_cast<f32x4*>(wa + 32 * db + 8 * j) =
                 f32x4{acc[db][4 * j], acc[db][4 * j + 1], acc[db][4 * j + 2], acc[db][4 * j + 3]};
         if (hh_e == 0) {
-          if constexpr (MOD) p.ws_m[row] = m_run == -__builtin_inff() ? kEmptyRef : m_run * c;
+          if constexpr (MOD) p.ws_m[row] = m_run == -__builtin_inff() ? kEmptyRef : log2_ref(p, m_run, c);
           else p.ws_m[row] = ie.skv == 0 ? 0.f : m_run * c;
           p.ws_l[row] = l_tot;
         }
@@ -680,7 +689,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(D == 64 && 
         // (B, Hq, Sq), or (tokens, Hq) with variable lengths.
         const int64_t li = varlen ? (ie.tok0 + ie.pos) * dm.Hq + ie.head
                                   : ((int64_t)ie.b * dm.Hq + ie.head) * dm.Sq + ie.pos;
-        p.lse[li] = (m_run * c + __log2f(l_tot)) * kLn2;
+        p.lse[li] = (log2_ref(p, m_run, c) + __log2f(l_tot)) * kLn2;
       }
       {
         // The wave's 32 x D output tile goes through LDS (row-major, 16-byte
@@ -814,7 +823,7 @@ static hipError_t launch_fwd_t(P p, hipStream_t stream) {
   p.div_hkv = make_fast_div((uint32_t)p.dm.Hkv);
   p.bm_mul = (65536u + (uint32_t)p.block_m - 1) / (uint32_t)p.block_m;
   int grid = total;
-  if (PG == 0 && D == 128) {
+  if (PG == 0 && D == 128 && !kHasMod<P>) {
     grid = cus > 0 ? std::min(total, cus) : total;
     p.n_wg = grid;
     // The dynamic schedule pays for its claims (atomic round trips of ~2 us,

@@ -161,17 +161,24 @@ struct ReduceParams {
 };
 
 // Changed scores (gqa_score.hpp): what a kernel does to s = q . k before the
-// softmax, in units of the raw product (scores divided by the score scale).
+// softmax.  Its units are the kernel's: Dims::c turns them into exponents of
+// two.  Without a cap, and under a wide one, they are those of the raw product;
+// under a usual cap the kernel's score is -1 / (1 + exp(2 score / softcap)), which
+// is (capped score - softcap) / (2 softcap).
 struct ScoreMod {
-  float cap;           // softcap / scale: s <- cap tanh(s / cap); 0: none
-  float cap_exp;       // 2 log2(e) / cap
-  const float* slopes; // (Hq): s <- s - slope |p - j| / scale; nullptr: none
-  float inv_scale;
+  float cap_exp;       // usual cap: 2 log2(e) scale / softcap; 0: none
+  float cap;           // wide cap: softcap / scale; 0: none
+  float shift2;        // what a row's log2 sum lacks: softcap log2(e) under a usual cap
+  const float* slopes; // (Hq): score - slope |p - j|; nullptr: none
+  float unit;          // kernel units of a score of 1
   const int* prefix;   // (B): keys below prefix[b] are visible to every row (causal only); nullptr: none
   // (B, Skv): the keys [span_lo, span_hi) of the document of each position;
   // nullptr: one document.  Contiguous K/V with Sq <= Skv only.
   const int* span_lo;
   const int* span_hi;
+  // Wide cap: tanh(x) = x (1 + u P(u)), u = x^2 = (s / cap)^2: P's coefficients for
+  // |s| up to lim3, their powers of 1 / cap folded in (set_wide_cap).
+  float wide_exp, lim3, p3[3];
 };
 
 // Packed query rows per single-pass workgroup (8 waves x 32 rows).
@@ -224,6 +231,21 @@ struct CacheWriteParams {
   int n_tokens, Hkv, D, block_shift;
   int elem_bytes;
 };
+
+// Softcaps up to this are usual ones: their form is off by 2^-22 of the softcap.
+constexpr float kUsualCap = 128.f;
+
+// A wide cap (in raw units) and its polynomial (a least-squares fit iterated to
+// equal ripple, of relative error 7e-8 on |x| <= 0.375).  The widest: up to where
+// the folded coefficients are normal numbers.
+inline void set_wide_cap(ScoreMod& m, float cap) {
+  constexpr double kP3[3] = {-0.33332332968711853, 0.1328972578048706, -0.04848729446530342};
+  m.cap = cap;
+  m.wide_exp = 2.0f * 1.44269504088896340736f / cap;
+  m.lim3 = cap > 262144.f ? cap / 64.f : 0.375f * cap;
+  double f = 1.0;
+  for (int i = 0; i < 3; ++i) m.p3[i] = (float)(kP3[i] * (f /= (double)cap * cap));
+}
 
 struct FwdModParams : FwdParams {
   ScoreMod mod;

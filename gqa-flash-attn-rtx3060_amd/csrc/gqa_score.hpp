@@ -5,13 +5,23 @@
 //   s <- cap tanh(s / cap),  s <- s - slope |p - j|,  visible keys by causal
 //   order, a prefix and documents,
 //
-// p the query's position in key coordinates (row + Skv - Sq), j the key's, all
-// in units of the raw product s = q . k: the softmax applies the score scale
-// as it does without changes.  A row that sees no key gives zeros and LSE
-// -inf here (without changes it gives the reference's 0 / 0 = NaN).
+// p the query's position in key coordinates (row + Skv - Sq), j the key's.  A
+// row that sees no key gives zeros and LSE -inf here (without changes it gives
+// the reference's 0 / 0 = NaN).
 //
-// What bounds them is the vector ALU: a plain tile costs a score one exp2 and
-// about four further instructions, next to the matrix product it hides.
+// What bounds them is the number of vector instructions a score: three and a
+// half without changes (fma, exp2, sum, half a conversion), beside the matrix
+// products that they hide.  An instruction more costs 8192 causal tokens (G = 4,
+// head_dim 128) about 35 us of 470, exp2 and reciprocals like any other: five
+// instructions of a cap in place of the raw score 646 us, a polynomial tanh of
+// five and a half 663.
+//
+// So a usual cap takes four, by changing the unit:
+//   cap tanh(s / cap) = cap - 2 cap / (1 + exp(2 s / cap))
+// is 2 cap times s' = -1 / (1 + 2^(cap_exp s)) plus a constant, which the softmax
+// does not see (the log-sum-exp gets it back: shift2); Dims::c is 2 softcap
+// log2(e).  A distance bias of keys that no row precedes is one: the row's own
+// part, slope (first key - p), goes into the exponent's offset.
 #pragma once
 
 #include <type_traits>
@@ -30,33 +40,98 @@ template <typename P> constexpr bool kHasMod = std::is_same<P, FwdModParams>::va
 // combine of empty partials alone, l = 0, gives zeros).
 constexpr float kEmptyRef = -1e30f;
 
-// The scores of one tile in W-wide register vectors.
+// v_max3_f32 of a and the sizes of b and c.
+__device__ __forceinline__ float vmax3_abs(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// The scores of one tile are in W-wide register vectors (N * W a multiple of 8).
 //
-// s <- cap tanh(s / cap) = cap - 2 cap / (1 + 2^(s cap_exp)); the ends follow
-// from 1 / (1 + inf) = 0 and 1 / (1 + 0) = 1.
+// s <- cap tanh(s / cap) for wide caps, where a rounding of the other form, 2^-22
+// of the cap, would be lost to scores far below it.  By the largest |s| of the
+// wave's tile: s (1 + u P(u)), u = s^2, or cap - 2 cap / (1 + exp(2 s / cap)).
 template <int W, typename V, int N>
-__device__ __forceinline__ void cap_scores(V (&s)[N], const ScoreMod& m) {
+__device__ __forceinline__ void wide_cap_scores(V (&s)[N], const ScoreMod& m) {
+  constexpr int E = N * W;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int e = 0; e < N * W; ++e) {
-    const float x = fast_exp2(s[e / W][e % W] * m.cap_exp);
-    s[e / W][e % W] = __builtin_fmaf(-2.f * m.cap, __builtin_amdgcn_rcpf(1.f + x), m.cap);
+  for (int e = 0; e < E; e += 8)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      t[k] = vmax3_abs(t[k], s[(e + 2 * k) / W][(e + 2 * k) % W], s[(e + 2 * k + 1) / W][(e + 2 * k + 1) % W]);
+  const float mx = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+  if (__builtin_amdgcn_ballot_w64(!(mx <= m.lim3)) == 0) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float x = s[e / W][e % W], u = x * x;
+      s[e / W][e % W] = __builtin_fmaf(x * u, __builtin_fmaf(__builtin_fmaf(m.p3[2], u, m.p3[1]), u, m.p3[0]), x);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float x = fast_exp2(s[e / W][e % W] * m.wide_exp);
+      s[e / W][e % W] = __builtin_fmaf(-2.f * m.cap, __builtin_amdgcn_rcpf(1.f + x), m.cap);
+    }
   }
 }
 
-// s <- s - slope |p - j|, slope in raw units; rel: (this lane's first key) - p,
-// off(e): the key of value e counted from the lane's first.  `past`
-// (wave-uniform): no key of the tile lies behind any row's own position.
+// The cap (the ends of the usual form follow from 1 / (1 + inf) = 0 and 1 / (1 +
+// 0) = 1; NaN stays NaN).
+template <int W, typename V, int N>
+__device__ __forceinline__ void cap_scores(V (&s)[N], const ScoreMod& m) {
+  if (m.cap_exp > 0.f) {
+#pragma unroll
+    for (int e = 0; e < N * W; ++e)
+      s[e / W][e % W] = __builtin_amdgcn_rcpf(-1.f - fast_exp2(s[e / W][e % W] * m.cap_exp));
+  } else if (m.cap > 0.f) {
+    wide_cap_scores<W>(s, m);
+  }
+}
+
+// score - slope |p - j|; rel: (this lane's first key) - p, off(e): the key of value
+// e counted from the lane's first.  Returns what is left to be added to every
+// score of the lane: slope rel, if (`past`, wave-uniform) no key of the tile lies
+// behind any row's own position, else 0.
 template <int W, typename V, int N, typename F>
-__device__ __forceinline__ void bias_scores(V (&s)[N], float slope, int rel, bool past, F off) {
+__device__ __forceinline__ float bias_scores(V (&s)[N], float slope, int rel, bool past, F off) {
   const float r = (float)rel;
   if (past) {
 #pragma unroll
-    for (int e = 0; e < N * W; ++e) s[e / W][e % W] = __builtin_fmaf(slope, r + (float)off(e), s[e / W][e % W]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < N * W; ++e)
-      s[e / W][e % W] = __builtin_fmaf(-slope, __builtin_fabsf(r + (float)off(e)), s[e / W][e % W]);
+    for (int e = 0; e < N * W; ++e) s[e / W][e % W] = __builtin_fmaf(slope, (float)off(e), s[e / W][e % W]);
+    return slope * r;
   }
+#pragma unroll
+  for (int e = 0; e < N * W; ++e)
+    s[e / W][e % W] = __builtin_fmaf(-slope, __builtin_fabsf(r + (float)off(e)), s[e / W][e % W]);
+  return 0.f;
+}
+
+// softmax_rebase (gqa_fwd_parts.hpp) for scores s + t, t the lane's own.
+// Returns (t - m_ref) c, the offset of the exponent.
+template <int NACC>
+__device__ __forceinline__ float softmax_rebase_at(const f32x16 (&s)[2], float t, float& m_ref, float& l_run,
+                                                   f32x16 (&acc)[NACC], float c) {
+  float a[4] = {s[0][0], s[0][1], s[1][0], s[1][1]};
+#pragma unroll
+  for (int v = 2; v < 16; v += 4)
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb) {
+      a[2 * mb] = vmax3(a[2 * mb], s[mb][v], s[mb][v + 1]);
+      if (v + 2 < 16) a[2 * mb + 1] = vmax3(a[2 * mb + 1], s[mb][v + 2], s[mb][v + 3]);
+    }
+  const float mx = xhalf_max(vmax3(vmax3(a[0], a[1], a[2]), a[3], a[3]) + t);
+  const float m_new = fmaxf(m_ref, mx);
+  const float m_use = (m_new == -__builtin_inff()) ? 0.f : m_new;
+  const float alpha = fast_exp2((m_ref - m_use) * c);
+  l_run *= alpha;
+#pragma unroll
+  for (int db = 0; db < NACC; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[db][v] *= alpha;
+  m_ref = m_new;
+  return (t - m_use) * c;
 }
 
 // mask_tile with a first visible key: `lim` and `low` counted from the tile's
@@ -70,27 +145,43 @@ __device__ __forceinline__ void mask_tile_span(f32x16 (&s)[2], int lim, int low)
       s[mb][v] = (uint32_t)(32 * mb + key_of(v, 0) - low) >= n ? -__builtin_inff() : s[mb][v];
 }
 
-// A query row's slope in raw units (0 without a distance bias), a sequence's
+// Tile order: with a distance bias in causal order the last keys weigh most, so
+// the tiles are taken from the last one back and a row's reference point is
+// settled by its first tiles, where ascending tiles raise it again and again
+// (head slopes 2^-1/4 to 2^-8, 8192 tokens: AAAA us -> BBBB).  Place it of n tiles
+// from tb on (places past the end stay there: their loads read zeros).
+__device__ __forceinline__ int tile_at(int tb, int n, int it, bool back) {
+  return tb + (back && it < n ? n - 1 - it : it);
+}
+
+// A query row's slope in kernel units (0 without a distance bias), a sequence's
 // prefix among its skv keys (0 without one; any value of the caller's comes to
 // one in [0, skv], so that sums with it stay in range).
 __device__ __forceinline__ float row_slope(const ScoreMod& m, int head) {
-  return m.slopes != nullptr ? m.slopes[head] * m.inv_scale : 0.f;
+  return m.slopes != nullptr ? m.slopes[head] * m.unit : 0.f;
 }
 __device__ __forceinline__ int seq_prefix(const ScoreMod& m, int b, int skv) {
   return m.prefix != nullptr ? min(max(load_uniform(m.prefix + b), 0), skv) : 0;
 }
 
-// Smallest and largest over the wave.
+// A row's reference point in log2 units, as partials and the log-sum-exp take it.
+template <typename P> __device__ __forceinline__ float log2_ref(const P& p, float m, float c) {
+  if constexpr (kHasMod<P>) return __builtin_fmaf(m, c, p.mod.shift2);
+  else return m * c;
+}
+
+// Smallest and largest over the wave (row shifts, then row broadcasts, into
+// lane 63; a lane without a source keeps its own).
 __device__ __forceinline__ int wave_min(int x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));
-  return __builtin_amdgcn_readfirstlane(x);
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xF, 0xF, false));
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xF, 0xF, false));
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xF, 0xF, false));
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xF, 0xF, false));
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xA, 0xF, false));
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xC, 0xF, false));
+  return __builtin_amdgcn_readlane(x, 63);
 }
-__device__ __forceinline__ int wave_max(int x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
-  return __builtin_amdgcn_readfirstlane(x);
-}
+__device__ __forceinline__ int wave_max(int x) { return -wave_min(-x); }
 
 // What a query block of the single pass sees under changed scores: keys [beg,
 // end) over its rows (none: beg = end = 0); every row of the wave sees [full_lo,
@@ -117,9 +208,8 @@ __device__ __forceinline__ RowSpan row_span(const ScoreMod& m, const Dims& dm, i
     const int* ql = m.span_lo + (int64_t)b * dm.Skv + off;
     const int* qh = m.span_hi + (int64_t)b * dm.Skv + off;
     const int row = valid ? pos : pos_lo;
-    x.lo = min(max(ql[row], 0), skv);
-    x.vis = min(x.vis, valid ? max(qh[row], 0) : 0);
-    int first = 0x7fffffff, last = 0;
+    const int lo = ql[row], hi = qh[row];
+    int first = skv, last = 0;
     for (int ps = pos_lo + lane; ps <= pos_hi; ps += 64) {
       const int l = max(ql[ps], 0), h = min(qh[ps], end_of(ps));
       if (l < h) {
@@ -127,10 +217,12 @@ __device__ __forceinline__ RowSpan row_span(const ScoreMod& m, const Dims& dm, i
         last = max(last, h);
       }
     }
+    x.lo = min(max(lo, 0), skv);
+    x.vis = min(x.vis, valid ? max(hi, 0) : 0);
     x.end = wave_max(last);
-    x.beg = x.end > 0 ? wave_min(first) : 0;
+    x.beg = min(wave_min(first), x.end);
     x.full_lo = wave_max(valid ? x.lo : 0);
-    x.full_hi = wave_min(valid ? x.vis : 0x7fffffff);
+    x.full_hi = wave_min(valid ? x.vis : skv);
   }
   x.lo -= 8 * hh;
   x.vis -= 8 * hh;

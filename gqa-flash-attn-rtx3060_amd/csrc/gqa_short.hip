@@ -116,15 +116,21 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       (uint32_t)(lrow * kssb) + 16u * (uint32_t)((lane % CPR) ^ ST::gk((gw * ST::RPI + lrow) & 15));
   const uint32_t voff = (uint32_t)(lrow * vssb) + 16u * (uint32_t)((lane % CPR) ^ ST::sv(lrow));
   using Blocks = FwdTileBlocks<D, PG>;
+  bool back = false;
+  if constexpr (MOD) back = p.mod.slopes != nullptr && dm.causal;
+  auto tile_of = [&](int j) __attribute__((always_inline)) -> int {  // this group's j-th tile
+    if constexpr (MOD) return tile_at(tb, 2 * steps, 2 * j + grp, back);
+    else return 2 * j + grp;
+  };
   auto ids = [&](int j) __attribute__((always_inline)) -> Blocks {  // block(s) of this group's tile j
-    return tile_blocks<D, PG>(table_row, p.block_shift, rows_ld, tb + 2 * j + grp, gw);
+    return tile_blocks<D, PG>(table_row, p.block_shift, rows_ld, tile_of(j), gw);
   };
   auto issue_k = [&](char* stage, int j, const Blocks& blk) __attribute__((always_inline)) {
-    issue_fwd_tile<D, PG>(stage + grp * TB, kbh, rk, kssb, koff, p.k.sb, p.block_shift, rows_ld, tb + 2 * j + grp, blk, true,
+    issue_fwd_tile<D, PG>(stage + grp * TB, kbh, rk, kssb, koff, p.k.sb, p.block_shift, rows_ld, tile_of(j), blk, true,
                           gw, lane);
   };
   auto issue_v = [&](char* stage, int j, const Blocks& blk) __attribute__((always_inline)) {
-    issue_fwd_tile<D, PG>(stage + grp * TB, vbh, rv, vssb, voff, p.v.sb, p.block_shift, rows_ld, tb + 2 * j + grp, blk,
+    issue_fwd_tile<D, PG>(stage + grp * TB, vbh, rv, vssb, voff, p.v.sb, p.block_shift, rows_ld, tile_of(j), blk,
                           false, gw, lane);
   };
 
@@ -276,11 +282,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     issue_v(PAR == 0 ? lds0_v1 : lds0_v0, j + 1, id_v);
     id_v = id_k;
     id_k = ids(j + 3);
-    const int key0 = (tb + 2 * j + grp) * ST::kKeys;
+    const int key0 = tile_of(j) * ST::kKeys;
+    [[maybe_unused]] float row_t = 0.f;  // changed scores: added to every score of the lane
     if constexpr (MOD) {
-      if (p.mod.cap > 0.f) cap_scores<16>(sc, p.mod);
+      cap_scores<16>(sc, p.mod);
       if (p.mod.slopes != nullptr)
-        bias_scores<16>(sc, slope, key0 + span.rel0, key0 + ST::kKeys - 1 <= qpos_lo,
+        row_t = bias_scores<16>(sc, slope, key0 + span.rel0, key0 + ST::kKeys - 1 <= qpos_lo,
                         [](int e) { return 32 * (e >> 4) + key_of(e & 15, 0); });
       if (key0 + ST::kKeys > span.full_hi || key0 < span.full_lo) mask_tile_span(sc, span.vis - key0, span.lo - key0);
     } else {
@@ -291,7 +298,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     bool keep = false;
     if constexpr (!FIRST) keep = __builtin_amdgcn_ballot_w64(m_run == -__builtin_inff()) == 0;
     if (keep) {
-      const float nmc = -m_run * c;
+      const float nmc = MOD ? (row_t - m_run) * c : -m_run * c;
       rs0 = softmax_exp<DT>(sc[0], nmc, c, pk[0]);
       rs1 = softmax_exp<DT>(sc[1], nmc, c, pk[1]);
       keep = __builtin_amdgcn_ballot_w64(!(rs0 + rs1 <= kRescaleSum)) == 0;
@@ -300,9 +307,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       float nmc;
       if constexpr (FIRST) {  // (nothing to rescale yet)
         f32x16 none[1] = {f32x16{}};
-        nmc = softmax_rebase<1>(sc, m_run, l_run, none, c);
+        if constexpr (MOD) nmc = softmax_rebase_at<1>(sc, row_t, m_run, l_run, none, c);
+        else nmc = softmax_rebase<1>(sc, m_run, l_run, none, c);
       } else {
-        nmc = softmax_rebase<NDB>(sc, m_run, l_run, acc, c);
+        if constexpr (MOD) nmc = softmax_rebase_at<NDB>(sc, row_t, m_run, l_run, acc, c);
+        else nmc = softmax_rebase<NDB>(sc, m_run, l_run, acc, c);
       }
       rs0 = softmax_exp<DT>(sc[0], nmc, c, pk[0]);
       rs1 = softmax_exp<DT>(sc[1], nmc, c, pk[1]);
@@ -395,7 +404,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const float inv = (MOD ? l_tot == 0.f : skv == 0) ? 0.f : 1.0f / l_tot;  // (a sequence without keys: zero rows)
   if (p.lse != nullptr && valid && grp == 0 && hh == 0) {
     const int64_t li = varlen ? (tok0 + pos) * dm.Hq + head : ((int64_t)b * dm.Hq + head) * dm.Sq + pos;
-    p.lse[li] = (mm * c + __log2f(l_tot)) * kLn2;
+    p.lse[li] = (log2_ref(p, mm, c) + __log2f(l_tot)) * kLn2;
   }
   // The output block goes through LDS (row-major, 16-byte chunks XOR-swizzled
   // by row), so that it leaves as whole rows.

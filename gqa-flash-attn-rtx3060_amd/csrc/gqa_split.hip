@@ -309,11 +309,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int kb0 = key0 + 32 * wave;  // this wave's 32 keys
     if (kb0 >= c1) continue;           // wave-uniform: nothing visible here
     f32x16 sc = qk_block<DT, D>(mytile, qreg, mb, lane);
+    [[maybe_unused]] float row_t = 0.f;  // changed scores: added to every score of the lane
     if constexpr (MOD) {
       f32x16 s1[1] = {sc};
-      if (p.mod.cap > 0.f) cap_scores<16>(s1, p.mod);
+      cap_scores<16>(s1, p.mod);
       if (p.mod.slopes != nullptr)
-        bias_scores<16>(s1, slope, kb0 + 8 * hh - qpos, kb0 + 31 <= qpos_lo, [](int e) { return key_of(e, 0); });
+        row_t = bias_scores<16>(s1, slope, kb0 + 8 * hh - qpos, kb0 + 31 <= qpos_lo, [](int e) { return key_of(e, 0); });
       sc = s1[0];
     }
     // The last keys that this row, and every row of the block, sees.
@@ -329,11 +330,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     float mx = sc[0];
 #pragma unroll
     for (int v = 1; v < 16; ++v) mx = fmaxf(mx, sc[v]);
+    if constexpr (MOD) mx += row_t;
     mx = xhalf_max(mx);
     const float m_new = fmaxf(m_run, mx);
     const float m_use = (m_new == -__builtin_inff()) ? 0.f : m_new;
     const float alpha = fast_exp2((m_run - m_use) * c);
-    const float nmc = -m_use * c;
+    const float nmc = MOD ? (row_t - m_use) * c : -m_use * c;
     float pv[16];
     float rs = 0.f;
 #pragma unroll
@@ -407,7 +409,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       // otherwise: the chunk's largest score contributes exp2(0) = 1 to l),
       // which the combine turns into a zero row.
       if (db == 0 && hh == 0) {
-        if constexpr (MOD) store_coherent(p.ws_m + row, mstar == -__builtin_inff() ? kEmptyRef : mstar * c);
+        if constexpr (MOD) store_coherent(p.ws_m + row, mstar == -__builtin_inff() ? kEmptyRef : log2_ref(p, mstar, c));
         else store_coherent(p.ws_m + row, skv == 0 ? 0.f : mstar * c);
         store_coherent(p.ws_l + row, lsum);
       }
