@@ -90,7 +90,7 @@ int gqa_qk_norm_rope_launch(const void* q, const int64_t q_stride[4], const void
     p.k = ref4(k, k_stride);
     p.ko = ref4(k_out, k_out_stride);
   }
-  p.n_tokens = (int64_t)batch * seq;
+  p.n_tokens = batch * seq;
   p.S = seq;
   p.Hq = num_heads;
   p.Hkv = num_kv_heads;

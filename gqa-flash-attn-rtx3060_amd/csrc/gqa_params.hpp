@@ -264,13 +264,15 @@ struct RopeParams {
   const float* table;         // (max_pos, R / 2) pairs (cos, sin), or nullptr: no rotation
   const void* pos;            // (axes, B * S) int32 or int64
   const int64_t* slots;       // (B * S), negative: not stored
-  int64_t n_tokens;           // B * S
+  int n_tokens;               // B * S
   int S, Hq, Hkv, D, R, max_pos;
   int axes, pos64, interleaved, w32, block_shift;
   uint32_t pair_axis[4];      // 2 bits a pair
   float eps;
-  int parts;                  // waves a token's heads are dealt to (set by the launcher)
-  FastDiv div_parts;
+  // Set by the launcher: waves a token's rows are dealt to, divisions by it and
+  // by S.
+  int parts;
+  FastDiv div_parts, div_s;
 };
 
 // The spans of documents, runs of equal ids (gqa_tables.hip).

@@ -14,6 +14,7 @@
 // hold a (token, head) row, 16 values each, as the two 8-value chunks whose
 // pairs they rotate: no exchange but the sum of squares.  A wave takes rows of
 // one token, so its cos and sin stay in registers over the heads.
+#include <algorithm>
 #include <type_traits>
 
 #include "gqa_common.hpp"
@@ -74,66 +75,96 @@ __device__ inline void load_weights(const void* w, int w32, int ca, int cb, floa
 }  // namespace
 
 // Wave: token, and units part, part + parts, ... of its rows; a unit is RPW
-// heads of q, of k or of v.
+// heads of q, of k or of v.  The next unit's rows are loaded while one is worked
+// on.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void gqa_rope_kernel(RopeParams p) {
   using T = typename Elem<DT>::T;
   constexpr int LPR = D / 16, RPW = 64 / LPR;
   const int lane = threadIdx.x & 63;
-  const int64_t wid = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (wid >= p.n_tokens * p.parts) return;
-  const int64_t tok = wid / p.parts;
-  const int part = (int)(wid - tok * p.parts);
-  const int64_t b = tok / p.S, s = tok - b * p.S;
+  const int wid = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tok = fast_div(wid, p.div_parts.mul, p.div_parts.shift);
+  if (tok >= p.n_tokens) return;
+  const int part = wid - tok * p.parts;
+  const int b = fast_div(tok, p.div_s.mul, p.div_s.shift), s = tok - b * p.S;
   const int j = lane % LPR, row = lane / LPR;
   // This lane's chunks (8 values each): a rotated pair of them, or two behind
   // the rotated dimensions.
   const int rl = p.table != nullptr ? p.R / 16 : 0;  // lanes with rotated chunks
   const bool rot = j < rl;
-  int ca, cb;
-  if (rot && !p.interleaved) {
-    ca = j;
-    cb = p.R / 16 + j;
-  } else {
-    ca = 2 * j;
-    cb = 2 * j + 1;
-  }
-  // cos and sin of its pairs: 8 of the half form, or 4 of each chunk.
-  float cs[8], sn[8];
-  if (rot) {
-    const int first = 8 * j;  // (interleaved: chunks 2 j and 2 j + 1 hold pairs 8 j .. 8 j + 7)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int pair = first + i;
-      const int axis = p.axes > 1 ? (p.pair_axis[pair >> 4] >> (2 * (pair & 15))) & 3 : 0;
-      const int64_t at = (int64_t)axis * p.n_tokens + tok;
-      const int64_t ps = p.pos64 ? static_cast<const int64_t*>(p.pos)[at] : (int64_t)static_cast<const int*>(p.pos)[at];
-      const int64_t in = ps < 0 ? 0 : (ps < p.max_pos ? ps : p.max_pos - 1);
-      const float* e = p.table + (in * (p.R / 2) + pair) * 2;
-      cs[i] = ps < p.max_pos ? e[0] : __builtin_nanf("");
-      sn[i] = ps < p.max_pos ? e[1] : __builtin_nanf("");
-    }
-  }
-  const int64_t slot = p.kc.ptr != nullptr ? p.slots[tok] : -1;
-  const int64_t blk = slot >> p.block_shift, off = slot & ((1 << p.block_shift) - 1);
+  const bool apart = rot && !p.interleaved;
+  const int ca = apart ? j : 2 * j, cb = apart ? p.R / 16 + j : 2 * j + 1;
 
   const int nq = (p.Hq + RPW - 1) / RPW, nk = p.k.ptr != nullptr ? (p.Hkv + RPW - 1) / RPW : 0;
-  const int nv = p.kc.ptr != nullptr ? nk : 0;
-  for (int u = part; u < nq + nk + nv; u += p.parts) {
+  const int units = nq + nk + (p.kc.ptr != nullptr ? nk : 0);
+  const T* qr = static_cast<const T*>(p.q.ptr) + b * p.q.sb + s * p.q.ss;
+  const T* kr = static_cast<const T*>(p.k.ptr) + b * p.k.sb + s * p.k.ss;
+  const T* vr = static_cast<const T*>(p.v.ptr) + b * p.v.sb + s * p.v.ss;
+  u32x4 xa, xb;
+  const auto fetch = [&](int u) {
     const int kind = u < nq ? 0 : u < nq + nk ? 1 : 2;
     const int h = (kind == 0 ? u : kind == 1 ? u - nq : u - nq - nk) * RPW + row;
-    const bool in = h < (kind == 0 ? p.Hq : p.Hkv);
-    const TensorRef& src = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
-    u32x4 xa = {0u, 0u, 0u, 0u}, xb = xa;
-    if (in) {
-      const T* r = static_cast<const T*>(src.ptr) + b * src.sb + s * src.ss + (int64_t)h * src.sh;
+    const T* r = kind == 0 ? qr + h * p.q.sh : kind == 1 ? kr + h * p.k.sh : vr + h * p.v.sh;
+    xa = xb = u32x4{0u, 0u, 0u, 0u};
+    if (u < units && h < (kind == 0 ? p.Hq : p.Hkv)) {
       xa = *reinterpret_cast<const u32x4*>(r + 8 * ca);
       xb = *reinterpret_cast<const u32x4*>(r + 8 * cb);
     }
+  };
+  fetch(part);
+
+  // cos and sin of this lane's 8 pairs: of the half form, or 4 of each chunk
+  // (interleaved chunks 2 j and 2 j + 1 hold pairs 8 j .. 8 j + 7).
+  float cs[8], sn[8];
+  int64_t slot = -1;
+  if (p.kc.ptr != nullptr) slot = p.slots[tok];
+  const auto position = [&](int axis) -> int64_t {
+    const int64_t at = (int64_t)axis * p.n_tokens + tok;
+    return p.pos64 ? static_cast<const int64_t*>(p.pos)[at] : (int64_t)static_cast<const int*>(p.pos)[at];
+  };
+  const auto line = [&](int64_t ps) {  // the table's row of a position, in it
+    return p.table + (ps < 0 ? 0 : ps < p.max_pos ? ps : p.max_pos - 1) * p.R;
+  };
+  if (rl > 0) {
+    if (p.axes == 1) {
+      const int64_t ps = position(0);
+      const f32x4* e = reinterpret_cast<const f32x4*>(line(ps)) + 4 * (rot ? j : 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 x = e[i];
+        cs[2 * i] = x[0], sn[2 * i] = x[1], cs[2 * i + 1] = x[2], sn[2 * i + 1] = x[3];
+      }
+      if (ps >= p.max_pos)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) cs[i] = sn[i] = __builtin_nanf("");
+    } else {
+      const int64_t p0 = position(0), p1 = position(1), p2 = p.axes > 2 ? position(2) : 0,
+                    p3 = p.axes > 3 ? position(3) : 0;
+      typedef float f32x2 __attribute__((__vector_size__(8)));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int pair = 8 * (rot ? j : 0) + i;
+        const int w = pair >> 4;
+        const uint32_t word = w == 0 ? p.pair_axis[0] : w == 1 ? p.pair_axis[1] : w == 2 ? p.pair_axis[2] : p.pair_axis[3];
+        const uint32_t axis = (word >> (2 * (pair & 15))) & 3;
+        const int64_t ps = axis == 0 ? p0 : axis == 1 ? p1 : axis == 2 ? p2 : p3;
+        const f32x2 x = reinterpret_cast<const f32x2*>(line(ps))[pair];
+        cs[i] = ps < p.max_pos ? x[0] : __builtin_nanf("");
+        sn[i] = ps < p.max_pos ? x[1] : __builtin_nanf("");
+      }
+    }
+  }
+  const int64_t blk = slot >> p.block_shift, off = slot & ((1 << p.block_shift) - 1);
+
+  for (int u = part; u < units; u += p.parts) {
+    const int kind = u < nq ? 0 : u < nq + nk ? 1 : 2;
+    const int h = (kind == 0 ? u : kind == 1 ? u - nq : u - nq - nk) * RPW + row;
+    u32x4 oa = xa, ob = xb;
+    fetch(u + p.parts);
     if (kind != 2) {
       float ya[8], yb[8];
-      unpack8<DT>(xa, ya);
-      unpack8<DT>(xb, yb);
+      unpack8<DT>(oa, ya);
+      unpack8<DT>(ob, yb);
       const void* w = kind == 0 ? p.wq : p.wk;
       if (w != nullptr) {
         float wa[8], wb[8], ss = 0.f;
@@ -167,31 +198,37 @@ __global__ __launch_bounds__(256) void gqa_rope_kernel(RopeParams p) {
           }
         }
       }
-      xa = pack8<DT>(ya);
-      xb = pack8<DT>(yb);
+      oa = pack8<DT>(ya);
+      ob = pack8<DT>(yb);
     }
-    if (!in) continue;
+    const bool cached = kind != 0 && p.kc.ptr != nullptr;
+    if (h >= (kind == 0 ? p.Hq : p.Hkv) || (cached && slot < 0)) continue;
     T* o;
-    if (kind == 0 || p.kc.ptr == nullptr) {
-      const TensorRef& dst = kind == 0 ? p.qo : p.ko;
-      o = static_cast<T*>(const_cast<void*>(dst.ptr)) + b * dst.sb + s * dst.ss + (int64_t)h * dst.sh;
-    } else {
-      if (slot < 0) continue;
+    if (cached) {
       const TensorRef& dst = kind == 1 ? p.kc : p.vc;
       o = static_cast<T*>(const_cast<void*>(dst.ptr)) + blk * dst.sb + off * dst.ss + (int64_t)h * dst.sh;
+    } else {
+      const TensorRef& dst = kind == 0 ? p.qo : p.ko;
+      o = static_cast<T*>(const_cast<void*>(dst.ptr)) + b * dst.sb + s * dst.ss + (int64_t)h * dst.sh;
     }
-    *reinterpret_cast<u32x4*>(o + 8 * ca) = xa;
-    *reinterpret_cast<u32x4*>(o + 8 * cb) = xb;
+    *reinterpret_cast<u32x4*>(o + 8 * ca) = oa;
+    *reinterpret_cast<u32x4*>(o + 8 * cb) = ob;
   }
 }
 
 hipError_t launch_rope(const RopeParams& in, int dtype, hipStream_t stream) {
   RopeParams p = in;
   if (p.n_tokens <= 0) return hipSuccess;
-  p.parts = 1;
-  const int64_t blocks = (p.n_tokens * p.parts + 3) / 4;
-  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)blocks), block(256);
+  // Few tokens: their rows over more waves, up to kRopeWaves in all.
+  const int rpw = 1024 / p.D, nk = p.k.ptr != nullptr ? (p.Hkv + rpw - 1) / rpw : 0;
+  const int units = (p.Hq + rpw - 1) / rpw + nk + (p.kc.ptr != nullptr ? nk : 0);
+  constexpr int kRopeWaves = 4096;
+  p.parts = std::min(units, std::max(1, kRopeWaves / p.n_tokens));
+  p.div_parts = make_fast_div((uint32_t)p.parts);
+  p.div_s = make_fast_div((uint32_t)p.S);
+  const int64_t waves = (int64_t)p.n_tokens * p.parts;
+  if (waves >= (int64_t)1 << 31) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
   if (dtype == 0) {
     if (p.D == 128) hipLaunchKernelGGL((gqa_rope_kernel<0, 128>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((gqa_rope_kernel<0, 64>), grid, block, 0, stream, p);

@@ -1,6 +1,8 @@
 // gqa_tables.hip — what describes a batch to the attention kernels, built on
 // the device: the spans of documents, and a step's block tables, slots and
 // positions from the requests' lengths and a free list that lives there too.
+#include <algorithm>
+
 #include "gqa_common.hpp"
 #include "gqa_params.hpp"
 
@@ -33,48 +35,122 @@ __device__ inline int64_t block_scan(int64_t x, int64_t* tmp, int64_t& total) {
 
 }  // namespace
 
-// One workgroup a row: thread t takes S / 1024 consecutive tokens; the start of
-// the run that reaches into them is the last change before them, the end of
-// the run that leaves them the first change behind.
-__global__ __launch_bounds__(kPlanThreads) void gqa_spans_kernel(SpanParams p) {
-  __shared__ int s_last[kPlanThreads], s_first[kPlanThreads];
-  const int t = threadIdx.x;
-  const int* ids = p.ids + blockIdx.x * p.stride;
-  int* lo = p.lo + (int64_t)blockIdx.x * p.S;
-  int* hi = p.hi + (int64_t)blockIdx.x * p.S;
-  const int per = (p.S + kPlanThreads - 1) / kPlanThreads;
-  const int a = min(t * per, p.S), e = min(a + per, p.S);
-  int first = p.S, last = -1;  // changes among the thread's tokens
-  for (int i = a; i < e; ++i)
-    if (i == 0 || ids[i] != ids[i - 1]) {
-      last = i;
-      if (first == p.S) first = i;
-    }
-  s_last[t] = last;
-  s_first[t] = first;
+// A workgroup a row's kSpanChunk tokens, kSpanPer a thread.  The run that
+// reaches into them starts at the last change before them, the one that leaves
+// them ends at the first change behind; both are looked for a chunk at a time
+// (the chunk beside it holds them unless a document is longer than that).
+constexpr int kSpanPer = 4, kSpanChunk = kPlanThreads * kSpanPer;
+
+// Inclusive running maximum over the workgroup; kPlanThreads / 64 ints.
+__device__ inline int block_max_scan(int x, int* tmp) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xF, 0xF, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xF, 0xF, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xF, 0xF, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xF, 0xF, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xA, 0xF, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xC, 0xF, false));
+  __syncthreads();  // tmp's readers of the call before
+  if (lane == 63) tmp[wave] = x;
   __syncthreads();
-  for (int o = 1; o < kPlanThreads; o <<= 1) {  // running maximum from the left, minimum from the right
-    const int x = t >= o ? s_last[t - o] : -1, y = t + o < kPlanThreads ? s_first[t + o] : p.S;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; ++w)
+    if (w < wave) x = max(x, tmp[w]);
+  return x;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void gqa_spans_kernel(SpanParams p) {
+  __shared__ int s_id[kSpanChunk + 2], s_scan[kPlanThreads], tmp[kPlanThreads / 64], s_found;
+  const int t = threadIdx.x;
+  const int* ids = p.ids + blockIdx.y * p.stride;
+  const int c0 = blockIdx.x * kSpanChunk, c1 = min(c0 + kSpanChunk, p.S);
+  int* lo = p.lo + (int64_t)blockIdx.y * p.S;
+  int* hi = p.hi + (int64_t)blockIdx.y * p.S;
+  // s_id[i]: the id of token c0 - 1 + i.
+  for (int i = t; i < c1 - c0 + 2; i += kPlanThreads) {
+    const int at = c0 - 1 + i;
+    s_id[i] = at >= 0 && at < p.S ? ids[at] : 0;
+  }
+  // The first change at or behind c1 (S: none), the last one at or before c0.
+  int behind = p.S, before = 0;
+  for (int a = c1; a < p.S; a += kPlanThreads) {
+    const int at = a + t;
+    if (t == 0) s_found = p.S;
     __syncthreads();
-    s_last[t] = max(s_last[t], x);
-    s_first[t] = min(s_first[t], y);
+    if (at < p.S && ids[at] != ids[at - 1]) atomicMin(&s_found, at);
     __syncthreads();
+    behind = s_found;
+    __syncthreads();
+    if (behind < p.S) break;
   }
-  int start = t > 0 ? s_last[t - 1] : -1;
-  for (int i = a; i < e; ++i) {
-    if (i == 0 || ids[i] != ids[i - 1]) start = i;
-    lo[i] = ids[i] < 0 ? 0 : start;
+  for (int a = c0; a > 0; a -= kPlanThreads) {
+    const int at = a - t;
+    if (t == 0) s_found = 0;
+    __syncthreads();
+    if (at > 0 && ids[at] != ids[at - 1]) atomicMax(&s_found, at);
+    __syncthreads();
+    before = s_found;
+    __syncthreads();
+    if (before > 0) break;
   }
-  int end = t + 1 < kPlanThreads ? s_first[t + 1] : p.S;
-  for (int i = e - 1; i >= a; --i) {
-    hi[i] = ids[i] < 0 ? 0 : end;
-    if (i == 0 || ids[i] != ids[i - 1]) end = i;
+  __syncthreads();  // s_id
+  // This thread's tokens a .. a + 3, and the changes among them.
+  const int a = t * kSpanPer;
+  int id[kSpanPer];
+  bool change[kSpanPer];
+  int last = -1, first = 0x7fffffff;
+#pragma unroll
+  for (int i = 0; i < kSpanPer; ++i) {
+    id[i] = a + i < c1 - c0 ? s_id[a + i + 1] : 0;
+    change[i] = a + i < c1 - c0 && (c0 + a + i == 0 || s_id[a + i] != id[i]);
+    if (change[i]) {
+      last = c0 + a + i;
+      first = min(first, c0 + a + i);
+    }
   }
+  // Running maximum of the last changes from the left, and (thread order turned
+  // round) of the negated first ones from the right.
+  s_scan[t] = block_max_scan(last, tmp);
+  __syncthreads();
+  int start = max(t > 0 ? s_scan[t - 1] : -1, before);
+  __syncthreads();
+  s_scan[kPlanThreads - 1 - t] = -first;
+  __syncthreads();
+  const int turned = block_max_scan(s_scan[t], tmp);
+  __syncthreads();
+  s_scan[t] = turned;
+  __syncthreads();
+  int end = t + 1 < kPlanThreads ? min(-s_scan[kPlanThreads - 2 - t], behind) : behind;
+  int st[kSpanPer], en[kSpanPer];
+#pragma unroll
+  for (int i = 0; i < kSpanPer; ++i) {
+    if (change[i]) start = c0 + a + i;
+    st[i] = id[i] < 0 ? 0 : start;
+  }
+#pragma unroll
+  for (int i = kSpanPer - 1; i >= 0; --i) {
+    en[i] = id[i] < 0 ? 0 : end;
+    if (change[i]) end = c0 + a + i;
+  }
+#pragma unroll
+  for (int i = 0; i < kSpanPer; ++i)
+    if (a + i < c1 - c0) {
+      lo[c0 + a + i] = st[i];
+      hi[c0 + a + i] = en[i];
+    }
 }
 
 hipError_t launch_spans(const SpanParams& p, hipStream_t stream) {
   if (p.B <= 0 || p.S <= 0) return hipSuccess;
-  hipLaunchKernelGGL(gqa_spans_kernel, dim3(p.B), dim3(kPlanThreads), 0, stream, p);
+  // (Rows in the grid's second dimension, at most 65535 a launch.)
+  for (int b = 0; b < p.B; b += 65535) {
+    SpanParams q = p;
+    q.ids += b * p.stride;
+    q.lo += (int64_t)b * p.S;
+    q.hi += (int64_t)b * p.S;
+    hipLaunchKernelGGL(gqa_spans_kernel, dim3((p.S + kSpanChunk - 1) / kSpanChunk, std::min(p.B - b, 65535)),
+                       dim3(kPlanThreads), 0, stream, q);
+  }
   return hipGetLastError();
 }
 
@@ -207,10 +283,159 @@ __global__ __launch_bounds__(256) void gqa_tables_expand_kernel(TablesParams p) 
   p.batch_tables[e] = x;
 }
 
+// The step in one launch, for batches whose plan fits LDS: every workgroup makes
+// the plan for itself (two dependent reads and two sums over the batch) and then
+// its share of the tokens and of the tables' rows; nothing that another
+// workgroup's plan reads is written (the pool's lengths and the free count move
+// on in a launch behind, gqa_tables_update_kernel).
+constexpr int kStepMaxBatch = 2048, kStepMaxRows = 4096, kStepMaxTokens = 1 << 18;  // (48 KiB of LDS)
+
+__device__ inline int block_sum_scan(int x, int* tmp, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+  __syncthreads();  // tmp's readers of the call before
+  if (lane == 63) tmp[wave] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    const int y = tmp[w];
+    if (w < wave) before += y;
+    total += y;
+  }
+  return before + x;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void gqa_tables_step_kernel(TablesParams p) {
+  extern __shared__ int lds[];
+  __shared__ int tmp[kPlanThreads / 64], s_refused, s_taken;
+  int* s_start = lds;           // (B) first token
+  int* s_old = s_start + p.B;   // (B) keys before
+  int* s_new = s_old + p.B;     // (B) new tokens, 0 if refused
+  int* s_base = s_new + p.B;    // (B) free blocks taken before
+  int* owner = s_base + p.B;    // (n_rows), with rows
+  const int t = threadIdx.x;
+  const int have_free = min(max(load_uniform(p.free_count), 0), p.n_free);
+  const int mask = (1 << p.block_shift) - 1;
+  if (t == 0) s_refused = s_taken = 0;
+  if (p.rows != nullptr) {
+    for (int r = t; r < p.n_rows; r += kPlanThreads) owner[r] = 0x7fffffff;
+    __syncthreads();
+    for (int b = t; b < p.B; b += kPlanThreads) {
+      const int r = p.rows[b];
+      if (r >= 0 && r < p.n_rows) atomicMin(&owner[r], b);
+    }
+  }
+  __syncthreads();
+  int tokens = 0, blocks = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
+    const int b = b0 + t;
+    int r = -1, fresh = 0, old = 0;
+    bool fits = false;
+    if (b < p.B) {
+      r = p.rows != nullptr ? p.rows[b] : b;
+      fresh = min(max(p.new_lens[b], 0), p.n_tokens + 1);  // (more than there is room for is as good as one more)
+      fits = r >= 0 && r < p.n_rows && (p.rows == nullptr || owner[r] == b);
+      old = fits ? min(max(p.lens[r], 0), p.width << p.block_shift) : 0;
+    }
+    int total;
+    const int upto = block_sum_scan(fresh, tmp, total) + tokens;
+    tokens = min(tokens + total, 1 << 30);
+    const int64_t len = (int64_t)old + fresh;
+    fits = fits && len <= ((int64_t)p.width << p.block_shift) && upto <= p.n_tokens;
+    const int pages = (old + mask) >> p.block_shift;
+    const int need = fits ? (int)((len + mask) >> p.block_shift) - pages : 0;
+    const int bl = block_sum_scan(need, tmp, total) + blocks;
+    blocks += total;
+    const bool ok = fits && (need == 0 || bl <= have_free);
+    if (b < p.B) {
+      s_start[b] = upto - fresh;
+      s_old[b] = old;
+      s_new[b] = ok ? fresh : 0;
+      s_base[b] = bl - need;
+      if (ok && need > 0) atomicMax(&s_taken, bl);  // (served requests' sums come before any refused one's)
+      if (!ok && r >= 0) atomicAdd(&s_refused, 1);
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int b = t; b < p.B; b += kPlanThreads) {
+      p.seq_lens[b] = s_old[b] + s_new[b];
+      p.query_start[b] = s_start[b];
+      p.query_lens[b] = s_new[b];
+    }
+    if (t == 0) {
+      *p.new_free = have_free - s_taken;
+      *p.refused = s_refused;
+    }
+  }
+  // The block of page `page` of request b: the pool's, or a new one.
+  const auto block_of = [&](int b, int r, int page) {
+    const int pages = (s_old[b] + mask) >> p.block_shift;
+    return page >= pages ? p.free_blocks[have_free - 1 - s_base[b] - (page - pages)] : p.tables[r * p.stride + page];
+  };
+  // Tokens, one a thread; the request by bisection.
+  for (int i = blockIdx.x * kPlanThreads + t; i < p.n_tokens; i += gridDim.x * kPlanThreads) {
+    int b = 0;  // the last request that starts at or before token i
+    for (int n = p.B; n > 1;) {
+      const int half = n >> 1;
+      if (s_start[b + half] <= i) b += half;
+      n -= half;
+    }
+    int64_t slot = -1;
+    int pos = 0;
+    const int at = p.B > 0 ? i - s_start[b] : 0;
+    if (p.B > 0 && at < s_new[b]) {
+      pos = s_old[b] + at;
+      slot = ((int64_t)block_of(b, p.rows != nullptr ? p.rows[b] : b, pos >> p.block_shift) << p.block_shift) + (pos & mask);
+    }
+    p.slots[i] = slot;
+    p.positions[i] = pos;
+  }
+  // Table rows, one a wave.
+  const int lane = t & 63;
+  for (int b = blockIdx.x * (kPlanThreads / 64) + (t >> 6); b < p.B; b += gridDim.x * (kPlanThreads / 64)) {
+    const int r = p.rows != nullptr ? p.rows[b] : b;
+    const int n = (s_old[b] + s_new[b] + mask) >> p.block_shift, pages = (s_old[b] + mask) >> p.block_shift;
+    int* out = p.batch_tables + (int64_t)b * p.width;
+#pragma unroll 4
+    for (int page = lane; page < p.width; page += 64) {
+      int x = 0;
+      if (page < n) {
+        x = block_of(b, r, page);
+        if (page >= pages) p.tables[r * p.stride + page] = x;
+      }
+      out[page] = x;
+    }
+  }
+}
+
+// The pool moves on: lengths of the served requests, the free count.
+__global__ __launch_bounds__(256) void gqa_tables_update_kernel(TablesParams p) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b < p.B && p.query_lens[b] > 0) p.lens[p.rows != nullptr ? p.rows[b] : b] = p.seq_lens[b];
+  if (b == 0) *p.free_count = *p.new_free;
+}
+
 hipError_t launch_tables(const TablesParams& p, hipStream_t stream) {
-  if (p.B <= 0 && p.n_tokens <= 0) return hipSuccess;
+  const int64_t entries = (int64_t)p.B * p.width;
+  if (p.B <= kStepMaxBatch && p.n_rows <= kStepMaxRows && p.n_tokens < kStepMaxTokens && entries < (int64_t)1 << 30) {
+    // A table row a wave, a few thousand tokens a workgroup.
+    const int wgs = std::min(std::max({(p.B + 15) / 16, (p.n_tokens + 2047) / 2048, 1}), 256);
+    const size_t lds = sizeof(int) * (4 * (size_t)p.B + (p.rows != nullptr ? p.n_rows : 0));
+    hipLaunchKernelGGL(gqa_tables_step_kernel, dim3(wgs), dim3(kPlanThreads), lds, stream, p);
+    if (p.update)
+      hipLaunchKernelGGL(gqa_tables_update_kernel, dim3((p.B + 255) / 256 + (p.B == 0)), dim3(256), 0, stream, p);
+    return hipGetLastError();
+  }
   hipLaunchKernelGGL(gqa_tables_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
-  const int64_t items = p.n_tokens + (int64_t)p.B * p.width;
+  const int64_t items = p.n_tokens + entries;
   if (items > 0)
     hipLaunchKernelGGL(gqa_tables_expand_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, p);
   return hipGetLastError();

@@ -316,10 +316,66 @@ void check_rc(int rc, const char* what) {
   if (rc != GQA_OK) raise_rc(rc, what);
 }
 
+// A contiguous 1-d tensor of n values (or 2-d, rows x n), or false; None gives
+// nullptr.
+bool optional_values(const py::handle& h, at::ScalarType type, int64_t rows, int64_t n, int64_t dev, const void*& out) {
+  out = nullptr;
+  if (h.is_none()) return true;
+  const at::Tensor* t = plain(h);
+  if (t == nullptr || t->scalar_type() != type || !t->is_contiguous() || t->get_device() != dev || t->requires_grad())
+    return false;
+  if (rows < 0 ? t->dim() != 1 || t->size(0) != n : t->dim() != 2 || t->size(0) != rows || t->size(1) != n) return false;
+  out = t->data_ptr();
+  return true;
+}
+
+// What changes a call's scores (gqa_score); `any`: whether something does.
+struct Changes {
+  gqa_score score{};
+  bool any = false, spans = false;
+};
+bool read_changes(double softcap, const py::handle& slopes, const py::handle& prefix, const py::handle& starts,
+                  const py::handle& ends, int64_t B, int64_t Hq, int64_t Sq, int64_t Skv, bool causal, int64_t dev,
+                  Changes& c) {
+  c.any = softcap != 0.0 || !slopes.is_none() || !prefix.is_none() || !starts.is_none();
+  if (!c.any) return true;
+  const void *sl, *pr, *lo, *hi;
+  if (!optional_values(slopes, at::kFloat, -1, Hq, dev, sl) || !optional_values(prefix, at::kInt, -1, B, dev, pr) ||
+      !optional_values(starts, at::kInt, B, Skv, dev, lo) || !optional_values(ends, at::kInt, B, Skv, dev, hi) ||
+      (pr != nullptr && !causal) || (lo == nullptr) != (hi == nullptr) || (lo != nullptr && Sq > Skv))
+    return false;
+  c.spans = lo != nullptr;
+  c.score.softcap = static_cast<float>(softcap);
+  c.score.alibi_slopes = static_cast<const float*>(sl);
+  c.score.prefix_lens = static_cast<const int*>(pr);
+  c.score.span_lo = static_cast<const int*>(lo);
+  c.score.span_hi = static_cast<const int*>(hi);
+  return true;
+}
+bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t != nullptr && t->requires_grad()) return true;
+  return false;
+}
+
+// The workspace of a call with changed scores: the stream's, or (none large
+// enough, or a capture) one of its own.
+float* call_workspace(const py::dict& buffers, int64_t dev, hipStream_t stream, size_t bytes, const at::Tensor& like,
+                      at::Tensor& own) {
+  if (bytes == 0) return nullptr;
+  void* ws = capturing() ? nullptr : stream_buffer(buffers, dev, stream, bytes);
+  if (ws != nullptr) return static_cast<float*>(ws);
+  own = at::empty({static_cast<int64_t>((bytes + 3) / 4)}, like.options().dtype(at::kFloat));
+  return own.data_ptr<float>();
+}
+
 // gqa_flash_attn(q, k, v, causal, return_lse), or None.  workspaces, counters:
-// gqa_split's per-stream buffers.
+// gqa_split's per-stream buffers.  softcap (0: none) to ends (None: none):
+// changed scores.
 py::object flash_attn(const py::handle& hq, const py::handle& hk, const py::handle& hv, bool causal, bool return_lse,
-                      const py::dict& workspaces, const py::dict& counters) {
+                      const py::dict& workspaces, const py::dict& counters, double softcap, const py::handle& slopes,
+                      const py::handle& prefix, const py::handle& starts, const py::handle& ends) {
   const at::Tensor *pq = plain(hq), *pk = plain(hk), *pv = plain(hv);
   if (pq == nullptr || pk == nullptr || pv == nullptr || modes_active()) return py::none();
   const at::Tensor &q = *pq, &k = *pk, &v = *pv;
@@ -331,7 +387,11 @@ py::object flash_attn(const py::handle& hq, const py::handle& hk, const py::hand
   if (k.size(0) != B || k.size(3) != D || k.get_device() != dev || v.get_device() != dev ||
       c10::hip::current_device() != dev)
     return py::none();
-  const auto found = g_plans.find(Key{0, B, Hq, Hkv, Sq, Skv, D, causal, dev});
+  Changes ch;
+  if (!read_changes(softcap, slopes, prefix, starts, ends, B, Hq, Sq, Skv, causal, dev, ch) ||
+      (ch.any && wants_grad({pq, pk, pv})))
+    return py::none();
+  const auto found = g_plans.find(Key{ch.any ? 2 : 0, B, Hq, Hkv, Sq, Skv, D, causal, dev, ch.spans});
   if (found == g_plans.end() || !rows_ready(q) || !rows_ready(k) || !rows_ready(v)) return py::none();
   const Plan p = found->second;
   if (p.kind != kSingle && (Skv + 192) * std::max(k.stride(2), v.stride(2)) >= ((int64_t)1 << 30)) return py::none();
@@ -345,9 +405,13 @@ py::object flash_attn(const py::handle& hq, const py::handle& hk, const py::hand
     need = gqa_split_flat_workspace_bytes(B, Hq, Sq, D, p.n);
   else if (p.kind == kSingle)
     need = gqa_fwd_split_workspace_bytes(B, Hkv, D, p.n);
+  at::Tensor own;
   // (A captured call gets partials and counters of its own, in Python.)
-  if (need > 0 && (capturing() || (ws = stream_buffer(workspaces, dev, stream, need)) == nullptr)) return py::none();
-  if (p.kind == kSingle || p.kind == kChunks) {
+  if (ch.any)
+    ws = call_workspace(workspaces, dev, stream, need, q, own);
+  else if (need > 0 && (capturing() || (ws = stream_buffer(workspaces, dev, stream, need)) == nullptr))
+    return py::none();
+  if (ch.any ? p.kind == kSingle && p.n > 0 : p.kind == kSingle || p.kind == kChunks) {
     const size_t n = gqa_fwd_split_counters_count(B, Hkv, p.kind == kSingle ? p.n : 0);
     if (capturing() || (cnt = stream_buffer(counters, dev, stream, n * sizeof(int))) == nullptr) return py::none();
   }
@@ -369,7 +433,12 @@ py::object flash_attn(const py::handle& hq, const py::handle& hk, const py::hand
   void* op = o.data_ptr();
   int rc;
   const char* what;
-  if (p.kind == kSplit) {
+  if (ch.any) {
+    what = "gqa_scored_launch";
+    rc = gqa_scored_launch(p.kind, qp, qs, kp, ks, vp, vs, op, os, lse_p, wsf, cnti, p.n, b, hq_, hkv, sq, skv, d, sl2,
+                           c, dt, &ch.score, stream);
+    if (rc == GQA_E_FLAT || rc == GQA_E_SCORE) return py::none();
+  } else if (p.kind == kSplit) {
     what = "gqa_split_launch";
     rc = gqa_split_launch(qp, qs, kp, ks, vp, vs, op, os, lse_p, wsf, p.n, b, hq_, hkv, sq, skv, d, sl2, c, dt, stream);
   } else if (p.kind == kFlat) {
@@ -415,7 +484,8 @@ bool int_rows(const at::Tensor* t, int64_t n, int64_t dev) {
 py::object paged_attn(const py::handle& hq, const py::handle& hkc, const py::handle& hvc, const py::handle& htab,
                       const py::handle& hlens, bool causal, int64_t max_seq_len, double scale_log2, bool return_lse,
                       const py::handle& hout, const py::handle& hqs, const py::handle& hql, int64_t max_query_len,
-                      const py::dict& workspaces, const py::dict& counters) {
+                      const py::dict& workspaces, const py::dict& counters, double softcap, const py::handle& slopes,
+                      const py::handle& prefix) {
   const at::Tensor *pq = plain(hq), *pkc = plain(hkc), *pvc = plain(hvc), *ptab = plain(htab), *plens = plain(hlens);
   if (pq == nullptr || pkc == nullptr || pvc == nullptr || ptab == nullptr || plens == nullptr || modes_active())
     return py::none();
@@ -440,7 +510,11 @@ py::object paged_attn(const py::handle& hq, const py::handle& hkc, const py::han
   if (max_seq_len < 0) max_seq_len = capacity;
   if (max_seq_len > capacity) return py::none();
   const bool interleaved = kc.stride(1) != D || vc.stride(1) != D;
-  const auto found = g_plans.find(Key{1, B, H, Hkv, Sq, max_seq_len, D, causal, dev, bs, interleaved, varlen});
+  Changes ch;
+  if (!read_changes(softcap, slopes, prefix, py::none(), py::none(), B, H, Sq, max_seq_len, causal, dev, ch) ||
+      (ch.any && wants_grad({pq, pkc, pvc})))
+    return py::none();
+  const auto found = g_plans.find(Key{ch.any ? 3 : 1, B, H, Hkv, Sq, max_seq_len, D, causal, dev, bs, interleaved, varlen});
   if (found == g_plans.end()) return py::none();
   const Plan p = found->second;
   if (p.kind == kShort && std::max(kc.stride(1), vc.stride(1)) >= ((int64_t)1 << 24)) return py::none();
@@ -454,7 +528,11 @@ py::object paged_attn(const py::handle& hq, const py::handle& hkc, const py::han
   else if (p.kind == kSingle)
     need = gqa_fwd_split_workspace_bytes(B, Hkv, D, p.n);
   // (A captured call gets partials and counters of its own, in Python.)
-  if (need > 0 && (capturing() || (ws = stream_buffer(workspaces, dev, stream, need)) == nullptr)) return py::none();
+  at::Tensor own;
+  if (ch.any)
+    ws = call_workspace(workspaces, dev, stream, need, q, own);
+  else if (need > 0 && (capturing() || (ws = stream_buffer(workspaces, dev, stream, need)) == nullptr))
+    return py::none();
   if (p.kind == kSingle && p.n > 0) {
     const size_t n = gqa_fwd_split_counters_count(B, Hkv, p.n);
     if (capturing() || (cnt = stream_buffer(counters, dev, stream, n * sizeof(int))) == nullptr) return py::none();
@@ -494,7 +572,13 @@ py::object paged_attn(const py::handle& hq, const py::handle& hkc, const py::han
   float* wsf = static_cast<float*>(ws);
   const void *qp = q.data_ptr(), *kp = kc.data_ptr(), *vp = vc.data_ptr();
   void* op = out.data_ptr();
-  if (p.kind == kFlat) {
+  if (ch.any) {
+    const int rc = gqa_paged_scored_launch(p.kind, qp, qs, kp, ks, vp, vs, tp, ts, lp, qsp, qlp, bsz, ms, op, os, lse_p,
+                                           wsf, static_cast<int*>(cnt), p.n, b, h, hkv, sq, d, sl2, c, dt, &ch.score,
+                                           stream);
+    if (rc == GQA_E_FLAT || rc == GQA_E_SCORE) return py::none();
+    check_rc(rc, "gqa_paged_scored_launch");
+  } else if (p.kind == kFlat) {
     const int rc = gqa_paged_split_flat_launch(qp, qs, kp, ks, vp, vs, tp, ts, lp, qsp, qlp, bsz, ms, op, os, lse_p,
                                                wsf, p.n, b, h, hkv, sq, d, sl2, c, dt, stream);
     if (rc == GQA_E_FLAT) return py::none();
@@ -543,6 +627,190 @@ bool write_kv(const py::handle& hk, const py::handle& hv, const py::handle& hkc,
     return false;
   cache_write(*k, *v, *kc, *vc, *sl, dtype_code(*k));
   return true;
+}
+
+// ---------------------------------------------------------------------------
+// Around the attention: norms and rotation, document spans, block tables.  As
+// above: None (nothing launched) unless every check passes.
+// ---------------------------------------------------------------------------
+
+// A contiguous view of n values at `offset` of buffer `t`.
+at::Tensor part_of(const at::Tensor& t, int64_t offset, at::IntArrayRef sizes) {
+  auto impl = c10::make_intrusive<at::TensorImpl>(c10::Storage(t.storage()), t.key_set(), t.dtype());
+  impl->set_storage_offset(offset);
+  impl->set_sizes_contiguous(sizes);
+  return at::Tensor(std::move(impl));
+}
+
+// qk_norm_rope, or (k_cache given) qk_norm_rope_write: (q_out, k_out) or q_out.
+// table: RotaryTable's (tensor, address of its gqa_rope, axes), or None.
+py::object norm_rope(const py::handle& hq, const py::handle& hk, const py::handle& hv, const py::handle& hpos,
+                     const py::handle& table, const py::handle& hkc, const py::handle& hvc, const py::handle& hslots,
+                     const py::handle& hwq, const py::handle& hwk, double eps, const py::handle& hqo,
+                     const py::handle& hko) {
+  const bool write = !hkc.is_none();
+  const at::Tensor *q = plain(hq), *k = hk.is_none() ? nullptr : plain(hk);
+  if (q == nullptr || modes_active() || (!hk.is_none() && k == nullptr) || !half_type(*q)) return py::none();
+  const int64_t nd = q->dim(), dev = q->get_device();
+  if ((nd != 3 && nd != 4) || (write && nd != 3) || c10::hip::current_device() != dev || !rows_ready(*q))
+    return py::none();
+  const int64_t D = q->size(-1), B = nd == 4 ? q->size(0) : 1, S = nd == 4 ? q->size(2) : q->size(0), Hq = q->size(1);
+  if ((D != 64 && D != 128) || !(eps >= 0.0)) return py::none();
+  if (B * S == 0 || (k == nullptr && (write || !hwk.is_none() || !hko.is_none()))) return py::none();
+  if (k != nullptr &&
+      (k->dim() != nd || k->scalar_type() != q->scalar_type() || k->get_device() != dev || k->size(-1) != D ||
+       (nd == 4 ? k->size(0) != B || k->size(2) != S : k->size(0) != S) || !rows_ready(*k)))
+    return py::none();
+  gqa_rope r{};
+  if (table.is_none()) {
+    if (hwq.is_none() && hwk.is_none()) return py::none();
+  } else {
+    const py::tuple tt = py::reinterpret_borrow<py::tuple>(table);
+    const at::Tensor& data = THPVariable_Unpack(tt[0].ptr());
+    r = *reinterpret_cast<const gqa_rope*>(tt[1].cast<intptr_t>());
+    const int64_t axes = tt[2].cast<int64_t>();  // (0: positions without an axis dimension)
+    const at::Tensor* pos = plain(hpos);
+    if (data.get_device() != dev || tt[3].cast<int64_t>() != D || pos == nullptr || pos->get_device() != dev ||
+        !pos->is_contiguous() || (pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong))
+      return py::none();
+    const int64_t lead = axes > 0 ? 1 : 0, per = nd == 4 ? 2 : 1;
+    if (pos->dim() != lead + per || (lead && pos->size(0) != axes) || pos->size(lead) != (nd == 4 ? B : S) ||
+        (nd == 4 && pos->size(lead + 1) != S))
+      return py::none();
+    r.positions = pos->data_ptr();
+    r.positions64 = pos->scalar_type() == at::kLong;
+  }
+  const at::Tensor *wq = nullptr, *wk = nullptr;
+  for (int i = 0; i < 2; ++i) {
+    const py::handle& h = i == 0 ? hwq : hwk;
+    if (h.is_none()) continue;
+    const at::Tensor* w = plain(h);
+    if (w == nullptr || w->dim() != 1 || w->size(0) != D || w->get_device() != dev || !w->is_contiguous() ||
+        (w->scalar_type() != q->scalar_type() && w->scalar_type() != at::kFloat) ||
+        (reinterpret_cast<uintptr_t>(w->data_ptr()) & 15) != 0)
+      return py::none();
+    (i == 0 ? wq : wk) = w;
+  }
+  if (wq != nullptr && wk != nullptr && wq->scalar_type() != wk->scalar_type()) return py::none();
+  r.q_weight = wq == nullptr ? nullptr : wq->data_ptr();
+  r.k_weight = wk == nullptr ? nullptr : wk->data_ptr();
+  r.weights32 = wq != nullptr ? wq->scalar_type() == at::kFloat : wk != nullptr && wk->scalar_type() == at::kFloat;
+  r.eps = static_cast<float>(eps);
+  const at::Tensor *v = nullptr, *kc = nullptr, *vc = nullptr, *sl = nullptr;
+  if (write) {
+    v = plain(hv), kc = plain(hkc), vc = plain(hvc), sl = plain(hslots);
+    if (v == nullptr || kc == nullptr || vc == nullptr || sl == nullptr || v->sizes() != k->sizes() ||
+        v->scalar_type() != k->scalar_type() || v->get_device() != dev || !rows_ready(*v) || !caches_ready(*kc, *vc) ||
+        kc->get_device() != dev || kc->scalar_type() != k->scalar_type() || kc->size(2) != k->size(1) ||
+        kc->size(3) != D || sl->scalar_type() != at::kLong || sl->dim() != 1 || sl->size(0) != S ||
+        sl->get_device() != dev || !sl->is_contiguous())
+      return py::none();
+  }
+  if (wants_grad({q, k, v, wq, wk})) return py::none();
+  at::Tensor outs[2];
+  const at::Tensor* ins[2] = {q, k};
+  const py::handle* given[2] = {&hqo, &hko};
+  for (int i = 0; i < (write || k == nullptr ? 1 : 2); ++i) {
+    if (given[i]->is_none()) {
+      outs[i] = at::empty_like(*ins[i]);
+    } else {
+      const at::Tensor* o = plain(*given[i]);
+      if (o == nullptr || o->sizes() != ins[i]->sizes() || o->scalar_type() != ins[i]->scalar_type() ||
+          o->get_device() != dev)
+        return py::none();
+      outs[i] = *o;
+    }
+    if (!rows_ready(outs[i])) return py::none();
+  }
+  hipStream_t stream = c10::hip::getCurrentHIPStream(dev).stream();
+  int rc;
+  {
+    py::gil_scoped_release others;  // (one launch, as above)
+    if (write) {
+      int64_t kcs[4], vcs[4];
+      strides_of(*kc, kcs);
+      strides_of(*vc, vcs);
+      rc = gqa_qk_norm_rope_write_launch(q->data_ptr(), q->strides().data(), k->data_ptr(), k->strides().data(),
+                                         v->data_ptr(), v->strides().data(), outs[0].data_ptr(),
+                                         outs[0].strides().data(), kc->data_ptr(), kcs, vc->data_ptr(), vcs,
+                                         sl->data_ptr<int64_t>(), &r, static_cast<int>(S), static_cast<int>(Hq),
+                                         static_cast<int>(k->size(1)), static_cast<int>(D),
+                                         static_cast<int>(kc->size(1)), dtype_code(*q), stream);
+    } else {
+      int64_t st[4][4] = {};
+      const at::Tensor* four[4] = {q, k, &outs[0], &outs[1]};
+      for (int i = 0; i < 4; ++i) {
+        if (four[i] == nullptr || !four[i]->defined()) continue;
+        if (nd == 4) {
+          strides_of(*four[i], st[i]);
+        } else {
+          st[i][1] = four[i]->stride(1), st[i][2] = four[i]->stride(0), st[i][3] = 1;
+        }
+      }
+      rc = gqa_qk_norm_rope_launch(q->data_ptr(), st[0], k == nullptr ? nullptr : k->data_ptr(), st[1],
+                                   outs[0].data_ptr(), st[2], k == nullptr ? nullptr : outs[1].data_ptr(), st[3], &r,
+                                   static_cast<int>(B), static_cast<int>(Hq),
+                                   k == nullptr ? 1 : static_cast<int>(k->size(1)), static_cast<int>(S),
+                                   static_cast<int>(D), dtype_code(*q), stream);
+    }
+  }
+  check_rc(rc, write ? "gqa_qk_norm_rope_write_launch" : "gqa_qk_norm_rope_launch");
+  if (write) return py::cast(outs[0]);
+  return py::make_tuple(outs[0], k == nullptr ? py::none() : py::cast(outs[1]));
+}
+
+// document_spans: (starts, ends).
+py::object document_spans(const py::handle& hids) {
+  const at::Tensor* ids = plain(hids);
+  if (ids == nullptr || modes_active() || ids->scalar_type() != at::kInt || ids->dim() != 2 || ids->stride(1) != 1 ||
+      ids->stride(0) < ids->size(1) || ids->numel() == 0 || c10::hip::current_device() != ids->get_device())
+    return py::none();
+  const int64_t B = ids->size(0), S = ids->size(1);
+  at::Tensor both = at::empty({2, B, S}, ids->options());
+  at::Tensor lo = part_of(both, 0, {B, S}), hi = part_of(both, B * S, {B, S});
+  hipStream_t stream = c10::hip::getCurrentHIPStream(ids->get_device()).stream();
+  check_rc(gqa_document_spans_launch(ids->data_ptr<int>(), ids->stride(0), lo.data_ptr<int>(), hi.data_ptr<int>(),
+                                     static_cast<int>(B), static_cast<int>(S), stream), "gqa_document_spans_launch");
+  return py::make_tuple(lo, hi);
+}
+
+// extend_block_tables: the eight tensors of StepTables in order.
+py::object extend_tables(const py::handle& htab, const py::handle& hlens, const py::handle& hnew,
+                         const py::handle& hfree, const py::handle& hcount, int64_t block_size, int64_t num_tokens,
+                         const py::handle& hrows, bool update) {
+  const at::Tensor *tab = plain(htab), *lens = plain(hlens), *fresh = plain(hnew), *freeb = plain(hfree),
+                   *count = plain(hcount), *rows = hrows.is_none() ? nullptr : plain(hrows);
+  if (tab == nullptr || modes_active() || (rows == nullptr && !hrows.is_none())) return py::none();
+  const int64_t dev = tab->get_device();
+  if (tab->scalar_type() != at::kInt || tab->dim() != 2 || tab->size(1) < 1 || tab->stride(1) != 1 ||
+      c10::hip::current_device() != dev || num_tokens < 0 || num_tokens >= ((int64_t)1 << 31) || fresh == nullptr ||
+      fresh->dim() != 1)
+    return py::none();
+  const int64_t R = tab->size(0), W = tab->size(1), B = fresh->size(0);
+  if ((R > 1 && tab->stride(0) < W) || !int_rows(lens, R, dev) || !int_rows(fresh, B, dev) || freeb == nullptr ||
+      freeb->dim() != 1 || !int_rows(freeb, freeb->size(0), dev) || !int_rows(count, 1, dev) ||
+      (rows != nullptr ? !int_rows(rows, B, dev) : B > R) || block_size < 1 || block_size > GQA_MAX_BLOCK_SIZE ||
+      (block_size & (block_size - 1)) != 0 || W * block_size >= ((int64_t)1 << 31) || B == 0)
+    return py::none();
+  const int64_t scratch = R + 2 * B + 1;
+  at::Tensor small = at::empty({3 * B + num_tokens + 2 + scratch}, tab->options());
+  at::Tensor slots = at::empty({num_tokens}, tab->options().dtype(at::kLong));
+  at::Tensor tables = at::empty({B, W}, tab->options());
+  at::Tensor seq = part_of(small, 0, {B}), start = part_of(small, B, {B}), qlen = part_of(small, 2 * B, {B});
+  at::Tensor pos = part_of(small, 3 * B, {num_tokens}), left = part_of(small, 3 * B + num_tokens, {1});
+  at::Tensor refused = part_of(small, 3 * B + num_tokens + 1, {1});
+  int* scr = small.data_ptr<int>() + 3 * B + num_tokens + 2;
+  hipStream_t stream = c10::hip::getCurrentHIPStream(dev).stream();
+  check_rc(gqa_extend_tables_launch(tab->data_ptr<int>(), std::max(tab->stride(0), W), static_cast<int>(W),
+                                    lens->data_ptr<int>(), static_cast<int>(R),
+                                    rows == nullptr ? nullptr : rows->data_ptr<int>(), fresh->data_ptr<int>(),
+                                    freeb->data_ptr<int>(), count->data_ptr<int>(), static_cast<int>(freeb->size(0)),
+                                    static_cast<int>(block_size), update ? 1 : 0, static_cast<int>(B),
+                                    static_cast<int>(num_tokens), seq.data_ptr<int>(), start.data_ptr<int>(),
+                                    qlen.data_ptr<int>(), slots.data_ptr<int64_t>(), pos.data_ptr<int>(),
+                                    tables.data_ptr<int>(), left.data_ptr<int>(), refused.data_ptr<int>(), scr, stream),
+           "gqa_extend_tables_launch");
+  return py::make_tuple(seq, start, qlen, slots, pos, tables, left, refused);
 }
 
 // gqa_kernels.dispatch._list_makespan, step for step (its docstring describes
@@ -649,9 +917,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("scale_log2"), py::arg("causal"), py::arg("dtype"));
   m.def("cache_write", &cache_write, "store new tokens' K/V at their paged cache slots", py::arg("key"),
         py::arg("value"), py::arg("k_cache"), py::arg("v_cache"), py::arg("slot_mapping"), py::arg("dtype"));
-  m.def("flash_attn", &flash_attn, "gqa_flash_attn of a planned shape, or None");
-  m.def("paged_attn", &paged_attn, "paged_attention of a planned shape on its default route, or None");
+  const auto none = py::none();
+  m.def("flash_attn", &flash_attn, "gqa_flash_attn of a planned shape, or None", py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("causal"), py::arg("return_lse"), py::arg("workspaces"), py::arg("counters"),
+        py::arg("softcap") = 0.0, py::arg("slopes") = none, py::arg("prefix") = none, py::arg("starts") = none,
+        py::arg("ends") = none);
+  m.def("paged_attn", &paged_attn, "paged_attention of a planned shape on its default route, or None", py::arg("q"),
+        py::arg("k_cache"), py::arg("v_cache"), py::arg("block_table"), py::arg("seq_lens"), py::arg("causal"),
+        py::arg("max_seq_len"), py::arg("scale_log2"), py::arg("return_lse"), py::arg("out"), py::arg("query_start"),
+        py::arg("query_lens"), py::arg("max_query_len"), py::arg("workspaces"), py::arg("counters"),
+        py::arg("softcap") = 0.0, py::arg("slopes") = none, py::arg("prefix") = none);
   m.def("write_kv", &write_kv, "write_kv with its checks, or False");
+  m.def("norm_rope", &norm_rope, "qk_norm_rope or qk_norm_rope_write with its checks, or None");
+  m.def("document_spans", &document_spans, "document_spans with its checks, or None");
+  m.def("extend_tables", &extend_tables, "extend_block_tables with its checks, or None");
   m.def("set_plan", &set_plan, "register the route of a shape");
   m.def("list_makespan", &list_makespan, "run time of a list of items over the CUs (the routing models)");
   m.def("ints_to_device", &ints_to_device, "host ints to an int32 device tensor, asynchronously");

@@ -19,7 +19,7 @@ import torch
 from . import _lib
 from .gqa_split import (_counter_buffer, _counters, _decode_host, _workspace_buffer, _workspaces, decode_forward,
                         flat_forward, flat_workspace_bytes, stream_handle, workspace_bytes)
-from .scores import check_score, refuse_grad, scored_launch, workspace
+from .scores import DocumentSpans, check_score, refuse_grad, scored_launch, workspace
 
 __all__ = ["gqa_flash_attn", "Route", "choose_plan", "choose_route"]
 
@@ -793,10 +793,13 @@ def gqa_flash_attn(q, k, v, causal=True, *, return_lse=False, softcap=None, alib
         return_lse=True the pair (o, lse).
     """
     changed = softcap or alibi_slopes is not None or prefix_lens is not None or documents is not None
-    host = _lib._host if not changed else None
+    host = _lib._host
     if host is not None:
         # A planned shape with every check passed, natively; else None.
-        out = host.flash_attn(q, k, v, bool(causal), bool(return_lse), _workspaces, _counters)
+        if changed:
+            out = _native_scored(host, q, k, v, causal, return_lse, softcap, alibi_slopes, prefix_lens, documents)
+        else:
+            out = host.flash_attn(q, k, v, bool(causal), bool(return_lse), _workspaces, _counters)
         if out is not None:
             return out
     batch, num_heads, seq_q, head_dim = q.shape
@@ -816,7 +819,17 @@ def gqa_flash_attn(q, k, v, causal=True, *, return_lse=False, softcap=None, alib
         score = check_score(softcap, alibi_slopes, prefix_lens, documents, batch=batch, num_heads=num_heads,
                             seq_q=seq_q, seq_kv=seq_kv, causal=bool(causal), scale=head_dim ** -0.5, device=q.device)
         with torch.cuda.device(dev):
-            return _scored(q, k, v, causal, return_lse, dev, score, documents is not None)
+            route = _scored_route(q, k, v, causal, dev, documents is not None)
+            host = _decode_host()
+            if host is not None and batch > 0 and seq_q > 0:
+                host.set_plan([2, batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, int(bool(causal)), dev,
+                               int(documents is not None), 0, 0],
+                              _KIND_IDS[route.kind], route.fwd_split if route.kind == "single" else route.splits,
+                              (head_dim ** -0.5) * LOG2E)
+                out = _native_scored(host, q, k, v, causal, return_lse, softcap, alibi_slopes, prefix_lens, documents)
+                if out is not None:
+                    return out
+            return _scored(route, q, k, v, causal, return_lse, score)
     host = _decode_host()
     route = _plan_cached(batch, num_heads, num_kv_heads, seq_q, seq_kv, _cu_count(dev), bool(causal), head_dim)
     if host is not None and batch > 0 and seq_q > 0:
@@ -868,9 +881,33 @@ def _launch(route, q_in, k, v, causal, return_lse, dev):
     return single_pass_forward(q, k, v, o, causal, route.fwd_split, return_lse)
 
 
-def _scored(q_in, k, v, causal, return_lse, dev, score, spans):
-    """gqa_flash_attn with changed scores: the same routes, through
-    gqa_scored_launch."""
+def _native_scored(host, q, k, v, causal, return_lse, softcap, alibi_slopes, prefix_lens, documents):
+    """gqa_flash_attn with changed scores natively, or None."""
+    starts = ends = None
+    if documents is not None:
+        if not isinstance(documents, DocumentSpans):
+            return None
+        starts, ends = documents.starts, documents.ends
+    return host.flash_attn(q, k, v, bool(causal), bool(return_lse), _workspaces, _counters, softcap or 0.0,
+                           alibi_slopes, prefix_lens, starts, ends)
+
+
+def _scored_route(q, k, v, causal, dev, spans) -> Route:
+    """The route of a call with changed scores: choose_plan's, or with documents
+    one of those that start at a first visible key."""
+    batch, num_heads, seq_q, head_dim = q.shape
+    shape = (batch, num_heads, k.shape[1], seq_q, k.shape[2], _cu_count(dev), bool(causal), head_dim)
+    if spans:
+        return Route("single")
+    route = _plan_cached(*shape)
+    # As _launch: 32-bit byte offsets must span the keys.
+    if route.kind != "single" and (k.shape[2] + 192) * max(k.stride(2), v.stride(2)) >= 1 << 30:
+        route = _route_cached(*shape)
+    return route
+
+
+def _scored(route, q_in, k, v, causal, return_lse, score):
+    """gqa_flash_attn with changed scores through gqa_scored_launch."""
     batch, num_heads, seq_q, head_dim = q_in.shape
     _, num_kv_heads, seq_kv, _ = k.shape
     q, k, v = _kernel_ready(q_in), _kernel_ready(k), _kernel_ready(v)
@@ -878,14 +915,6 @@ def _scored(q_in, k, v, causal, return_lse, dev, score, spans):
     if not _is_kernel_ready(o):
         o = torch.empty_like(q_in, memory_format=torch.contiguous_format)
     lse = torch.empty(batch, num_heads, seq_q, dtype=torch.float32, device=q.device) if return_lse else None
-    cu = _cu_count(dev)
-    shape = (batch, num_heads, num_kv_heads, seq_q, seq_kv, cu, bool(causal), head_dim)
-    if spans:  # (the single pass alone has a first visible key)
-        route = Route("single")
-    else:
-        route = _plan_cached(*shape)
-        if route.kind != "single" and (seq_kv + 192) * max(k.stride(2), v.stride(2)) >= 1 << 30:
-            route = _route_cached(*shape)  # as _launch
     stream = stream_handle(q.device)
 
     def launch(route):
@@ -898,15 +927,14 @@ def _scored(q_in, k, v, causal, return_lse, dev, score, spans):
             parts = route.fwd_split
             if parts:
                 ws = workspace(lib.gqa_fwd_split_workspace_bytes(batch, num_kv_heads, head_dim, parts), q.device)
-        if route.kind in ("single", "chunks"):
-            cnt = _counter_buffer(q.device, stream, lib.gqa_fwd_split_counters_count(
-                batch, num_kv_heads, parts if route.kind == "single" else 0))
+                cnt = _counter_buffer(q.device, stream,
+                                      lib.gqa_fwd_split_counters_count(batch, num_kv_heads, parts))
         return scored_launch(_KIND_IDS[route.kind], parts, q, k, v, o, lse, ws, cnt, causal,
                              (head_dim ** -0.5) * LOG2E, _DTYPES[q.dtype], score, stream)
 
     rc = launch(route)
     if rc == _lib.GQA_E_FLAT:
-        rc = launch(_route_cached(*shape))
+        rc = launch(_base_route(q, k, causal, q.get_device()))
     _lib.check(rc)
     return o if lse is None else (o, lse)
 

@@ -424,14 +424,15 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
     varlen = query_start is not None
     changed = bool(softcap) or alibi_slopes is not None or prefix_lens is not None
     default_route = route is None and splits is None and (not varlen or query_lens is not None)
-    native = _lib._host if default_route and not changed else None
+    native = _lib._host if default_route else None
     if native is not None:
         # A planned shape with every check passed, natively; else None.
         res = native.paged_attn(q, k_cache, v_cache, block_table, seq_lens, bool(causal),
                                 -1 if max_seq_len is None or max_seq_len < 0 else max_seq_len,
                                 (q.shape[-1] ** -0.5 if scale is None else scale) * LOG2E, bool(return_lse), out,
                                 query_start, query_lens, -1 if max_query_len is None else int(max_query_len),
-                                _workspaces, _counters) if max_seq_len is None or max_seq_len >= 0 else None
+                                _workspaces, _counters, softcap or 0.0, alibi_slopes,
+                                prefix_lens) if max_seq_len is None or max_seq_len >= 0 else None
         if res is not None:
             return res
     qdev = q.device
@@ -499,8 +500,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
         refuse_grad("paged_attention with changed scores", q, k_cache, v_cache, alibi_slopes)
         score = check_score(softcap, alibi_slopes, prefix_lens, None, batch=batch, num_heads=num_heads, seq_q=seq_q,
                             seq_kv=max_seq_len, causal=bool(causal), scale=scale, device=qdev)
-    if default_route and not changed and batch > 0 and seq_q > 0:
-        plan_key = [1, batch, num_heads, num_kv_heads, seq_q, max_seq_len, head_dim, int(bool(causal)), dev, block_size,
+    if default_route and batch > 0 and seq_q > 0:
+        plan_key = [3 if changed else 1, batch, num_heads, num_kv_heads, seq_q, max_seq_len, head_dim, int(bool(causal)), dev, block_size,
                     int(interleaved), int(varlen)]
     kv_chunks = fwd_split = 0
     if route is None:
@@ -531,7 +532,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
         host.set_plan(plan_key, _KIND_IDS["flat" if flat else route], flat_slots if flat else n_parts, 0.0)
         res = host.paged_attn(q, k_cache, v_cache, block_table, seq_lens, bool(causal), max_seq_len, scale * LOG2E,
                               bool(return_lse), out, query_start, query_lens if varlen else None,
-                              seq_q if varlen else -1, _workspaces, _counters)
+                              seq_q if varlen else -1, _workspaces, _counters, softcap or 0.0, alibi_slopes,
+                              prefix_lens)
         if res is not None:
             return res
     lse = torch.empty(lse_shape, dtype=torch.float32, device=qdev) if return_lse else None

@@ -19,7 +19,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from .gqa_split import stream_handle
+from .gqa_split import _decode_host, stream_handle
 from .scores import refuse_grad
 
 __all__ = ["RotaryTable", "qk_norm_rope", "qk_norm_rope_write"]
@@ -80,6 +80,12 @@ class RotaryTable:
         for i, a in enumerate(axes or ()):
             words[i >> 4] |= a << (2 * (i & 15))
         self._pair_axis = (ctypes.c_uint32 * 4)(*words)
+        # For the native calls: the table, its gqa_rope, axes (0: positions
+        # without an axis dimension), head_dim.
+        r = self._rope = _lib.Rope()
+        r.table, r.max_positions, r.rotary_dim = self.table.data_ptr(), self.max_positions, self.rotary_dim
+        r.interleaved, r.axes, r.pair_axis = int(self.interleaved), self.num_axes, self._pair_axis
+        self._native = (self.table, ctypes.addressof(r), 0 if axes is None else self.num_axes, head_dim)
 
     @staticmethod
     def sections(sizes: Sequence[int]) -> list:
@@ -174,6 +180,12 @@ def qk_norm_rope(q, k, positions, table: Optional[RotaryTable] = None, *, q_weig
     Returns:
         (q, k) normed and rotated (k None without k).
     """
+    if _lib._host is not None:
+        # Every check passed, natively; else None.
+        res = _lib._host.norm_rope(q, k, None, positions, None if table is None else table._native, None, None, None,
+                                   q_weight, k_weight, eps, q_out, k_out)
+        if res is not None:
+            return res
     refuse_grad("qk_norm_rope", q, k, q_weight, k_weight)
     assert q.dim() in (3, 4), "q must be (batch, num_heads, seq, head_dim) or (num_tokens, num_heads, head_dim)"
     _check_qk(q, k, q.dim())
@@ -200,6 +212,7 @@ def qk_norm_rope(q, k, positions, table: Optional[RotaryTable] = None, *, q_weig
 
     qi, ki = _ready(q), None if k is None else _ready(k)
     batch, seq = tokens if len(tokens) == 2 else (1, tokens[0])
+    _decode_host()  # (the native call from here on)
     with torch.cuda.device(q.device):
         _lib.check(_lib.load().gqa_qk_norm_rope_launch(
             qi.data_ptr(), four(qi), None if ki is None else ki.data_ptr(), four(ki),
@@ -219,6 +232,12 @@ def qk_norm_rope_write(q, k, v, positions, table: Optional[RotaryTable], k_cache
     every other one lies inside the caches, no slot twice)."""
     from .paged import _check_cache
 
+    if _lib._host is not None:
+        # Every check passed, natively; else None.
+        res = _lib._host.norm_rope(q, k, v, positions, None if table is None else table._native, k_cache, v_cache,
+                                   slot_mapping, q_weight, k_weight, eps, q_out, None)
+        if res is not None:
+            return res
     refuse_grad("qk_norm_rope_write", q, k, v, q_weight, k_weight)
     _check_qk(q, k, 3)
     assert v is not None and tuple(v.shape) == tuple(k.shape) and v.dtype == k.dtype and v.device == k.device
@@ -233,6 +252,7 @@ def qk_norm_rope_write(q, k, v, positions, table: Optional[RotaryTable], k_cache
     keep: list = []
     rope = _rope(q, positions, table, q_weight, k_weight, eps, (q.shape[0],), keep)
     qi, ki, vi = _ready(q), _ready(k), _ready(v)
+    _decode_host()  # (the native call from here on)
     with torch.cuda.device(q.device):
         _lib.check(_lib.load().gqa_qk_norm_rope_write_launch(
             qi.data_ptr(), _lib.strides3(qi), ki.data_ptr(), _lib.strides3(ki), vi.data_ptr(), _lib.strides3(vi),

@@ -10,13 +10,12 @@ from __future__ import annotations
 
 import ctypes
 import math
-from dataclasses import dataclass
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
-from .gqa_split import stream_handle
+from .gqa_split import _decode_host, stream_handle
 
 __all__ = ["DocumentSpans", "document_spans"]
 
@@ -28,8 +27,7 @@ def refuse_grad(name: str, *tensors) -> None:
         raise NotImplementedError(f"{name} has no backward pass: call it under torch.no_grad()")
 
 
-@dataclass(frozen=True)
-class DocumentSpans:
+class DocumentSpans(NamedTuple):
     """For each position of a batch of packed sequences, the first key of its
     document and the first key behind it: int32 (batch, seq_kv), contiguous."""
 
@@ -47,10 +45,15 @@ def document_spans(document_ids: torch.Tensor) -> DocumentSpans:
     padding, which sees nothing and is seen by nothing.
     """
     ids = document_ids
+    if _lib._host is not None:
+        both = _lib._host.document_spans(ids)  # every check passed, natively; else None
+        if both is not None:
+            return DocumentSpans(*both)
     assert ids.dim() == 2 and ids.dtype == torch.int32, "document_ids must be int32 (batch, seq_kv)"
     assert ids.is_cuda
     if ids.stride(1) != 1 or ids.stride(0) < ids.shape[1]:
         ids = ids.contiguous()
+    _decode_host()  # (the native call from here on)
     both = torch.empty(2, *ids.shape, dtype=torch.int32, device=ids.device)
     with torch.cuda.device(ids.device):
         _lib.check(_lib.load().gqa_document_spans_launch(ids.data_ptr(), ids.stride(0), both[0].data_ptr(),

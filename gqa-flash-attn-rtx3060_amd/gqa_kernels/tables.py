@@ -9,19 +9,17 @@ names a paged cache as its next step.)
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
-from .gqa_split import stream_handle
+from .gqa_split import _decode_host, stream_handle
 
 __all__ = ["StepTables", "extend_block_tables", "release_blocks", "BlockPool"]
 
 
-@dataclass(frozen=True)
-class StepTables:
+class StepTables(NamedTuple):
     """What ``extend_block_tables`` makes of a step, all on the device: int32 but
     for slot_mapping (int64).
 
@@ -94,6 +92,11 @@ def extend_block_tables(block_tables, seq_lens, query_lens, free_blocks, free_co
     ends before its pages; requests behind one that the free list refused get
     no page either.
     """
+    if _lib._host is not None:
+        res = _lib._host.extend_tables(block_tables, seq_lens, query_lens, free_blocks, free_count, block_size,
+                                       num_tokens, rows, bool(update))  # every check passed, natively; else None
+        if res is not None:
+            return StepTables(*res)
     dev = _check_pool(block_tables, seq_lens, free_blocks, free_count, block_size)
     assert query_lens.dim() == 1 and num_tokens >= 0
     batch, (n_rows, width) = query_lens.shape[0], block_tables.shape
@@ -103,6 +106,7 @@ def extend_block_tables(block_tables, seq_lens, query_lens, free_blocks, free_co
     else:
         rows = _check_ints("rows", rows, dev, batch)
     lib = _lib.load()
+    _decode_host()  # (the native call from here on)
     # One int32 allocation for the small outputs and the scratch.
     counts = [batch, batch, batch, num_tokens, 1, 1, n_rows + 2 * batch + 1]
     seq, start, qlen, pos, left, refused, scratch = torch.empty(sum(counts), dtype=torch.int32, device=dev).split(counts)
