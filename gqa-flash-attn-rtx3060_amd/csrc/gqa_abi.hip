@@ -137,7 +137,8 @@ int fwd_impl(const void* q, const int64_t q_stride[4], const void* k, const int6
              bool short_form = false, const gqa::ScoreMod* mod = nullptr) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, dtype);
   if (rc) return rc;
-  const int G = num_heads / num_kv_heads, rows = short_form ? gqa::kShortRows : gqa::kFwdRows;
+  const int G = num_heads / num_kv_heads;
+  const int rows = short_form || mod != nullptr ? gqa::kShortRows : gqa::kFwdRows;
   if (G > rows) return GQA_E_GROUP;
   const int block_m = rows / G;
   const int n_mblk = (seq_q + block_m - 1) / block_m;
@@ -167,7 +168,8 @@ int fwd_impl(const void* q, const int64_t q_stride[4], const void* k, const int6
   // The scheduling counters follow the split blocks' counters.
   p.sched = part_cnt != nullptr ? part_cnt + (size_t)batch * num_kv_heads * n_split : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return to_code(short_form ? gqa::launch_short(p, dtype, st, mod) : gqa::launch_fwd(p, dtype, st, mod));
+  if (mod != nullptr && !short_form) return to_code(gqa::launch_scored(p, dtype, st, *mod));
+  return to_code(short_form ? gqa::launch_short(p, dtype, st, mod) : gqa::launch_fwd(p, dtype, st));
 }
 
 // Variable query lengths: q_start and q_len both NULL (uniform seq_q) or
@@ -726,8 +728,8 @@ int fwd_chunks_impl(const void* q, const int64_t q_stride[4], const void* k, con
                           int dtype, void* stream, const gqa::ScoreMod* mod = nullptr) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, dtype);
   if (rc) return rc;
-  const int G = num_heads / num_kv_heads;
-  if (G > gqa::kFwdRows) return GQA_E_GROUP;
+  const int G = num_heads / num_kv_heads, block_rows = mod != nullptr ? gqa::kShortRows : gqa::kFwdRows;
+  if (G > block_rows) return GQA_E_GROUP;
   if (kv_splits < 1 || kv_splits > GQA_MAX_SPLITS) return GQA_E_SPLITS;
   if (batch == 0 || seq_q == 0) return GQA_OK;
   if (workspace == nullptr) return GQA_E_NULL;
@@ -744,7 +746,7 @@ int fwd_chunks_impl(const void* q, const int64_t q_stride[4], const void* k, con
   p.v = ref(v, v_stride);
   p.o = ref(o, o_stride);
   p.dm = Dims{batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, G, scale_log2, causal ? 1 : 0};
-  p.block_m = gqa::kFwdRows / G;
+  p.block_m = block_rows / G;
   p.n_mblk = (seq_q + p.block_m - 1) / p.block_m;
   p.lse = nullptr;  // written by the combine
   p.sched = counters;
@@ -755,7 +757,8 @@ int fwd_chunks_impl(const void* q, const int64_t q_stride[4], const void* k, con
   p.ws_acc = workspace;
   p.ws_m = workspace + rows * head_dim;
   p.ws_l = p.ws_m + rows;
-  rc = to_code(gqa::launch_fwd(p, dtype, static_cast<hipStream_t>(stream), mod));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  rc = to_code(mod != nullptr ? gqa::launch_scored(p, dtype, st, *mod) : gqa::launch_fwd(p, dtype, st));
   if (rc) return rc;
   return reduce_impl(workspace, kv_splits, o, o_stride, lse, batch, num_heads, seq_q, head_dim, dtype, stream);
 }
@@ -830,7 +833,8 @@ int paged_fwd_impl(const void* q, const int64_t q_stride[4], const void* k_cache
                    int n_split, float* part_ws, int* part_cnt, bool short_form, const gqa::ScoreMod* mod) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, max_seq_len, head_dim, dtype);
   if (rc) return rc;
-  const int G = num_heads / num_kv_heads, block_rows = short_form ? gqa::kShortRows : gqa::kFwdRows;
+  const int G = num_heads / num_kv_heads;
+  const int block_rows = short_form || mod != nullptr ? gqa::kShortRows : gqa::kFwdRows;
   if (G > block_rows) return GQA_E_GROUP;
   // Each LDS-DMA instruction loads 512 / head_dim rows, which must lie in
   // one block.
@@ -883,8 +887,12 @@ int paged_fwd_impl(const void* q, const int64_t q_stride[4], const void* k_cache
   p.block_shift = shift;
   p.q_start = q_start;
   p.q_len = q_len;
-  if (short_form) return to_code(gqa::launch_short(p, dtype, static_cast<hipStream_t>(stream), mod));
-  if (kv_splits == 0) return to_code(gqa::launch_paged_fwd(p, dtype, static_cast<hipStream_t>(stream), mod));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (short_form) return to_code(gqa::launch_short(p, dtype, st, mod));
+  const auto launch = [&] {
+    return to_code(mod != nullptr ? gqa::launch_scored(p, dtype, st, *mod) : gqa::launch_paged_fwd(p, dtype, st));
+  };
+  if (kv_splits == 0) return launch();
   // Key chunks: chunk c of every query block covers key tiles [c * ct,
   // (c + 1) * ct) of the longest sequence's range; the partials go to the
   // split-KV workspace layout and the split combine writes o (and lse),
@@ -897,7 +905,7 @@ int paged_fwd_impl(const void* q, const int64_t q_stride[4], const void* k_cache
   p.ws_acc = workspace;
   p.ws_m = workspace + rows * head_dim;
   p.ws_l = p.ws_m + rows;
-  rc = to_code(gqa::launch_paged_fwd(p, dtype, static_cast<hipStream_t>(stream), mod));
+  rc = launch();
   if (rc) return rc;
   return reduce_impl(workspace, kv_splits, o, o_stride, lse, batch, num_heads, seq_q, head_dim, dtype, stream,
                      q_start, q_len);
@@ -1016,7 +1024,7 @@ extern "C" {
 
 int gqa_scored_launch(int form, const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
                       const void* v, const int64_t v_stride[4], void* o, const int64_t o_stride[4], float* lse,
-                      float* workspace, int* counters, int parts, int batch, int num_heads, int num_kv_heads,
+                      float* workspace, int parts, int batch, int num_heads, int num_kv_heads,
                       int seq_q, int seq_kv, int head_dim, float scale_log2, int causal, int dtype,
                       const gqa_score* score, void* stream) {
   gqa::ScoreMod m;
@@ -1032,18 +1040,16 @@ int gqa_scored_launch(int form, const void* q, const int64_t q_stride[4], const 
       return rc ? rc
                 : reduce_impl(workspace, parts, o, o_stride, lse, batch, num_heads, seq_q, head_dim, dtype, stream);
     case GQA_FORM_SINGLE:
+    case GQA_FORM_SHORT:
       return fwd_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, batch, num_heads, num_kv_heads, seq_q,
-                      seq_kv, head_dim, scale_log2, causal, dtype, stream, parts, workspace, counters, false, &m);
+                      seq_kv, head_dim, scale_log2, causal, dtype, stream, 0, nullptr, nullptr,
+                      form == GQA_FORM_SHORT, &m);
     case GQA_FORM_CHUNKS:
-      return fwd_chunks_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, counters, parts,
-                             batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype,
+      return fwd_chunks_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, nullptr, parts, batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype,
                              stream, &m);
     case GQA_FORM_FLAT:
       return split_flat_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, parts, batch,
                              num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream, &m);
-    case GQA_FORM_SHORT:
-      return fwd_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, batch, num_heads, num_kv_heads, seq_q,
-                      seq_kv, head_dim, scale_log2, causal, dtype, stream, 0, nullptr, nullptr, true, &m);
     default: return GQA_E_SCORE;
   }
 }
@@ -1052,7 +1058,7 @@ int gqa_paged_scored_launch(int form, const void* q, const int64_t q_stride[4], 
                             const int64_t k_cache_stride[4], const void* v_cache, const int64_t v_cache_stride[4],
                             const int* block_table, int table_stride, const int* seq_lens, const int* q_start,
                             const int* q_len, int block_size, int max_seq_len, void* o, const int64_t o_stride[4],
-                            float* lse, float* workspace, int* counters, int parts, int batch, int num_heads,
+                            float* lse, float* workspace, int parts, int batch, int num_heads,
                             int num_kv_heads, int seq_q, int head_dim, float scale_log2, int causal, int dtype,
                             const gqa_score* score, void* stream) {
   gqa::ScoreMod m;
@@ -1078,12 +1084,10 @@ int gqa_paged_scored_launch(int form, const void* q, const int64_t q_stride[4], 
     case GQA_FORM_CHUNKS:
     case GQA_FORM_SHORT: {
       if (form == GQA_FORM_CHUNKS && (parts < 1 || parts > GQA_MAX_SPLITS)) return GQA_E_SPLITS;
-      const bool single = form == GQA_FORM_SINGLE;
       return paged_fwd_impl(q, q_stride, k_cache, k_cache_stride, v_cache, v_cache_stride, block_table, table_stride,
                             seq_lens, q_start, q_len, block_size, max_seq_len, o, o_stride, lse, workspace,
                             form == GQA_FORM_CHUNKS ? parts : 0, batch, num_heads, num_kv_heads, seq_q, head_dim,
-                            scale_log2, causal, dtype, stream, single ? parts : 0, single ? workspace : nullptr,
-                            single ? counters : nullptr, form == GQA_FORM_SHORT, &m);
+                            scale_log2, causal, dtype, stream, 0, nullptr, nullptr, form == GQA_FORM_SHORT, &m);
     }
     default: return GQA_E_SCORE;
   }

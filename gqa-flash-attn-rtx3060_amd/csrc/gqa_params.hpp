@@ -328,11 +328,12 @@ inline int device_cu_count() {
   return n;
 }
 
-// `mod`: changed scores, or nullptr.
-hipError_t launch_fwd(const FwdParams& p, int dtype, hipStream_t stream, const ScoreMod* mod = nullptr);
-hipError_t launch_paged_fwd(const FwdParams& p, int dtype, hipStream_t stream, const ScoreMod* mod = nullptr);
-// (gqa_fwd_mod.hip: both, with changed scores.)
-hipError_t launch_fwd_mod(const FwdParams& p, int dtype, hipStream_t stream, const ScoreMod& mod);
+hipError_t launch_fwd(const FwdParams& p, int dtype, hipStream_t stream);
+hipError_t launch_paged_fwd(const FwdParams& p, int dtype, hipStream_t stream);
+// Single pass with changed scores (gqa_scored.hip): contiguous or paged, over
+// key chunks with p.kv_splits > 0; kShortRows rows a block.
+hipError_t launch_scored(const FwdParams& p, int dtype, hipStream_t stream, const ScoreMod& mod);
+// In the other launchers, `mod`: changed scores, or nullptr.
 // Single pass of short calls (gqa_short.hip): contiguous, or paged when
 // p.block_table is set; no split blocks, no key chunks.
 hipError_t launch_short(const FwdParams& p, int dtype, hipStream_t stream, const ScoreMod* mod = nullptr);

@@ -1,6 +1,6 @@
-// gqa_score.hpp — changed scores (ScoreMod): what the attention kernels' second
-// instances, built with FwdModParams or SplitModParams, do between the product
-// of queries and keys and the softmax.
+// gqa_score.hpp — changed scores (ScoreMod): what gqa_scored.hip, and the other
+// attention kernels' second instances, built with FwdModParams or
+// SplitModParams, do between the product of queries and keys and the softmax.
 //
 //   s <- cap tanh(s / cap),  s <- s - slope |p - j|,  visible keys by causal
 //   order, a prefix and documents,
@@ -189,7 +189,6 @@ __device__ __forceinline__ int wave_max(int x) { return -wave_min(-x); }
 // them; rel0: (8 hh) - its position.
 struct RowSpan {
   int beg, end, full_lo, full_hi, lo, vis, rel0;
-  int chunk;  // key chunks: the item's
 };
 // The block's rows are positions [pos_lo, pos_hi] of sequence b (pos_hi at most
 // sq - 1, at least pos_lo); the lane's row is `pos`, if `valid`.

@@ -403,7 +403,7 @@ py::object flash_attn(const py::handle& hq, const py::handle& hk, const py::hand
     need = gqa_split_workspace_bytes(B, Hq, Sq, D, p.n);
   else if (p.kind == kFlat)
     need = gqa_split_flat_workspace_bytes(B, Hq, Sq, D, p.n);
-  else if (p.kind == kSingle)
+  else if (p.kind == kSingle && !ch.any)
     need = gqa_fwd_split_workspace_bytes(B, Hkv, D, p.n);
   at::Tensor own;
   // (A captured call gets partials and counters of its own, in Python.)
@@ -411,7 +411,7 @@ py::object flash_attn(const py::handle& hq, const py::handle& hk, const py::hand
     ws = call_workspace(workspaces, dev, stream, need, q, own);
   else if (need > 0 && (capturing() || (ws = stream_buffer(workspaces, dev, stream, need)) == nullptr))
     return py::none();
-  if (ch.any ? p.kind == kSingle && p.n > 0 : p.kind == kSingle || p.kind == kChunks) {
+  if (!ch.any && (p.kind == kSingle || p.kind == kChunks)) {
     const size_t n = gqa_fwd_split_counters_count(B, Hkv, p.kind == kSingle ? p.n : 0);
     if (capturing() || (cnt = stream_buffer(counters, dev, stream, n * sizeof(int))) == nullptr) return py::none();
   }
@@ -435,7 +435,7 @@ py::object flash_attn(const py::handle& hq, const py::handle& hk, const py::hand
   const char* what;
   if (ch.any) {
     what = "gqa_scored_launch";
-    rc = gqa_scored_launch(p.kind, qp, qs, kp, ks, vp, vs, op, os, lse_p, wsf, cnti, p.n, b, hq_, hkv, sq, skv, d, sl2,
+    rc = gqa_scored_launch(p.kind, qp, qs, kp, ks, vp, vs, op, os, lse_p, wsf, p.n, b, hq_, hkv, sq, skv, d, sl2,
                            c, dt, &ch.score, stream);
     if (rc == GQA_E_FLAT || rc == GQA_E_SCORE) return py::none();
   } else if (p.kind == kSplit) {
@@ -525,7 +525,7 @@ py::object paged_attn(const py::handle& hq, const py::handle& hkc, const py::han
     need = gqa_split_workspace_bytes(B, H, Sq, D, p.n);
   else if (p.kind == kFlat)
     need = gqa_split_flat_workspace_bytes(B, H, Sq, D, p.n);
-  else if (p.kind == kSingle)
+  else if (p.kind == kSingle && !ch.any)
     need = gqa_fwd_split_workspace_bytes(B, Hkv, D, p.n);
   // (A captured call gets partials and counters of its own, in Python.)
   at::Tensor own;
@@ -533,7 +533,7 @@ py::object paged_attn(const py::handle& hq, const py::handle& hkc, const py::han
     ws = call_workspace(workspaces, dev, stream, need, q, own);
   else if (need > 0 && (capturing() || (ws = stream_buffer(workspaces, dev, stream, need)) == nullptr))
     return py::none();
-  if (p.kind == kSingle && p.n > 0) {
+  if (!ch.any && p.kind == kSingle && p.n > 0) {
     const size_t n = gqa_fwd_split_counters_count(B, Hkv, p.n);
     if (capturing() || (cnt = stream_buffer(counters, dev, stream, n * sizeof(int))) == nullptr) return py::none();
   }
@@ -574,7 +574,7 @@ py::object paged_attn(const py::handle& hq, const py::handle& hkc, const py::han
   void* op = out.data_ptr();
   if (ch.any) {
     const int rc = gqa_paged_scored_launch(p.kind, qp, qs, kp, ks, vp, vs, tp, ts, lp, qsp, qlp, bsz, ms, op, os, lse_p,
-                                           wsf, static_cast<int*>(cnt), p.n, b, h, hkv, sq, d, sl2, c, dt, &ch.score,
+                                           wsf, p.n, b, h, hkv, sq, d, sl2, c, dt, &ch.score,
                                            stream);
     if (rc == GQA_E_FLAT || rc == GQA_E_SCORE) return py::none();
     check_rc(rc, "gqa_paged_scored_launch");

@@ -144,12 +144,12 @@ SIGNATURES = {
     ),
     "gqa_scored_launch": (
         _i,
-        [_i, _p, _i64x4, _p, _i64x4, _p, _i64x4, _p, _i64x4, _p, _p, _p, _i,
+        [_i, _p, _i64x4, _p, _i64x4, _p, _i64x4, _p, _i64x4, _p, _p, _i,
          _i, _i, _i, _i, _i, _i, _f, _i, _i, ctypes.POINTER(Score), _p],
     ),
     "gqa_paged_scored_launch": (
         _i,
-        [_i, _p, _i64x4, _p, _i64x4, _p, _i64x4, _p, _i, _p, _p, _p, _i, _i, _p, _i64x4, _p, _p, _p, _i,
+        [_i, _p, _i64x4, _p, _i64x4, _p, _i64x4, _p, _i, _p, _p, _p, _i, _i, _p, _i64x4, _p, _p, _i,
          _i, _i, _i, _i, _i, _f, _i, _i, ctypes.POINTER(Score), _p],
     ),
     "gqa_qk_norm_rope_launch": (

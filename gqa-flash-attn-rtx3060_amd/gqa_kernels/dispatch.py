@@ -918,18 +918,12 @@ def _scored(route, q_in, k, v, causal, return_lse, score):
     stream = stream_handle(q.device)
 
     def launch(route):
-        lib, ws, cnt, parts = _lib.load(), None, None, route.splits
+        ws = None
         if route.kind in ("split", "chunks"):
-            ws = workspace(workspace_bytes(batch, num_heads, seq_q, head_dim, parts), q.device)
+            ws = workspace(workspace_bytes(batch, num_heads, seq_q, head_dim, route.splits), q.device)
         elif route.kind == "flat":
-            ws = workspace(flat_workspace_bytes(batch, num_heads, seq_q, head_dim, parts), q.device)
-        elif route.kind == "single":
-            parts = route.fwd_split
-            if parts:
-                ws = workspace(lib.gqa_fwd_split_workspace_bytes(batch, num_kv_heads, head_dim, parts), q.device)
-                cnt = _counter_buffer(q.device, stream,
-                                      lib.gqa_fwd_split_counters_count(batch, num_kv_heads, parts))
-        return scored_launch(_KIND_IDS[route.kind], parts, q, k, v, o, lse, ws, cnt, causal,
+            ws = workspace(flat_workspace_bytes(batch, num_heads, seq_q, head_dim, route.splits), q.device)
+        return scored_launch(_KIND_IDS[route.kind], route.splits, q, k, v, o, lse, ws, causal,
                              (head_dim ** -0.5) * LOG2E, _DTYPES[q.dtype], score, stream)
 
     rc = launch(route)

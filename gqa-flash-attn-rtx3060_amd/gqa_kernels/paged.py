@@ -647,21 +647,17 @@ def _paged_scored(kind, parts, q, k_cache, v_cache, block_table, table_stride, s
     stream = stream_handle(dev)
 
     def launch(kind, parts):
-        ws = cnt = None
+        ws = None
         if kind in ("split", "chunks"):
             ws = own_workspace(workspace_bytes(batch, num_heads, seq_q, head_dim, parts), dev)
         elif kind == "flat":
             ws = own_workspace(flat_workspace_bytes(batch, num_heads, seq_q, head_dim, parts), dev)
-        elif kind == "single" and parts:
-            ws = own_workspace(lib.gqa_fwd_split_workspace_bytes(batch, num_kv_heads, head_dim, parts), dev)
-            cnt = _counter_buffer(dev, stream, lib.gqa_fwd_split_counters_count(batch, num_kv_heads, parts))
         return lib.gqa_paged_scored_launch(
             _KIND_IDS[kind], q.data_ptr(), _row_strides(q, varlen), k_cache.data_ptr(), _lib.strides(k_cache),
             v_cache.data_ptr(), _lib.strides(v_cache), block_table.data_ptr(), table_stride, seq_lens.data_ptr(),
             query_start.data_ptr() if varlen else None, query_lens.data_ptr() if varlen else None, block_size,
             max_seq_len, out.data_ptr(), _row_strides(out, varlen), None if lse is None else lse.data_ptr(),
-            None if ws is None else ws.data_ptr(), None if cnt is None else cnt.data_ptr(), parts, batch, num_heads,
-            num_kv_heads, seq_q, head_dim, scale_log2, int(bool(causal)), dtype, ctypes.byref(score), stream)
+            None if ws is None else ws.data_ptr(), parts, batch, num_heads, num_kv_heads, seq_q, head_dim, scale_log2, int(bool(causal)), dtype, ctypes.byref(score), stream)
 
     rc = launch(kind, parts)
     if rc == _lib.GQA_E_FLAT:

@@ -98,16 +98,15 @@ def check_score(softcap, alibi_slopes, prefix_lens, documents, *, batch: int, nu
     return s
 
 
-def scored_launch(form: int, parts: int, q, k, v, o, lse, workspace, counters, causal: bool, scale_log2: float,
-                  dtype: int, score: "_lib.Score", stream: int) -> int:
+def scored_launch(form: int, parts: int, q, k, v, o, lse, workspace, causal: bool, scale_log2: float, dtype: int,
+                  score: "_lib.Score", stream: int) -> int:
     """gqa_scored_launch on kernel-ready tensors; its return code."""
     batch, num_heads, seq_q, head_dim = q.shape
     return _lib.load().gqa_scored_launch(
         form, q.data_ptr(), _lib.strides(q), k.data_ptr(), _lib.strides(k), v.data_ptr(), _lib.strides(v),
         o.data_ptr(), _lib.strides(o), None if lse is None else lse.data_ptr(),
-        None if workspace is None else workspace.data_ptr(), None if counters is None else counters.data_ptr(), parts,
-        batch, num_heads, k.shape[1], seq_q, k.shape[2], head_dim, scale_log2, int(bool(causal)), dtype,
-        ctypes.byref(score), stream)
+        None if workspace is None else workspace.data_ptr(), parts, batch, num_heads, k.shape[1], seq_q,
+        k.shape[2], head_dim, scale_log2, int(bool(causal)), dtype, ctypes.byref(score), stream)
 
 
 def workspace(nbytes: int, device) -> Optional[torch.Tensor]:

@@ -476,11 +476,14 @@ typedef struct gqa_score {
   const int* span_hi;        /* (batch, seq_kv) */
 } gqa_score;
 
-/* form: the launch whose work decomposition (and meaning of workspace, counters
- * and parts) the call takes: gqa_split_launch (parts: splits),
- * gqa_fwd_split_launch (n_split), gqa_fwd_chunks_launch (kv_splits),
- * gqa_split_flat_launch (slots), gqa_fwd_short_launch (0), or their paged
- * counterparts, whose other arguments and errors hold. */
+/* form: how the work is cut, with the arguments and errors of the launch (paged:
+ * of its paged counterpart) named here.  GQA_FORM_SPLIT: gqa_split_launch, parts
+ * splits; GQA_FORM_SINGLE: gqa_fwd_lse_launch, in blocks of 128 packed rows;
+ * GQA_FORM_CHUNKS: the same over parts key chunks, as gqa_fwd_chunks_launch;
+ * GQA_FORM_FLAT: gqa_split_flat_launch, parts slots; GQA_FORM_SHORT:
+ * gqa_fwd_short_launch.  workspace: that launch's (NULL for single and short);
+ * lse may be NULL.  The group size is at most 128 in the single, chunk and
+ * short forms (GQA_E_GROUP). */
 #define GQA_FORM_SPLIT 0
 #define GQA_FORM_SINGLE 1
 #define GQA_FORM_CHUNKS 2
@@ -491,7 +494,7 @@ int gqa_scored_launch(int form,
                       const void* k, const int64_t k_stride[4],
                       const void* v, const int64_t v_stride[4],
                       void* o, const int64_t o_stride[4], float* lse,
-                      float* workspace, int* counters, int parts,
+                      float* workspace, int parts,
                       int batch, int num_heads, int num_kv_heads,
                       int seq_q, int seq_kv, int head_dim,
                       float scale_log2, int causal, int dtype,
@@ -505,7 +508,7 @@ int gqa_paged_scored_launch(int form,
                             const int* seq_lens, const int* q_start, const int* q_len,
                             int block_size, int max_seq_len,
                             void* o, const int64_t o_stride[4], float* lse,
-                            float* workspace, int* counters, int parts,
+                            float* workspace, int parts,
                             int batch, int num_heads, int num_kv_heads,
                             int seq_q, int head_dim,
                             float scale_log2, int causal, int dtype,
