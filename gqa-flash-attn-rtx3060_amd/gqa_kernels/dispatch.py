@@ -190,6 +190,19 @@ COMBINE_BYTES_PER_US = 5.0e6
 # the first pass, read back by the combine (fitted: 1.5).
 CHUNK_PARTIAL_PASSES = 1.5
 
+# Changed scores (scores.py): run time in us of the single pass in 128-row
+# workgroups, two a CU (gqa_scored.hip), plain or over key chunks, and of the
+# short form with the same changes: base + the longest slot's sum of (item +
+# tiles x step), the step's time as _step_us has it; the combine: launch + rows
+# + partials.  Fitted to 34 prompts and chunks at each head_dim (64-4096 new
+# tokens, up to 16384 keys, 7-32 query heads, batches of 1-8, capped scores):
+# chunk forms within 8 % in the mean, the short one within 4 %.  The fastest of
+# the modelled times took 1.01 times the fastest measured in the mean, 1.20 at
+# worst (without the short form 1.04 and 1.5).
+SCORED_PASS_US = {128: (2.4, 3.9, 1.58, 2.35), 64: (2.4, 2.5, 1.23, 1.63)}
+SCORED_SHORT_US = {128: (3.5, 4.7, 2.15, 2.46), 64: (2.7, 3.8, 1.93, 1.96)}
+SCORED_COMBINE_US = {128: (3.5, 0.36e-3, 0.30e-6), 64: (4.0, 0.90e-3, 0.17e-6)}  # launch, per row, per byte
+
 # Route kinds as the native calls number them (gqa_host.cpp).
 _KIND_IDS = {"split": 0, "single": 1, "chunks": 2, "flat": 3, "short": 4}
 
@@ -817,7 +830,7 @@ def gqa_flash_attn(q, k, v, causal=True, *, return_lse=False, softcap=None, alib
     if changed:
         refuse_grad("gqa_flash_attn with changed scores", q, k, v, alibi_slopes)
         score = check_score(softcap, alibi_slopes, prefix_lens, documents, batch=batch, num_heads=num_heads,
-                            seq_q=seq_q, seq_kv=seq_kv, causal=bool(causal), scale=head_dim ** -0.5, device=q.device)
+                            num_kv_heads=num_kv_heads, seq_q=seq_q, seq_kv=seq_kv, causal=bool(causal), scale=head_dim ** -0.5, device=q.device)
         with torch.cuda.device(dev):
             route = _scored_route(q, k, v, causal, dev, documents is not None)
             host = _decode_host()
@@ -892,18 +905,75 @@ def _native_scored(host, q, k, v, causal, return_lse, softcap, alibi_slopes, pre
                            alibi_slopes, prefix_lens, starts, ends)
 
 
+def _slots_us(model, runs, n_bh: int, slots: int, work: int, longest: int) -> float:
+    """base + the longest of `slots` slots' (item + tiles x step) sums; runs:
+    [tiles, count] of one (b, kv head) in the kernel's order."""
+    base, item, lo, hi = model
+    step = _step_us(lo, hi, work, longest, slots)
+    return base + _list_makespan([[item + step * t, n] for t, n in runs], n_bh, slots)
+
+
+@functools.lru_cache(maxsize=4096)
+def scored_plan(batch: int, num_heads: int, num_kv_heads: int, seq_q: int, seq_kv: int, cu_count: int,
+                causal: bool = True, head_dim: int = 128) -> Route:
+    """The form of the single pass for a call with changed scores: "single",
+    "chunks" or "short", by the modelled times above."""
+    group = num_heads // num_kv_heads
+    block_m = SHORT_ROWS // group
+    n_mblk, n_bh = _cdiv(seq_q, block_m), batch * num_kv_heads
+    if n_mblk * n_bh == 0 or seq_kv == 0:
+        return Route("single")
+    if n_mblk * n_bh >= 8 * cu_count:  # (four rounds of workgroups: nothing to split)
+        return Route("single", 1, n_mblk * n_bh)
+    tiles = _fwd_block_tiles(n_mblk, block_m, seq_q, seq_kv, causal)
+    order = tiles[::-1] if causal else tiles
+    work, slots = sum(tiles) * n_bh, 2 * cu_count
+
+    def runs_of(items):
+        runs = []
+        for t in items:
+            _push_run(runs, t, 1)
+        return runs
+
+    best = _slots_us(SCORED_PASS_US[head_dim], runs_of(order), n_bh, slots, work, max(tiles))
+    route = Route("single", 1, n_mblk * n_bh)
+    # (Short: two tiles a step, one workgroup a CU; within what its models were fitted to.)
+    if n_mblk * n_bh <= SHORT_MAX_WG_PER_CU * cu_count:
+        base, item, lo, hi = SCORED_SHORT_US[head_dim]
+        step = _step_us(lo, hi, work, max(tiles), cu_count)
+        t = base + _list_makespan([[item + step * _cdiv(t, 2), n] for t, n in runs_of(order)], n_bh, cu_count)
+        if t < best:
+            best, route = t, Route("short", 1, n_mblk * n_bh)
+    launch, per_row, per_byte = SCORED_COMBINE_US[head_dim]
+    rows, s = batch * num_heads * seq_q, 2
+    while s <= _lib.GQA_MAX_SPLITS and _cdiv(_cdiv(seq_kv, FWD_TILE), s) >= 2 and n_mblk * n_bh * s <= 8 * slots:
+        ct = _cdiv(_cdiv(seq_kv, FWD_TILE), s)
+        items = [max(0, min(t - c * ct, ct)) for c in range(s) for t in order]
+        t = _slots_us(SCORED_PASS_US[head_dim], runs_of(items), n_bh, slots, work, max(items))
+        t += launch + per_row * rows + per_byte * rows * s * (head_dim + 2) * 4
+        if t < best:
+            best, route = t, Route("chunks", s, n_mblk * n_bh * s)
+        s *= 2
+    return route
+
+
 def _scored_route(q, k, v, causal, dev, spans) -> Route:
-    """The route of a call with changed scores: choose_plan's, or with documents
-    one of those that start at a first visible key."""
+    """The route of a call with changed scores: few packed rows per kv head as
+    choose_plan has them, others by scored_plan; with documents the single pass
+    alone, which starts at a block's first visible key."""
     batch, num_heads, seq_q, head_dim = q.shape
     shape = (batch, num_heads, k.shape[1], seq_q, k.shape[2], _cu_count(dev), bool(causal), head_dim)
     if spans:
         return Route("single")
-    route = _plan_cached(*shape)
-    # As _launch: 32-bit byte offsets must span the keys.
-    if route.kind != "single" and (k.shape[2] + 192) * max(k.stride(2), v.stride(2)) >= 1 << 30:
-        route = _route_cached(*shape)
-    return route
+    far = (k.shape[2] + 192) * max(k.stride(2), v.stride(2)) >= 1 << 30  # as _launch: 32-bit byte offsets
+    if num_heads // k.shape[1] * seq_q <= split_max_rows(head_dim):
+        route = _plan_cached(*shape)
+        if route.kind in ("split", "flat") and not far:
+            return route
+        if far:  # the split-KV pass alone takes such rows
+            route = _route_cached(*shape)
+            return route if route.kind == "split" else Route("split", 1)
+    return scored_plan(*shape)
 
 
 def _scored(route, q_in, k, v, causal, return_lse, score):
@@ -928,7 +998,7 @@ def _scored(route, q_in, k, v, causal, return_lse, score):
 
     rc = launch(route)
     if rc == _lib.GQA_E_FLAT:
-        rc = launch(_base_route(q, k, causal, q.get_device()))
+        rc = launch(Route("split", _base_route(q, k, causal, q.get_device()).splits))
     _lib.check(rc)
     return o if lse is None else (o, lse)
 

@@ -42,7 +42,7 @@ import torch
 
 from . import _lib
 from .dispatch import (_KIND_IDS, FWD_ROWS, SPLIT_MIN_KV, _fwd_block_tiles, choose_fwd_split, choose_kv_chunks, flat_max_rows,
-                       flat_piece_steps, flat_steps, fwd_split_makespan, use_short)
+                       flat_piece_steps, flat_steps, fwd_split_makespan, scored_plan, use_short)
 from .gqa_split import (_counter_buffer, _counters, _decode_host, _workspace_buffer, _workspaces,
                         flat_workspace_bytes, stream_handle, workspace_bytes)
 from .rotary import qk_norm_rope, qk_norm_rope_write
@@ -498,8 +498,9 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
     score = None
     if changed:
         refuse_grad("paged_attention with changed scores", q, k_cache, v_cache, alibi_slopes)
-        score = check_score(softcap, alibi_slopes, prefix_lens, None, batch=batch, num_heads=num_heads, seq_q=seq_q,
-                            seq_kv=max_seq_len, causal=bool(causal), scale=scale, device=qdev)
+        score = check_score(softcap, alibi_slopes, prefix_lens, None, batch=batch, num_heads=num_heads,
+                            num_kv_heads=num_kv_heads, seq_q=seq_q, seq_kv=max_seq_len, causal=bool(causal),
+                            scale=scale, device=qdev)
     if default_route and batch > 0 and seq_q > 0:
         plan_key = [3 if changed else 1, batch, num_heads, num_kv_heads, seq_q, max_seq_len, head_dim, int(bool(causal)), dev, block_size,
                     int(interleaved), int(varlen)]
@@ -512,13 +513,20 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
         # route that this call's strides refuse is not the shape's.
         if short and max(k_cache.stride(1), v_cache.stride(1)) >= 1 << 24:
             short, plan_key = False, None
-        if short:
+        if changed and route == "single":
+            planned = scored_plan(batch, num_heads, num_kv_heads, seq_q, max_seq_len, _cu_count(dev), bool(causal),
+                                  head_dim)
+            route, kv_chunks = planned.kind, planned.splits if planned.kind == "chunks" else 0
+            if route == "short" and max(k_cache.stride(1), v_cache.stride(1)) >= 1 << 24:
+                route, plan_key = "single", None
+        elif short:
             route = "short"
         elif route == "single":
             kv_chunks, fwd_split = paged_single_plan(batch, num_heads, num_kv_heads, seq_q, max_seq_len,
                                                      _cu_count(dev), bool(causal), head_dim)
             route = "chunks" if kv_chunks else route
     elif route == "single":
+        assert not (changed and splits_given and splits), "changed scores: the single pass has no split blocks"
         fwd_split = splits if splits_given else 0
     elif route == "chunks":
         kv_chunks = splits if splits_given else max(2, paged_kv_chunks(

@@ -62,11 +62,12 @@ def document_spans(document_ids: torch.Tensor) -> DocumentSpans:
     return DocumentSpans(both[0], both[1])
 
 
-def check_score(softcap, alibi_slopes, prefix_lens, documents, *, batch: int, num_heads: int, seq_q: int,
-                seq_kv: int, causal: bool, scale: float, device) -> _lib.Score:
+def check_score(softcap, alibi_slopes, prefix_lens, documents, *, batch: int, num_heads: int, num_kv_heads: int,
+                seq_q: int, seq_kv: int, causal: bool, scale: float, device) -> _lib.Score:
     """The changes as the C entry points take them, their arguments checked.
     (The struct holds addresses: the caller keeps the tensors.)"""
     s = _lib.Score()
+    assert num_heads <= 128 * num_kv_heads, "changed scores take groups of at most 128 query heads per kv head"
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"changed scores need a positive scale, not {scale}")
     if softcap:

@@ -22,9 +22,9 @@ def scored(lib, form=1, parts=0, paged=False, softcap=10.0, slopes=None, prefix=
            ws=None, lse=None, head_dim=128, dtype=0, batch=1):
     s = _lib.Score(softcap, slopes, prefix, lo, hi)
     if paged:
-        return lib.gqa_paged_scored_launch(form, P, ST, P, ST, P, ST, P, 8, P, None, None, 16, seq_kv, P, ST, lse, ws, None, parts, batch, 8, 2, seq_q,
+        return lib.gqa_paged_scored_launch(form, P, ST, P, ST, P, ST, P, 8, P, None, None, 16, seq_kv, P, ST, lse, ws, parts, batch, 8, 2, seq_q,
                                            head_dim, scale, causal, dtype, ctypes.byref(s), None)
-    return lib.gqa_scored_launch(form, P, ST, P, ST, P, ST, P, ST, lse, ws, None, parts, batch, 8, 2, seq_q, seq_kv, head_dim, scale, causal, dtype,
+    return lib.gqa_scored_launch(form, P, ST, P, ST, P, ST, P, ST, lse, ws, parts, batch, 8, 2, seq_q, seq_kv, head_dim, scale, causal, dtype,
                                  ctypes.byref(s), None)
 
 
@@ -98,7 +98,7 @@ def test_table_and_span_refusals(lib):
 
 def test_python_checks_without_a_device():
     dev = torch.device("cpu")
-    kw = dict(batch=2, num_heads=4, seq_q=8, seq_kv=8, causal=True, scale=0.1, device=dev)
+    kw = dict(batch=2, num_heads=4, num_kv_heads=2, seq_q=8, seq_kv=8, causal=True, scale=0.1, device=dev)
     z = torch.zeros(2, 8, dtype=torch.int32)
     assert check_score(0.0, None, None, None, **kw).softcap == 0.0 and check_score(2.0, None, None, None, **kw).softcap == 2.0
     for cap in (-1.0, float("nan"), 1e-6, 1e12, float("inf")):
