@@ -957,6 +957,28 @@ def scored_plan(batch: int, num_heads: int, num_kv_heads: int, seq_q: int, seq_k
     return route
 
 
+# Chunks of at most this many 64-key tiles stay ahead of the flat split.
+SCORED_CHUNK_TILES = 8
+
+
+def scored_fine_split(batch: int, num_kv_heads: int, rows: int, seq_kv: int, cu_count: int, head_dim: int) -> tuple:
+    """(splits, 64-key tiles a chunk) of the split pass with changed scores that
+    keeps its workgroups within the compute units, down to one tile a chunk;
+    (0, 0) without keys or over the rows of the split pass measured here (32, at
+    head_dim 64 16).
+
+    A step costs more than with plain scores (a bound on the vector ALU), the
+    combine the same.  Contiguous, bf16, head_dim 128, us, choose_plan's count /
+    this: one token over 300 keys of 8 kv heads 9.0 / 7.3, 700 9.1 / 7.5, 1500 9.6
+    / 8.1, 8000 11.8 / 11.8; 3 x 700 with 4 tokens 9.7 / 7.9; 8 x 300 10.0 / 9.0;
+    over pages in paged.scored_split."""
+    tiles = _cdiv(seq_kv, 64)
+    if not 0 < rows <= (32 if head_dim == 128 else 16) or tiles == 0 or batch == 0:
+        return 0, 0
+    fine = max(1, min(tiles, cu_count // (batch * num_kv_heads), _lib.GQA_MAX_SPLITS))
+    return fine, _cdiv(tiles, fine)
+
+
 def _scored_route(q, k, v, causal, dev, spans) -> Route:
     """The route of a call with changed scores: few packed rows per kv head as
     choose_plan has them, others by scored_plan; with documents the single pass
@@ -969,7 +991,11 @@ def _scored_route(q, k, v, causal, dev, spans) -> Route:
     if num_heads // k.shape[1] * seq_q <= split_max_rows(head_dim):
         route = _plan_cached(*shape)
         if route.kind in ("split", "flat") and not far:
-            return route
+            fine, chunk = scored_fine_split(batch, k.shape[1], num_heads // k.shape[1] * seq_q, k.shape[2], shape[5],
+                                            head_dim)
+            if not fine or chunk > SCORED_CHUNK_TILES:
+                return route
+            return Route("split", max(fine, route.splits if route.kind == "split" else 0))
         if far:  # the split-KV pass alone takes such rows
             route = _route_cached(*shape)
             return route if route.kind == "split" else Route("split", 1)

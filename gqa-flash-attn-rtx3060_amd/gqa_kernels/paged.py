@@ -41,8 +41,9 @@ from typing import Dict, Hashable, List, Optional, Sequence
 import torch
 
 from . import _lib
-from .dispatch import (_KIND_IDS, FWD_ROWS, SPLIT_MIN_KV, _fwd_block_tiles, choose_fwd_split, choose_kv_chunks, flat_max_rows,
-                       flat_piece_steps, flat_steps, fwd_split_makespan, scored_plan, use_short)
+from .dispatch import (_KIND_IDS, FWD_ROWS, SCORED_CHUNK_TILES, SPLIT_MIN_KV, _fwd_block_tiles, choose_fwd_split,
+                       choose_kv_chunks, flat_max_rows, flat_piece_steps, flat_steps, fwd_split_makespan,
+                       scored_fine_split, scored_plan, use_short)
 from .gqa_split import (_counter_buffer, _counters, _decode_host, _workspace_buffer, _workspaces,
                         flat_workspace_bytes, stream_handle, workspace_bytes)
 from .rotary import qk_norm_rope, qk_norm_rope_write
@@ -113,6 +114,7 @@ _SPLIT_WG_PER_CU = 2
 _LDS_WG_PER_CU = 1
 _LDS_WG_PER_CU_INTERLEAVED = 4
 _MIN_CHUNK = 256
+SCORED_SLOT_TILES = 32  # 64-key tiles a slot, scored_split
 # Tile steps a piece of the flat split keeps, and steps that its ranges are
 # shorter than the fixed count's chunks (paged_flat_slots): head_dim 64,
 # head_dim 128 up to 16 packed rows, 17-32 rows.
@@ -252,6 +254,36 @@ def paged_flat_slots(batch: int, num_heads: int, num_kv_heads: int, seq_q: int, 
     saved = -(-steps // splits) - batch * steps / slots
     least = (_FLAT_MIN_SAVED_WIDE if wide else _FLAT_MIN_SAVED[head_dim]) + (splits == 1)
     return slots if saved >= least else 0
+
+
+@functools.lru_cache(maxsize=4096)
+def scored_split(batch: int, num_heads: int, num_kv_heads: int, seq_q: int, max_seq_len: int, cu_count: int,
+                 block_size: int = 64, head_dim: int = 128, heads_interleaved: bool = False) -> tuple:
+    """(slots of the flat split or 0, split count) of a paged split call with
+    changed scores.
+
+    The fine split of scored_fine_split, ahead of the flat split where its chunks
+    are at most SCORED_CHUNK_TILES tiles; a flat split of up to 16 rows whose
+    slots have SCORED_SLOT_TILES tiles and more takes two workgroups a CU.
+    Measured on MI355X (bf16, us, paged_splits and paged_flat_slots / this):
+    one token over 700 keys of 8 kv heads 12.3 / 7.5, 3000 13.0 / 8.9, 8000
+    15.8 / 12.1; B = 2 of 4000 14.1 / 11.5; B = 8 of 300 (2 kv heads) 9.7 /
+    7.6; B = 32 of 100-8000 55.1 / 51.1, of 2204-14176 (head_dim 64, 4 kv
+    heads) 69.8 / 59.1.  87 batches against the best of all counts: 1.19 / 1.03
+    times its time in the mean (worst 1.75 / 1.30, 16 x 9000 of 2 kv heads at
+    head_dim 64, where paged_splits' 32 parts stay)."""
+    slots = paged_flat_slots(batch, num_heads, num_kv_heads, seq_q, max_seq_len, cu_count, block_size, head_dim,
+                             heads_interleaved)
+    splits = paged_splits(batch, num_heads, num_kv_heads, seq_q, max_seq_len, cu_count, block_size, head_dim,
+                          heads_interleaved)
+    rows = num_heads // num_kv_heads * seq_q
+    fine, chunk = scored_fine_split(batch, num_kv_heads, rows, max_seq_len, cu_count, head_dim)
+    if fine and (not slots or chunk <= SCORED_CHUNK_TILES):
+        return 0, max(fine, splits)
+    if (rows <= _DEC16_ROWS and 2 * slots <= _lib.GQA_MAX_SPLITS
+            and batch * max_seq_len >= 64 * SCORED_SLOT_TILES * slots):
+        slots *= 2
+    return slots, splits
 
 
 def _paged_host():
@@ -475,7 +507,10 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
     splits_given = splits is not None
     flat_slots = 0
     interleaved = k_cache.stride(1) != head_dim or v_cache.stride(1) != head_dim
-    if splits is None and route in (None, "split"):
+    if changed and splits is None and route in (None, "split"):
+        flat_slots, splits = scored_split(batch, num_heads, num_kv_heads, seq_q, max_seq_len, _cu_count(dev),
+                                          block_size, head_dim, interleaved)
+    elif splits is None and route in (None, "split"):
         flat_slots = paged_flat_slots(batch, num_heads, num_kv_heads, seq_q, max_seq_len, _cu_count(dev), block_size,
                                       head_dim, interleaved)
     if splits is None and (not flat_slots or max_seq_len > 1 << 20):  # (only there can it refuse the call)
@@ -502,8 +537,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
                             num_kv_heads=num_kv_heads, seq_q=seq_q, seq_kv=max_seq_len, causal=bool(causal),
                             scale=scale, device=qdev)
     if default_route and batch > 0 and seq_q > 0:
-        plan_key = [3 if changed else 1, batch, num_heads, num_kv_heads, seq_q, max_seq_len, head_dim, int(bool(causal)), dev, block_size,
-                    int(interleaved), int(varlen)]
+        plan_key = [3 if changed else 1, batch, num_heads, num_kv_heads, seq_q, max_seq_len, head_dim,
+                    int(bool(causal)), dev, block_size, int(interleaved), int(varlen)]
     kv_chunks = fwd_split = 0
     if route is None:
         route = paged_route(num_heads, num_kv_heads, seq_q, block_size, head_dim)
@@ -551,10 +586,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
             return _paged_scored("flat" if flat else route, flat_slots if flat else n_parts, q, k_cache, v_cache,
                                  block_table, table_stride, seq_lens, query_start if varlen else None,
                                  query_lens if varlen else None, block_size, max_seq_len, out, lse, batch, seq_q,
-                                 scale * LOG2E, causal, dtype, score,
-                                 lambda: splits if splits is not None else paged_splits(
-                                     batch, num_heads, num_kv_heads, seq_q, max_seq_len, _cu_count(dev), block_size,
-                                     head_dim, interleaved))
+                                 scale * LOG2E, causal, dtype, score, splits)
     if flat:
         workspace = _workspace_buffer(qdev, stream, flat_workspace_bytes(batch, num_heads, seq_q, head_dim, flat_slots))
         if host is not None:
@@ -647,9 +679,9 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
 
 
 def _paged_scored(kind, parts, q, k_cache, v_cache, block_table, table_stride, seq_lens, query_start, query_lens,
-                  block_size, max_seq_len, out, lse, batch, seq_q, scale_log2, causal, dtype, score, fixed_splits):
+                  block_size, max_seq_len, out, lse, batch, seq_q, scale_log2, causal, dtype, score, splits):
     """paged_attention's launch with changed scores (gqa_paged_scored_launch);
-    ``fixed_splits``: the split count where the flat split is refused."""
+    ``splits``: the count where the flat split is refused."""
     lib, dev, varlen = _lib.load(), q.device, query_start is not None
     num_heads, head_dim, num_kv_heads = q.shape[1], q.shape[-1], k_cache.shape[2]
     stream = stream_handle(dev)
@@ -665,11 +697,12 @@ def _paged_scored(kind, parts, q, k_cache, v_cache, block_table, table_stride, s
             v_cache.data_ptr(), _lib.strides(v_cache), block_table.data_ptr(), table_stride, seq_lens.data_ptr(),
             query_start.data_ptr() if varlen else None, query_lens.data_ptr() if varlen else None, block_size,
             max_seq_len, out.data_ptr(), _row_strides(out, varlen), None if lse is None else lse.data_ptr(),
-            None if ws is None else ws.data_ptr(), parts, batch, num_heads, num_kv_heads, seq_q, head_dim, scale_log2, int(bool(causal)), dtype, ctypes.byref(score), stream)
+            None if ws is None else ws.data_ptr(), parts, batch, num_heads, num_kv_heads, seq_q, head_dim,
+            scale_log2, int(bool(causal)), dtype, ctypes.byref(score), stream)
 
     rc = launch(kind, parts)
     if rc == _lib.GQA_E_FLAT:
-        rc = launch("split", fixed_splits())
+        rc = launch("split", splits)
     _lib.check(rc)
     return out if lse is None else (out, lse)
 
