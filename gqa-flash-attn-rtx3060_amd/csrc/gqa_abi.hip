@@ -262,10 +262,10 @@ int gqa_paged_fwd_short_launch(const void* q, const int64_t q_stride[4], const v
 
 namespace {
 
-int split_first_impl(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
-                           const void* v, const int64_t v_stride[4], float* workspace, int splits, int batch,
-                           int num_heads, int num_kv_heads, int seq_q, int seq_kv, int head_dim,
-                           float scale_log2, int causal, int dtype, void* stream, const gqa::ScoreMod* mod = nullptr) {
+int split_first_impl(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4], const void* v,
+                     const int64_t v_stride[4], float* workspace, int splits, int batch, int num_heads,
+                     int num_kv_heads, int seq_q, int seq_kv, int head_dim, float scale_log2, int causal, int dtype,
+                     void* stream, const gqa::ScoreMod* mod = nullptr) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, dtype);
   if (rc) return rc;
   if (splits < 1 || splits > GQA_MAX_SPLITS) return GQA_E_SPLITS;
@@ -303,7 +303,8 @@ int gqa_split_first_launch(const void* q, const int64_t q_stride[4], const void*
                            const void* v, const int64_t v_stride[4], float* workspace, int splits, int batch,
                            int num_heads, int num_kv_heads, int seq_q, int seq_kv, int head_dim,
                            float scale_log2, int causal, int dtype, void* stream) {
-  return split_first_impl(q, q_stride, k, k_stride, v, v_stride, workspace, splits, batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream);
+  return split_first_impl(q, q_stride, k, k_stride, v, v_stride, workspace, splits, batch, num_heads, num_kv_heads,
+                          seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream);
 }
 
 }  // extern "C"
@@ -311,12 +312,11 @@ int gqa_split_first_launch(const void* q, const int64_t q_stride[4], const void*
 namespace {
 
 int paged_split_first_impl(const void* q, const int64_t q_stride[4], const void* k_cache,
-                                 const int64_t k_cache_stride[4], const void* v_cache,
-                                 const int64_t v_cache_stride[4], const int* block_table, int table_stride,
-                                 const int* seq_lens, const int* q_start, const int* q_len, int block_size,
-                                 int max_seq_len, float* workspace, int splits, int batch, int num_heads,
-                                 int num_kv_heads, int seq_q, int head_dim, float scale_log2, int causal, int dtype,
-                                 void* stream, const gqa::ScoreMod* mod = nullptr) {
+                           const int64_t k_cache_stride[4], const void* v_cache, const int64_t v_cache_stride[4],
+                           const int* block_table, int table_stride, const int* seq_lens, const int* q_start,
+                           const int* q_len, int block_size, int max_seq_len, float* workspace, int splits, int batch,
+                           int num_heads, int num_kv_heads, int seq_q, int head_dim, float scale_log2, int causal,
+                           int dtype, void* stream, const gqa::ScoreMod* mod = nullptr) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, max_seq_len, head_dim, dtype);
   if (rc) return rc;
   if (block_size < 1 || block_size > GQA_MAX_BLOCK_SIZE || (block_size & (block_size - 1)) != 0)
@@ -379,7 +379,9 @@ int gqa_paged_split_first_launch(const void* q, const int64_t q_stride[4], const
                                  int max_seq_len, float* workspace, int splits, int batch, int num_heads,
                                  int num_kv_heads, int seq_q, int head_dim, float scale_log2, int causal, int dtype,
                                  void* stream) {
-  return paged_split_first_impl(q, q_stride, k_cache, k_cache_stride, v_cache, v_cache_stride, block_table, table_stride, seq_lens, q_start, q_len, block_size, max_seq_len, workspace, splits, batch, num_heads, num_kv_heads, seq_q, head_dim, scale_log2, causal, dtype, stream);
+  return paged_split_first_impl(q, q_stride, k_cache, k_cache_stride, v_cache, v_cache_stride, block_table,
+                                table_stride, seq_lens, q_start, q_len, block_size, max_seq_len, workspace, splits,
+                                batch, num_heads, num_kv_heads, seq_q, head_dim, scale_log2, causal, dtype, stream);
 }
 
 int gqa_paged_fwd_launch(const void* q, const int64_t q_stride[4], const void* k_cache,
@@ -603,10 +605,10 @@ size_t gqa_split_flat_workspace_bytes(int batch, int num_heads, int seq_q, int h
 
 namespace {
 
-int split_flat_impl(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
-                          const void* v, const int64_t v_stride[4], void* o, const int64_t o_stride[4], float* lse,
-                          float* workspace, int slots, int batch, int num_heads, int num_kv_heads, int seq_q,
-                          int seq_kv, int head_dim, float scale_log2, int causal, int dtype, void* stream, const gqa::ScoreMod* mod = nullptr) {
+int split_flat_impl(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4], const void* v,
+                    const int64_t v_stride[4], void* o, const int64_t o_stride[4], float* lse, float* workspace,
+                    int slots, int batch, int num_heads, int num_kv_heads, int seq_q, int seq_kv, int head_dim,
+                    float scale_log2, int causal, int dtype, void* stream, const gqa::ScoreMod* mod = nullptr) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, dtype);
   if (rc) return rc;
   if (slots < 1 || slots > GQA_MAX_SPLITS || seq_kv < 1) return GQA_E_FLAT;
@@ -641,7 +643,8 @@ int gqa_split_flat_launch(const void* q, const int64_t q_stride[4], const void* 
                           const void* v, const int64_t v_stride[4], void* o, const int64_t o_stride[4], float* lse,
                           float* workspace, int slots, int batch, int num_heads, int num_kv_heads, int seq_q,
                           int seq_kv, int head_dim, float scale_log2, int causal, int dtype, void* stream) {
-  return split_flat_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, slots, batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream);
+  return split_flat_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, slots, batch, num_heads,
+                         num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream);
 }
 
 }  // extern "C"
@@ -649,12 +652,12 @@ int gqa_split_flat_launch(const void* q, const int64_t q_stride[4], const void* 
 namespace {
 
 int paged_split_flat_impl(const void* q, const int64_t q_stride[4], const void* k_cache,
-                                const int64_t k_cache_stride[4], const void* v_cache,
-                                const int64_t v_cache_stride[4], const int* block_table, int table_stride,
-                                const int* seq_lens, const int* q_start, const int* q_len, int block_size,
-                                int max_seq_len, void* o, const int64_t o_stride[4], float* lse, float* workspace,
-                                int slots, int batch, int num_heads, int num_kv_heads, int seq_q, int head_dim,
-                                float scale_log2, int causal, int dtype, void* stream, const gqa::ScoreMod* mod = nullptr) {
+                          const int64_t k_cache_stride[4], const void* v_cache, const int64_t v_cache_stride[4],
+                          const int* block_table, int table_stride, const int* seq_lens, const int* q_start,
+                          const int* q_len, int block_size, int max_seq_len, void* o, const int64_t o_stride[4],
+                          float* lse, float* workspace, int slots, int batch, int num_heads, int num_kv_heads,
+                          int seq_q, int head_dim, float scale_log2, int causal, int dtype, void* stream,
+                          const gqa::ScoreMod* mod = nullptr) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, max_seq_len, head_dim, dtype);
   if (rc) return rc;
   if (block_size < 1 || block_size > GQA_MAX_BLOCK_SIZE || (block_size & (block_size - 1)) != 0)
@@ -701,7 +704,9 @@ int gqa_paged_split_flat_launch(const void* q, const int64_t q_stride[4], const 
                                 int max_seq_len, void* o, const int64_t o_stride[4], float* lse, float* workspace,
                                 int slots, int batch, int num_heads, int num_kv_heads, int seq_q, int head_dim,
                                 float scale_log2, int causal, int dtype, void* stream) {
-  return paged_split_flat_impl(q, q_stride, k_cache, k_cache_stride, v_cache, v_cache_stride, block_table, table_stride, seq_lens, q_start, q_len, block_size, max_seq_len, o, o_stride, lse, workspace, slots, batch, num_heads, num_kv_heads, seq_q, head_dim, scale_log2, causal, dtype, stream);
+  return paged_split_flat_impl(q, q_stride, k_cache, k_cache_stride, v_cache, v_cache_stride, block_table, table_stride,
+                               seq_lens, q_start, q_len, block_size, max_seq_len, o, o_stride, lse, workspace, slots,
+                               batch, num_heads, num_kv_heads, seq_q, head_dim, scale_log2, causal, dtype, stream);
 }
 
 int gqa_split_reduce_launch(const float* workspace, int splits, void* o, const int64_t o_stride[4], int batch,
@@ -721,11 +726,11 @@ int gqa_split_reduce_lse_launch(const float* workspace, int splits, void* o, con
 
 namespace {
 
-int fwd_chunks_impl(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4],
-                          const void* v, const int64_t v_stride[4], void* o, const int64_t o_stride[4], float* lse,
-                          float* workspace, int* counters, int kv_splits, int batch, int num_heads,
-                          int num_kv_heads, int seq_q, int seq_kv, int head_dim, float scale_log2, int causal,
-                          int dtype, void* stream, const gqa::ScoreMod* mod = nullptr) {
+int fwd_chunks_impl(const void* q, const int64_t q_stride[4], const void* k, const int64_t k_stride[4], const void* v,
+                    const int64_t v_stride[4], void* o, const int64_t o_stride[4], float* lse, float* workspace,
+                    int* counters, int kv_splits, int batch, int num_heads, int num_kv_heads, int seq_q, int seq_kv,
+                    int head_dim, float scale_log2, int causal, int dtype, void* stream,
+                    const gqa::ScoreMod* mod = nullptr) {
   int rc = check_dims(batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, dtype);
   if (rc) return rc;
   const int G = num_heads / num_kv_heads, block_rows = mod != nullptr ? gqa::kShortRows : gqa::kFwdRows;
@@ -772,7 +777,8 @@ int gqa_fwd_chunks_launch(const void* q, const int64_t q_stride[4], const void* 
                           float* workspace, int* counters, int kv_splits, int batch, int num_heads,
                           int num_kv_heads, int seq_q, int seq_kv, int head_dim, float scale_log2, int causal,
                           int dtype, void* stream) {
-  return fwd_chunks_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, counters, kv_splits, batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream);
+  return fwd_chunks_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, counters, kv_splits, batch,
+                         num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream);
 }
 
 int gqa_split_reduce_varlen_launch(const float* workspace, int splits, void* o, const int64_t o_stride[4],
@@ -1045,8 +1051,8 @@ int gqa_scored_launch(int form, const void* q, const int64_t q_stride[4], const 
                       seq_kv, head_dim, scale_log2, causal, dtype, stream, 0, nullptr, nullptr,
                       form == GQA_FORM_SHORT, &m);
     case GQA_FORM_CHUNKS:
-      return fwd_chunks_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, nullptr, parts, batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype,
-                             stream, &m);
+      return fwd_chunks_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, nullptr, parts, batch,
+                             num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream, &m);
     case GQA_FORM_FLAT:
       return split_flat_impl(q, q_stride, k, k_stride, v, v_stride, o, o_stride, lse, workspace, parts, batch,
                              num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale_log2, causal, dtype, stream, &m);

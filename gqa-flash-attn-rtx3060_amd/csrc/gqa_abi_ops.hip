@@ -75,7 +75,7 @@ int gqa_qk_norm_rope_launch(const void* q, const int64_t q_stride[4], const void
                             void* q_out, const int64_t q_out_stride[4], void* k_out, const int64_t k_out_stride[4],
                             const gqa_rope* rope, int batch, int num_heads, int num_kv_heads, int seq, int head_dim,
                             int dtype, void* stream) {
-  if (batch < 0 || seq < 0 || num_heads <= 0 || num_kv_heads <= 0 || (int64_t)batch * seq >= ((int64_t)1 << 31))
+  if (batch < 0 || seq < 0 || num_heads <= 0 || num_kv_heads <= 0 || (int64_t)batch * seq >= GQA_MAX_ROPE_TOKENS)
     return GQA_E_SHAPE;
   gqa::RopeParams p{};
   int rc = rope_params(rope, head_dim, dtype, (int64_t)batch * seq, p);
@@ -103,7 +103,7 @@ int gqa_qk_norm_rope_write_launch(const void* q, const int64_t q_stride[3], cons
                                   void* v_cache, const int64_t v_cache_stride[4], const int64_t* slot_mapping,
                                   const gqa_rope* rope, int num_tokens, int num_heads, int num_kv_heads, int head_dim,
                                   int block_size, int dtype, void* stream) {
-  if (num_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0) return GQA_E_SHAPE;
+  if (num_tokens < 0 || num_tokens >= GQA_MAX_ROPE_TOKENS || num_heads <= 0 || num_kv_heads <= 0) return GQA_E_SHAPE;
   if (bad_block(block_size)) return GQA_E_BLOCK;
   gqa::RopeParams p{};
   int rc = rope_params(rope, head_dim, dtype, num_tokens, p);
@@ -131,7 +131,7 @@ int gqa_qk_norm_rope_write_launch(const void* q, const int64_t q_stride[3], cons
 }
 
 int gqa_document_spans_launch(const int* ids, int64_t row_stride, int* lo, int* hi, int batch, int seq, void* stream) {
-  if (batch < 0 || seq < 0 || row_stride < 0) return GQA_E_SHAPE;
+  if (batch < 0 || seq < 0 || seq > (1 << 30) || row_stride < 0) return GQA_E_SHAPE;
   if (batch == 0 || seq == 0) return GQA_OK;
   if (ids == nullptr || lo == nullptr || hi == nullptr) return GQA_E_NULL;
   if (unaligned(ids, 3u) || unaligned(lo, 3u) || unaligned(hi, 3u)) return GQA_E_STRIDE;
@@ -155,7 +155,7 @@ int gqa_extend_tables_launch(int* block_tables, int64_t table_stride, int table_
   if (bad_block(block_size) || (int64_t)table_width * block_size >= ((int64_t)1 << 31) ||
       (int64_t)num_blocks * block_size >= ((int64_t)1 << 40))
     return GQA_E_BLOCK;
-  if ((int64_t)batch * table_width + num_tokens >= ((int64_t)1 << 39)) return GQA_E_SHAPE;
+  if ((int64_t)batch * table_width + num_tokens >= ((int64_t)1 << 31)) return GQA_E_SHAPE;  // (an item a thread)
   if (free_count == nullptr || new_free_count == nullptr || refused == nullptr || scratch == nullptr) return GQA_E_NULL;
   if (num_blocks > 0 && free_blocks == nullptr) return GQA_E_NULL;
   if (batch > 0 && (block_tables == nullptr || pool_lens == nullptr || query_lens == nullptr || seq_lens == nullptr ||

@@ -11,7 +11,8 @@ bool decode_kernel_fits(const SplitParams& p) {
   const bool flat = p.slots > 0;
   if (flat && (p.n_rblk != 1 || p.counters != nullptr)) return false;
   const int unit = decode_unit(D);
-  if (flat && ((int64_t)((p.dm.Skv + unit - 1) / unit) * p.dm.B + 1) * (p.slots + 1) >= ((int64_t)1 << 31)) return false;
+  if (flat && ((int64_t)((p.dm.Skv + unit - 1) / unit) * p.dm.B + 1) * (p.slots + 1) >= ((int64_t)1 << 31))
+    return false;
   // Head_dim 64: the 16-row first pass only (at most 16 packed rows per kv
   // head), in the two-launch form (no fused combine at that width).
   if (D == 64) {

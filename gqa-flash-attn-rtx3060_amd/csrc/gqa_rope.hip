@@ -145,7 +145,10 @@ __global__ __launch_bounds__(256) void gqa_rope_kernel(RopeParams p) {
       for (int i = 0; i < 8; ++i) {
         const int pair = 8 * (rot ? j : 0) + i;
         const int w = pair >> 4;
-        const uint32_t word = w == 0 ? p.pair_axis[0] : w == 1 ? p.pair_axis[1] : w == 2 ? p.pair_axis[2] : p.pair_axis[3];
+        const uint32_t word = w == 0   ? p.pair_axis[0]
+                              : w == 1 ? p.pair_axis[1]
+                              : w == 2 ? p.pair_axis[2]
+                                       : p.pair_axis[3];
         const uint32_t axis = (word >> (2 * (pair & 15))) & 3;
         const int64_t ps = axis == 0 ? p0 : axis == 1 ? p1 : axis == 2 ? p2 : p3;
         const f32x2 x = reinterpret_cast<const f32x2*>(line(ps))[pair];
@@ -227,7 +230,6 @@ hipError_t launch_rope(const RopeParams& in, int dtype, hipStream_t stream) {
   p.div_parts = make_fast_div((uint32_t)p.parts);
   p.div_s = make_fast_div((uint32_t)p.S);
   const int64_t waves = (int64_t)p.n_tokens * p.parts;
-  if (waves >= (int64_t)1 << 31) return hipErrorInvalidValue;
   const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
   if (dtype == 0) {
     if (p.D == 128) hipLaunchKernelGGL((gqa_rope_kernel<0, 128>), grid, block, 0, stream, p);

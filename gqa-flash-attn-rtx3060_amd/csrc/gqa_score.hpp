@@ -12,9 +12,10 @@
 // What bounds them is the number of vector instructions a score: three and a
 // half without changes (fma, exp2, sum, half a conversion), beside the matrix
 // products that they hide.  An instruction more costs 8192 causal tokens (G = 4,
-// head_dim 128) about 35 us of 470, exp2 and reciprocals like any other: five
+// head_dim 128) about 35 us of 460, exp2 and reciprocals like any other: five
 // instructions of a cap in place of the raw score 646 us, a polynomial tanh of
-// five and a half 663.
+// five and a half 663, the four below 594 (gqa_scored.hip: 925 TFLOP/s, the
+// vector unit 67 % busy, the matrix unit 43 %).
 //
 // So a usual cap takes four, by changing the unit:
 //   cap tanh(s / cap) = cap - 2 cap / (1 + exp(2 s / cap))
@@ -33,7 +34,8 @@
 namespace gqa {
 
 // Instances with changed scores carry their parameters in a type of their own.
-template <typename P> constexpr bool kHasMod = std::is_same<P, FwdModParams>::value || std::is_same<P, SplitModParams>::value;
+template <typename P>
+constexpr bool kHasMod = std::is_same<P, FwdModParams>::value || std::is_same<P, SplitModParams>::value;
 
 // The reference point stored with the partial of a row that saw no key: below
 // every score (so a real partial of the row outweighs it), finite (so the
@@ -148,7 +150,8 @@ __device__ __forceinline__ void mask_tile_span(f32x16 (&s)[2], int lim, int low)
 // Tile order: with a distance bias in causal order the last keys weigh most, so
 // the tiles are taken from the last one back and a row's reference point is
 // settled by its first tiles, where ascending tiles raise it again and again
-// (head slopes 2^-1/4 to 2^-8, 8192 tokens: AAAA us -> BBBB).  Place it of n tiles
+// (head slopes 2^-1/4 to 2^-8, 8192 tokens, head_dim 128, in the single pass of
+// gqa_fwd.hip's shape: 677 us -> 493).  Place it of n tiles
 // from tb on (places past the end stay there: their loads read zeros).
 __device__ __forceinline__ int tile_at(int tb, int n, int it, bool back) {
   return tb + (back && it < n ? n - 1 - it : it);

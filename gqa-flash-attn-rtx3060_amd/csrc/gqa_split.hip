@@ -314,7 +314,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       f32x16 s1[1] = {sc};
       cap_scores<16>(s1, p.mod);
       if (p.mod.slopes != nullptr)
-        row_t = bias_scores<16>(s1, slope, kb0 + 8 * hh - qpos, kb0 + 31 <= qpos_lo, [](int e) { return key_of(e, 0); });
+        row_t = bias_scores<16>(s1, slope, kb0 + 8 * hh - qpos, kb0 + 31 <= qpos_lo,
+                                [](int e) { return key_of(e, 0); });
       sc = s1[0];
     }
     // The last keys that this row, and every row of the block, sees.

@@ -393,7 +393,8 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_tables_step_kernel(TablesPar
     const int at = p.B > 0 ? i - s_start[b] : 0;
     if (p.B > 0 && at < s_new[b]) {
       pos = s_old[b] + at;
-      slot = ((int64_t)block_of(b, p.rows != nullptr ? p.rows[b] : b, pos >> p.block_shift) << p.block_shift) + (pos & mask);
+      const int r = p.rows != nullptr ? p.rows[b] : b;
+      slot = ((int64_t)block_of(b, r, pos >> p.block_shift) << p.block_shift) + (pos & mask);
     }
     p.slots[i] = slot;
     p.positions[i] = pos;
@@ -454,8 +455,10 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_release_kernel(ReleaseParams
     int r = -1, n = 0;
     if (b < p.B) {
       r = p.rows[b];
-      if (r >= 0 && r < p.n_rows && owns(p.scratch, r, b)) n = (min(max(p.lens[r], 0), p.width << p.block_shift) + mask) >> p.block_shift;
-      else r = -1;
+      if (r >= 0 && r < p.n_rows && owns(p.scratch, r, b))
+        n = (min(max(p.lens[r], 0), p.width << p.block_shift) + mask) >> p.block_shift;
+      else
+        r = -1;
     }
     int64_t total;
     const int64_t upto = block_scan(n, tmp, total);

@@ -324,7 +324,8 @@ bool optional_values(const py::handle& h, at::ScalarType type, int64_t rows, int
   const at::Tensor* t = plain(h);
   if (t == nullptr || t->scalar_type() != type || !t->is_contiguous() || t->get_device() != dev || t->requires_grad())
     return false;
-  if (rows < 0 ? t->dim() != 1 || t->size(0) != n : t->dim() != 2 || t->size(0) != rows || t->size(1) != n) return false;
+  if (rows < 0 ? t->dim() != 1 || t->size(0) != n : t->dim() != 2 || t->size(0) != rows || t->size(1) != n)
+    return false;
   out = t->data_ptr();
   return true;
 }
@@ -514,7 +515,8 @@ py::object paged_attn(const py::handle& hq, const py::handle& hkc, const py::han
   if (!read_changes(softcap, slopes, prefix, py::none(), py::none(), B, H, Sq, max_seq_len, causal, dev, ch) ||
       (ch.any && wants_grad({pq, pkc, pvc})))
     return py::none();
-  const auto found = g_plans.find(Key{ch.any ? 3 : 1, B, H, Hkv, Sq, max_seq_len, D, causal, dev, bs, interleaved, varlen});
+  const auto found =
+      g_plans.find(Key{ch.any ? 3 : 1, B, H, Hkv, Sq, max_seq_len, D, causal, dev, bs, interleaved, varlen});
   if (found == g_plans.end()) return py::none();
   const Plan p = found->second;
   if (p.kind == kShort && std::max(kc.stride(1), vc.stride(1)) >= ((int64_t)1 << 24)) return py::none();
@@ -574,8 +576,7 @@ py::object paged_attn(const py::handle& hq, const py::handle& hkc, const py::han
   void* op = out.data_ptr();
   if (ch.any) {
     const int rc = gqa_paged_scored_launch(p.kind, qp, qs, kp, ks, vp, vs, tp, ts, lp, qsp, qlp, bsz, ms, op, os, lse_p,
-                                           wsf, p.n, b, h, hkv, sq, d, sl2, c, dt, &ch.score,
-                                           stream);
+                                           wsf, p.n, b, h, hkv, sq, d, sl2, c, dt, &ch.score, stream);
     if (rc == GQA_E_FLAT || rc == GQA_E_SCORE) return py::none();
     check_rc(rc, "gqa_paged_scored_launch");
   } else if (p.kind == kFlat) {
@@ -656,7 +657,7 @@ py::object norm_rope(const py::handle& hq, const py::handle& hk, const py::handl
     return py::none();
   const int64_t D = q->size(-1), B = nd == 4 ? q->size(0) : 1, S = nd == 4 ? q->size(2) : q->size(0), Hq = q->size(1);
   if ((D != 64 && D != 128) || !(eps >= 0.0)) return py::none();
-  if (B * S == 0 || (k == nullptr && (write || !hwk.is_none() || !hko.is_none()))) return py::none();
+  if (B * S == 0 || B * S >= GQA_MAX_ROPE_TOKENS || (k == nullptr && (write || !hwk.is_none() || !hko.is_none()))) return py::none();
   if (k != nullptr &&
       (k->dim() != nd || k->scalar_type() != q->scalar_type() || k->get_device() != dev || k->size(-1) != D ||
        (nd == 4 ? k->size(0) != B || k->size(2) != S : k->size(0) != S) || !rows_ready(*k)))

@@ -830,11 +830,13 @@ def gqa_flash_attn(q, k, v, causal=True, *, return_lse=False, softcap=None, alib
     if changed:
         refuse_grad("gqa_flash_attn with changed scores", q, k, v, alibi_slopes)
         score = check_score(softcap, alibi_slopes, prefix_lens, documents, batch=batch, num_heads=num_heads,
-                            num_kv_heads=num_kv_heads, seq_q=seq_q, seq_kv=seq_kv, causal=bool(causal), scale=head_dim ** -0.5, device=q.device)
+                            num_kv_heads=num_kv_heads, seq_q=seq_q, seq_kv=seq_kv, causal=bool(causal),
+                            scale=head_dim ** -0.5, device=q.device)
         with torch.cuda.device(dev):
             route = _scored_route(q, k, v, causal, dev, documents is not None)
             host = _decode_host()
-            if host is not None and batch > 0 and seq_q > 0:
+            # (A route that these strides chose is not the shape's.)
+            if host is not None and batch > 0 and seq_q > 0 and not _far_rows(k, v):
                 host.set_plan([2, batch, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, int(bool(causal)), dev,
                                int(documents is not None), 0, 0],
                               _KIND_IDS[route.kind], route.fwd_split if route.kind == "single" else route.splits,
@@ -979,6 +981,11 @@ def scored_fine_split(batch: int, num_kv_heads: int, rows: int, seq_kv: int, cu_
     return fine, _cdiv(tiles, fine)
 
 
+def _far_rows(k, v) -> bool:
+    """Rows so far apart that 32-bit byte offsets cannot span the keys (as _launch)."""
+    return (k.shape[2] + 192) * max(k.stride(2), v.stride(2)) >= 1 << 30
+
+
 def _scored_route(q, k, v, causal, dev, spans) -> Route:
     """The route of a call with changed scores: few packed rows per kv head as
     choose_plan has them, others by scored_plan; with documents the single pass
@@ -987,7 +994,7 @@ def _scored_route(q, k, v, causal, dev, spans) -> Route:
     shape = (batch, num_heads, k.shape[1], seq_q, k.shape[2], _cu_count(dev), bool(causal), head_dim)
     if spans:
         return Route("single")
-    far = (k.shape[2] + 192) * max(k.stride(2), v.stride(2)) >= 1 << 30  # as _launch: 32-bit byte offsets
+    far = _far_rows(k, v)
     if num_heads // k.shape[1] * seq_q <= split_max_rows(head_dim):
         route = _plan_cached(*shape)
         if route.kind in ("split", "flat") and not far:

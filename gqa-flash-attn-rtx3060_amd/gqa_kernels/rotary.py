@@ -26,6 +26,7 @@ __all__ = ["RotaryTable", "qk_norm_rope", "qk_norm_rope_write"]
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 _MAX_AXES = 4
+_MAX_TOKENS = 1 << 26  # GQA_MAX_ROPE_TOKENS
 
 
 class RotaryTable:
@@ -210,8 +211,9 @@ def qk_norm_rope(q, k, positions, table: Optional[RotaryTable] = None, *, q_weig
             return _lib.strides(t)
         return _lib._i64x4(0, t.stride(1), t.stride(0), 1)
 
-    qi, ki = _ready(q), None if k is None else _ready(k)
     batch, seq = tokens if len(tokens) == 2 else (1, tokens[0])
+    assert batch * seq < _MAX_TOKENS, f"qk_norm_rope takes fewer than {_MAX_TOKENS} tokens"
+    qi, ki = _ready(q), None if k is None else _ready(k)
     _decode_host()  # (the native call from here on)
     with torch.cuda.device(q.device):
         _lib.check(_lib.load().gqa_qk_norm_rope_launch(
@@ -242,6 +244,7 @@ def qk_norm_rope_write(q, k, v, positions, table: Optional[RotaryTable], k_cache
     _check_qk(q, k, 3)
     assert v is not None and tuple(v.shape) == tuple(k.shape) and v.dtype == k.dtype and v.device == k.device
     assert k.shape[0] == q.shape[0], "q and k have different tokens"
+    assert q.shape[0] < _MAX_TOKENS, f"qk_norm_rope_write takes fewer than {_MAX_TOKENS} tokens"
     block_size = _check_cache(k_cache, v_cache)
     assert k_cache.shape[2] == k.shape[1] and k_cache.shape[3] == k.shape[2] and k_cache.dtype == k.dtype
     assert k_cache.device == q.device

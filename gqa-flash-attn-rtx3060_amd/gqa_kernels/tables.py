@@ -109,7 +109,8 @@ def extend_block_tables(block_tables, seq_lens, query_lens, free_blocks, free_co
     _decode_host()  # (the native call from here on)
     # One int32 allocation for the small outputs and the scratch.
     counts = [batch, batch, batch, num_tokens, 1, 1, n_rows + 2 * batch + 1]
-    seq, start, qlen, pos, left, refused, scratch = torch.empty(sum(counts), dtype=torch.int32, device=dev).split(counts)
+    seq, start, qlen, pos, left, refused, scratch = torch.empty(sum(counts), dtype=torch.int32,
+                                                                device=dev).split(counts)
     slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
     tables = torch.empty(batch, width, dtype=torch.int32, device=dev)
     with torch.cuda.device(dev):

@@ -566,7 +566,9 @@ typedef struct gqa_rope {
 
 /* q, k: (batch, heads, seq, head_dim) with element strides (last 1, rows
  * 16-byte aligned); q_out and k_out likewise, and may be q and k.  k and k_out
- * NULL: queries alone.  Token (b, s) is token b * seq + s of the positions. */
+ * NULL: queries alone.  Token (b, s) is token b * seq + s of the positions.
+ * Fewer than GQA_MAX_ROPE_TOKENS tokens, here and below (else GQA_E_SHAPE). */
+#define GQA_MAX_ROPE_TOKENS (1 << 26)
 int gqa_qk_norm_rope_launch(const void* q, const int64_t q_stride[4],
                             const void* k, const int64_t k_stride[4],
                             void* q_out, const int64_t q_out_stride[4],
@@ -591,7 +593,7 @@ int gqa_qk_norm_rope_write_launch(const void* q, const int64_t q_stride[3],
 
 /* lo, hi (batch, seq) <- the first token, and the first behind the last, of each
  * token's document: a run of equal ids in its row of ids (batch, seq; int32, rows
- * row_stride apart).  Tokens of negative ids (padding): [0, 0). */
+ * row_stride apart; seq at most 2^30).  Tokens of negative ids (padding): [0, 0). */
 int gqa_document_spans_launch(const int* ids, int64_t row_stride, int* lo, int* hi,
                               int batch, int seq, void* stream);
 
@@ -611,7 +613,8 @@ int gqa_document_spans_launch(const int* ids, int64_t row_stride, int* lo, int* 
  * the table's width, or the blocks that it and the requests before it need the
  * free list.  A negative row is an empty place, not counted in refused.
  * scratch: gqa_extend_tables_scratch_bytes bytes.  Calls that share a pool or a
- * scratch are ordered on one stream. */
+ * scratch are ordered on one stream.  batch * table_width + num_tokens below
+ * 2^31 (else GQA_E_SHAPE). */
 size_t gqa_extend_tables_scratch_bytes(int pool_rows, int batch);
 int gqa_extend_tables_launch(int* block_tables, int64_t table_stride, int table_width,
                              int* pool_lens, int pool_rows, const int* rows,

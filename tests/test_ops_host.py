@@ -5,7 +5,8 @@ import pytest
 import torch
 
 from gqa_kernels import RotaryTable, _lib, document_spans, qk_norm_rope
-from gqa_kernels.paged import BlockPool, extend_block_tables
+from gqa_kernels.dispatch import scored_fine_split
+from gqa_kernels.paged import BlockPool, extend_block_tables, scored_split
 from gqa_kernels.scores import DocumentSpans, check_score
 
 SHAPE, HEAD, DTYPE, STRIDE, SPLITS, NULL, BLOCK = -1, -2, -3, -4, -5, -7, -8
@@ -136,3 +137,34 @@ def test_rotary_table_values_and_checks():
         with pytest.raises(AssertionError):
             RotaryTable(**{**dict(head_dim=64, max_positions=4, device="cpu"), **kw})
     assert RotaryTable.sections((2, 1, 3)) == [0, 0, 1, 2, 2, 2]
+
+
+def test_sizes_past_what_a_launch_spans(lib):
+    def rope(write, tokens):
+        r = _lib.Rope(table=P, max_positions=10, rotary_dim=128, positions=P, axes=1)
+        t3 = _lib._i64x3(1024, 128, 1)
+        if write:
+            return lib.gqa_qk_norm_rope_write_launch(P, t3, P, t3, P, t3, P, t3, P, ST, P, ST, P, ctypes.byref(r),
+                                                     tokens, 8, 2, 128, 16, 0, None)
+        return lib.gqa_qk_norm_rope_launch(P, ST, P, ST, P, ST, P, ST, ctypes.byref(r), 1, 8, 2, tokens, 128, 0, None)
+
+    assert rope(False, 1 << 26) == SHAPE and rope(True, 1 << 26) == SHAPE
+    assert lib.gqa_document_spans_launch(P, 8, P, P, 1, (1 << 30) + 1, None) == SHAPE
+    wide = 1 << 20
+    assert lib.gqa_extend_tables_launch(P, wide, wide, P, 4096, P, P, P, P, 5, 16, 1, 2048, 2, P, P, P, P, P, P, P, P, P,
+                                        None) == SHAPE
+
+
+def test_scored_split_counts():
+    def split(B, ml, Hq=32, Hkv=8, Sq=1, D=128, block=16):
+        return scored_split(B, Hq, Hkv, Sq, ml, 256, block, D, True)
+
+    assert split(1, 1) == (0, 1) and split(1, 64) == (0, 1) and split(1, 700) == (0, 11) and split(1, 3000) == (0, 32)
+    assert split(1, 0)[0] == 0 and split(0, 700)[1] >= 1
+    assert split(32, 8000)[0] == 64  # two workgroups a compute unit
+    assert split(32, 8000, Sq=8)[0] in (0, 32)  # 32 rows: one
+    assert scored_fine_split(1, 8, 33, 700, 256, 128) == (0, 0) and scored_fine_split(1, 8, 17, 700, 256, 64) == (0, 0)
+    for B in (1, 3, 7, 40, 300):
+        for ml in (1, 65, 777, 5000, 100000):
+            slots, splits = split(B, ml)
+            assert 1 <= splits <= _lib.GQA_MAX_SPLITS and 0 <= slots <= _lib.GQA_MAX_SPLITS

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from gqa_kernels import document_spans, gqa_flash_attn
-from gqa_kernels.paged import GQAPagedAttention, PagedAttentionMetadata, paged_attention
+from gqa_kernels.paged import GQAPagedAttention, PagedAttentionMetadata, paged_attention, scored_split
 from ops_reference import attend64, check_attention
 
 pytestmark = pytest.mark.gpu
@@ -273,6 +273,38 @@ def test_paged(case, kind):
     for b, n in enumerate(lens):
         check_attention(o[b], lse[b], attend64(q[b], rows_of(kc, table[b], n), rows_of(vc, table[b], n), softcap=cap or 0.0, slopes=slopes,
                                                prefix=None if prefix is None else prefix[b]))
+
+
+@pytest.mark.parametrize("Hkv,D", [(8, 64), (4, 128)])
+def test_paged_long_flat_splits(Hkv, D):
+    """Unequal lengths, two slots of the flat split a compute unit."""
+    lens = [3600 if b == 3 else 1 + 171 * b for b in range(20)]
+    slots = scored_split(20, 2 * Hkv, Hkv, 1, 3600 if Hkv == 8 else 7000, 256, 16, D, True)[0]
+    assert slots == 512 // Hkv
+    q, kc, vc, table, sl = make_paged(lens if Hkv == 8 else [2 * n - 200 * (n == 3600) for n in lens], 2 * Hkv, Hkv, 1, D, 16, seed=5)
+    slopes = slopes_of(2 * Hkv)
+    o, lse = paged_attention(q, kc, vc, table, sl, True, return_lse=True, softcap=15.0, alibi_slopes=slopes)
+    for b, n in enumerate(sl.tolist()):
+        check_attention(o[b], lse[b], attend64(q[b], rows_of(kc, table[b], n), rows_of(vc, table[b], n), softcap=15.0,
+                                               slopes=slopes))
+
+
+@pytest.mark.parametrize("Sq", [1, 4])
+def test_rows_far_apart(Sq):
+    """K and V rows that 32-bit offsets cannot span, before and after calls of the same shape with rows close by."""
+    q, k, v = make(1, 8, 2, Sq, 300, 64, seed=6)
+    step = (1 << 30) // 492 // 8 * 8 + 8
+    base = torch.empty(2, 299 * step + 128, dtype=BF, device="cuda")
+    kf, vf = (t.as_strided((1, 2, 300, 64), (300 * step, 64, step, 1)) for t in base)
+    kf.copy_(k)
+    vf.copy_(v)
+    first = check(q, kf, vf, softcap=20.0)
+    near = check(q, k, v, softcap=20.0)
+    again = check(q, kf, vf, softcap=20.0)
+    assert torch.equal(first[0], again[0])
+    assert torch.equal(near[0], check(q, k, v, softcap=20.0)[0])
+    with pytest.raises(Exception, match="stride|aligned"):
+        gqa_flash_attn(q, kf, vf, documents=document_spans(torch.zeros(1, 300, dtype=torch.int32).cuda()))
 
 
 @pytest.mark.parametrize("route", ["split", "single", "chunks", "short"])
