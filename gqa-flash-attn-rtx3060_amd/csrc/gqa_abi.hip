@@ -512,7 +512,7 @@ int fused_impl(const void* q, const int64_t q_stride[4], const void* k, const in
 
 int reduce_impl(const float* workspace, int splits, void* o, const int64_t o_stride[4], float* lse, int batch,
                 int num_heads, int seq_q, int head_dim, int dtype, void* stream, const int* q_start = nullptr,
-                const int* q_len = nullptr);
+                const int* q_len = nullptr, bool scored_chunks = false);
 
 // A flat split (checked arguments): workspace as SplitParams::slots describes
 // it (acc, m, l, plan), first pass, then the combine unless the first pass
@@ -765,7 +765,8 @@ int fwd_chunks_impl(const void* q, const int64_t q_stride[4], const void* k, con
   hipStream_t st = static_cast<hipStream_t>(stream);
   rc = to_code(mod != nullptr ? gqa::launch_scored(p, dtype, st, *mod) : gqa::launch_fwd(p, dtype, st));
   if (rc) return rc;
-  return reduce_impl(workspace, kv_splits, o, o_stride, lse, batch, num_heads, seq_q, head_dim, dtype, stream);
+  return reduce_impl(workspace, kv_splits, o, o_stride, lse, batch, num_heads, seq_q, head_dim, dtype, stream, nullptr,
+                     nullptr, mod != nullptr);
 }
 
 }  // namespace
@@ -800,7 +801,7 @@ namespace {
 
 int reduce_impl(const float* workspace, int splits, void* o, const int64_t o_stride[4], float* lse, int batch,
                 int num_heads, int seq_q, int head_dim, int dtype, void* stream, const int* q_start,
-                const int* q_len) {
+                const int* q_len, bool scored_chunks) {
   if (batch < 0 || num_heads <= 0 || seq_q < 0) return GQA_E_SHAPE;
   if (head_dim != 64 && head_dim != 128) return GQA_E_HEAD_DIM;
   if (dtype != GQA_DTYPE_BF16 && dtype != GQA_DTYPE_FP16) return GQA_E_DTYPE;
@@ -824,7 +825,8 @@ int reduce_impl(const float* workspace, int splits, void* o, const int64_t o_str
   p.lse = lse;
   p.q_start = q_start;
   p.q_len = q_len;
-  return to_code(gqa::launch_split_reduce(p, dtype, static_cast<hipStream_t>(stream)));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return to_code(scored_chunks ? gqa::launch_scored_combine(p, dtype, st) : gqa::launch_split_reduce(p, dtype, st));
 }
 
 // The paged single pass (gqa_paged_fwd_launch) and, with kv_splits > 0, the
@@ -914,7 +916,7 @@ int paged_fwd_impl(const void* q, const int64_t q_stride[4], const void* k_cache
   rc = launch();
   if (rc) return rc;
   return reduce_impl(workspace, kv_splits, o, o_stride, lse, batch, num_heads, seq_q, head_dim, dtype, stream,
-                     q_start, q_len);
+                     q_start, q_len, mod != nullptr);
 }
 
 // ---------------------------------------------------------------------------

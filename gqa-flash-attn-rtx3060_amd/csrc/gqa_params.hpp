@@ -333,6 +333,8 @@ hipError_t launch_paged_fwd(const FwdParams& p, int dtype, hipStream_t stream);
 // Single pass with changed scores (gqa_scored.hip): contiguous or paged, over
 // key chunks with p.kv_splits > 0; kShortRows rows a block.
 hipError_t launch_scored(const FwdParams& p, int dtype, hipStream_t stream, const ScoreMod& mod);
+// The combine of its key chunks (partials without a sum hold no accumulators).
+hipError_t launch_scored_combine(const ReduceParams& p, int dtype, hipStream_t stream);
 // In the other launchers, `mod`: changed scores, or nullptr.
 // Single pass of short calls (gqa_short.hip): contiguous, or paged when
 // p.block_table is set; no split blocks, no key chunks.

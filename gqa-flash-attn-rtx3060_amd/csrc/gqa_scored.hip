@@ -95,6 +95,15 @@ __global__ __launch_bounds__(kScoredThreads) __attribute__((amdgpu_waves_per_eu(
     tb += skip;
     n = max(min(n - skip, p.kv_chunk_tiles), 0);
   }
+  // The chunk's partial of this lane's row, in the split workspace's layout.
+  const int64_t part = (((int64_t)b * dm.Hq + head) * dm.Sq + pos) * p.kv_splits + chunk;
+  if (KC && n == 0) {  // (no sum: the combine reads nothing else of it)
+    if (valid && hh == 0) {
+      p.ws_m[part] = kEmptyRef;
+      p.ws_l[part] = 0.f;
+    }
+    return;
+  }
   const bool back = p.mod.slopes != nullptr && dm.causal;
   auto tile_of = [&](int j) __attribute__((always_inline)) { return tile_at(tb, n, j, back); };
 
@@ -307,11 +316,9 @@ __global__ __launch_bounds__(kScoredThreads) __attribute__((amdgpu_waves_per_eu(
 
   const float l_tot = xhalf_sum(l_run);
   if constexpr (KC) {
-    // The chunk's partial of this lane's row, in the split workspace's layout.
-    // Lane (i, hh) holds dims 32 db + 8 j + 4 hh + 0..3 of it in acc[db][4 j ..].
+    // Lane (i, hh) holds dims 32 db + 8 j + 4 hh + 0..3 of its row in acc[db][4 j ..].
     if (!valid) return;
-    const int64_t row = (((int64_t)b * dm.Hq + head) * dm.Sq + pos) * p.kv_splits + chunk;
-    float* wa = p.ws_acc + row * D + 4 * hh;
+    float* wa = p.ws_acc + part * D + 4 * hh;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -319,8 +326,8 @@ __global__ __launch_bounds__(kScoredThreads) __attribute__((amdgpu_waves_per_eu(
         *reinterpret_cast<f32x4*>(wa + 32 * db + 8 * j) =
             f32x4{acc[db][4 * j], acc[db][4 * j + 1], acc[db][4 * j + 2], acc[db][4 * j + 3]};
     if (hh == 0) {
-      p.ws_m[row] = m_run == -__builtin_inff() ? kEmptyRef : log2_ref(p, m_run, c);
-      p.ws_l[row] = l_tot;
+      p.ws_m[part] = m_run == -__builtin_inff() ? kEmptyRef : log2_ref(p, m_run, c);
+      p.ws_l[part] = l_tot;
     }
     return;
   }
@@ -357,6 +364,110 @@ __global__ __launch_bounds__(kScoredThreads) __attribute__((amdgpu_waves_per_eu(
       *reinterpret_cast<u32x4*>(orow + 8 * cc) = x;
     }
   }
+}
+
+// Joins the key chunks' partials of each row: m* = max m_s, l = sum 2^(m_s - m*)
+// l_s, o = sum 2^(m_s - m*) acc_s / l, over the partials with a sum.  A row's D / 4
+// lanes take four columns each; NSG such groups share a row's chunks and meet in
+// LDS, 1024 / (D NSG) rows a workgroup.  Memory-bound: a group takes four chunks
+// at a time, and the accumulators of those with a sum.  Few chunks of many rows
+// want many rows a workgroup (gqa_split_reduce_kernel, one row a workgroup, / this,
+// us: 16000 rows of 4 chunks at head_dim 64 17.4 / 6.5, 32768 of 2 at head_dim 128
+// 23 / 9.8, 3.5 TB/s).
+template <int DT, int D, int NSG> __global__ __launch_bounds__(256) void gqa_scored_combine_kernel(ReduceParams p) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  constexpr int ND4 = D / 4, R = 256 / (ND4 * NSG), BATCH = 4;
+  const int t = threadIdx.x, d4 = t % ND4, sg = (t / ND4) % NSG, r = t / (ND4 * NSG);
+  const int row = xcd_remap(blockIdx.x, gridDim.x) * R + r;
+  const int bh = fast_div(row, p.div_sq.mul, p.div_sq.shift), pos = row - bh * p.Sq;
+  const int b = fast_div(bh, p.div_hq.mul, p.div_hq.shift), h = bh - b * p.Hq;
+  const bool varlen = p.q_len != nullptr;
+  const bool live = row < p.B * p.Hq * p.Sq && (!varlen || pos < p.q_len[b]);
+  const int S = live ? p.splits : 0;
+  const float* wm = p.ws_m + (int64_t)row * p.splits;
+  const float* wl = p.ws_l + (int64_t)row * p.splits;
+  const float* wa = p.ws_acc + (int64_t)row * p.splits * D + 4 * d4;
+  float m = kEmptyRef, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = sg; s0 < S; s0 += BATCH * NSG) {
+    float mv[BATCH], lv[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int s = s0 + k * NSG;
+      mv[k] = s < S ? wm[s] : kEmptyRef;
+      lv[k] = s < S ? wl[s] : 0.f;
+    }
+    f32x4 av[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      av[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (lv[k] != 0.f) av[k] = *reinterpret_cast<const f32x4*>(wa + (int64_t)(s0 + k * NSG) * D);
+    }
+    const float mb = fmaxf(fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])), m);
+    const float keep = fast_exp2(m - mb);
+    l *= keep;
+    o *= keep;
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const float a = fast_exp2(mv[k] - mb);
+      l += a * lv[k];
+      o += a * av[k];
+    }
+    m = mb;
+  }
+  if constexpr (NSG > 1) {
+    __shared__ float red_m[256], red_l[256];
+    __shared__ f32x4 red_o[256];
+    red_m[t] = m;
+    red_l[t] = l;
+    red_o[t] = o;
+    __syncthreads();
+    if (sg != 0) return;
+#pragma unroll
+    for (int k = 1; k < NSG; ++k) {
+      const int at = t + k * ND4;
+      const float mb = fmaxf(m, red_m[at]), a0 = fast_exp2(m - mb), a1 = fast_exp2(red_m[at] - mb);
+      l = l * a0 + red_l[at] * a1;
+      o = o * a0 + red_o[at] * a1;
+      m = mb;
+    }
+  }
+  if (!live) return;
+  const int64_t tok = varlen ? (int64_t)p.q_start[b] + pos : 0;
+  if (p.lse != nullptr && d4 == 0) p.lse[varlen ? tok * p.Hq + h : row] = (m + __log2f(l)) * kLn2;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;  // (a row that sees no key: zeros)
+  T* orow = static_cast<T*>(const_cast<void*>(p.o.ptr)) +
+            (varlen ? tok * p.o.ss + (int64_t)h * p.o.sh
+                    : (int64_t)b * p.o.sb + (int64_t)h * p.o.sh + (int64_t)pos * p.o.ss);
+  u32x2 x;
+  x[0] = E::pack2(o[0] * inv, o[1] * inv);
+  x[1] = E::pack2(o[2] * inv, o[3] * inv);
+  *reinterpret_cast<u32x2*>(orow + 4 * d4) = x;
+}
+
+template <int DT, int D> static hipError_t launch_combine_t(ReduceParams p, hipStream_t stream) {
+  const int64_t rows = (int64_t)p.B * p.Hq * p.Sq;
+  if (rows <= 0) return hipSuccess;
+  if (rows >= (int64_t)1 << 24) return hipErrorInvalidValue;
+  p.div_sq = make_fast_div((uint32_t)p.Sq);
+  p.div_hq = make_fast_div((uint32_t)p.Hq);
+  const auto grid = [&](int nsg) { return dim3((unsigned)((rows * (D / 4) * nsg + 255) / 256)); };
+  // (A thread's loop of chunks in at most two rounds of loads, up to one row a
+  // workgroup.)
+  constexpr int kMax = 1024 / D;
+  if (p.splits <= 8)
+    hipLaunchKernelGGL((gqa_scored_combine_kernel<DT, D, 1>), grid(1), dim3(256), 0, stream, p);
+  else if (p.splits <= 32)
+    hipLaunchKernelGGL((gqa_scored_combine_kernel<DT, D, 4>), grid(4), dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((gqa_scored_combine_kernel<DT, D, kMax>), grid(kMax), dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
+hipError_t launch_scored_combine(const ReduceParams& p, int dtype, hipStream_t stream) {
+  if (dtype == 0) return p.D == 128 ? launch_combine_t<0, 128>(p, stream) : launch_combine_t<0, 64>(p, stream);
+  return p.D == 128 ? launch_combine_t<1, 128>(p, stream) : launch_combine_t<1, 64>(p, stream);
 }
 
 template <int DT, int D, int PG> static hipError_t launch_scored_t(FwdModParams p, hipStream_t stream) {

@@ -191,17 +191,19 @@ COMBINE_BYTES_PER_US = 5.0e6
 CHUNK_PARTIAL_PASSES = 1.5
 
 # Changed scores (scores.py): run time in us of the single pass in 128-row
-# workgroups, two a CU (gqa_scored.hip), plain or over key chunks, and of the
-# short form with the same changes: base + the longest slot's sum of (item +
-# tiles x step), the step's time as _step_us has it; the combine: launch + rows
-# + partials.  Fitted to 34 prompts and chunks at each head_dim (64-4096 new
-# tokens, up to 16384 keys, 7-32 query heads, batches of 1-8, capped scores):
-# chunk forms within 8 % in the mean, the short one within 4 %.  The fastest of
-# the modelled times took 1.01 times the fastest measured in the mean, 1.20 at
-# worst (without the short form 1.04 and 1.5).
-SCORED_PASS_US = {128: (2.4, 3.9, 1.58, 2.35), 64: (2.4, 2.5, 1.23, 1.63)}
+# workgroups, two a CU (gqa_scored.hip), plain or over key chunks: base and the
+# longest of (a list of item + tiles x lo over two slots a CU), (all items and
+# tiles x hi, shared evenly) and, with more long items than CUs, (the longest one
+# at hi); hi is a step's time beside another workgroup's.  Of the short form with
+# the same changes: base + the longest slot's sum of (item + step x tiles / 2), as
+# _step_us has the step.  Of the combine: launch + partials.  Fitted to 162
+# prompts and chunks (48-4000 new tokens, up to 16384 keys, 2-64 query heads,
+# batches of 1-8, a quarter of them paged with unequal lengths, whose longest the
+# model knows): times within 10 % in the mean, and the fastest of the modelled
+# took 1.013 times the fastest measured in the mean, 1.14 at worst.
+SCORED_PASS_US = {128: (0.7, 5.8, 1.53, 1.88), 64: (2.7, 3.0, 1.07, 1.43)}
 SCORED_SHORT_US = {128: (3.5, 4.7, 2.15, 2.46), 64: (2.7, 3.8, 1.93, 1.96)}
-SCORED_COMBINE_US = {128: (3.5, 0.36e-3, 0.30e-6), 64: (4.0, 0.90e-3, 0.17e-6)}  # launch, per row, per byte
+SCORED_COMBINE_US = {128: (5.0, 0.237e-6), 64: (4.2, 0.206e-6)}  # launch, per byte
 
 # Route kinds as the native calls number them (gqa_host.cpp).
 _KIND_IDS = {"split": 0, "single": 1, "chunks": 2, "flat": 3, "short": 4}
@@ -907,12 +909,16 @@ def _native_scored(host, q, k, v, causal, return_lse, softcap, alibi_slopes, pre
                            alibi_slopes, prefix_lens, starts, ends)
 
 
-def _slots_us(model, runs, n_bh: int, slots: int, work: int, longest: int) -> float:
-    """base + the longest of `slots` slots' (item + tiles x step) sums; runs:
-    [tiles, count] of one (b, kv head) in the kernel's order."""
+def _scored_pass_us(model, runs, n_bh: int, cu_count: int) -> float:
+    """runs: [tiles, count] of one (b, kv head) in the kernel's order."""
     base, item, lo, hi = model
-    step = _step_us(lo, hi, work, longest, slots)
-    return base + _list_makespan([[item + step * t, n] for t, n in runs], n_bh, slots)
+    longest = max(t for t, _ in runs)
+    slots, live = 2 * cu_count, [(t, n * n_bh) for t, n in runs if t]
+    us = max(_list_makespan([[item + lo * t if t else 0.3, n] for t, n in runs], n_bh, slots),
+             sum((item + hi * t) * n for t, n in live) / slots)
+    if sum(n for t, n in live if t >= 0.75 * longest) > cu_count:
+        us = max(us, item + hi * longest)
+    return base + us
 
 
 @functools.lru_cache(maxsize=4096)
@@ -929,7 +935,6 @@ def scored_plan(batch: int, num_heads: int, num_kv_heads: int, seq_q: int, seq_k
         return Route("single", 1, n_mblk * n_bh)
     tiles = _fwd_block_tiles(n_mblk, block_m, seq_q, seq_kv, causal)
     order = tiles[::-1] if causal else tiles
-    work, slots = sum(tiles) * n_bh, 2 * cu_count
 
     def runs_of(items):
         runs = []
@@ -937,22 +942,21 @@ def scored_plan(batch: int, num_heads: int, num_kv_heads: int, seq_q: int, seq_k
             _push_run(runs, t, 1)
         return runs
 
-    best = _slots_us(SCORED_PASS_US[head_dim], runs_of(order), n_bh, slots, work, max(tiles))
-    route = Route("single", 1, n_mblk * n_bh)
+    whole, model = runs_of(order), SCORED_PASS_US[head_dim]
+    best, route = _scored_pass_us(model, whole, n_bh, cu_count), Route("single", 1, n_mblk * n_bh)
     # (Short: two tiles a step, one workgroup a CU; within what its models were fitted to.)
     if n_mblk * n_bh <= SHORT_MAX_WG_PER_CU * cu_count:
         base, item, lo, hi = SCORED_SHORT_US[head_dim]
-        step = _step_us(lo, hi, work, max(tiles), cu_count)
-        t = base + _list_makespan([[item + step * _cdiv(t, 2), n] for t, n in runs_of(order)], n_bh, cu_count)
+        step = _step_us(lo, hi, sum(tiles) * n_bh, max(tiles), cu_count)
+        t = base + _list_makespan([[item + step * _cdiv(t, 2), n] for t, n in whole], n_bh, cu_count)
         if t < best:
             best, route = t, Route("short", 1, n_mblk * n_bh)
-    launch, per_row, per_byte = SCORED_COMBINE_US[head_dim]
+    launch, per_byte = SCORED_COMBINE_US[head_dim]
     rows, s = batch * num_heads * seq_q, 2
-    while s <= _lib.GQA_MAX_SPLITS and _cdiv(_cdiv(seq_kv, FWD_TILE), s) >= 2 and n_mblk * n_bh * s <= 8 * slots:
+    while s <= _lib.GQA_MAX_SPLITS and _cdiv(_cdiv(seq_kv, FWD_TILE), s) >= 2 and n_mblk * n_bh * s <= 16 * cu_count:
         ct = _cdiv(_cdiv(seq_kv, FWD_TILE), s)
-        items = [max(0, min(t - c * ct, ct)) for c in range(s) for t in order]
-        t = _slots_us(SCORED_PASS_US[head_dim], runs_of(items), n_bh, slots, work, max(items))
-        t += launch + per_row * rows + per_byte * rows * s * (head_dim + 2) * 4
+        parts = runs_of(max(0, min(t - c * ct, ct)) for c in range(s) for t in order)
+        t = _scored_pass_us(model, parts, n_bh, cu_count) + launch + per_byte * rows * s * (head_dim + 2) * 4
         if t < best:
             best, route = t, Route("chunks", s, n_mblk * n_bh * s)
         s *= 2

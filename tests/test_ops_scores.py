@@ -381,3 +381,28 @@ def test_layer_with_changed_scores():
             want = attend64(qb, rows_of(kc, table[b], n), rows_of(vc, table[b], n), softcap=20.0, slopes=slopes, prefix=int(pre[b]))
             check_attention(o[t:t + qlens[b]].view(-1, Hq, D).transpose(0, 1), None, want)
             t += qlens[b]
+
+
+@pytest.mark.parametrize("chunks", [2, 8, 9, 32, 40])
+@pytest.mark.parametrize("D", [64, 128])
+def test_key_chunks_and_their_combine(chunks, D):
+    """Chunk counts on both sides of the combine's forms, chunks that no row sees, a sequence shorter than a chunk and one without keys."""
+    lens = [2600, 130, 0, 1999]
+    q, kc, vc, table, sl = make_paged(lens, 6, 2, 43, D, 16, seed=chunks)
+    slopes = slopes_of(6)
+    o, lse = paged_attention(q, kc, vc, table, sl, True, return_lse=True, softcap=15.0, alibi_slopes=slopes, route="chunks",
+                             splits=chunks)
+    for b, n in enumerate(lens):
+        check_attention(o[b], lse[b], attend64(q[b], rows_of(kc, table[b], n), rows_of(vc, table[b], n), softcap=15.0,
+                                               slopes=slopes))
+    start, qlens = [0, 43, 44, 44], [43, 1, 0, 20]
+    ints = lambda x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    tokens = torch.cat([q[b, :, :n].transpose(0, 1) for b, n in enumerate(qlens)] + [q[0, :, :2].transpose(0, 1)]).contiguous()
+    out = torch.full_like(tokens, 7.0)
+    o, lse = paged_attention(tokens, kc, vc, table, sl, True, query_start=ints(start), query_lens=ints(qlens), max_query_len=43,
+                             out=out, return_lse=True, softcap=15.0, alibi_slopes=slopes, route="chunks", splits=chunks)
+    for b, n in enumerate(lens):
+        a, e = start[b], start[b] + qlens[b]
+        check_attention(o[a:e].transpose(0, 1), lse[a:e].T, attend64(tokens[a:e].transpose(0, 1), rows_of(kc, table[b], n),
+                                                                     rows_of(vc, table[b], n), softcap=15.0, slopes=slopes))
+    assert (o[64:] == 7.0).all()
