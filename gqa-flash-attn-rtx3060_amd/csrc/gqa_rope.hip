@@ -13,7 +13,12 @@
 // Bound by memory: q, k (and v) are read once and written once.  D / 16 lanes
 // hold a (token, head) row, 16 values each, as the two 8-value chunks whose
 // pairs they rotate: no exchange but the sum of squares.  A wave takes rows of
-// one token, so its cos and sin stay in registers over the heads.
+// one token, so its cos and sin stay in registers over the heads.  Measured, bf16,
+// head_dim 128, 32/8 heads: 16384 tokens 72.4 us, 4.64 TB/s (a large copy reaches
+// 4.9-5.0); 5003 tokens of three axes into a paged cache 27.2 us, 4.53 TB/s; 64
+// tokens into it 3.2 us, bound by two dependent reads (position, table row), with
+// a token's rows over as many waves as 4096 allow.  A wave a token with its loads
+// where they are used: 87.5 and 9.3 us for the first and the last.
 #include <algorithm>
 #include <type_traits>
 

@@ -38,7 +38,8 @@ __device__ inline int64_t block_scan(int64_t x, int64_t* tmp, int64_t& total) {
 // A workgroup a row's kSpanChunk tokens, kSpanPer a thread.  The run that
 // reaches into them starts at the last change before them, the one that leaves
 // them ends at the first change behind; both are looked for a chunk at a time
-// (the chunk beside it holds them unless a document is longer than that).
+// (the chunk beside it holds them unless a document is longer than that).  2 x 8192
+// ids: 8 us, of barriers and dependent reads (bytes: 0.03 us).
 constexpr int kSpanPer = 4, kSpanChunk = kPlanThreads * kSpanPer;
 
 // Inclusive running maximum over the workgroup; kPlanThreads / 64 ints.
@@ -287,7 +288,9 @@ __global__ __launch_bounds__(256) void gqa_tables_expand_kernel(TablesParams p) 
 // the plan for itself (two dependent reads and two sums over the batch) and then
 // its share of the tokens and of the tables' rows; nothing that another
 // workgroup's plan reads is written (the pool's lengths and the free count move
-// on in a launch behind, gqa_tables_update_kernel).
+// on in a launch behind, gqa_tables_update_kernel).  Bound by that chain of reads,
+// not by its bytes: 256 requests of up to 8000 keys 5.9 us with the update (plan
+// and expansion in a launch each: 15.3), 41663 tokens of 48 prompts 7.1.
 constexpr int kStepMaxBatch = 2048, kStepMaxRows = 4096, kStepMaxTokens = 1 << 18;  // (48 KiB of LDS)
 
 __device__ inline int block_sum_scan(int x, int* tmp, int& total) {
