@@ -66,6 +66,7 @@ __global__ __launch_bounds__(kScoredThreads) __attribute__((amdgpu_waves_per_eu(
   const int w = xcd_remap(blockIdx.x, n_items * dm.Hkv * dm.B);
   int bh, mrank, chunk = 0;
   item_of(p, w, n_items, bh, mrank);
+  if (PAGED && p.xcd_heads > 1) bh = turned_pair(p, bh, mrank);
   if constexpr (KC) {
     chunk = fast_div(mrank, p.div_mblk.mul, p.div_mblk.shift);
     mrank -= chunk * p.n_mblk;

@@ -406,3 +406,14 @@ def test_key_chunks_and_their_combine(chunks, D):
         check_attention(o[a:e].transpose(0, 1), lse[a:e].T, attend64(tokens[a:e].transpose(0, 1), rows_of(kc, table[b], n),
                                                                      rows_of(vc, table[b], n), softcap=15.0, slopes=slopes))
     assert (o[64:] == 7.0).all()
+
+
+@pytest.mark.parametrize("B,Hkv", [(2, 8), (4, 8), (8, 4), (6, 4), (6, 8), (3, 8), (5, 8)])
+def test_batches_over_pages_of_every_dealing(B, Hkv):
+    """Pairs of (sequence, kv head) per compute die: 2, 4, 4, 3, 6, 3 and 5, each item once, in one pass and in chunks."""
+    lens = [40 + (977 * b) % 1100 for b in range(B)]
+    q, kc, vc, table, sl = make_paged(lens, 2 * Hkv, Hkv, 150, 64, 16, seed=B)
+    for route, splits in (("single", None), ("chunks", 3), (None, None)):
+        o, lse = paged_attention(q, kc, vc, table, sl, True, return_lse=True, softcap=15.0, route=route, splits=splits)
+        for b, n in enumerate(lens):
+            check_attention(o[b], lse[b], attend64(q[b], rows_of(kc, table[b], n), rows_of(vc, table[b], n), softcap=15.0))
