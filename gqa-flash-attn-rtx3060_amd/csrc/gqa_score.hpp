@@ -157,12 +157,13 @@ __device__ __forceinline__ int tile_at(int tb, int n, int it, bool back) {
   return tb + (back && it < n ? n - 1 - it : it);
 }
 
-// Dealt items (item_of) over pages: the pair that takes the place of `bh` among
+// Dealt items (item_of): the pair that takes the place of `bh` among
 // the XCD's idx-th items.  An XCD hands its workgroups to its four shader engines
 // in turn, whichever of them is free, so a sequence whose place has a period of
 // two or four stays on one engine, or two, and the long ones' engines run on while
 // the others idle; turned by one place a round it comes to all four.  4 x 256
-// tokens over 2000-9000 keys with a cap, in 3 chunks: 184 us -> 128, in 8 180 -> 144.
+// tokens over 2000-9000 keys with a cap, in 3 chunks: 184 us -> 128, in 8 180 -> 144;
+// documents in 2 x 8192 173 -> 169.5, 4 x 777 with prefixes 42.5 -> 42.
 __device__ __forceinline__ int turned_pair(const FwdParams& p, int bh, int idx) {
   if (p.xcd_heads & 1) return bh;  // (it comes to all of them by itself)
   const int x = bh & 7, at = (bh >> 3) + (p.xcd_heads & 2 ? idx >> 1 : idx);

@@ -11,7 +11,7 @@
 // the two wave groups of gqa_fwd.hip's workgroup wait for each other every phase.
 // Measured, us, gqa_fwd.hip's form with the same changes / this one: 8192 causal
 // tokens with a cap, head_dim 128 607 / 594, head_dim 64 500 / 406; with a distance
-// bias, head_dim 64 380 / 309; documents in 2 x 8192 tokens 208 / 173 (570 TFLOP/s
+// bias, head_dim 64 380 / 309; documents in 2 x 8192 tokens 208 / 170 (580 TFLOP/s
 // of visible pairs); 4 x 777 with a cap and a prefix 42.7 / 39.9; 500 tokens over
 // 6001 keys in 4 chunks 56.2 / 54.8.  Wave priorities by phase or by slot, a
 // workgroup started half a tile late and Q loaded ahead of the spans: all within
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(kScoredThreads) __attribute__((amdgpu_waves_per_eu(
   const int w = xcd_remap(blockIdx.x, n_items * dm.Hkv * dm.B);
   int bh, mrank, chunk = 0;
   item_of(p, w, n_items, bh, mrank);
-  if (PAGED && p.xcd_heads > 1) bh = turned_pair(p, bh, mrank);
+  if (p.xcd_heads > 1) bh = turned_pair(p, bh, mrank);
   if constexpr (KC) {
     chunk = fast_div(mrank, p.div_mblk.mul, p.div_mblk.shift);
     mrank -= chunk * p.n_mblk;
