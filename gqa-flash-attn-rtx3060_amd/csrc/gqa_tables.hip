@@ -288,9 +288,10 @@ __global__ __launch_bounds__(256) void gqa_tables_expand_kernel(TablesParams p) 
 // the plan for itself (two dependent reads and two sums over the batch) and then
 // its share of the tokens and of the tables' rows; nothing that another
 // workgroup's plan reads is written (the pool's lengths and the free count move
-// on in a launch behind, gqa_tables_update_kernel).  Bound by that chain of reads,
-// not by its bytes: 256 requests of up to 8000 keys 5.9 us with the update (plan
-// and expansion in a launch each: 15.3), 41663 tokens of 48 prompts 7.1.
+// on in a launch behind, gqa_tables_update_kernel; with one workgroup at its end).
+// Bound by that chain of reads, not by its bytes: 256 requests of up to 8000 keys
+// 5.9 us with the update (plan and expansion in a launch each: 15.3), 41663 tokens
+// of 48 prompts 7.1.
 constexpr int kStepMaxBatch = 2048, kStepMaxRows = 4096, kStepMaxTokens = 1 << 18;  // (48 KiB of LDS)
 
 __device__ inline int block_sum_scan(int x, int* tmp, int& total) {
@@ -418,6 +419,11 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_tables_step_kernel(TablesPar
       out[page] = x;
     }
   }
+  if (gridDim.x > 1 || !p.update) return;
+  // One workgroup, which has read all that its plan reads: the pool moves on here.
+  for (int b = t; b < p.B; b += kPlanThreads)
+    if (s_new[b] > 0) p.lens[p.rows != nullptr ? p.rows[b] : b] = s_old[b] + s_new[b];
+  if (t == 0) *p.free_count = have_free - s_taken;
 }
 
 // The pool moves on: lengths of the served requests, the free count.
@@ -430,11 +436,16 @@ __global__ __launch_bounds__(256) void gqa_tables_update_kernel(TablesParams p) 
 hipError_t launch_tables(const TablesParams& p, hipStream_t stream) {
   const int64_t entries = (int64_t)p.B * p.width;
   if (p.B <= kStepMaxBatch && p.n_rows <= kStepMaxRows && p.n_tokens < kStepMaxTokens && entries < (int64_t)1 << 30) {
-    // A table row a wave, a few thousand tokens a workgroup.
-    const int wgs = std::min(std::max({(p.B + 15) / 16, (p.n_tokens + 2047) / 2048, 1}), 256);
+    // A table row a wave, a few thousand tokens a workgroup.  Small steps that move
+    // the pool on: one workgroup, and no launch behind it (us on the GPU and on the
+    // host, several / one: 1-16 requests of 500 pages 6.0 and 8.8 / 4.8 and 6.0, 32 of
+    // them 6.2 and 8.8 / 6.5 and 5.8, 8 with 4096 tokens 5.2 and 8.9 / 4.4 and 5.9; more
+    // rows, 256 of 32 pages 5.1 / 8.6, or tokens, 8192 of 48 5.9 / 8.0, not).
+    int wgs = std::min(std::max({(p.B + 15) / 16, (p.n_tokens + 2047) / 2048, 1}), 256);
+    if (p.update && p.B <= 32 && p.n_tokens <= 4096 && entries <= 16 * kPlanThreads) wgs = 1;
     const size_t lds = sizeof(int) * (4 * (size_t)p.B + (p.rows != nullptr ? p.n_rows : 0));
     hipLaunchKernelGGL(gqa_tables_step_kernel, dim3(wgs), dim3(kPlanThreads), lds, stream, p);
-    if (p.update)
+    if (p.update && wgs > 1)
       hipLaunchKernelGGL(gqa_tables_update_kernel, dim3((p.B + 255) / 256 + (p.B == 0)), dim3(256), 0, stream, p);
     return hipGetLastError();
   }

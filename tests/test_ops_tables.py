@@ -211,3 +211,24 @@ def test_decode_loop_in_a_graph():
             qr, _ = qk_norm_rope(q[i, -1:], None, pos[-1:], rot, q_weight=w)
             want = attend64(qr.transpose(0, 1), kv[0][at].transpose(0, 1), kv[1][at].transpose(0, 1), softcap=20.0)
             check_attention(out[i].unsqueeze(1), None, want)
+
+
+@pytest.mark.parametrize("B,width,new", [(1, 600, 1), (31, 500, 3), (32, 512, 128), (32, 513, 1), (33, 100, 1), (32, 40, 129)])
+def test_sizes_around_one_workgroup(B, width, new):
+    """Steps on both sides of the form that moves the pool on in its only workgroup: three in a row, against the host."""
+    p = BlockPool(B * 30 + 7, 16, B + 3, width * 16)
+    rows = ints([(5 * b + 2) % (B + 3) for b in range(B)] if (B + 3) % 5 else list(range(B)))
+    for step in range(3):
+        table, lens = p.block_tables.tolist(), p.seq_lens.tolist()
+        free = p.free_blocks[:int(p.free_count)].tolist()
+        r = p.step(ints([new] * B), B * new, rows=rows)
+        slots, at = [], 0
+        for b, row in enumerate(rows.tolist()):
+            first, lens[row] = lens[row], lens[row] + new
+            for page in range(-(-first // 16), -(-lens[row] // 16)):
+                table[row][page] = free.pop()
+            slots += [table[row][i // 16] * 16 + i % 16 for i in range(first, lens[row])]
+        assert p.block_tables.tolist() == table and p.seq_lens.tolist() == lens
+        assert int(p.free_count) == len(free) == int(r.free_count) and int(r.refused) == 0
+        assert r.slot_mapping.tolist() == slots and r.seq_lens.tolist() == [lens[i] for i in rows.tolist()]
+        assert r.block_tables.tolist() == [table[i][:-(-lens[i] // 16)] + [0] * (width - -(-lens[i] // 16)) for i in rows.tolist()]
