@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from gqa_kernels import RotaryTable, _lib, document_spans, qk_norm_rope
-from gqa_kernels.dispatch import scored_fine_split
+from gqa_kernels.dispatch import _cu_count, _scored_route, scored_fine_split
 from gqa_kernels.paged import BlockPool, extend_block_tables, scored_split
 from gqa_kernels.scores import DocumentSpans, check_score
 
@@ -168,3 +168,21 @@ def test_scored_split_counts():
         for ml in (1, 65, 777, 5000, 100000):
             slots, splits = split(B, ml)
             assert 1 <= splits <= _lib.GQA_MAX_SPLITS and 0 <= slots <= _lib.GQA_MAX_SPLITS
+
+
+def test_scored_routes_of_few_rows():
+    def route(B, Skv, Hkv=8, G=4, Sq=1, D=128):
+        q, k = torch.empty(B, Hkv * G, Sq, D, device="meta"), torch.empty(B, Hkv, Skv, D, device="meta")
+        return _scored_route(q, k, k, True, 0, False)
+
+    _cu_count.cache_clear()
+    try:
+        with pytest.MonkeyPatch.context() as mp:
+            mp.setattr("gqa_kernels.dispatch._cu_count", lambda dev: 256)
+            assert (route(1, 700).kind, route(1, 700).splits) == ("split", 11)
+            assert (route(8, 300, Hkv=2).kind, route(8, 300, Hkv=2).splits) == ("split", 5)
+            for B, Skv in ((64, 300), (32, 64)):  # one launch: a slot a sequence
+                assert (route(B, Skv).kind, route(B, Skv).splits) == ("flat", B)
+            assert route(1, 3000, Sq=64).kind in ("single", "chunks", "short")
+    finally:
+        _cu_count.cache_clear()
