@@ -1,5 +1,6 @@
 """Attention with changed scores (softcap, distance bias, prefix and document masks) against float64, over contiguous and paged K/V."""
 import math
+import threading
 
 import pytest
 import torch
@@ -417,3 +418,33 @@ def test_batches_over_pages_of_every_dealing(B, Hkv):
         o, lse = paged_attention(q, kc, vc, table, sl, True, return_lse=True, softcap=15.0, route=route, splits=splits)
         for b, n in enumerate(lens):
             check_attention(o[b], lse[b], attend64(q[b], rows_of(kc, table[b], n), rows_of(vc, table[b], n), softcap=15.0))
+
+
+def test_two_threads_at_once():
+    """Calls of two threads, on one stream and on streams of their own: each as it is alone."""
+    shapes = [(1, 16, 4, 1, 3000, 128), (1, 16, 4, 130, 4000, 128)]
+    sl = slopes_of(16)
+    data = [make(*s, seed=30 + i) for i, s in enumerate(shapes)]
+    paged = make_paged([900, 2500], 16, 4, 1, 64, 16, seed=31)
+    calls = [lambda d=d: gqa_flash_attn(*d, softcap=20.0, alibi_slopes=sl, return_lse=True) for d in data]
+    calls.append(lambda: paged_attention(*paged, True, softcap=20.0, return_lse=True))
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    for own in (False, True):
+        bad, streams = [], [torch.cuda.Stream() for _ in range(2)]
+
+        def work(i):
+            with torch.cuda.stream(streams[i] if own else torch.cuda.default_stream()):
+                for n in range(60):
+                    k = (n + i) % len(calls)
+                    o, lse = calls[k]()
+                    if not (torch.equal(o, want[k][0]) and torch.equal(lse, want[k][1])):
+                        bad.append((own, i, n, k))
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert not bad
