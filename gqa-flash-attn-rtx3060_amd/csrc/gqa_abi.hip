@@ -993,10 +993,9 @@ namespace {
 // scale_log2 becomes the kernel's Dims::c.
 int score_mod(const gqa_score* score, float& scale_log2, int causal, bool paged, int seq_q, int seq_kv,
               gqa::ScoreMod& m) {
-  constexpr float kLog2e = 1.44269504088896340736f;
   if (score == nullptr) return GQA_E_NULL;
   m = gqa::ScoreMod{};
-  const float scale = scale_log2 / kLog2e;
+  const float scale = scale_log2 / gqa::kLog2e;
   if (!(scale > 0.f) || !std::isfinite(scale)) return GQA_E_SCORE;
   m.unit = 1.f / scale;
   if (score->softcap != 0.f) {
@@ -1004,10 +1003,10 @@ int score_mod(const gqa_score* score, float& scale_log2, int causal, bool paged,
     const float cap = score->softcap / scale;
     if (!(cap >= GQA_MIN_RAW_SOFTCAP && cap <= GQA_MAX_RAW_SOFTCAP)) return GQA_E_SCORE;
     if (score->softcap <= gqa::kUsualCap) {
-      m.cap_exp = 2.f * kLog2e / cap;
-      m.shift2 = score->softcap * kLog2e;
+      m.cap_exp = 2.f * gqa::kLog2e / cap;
+      m.shift2 = score->softcap * gqa::kLog2e;
       m.unit = 0.5f / score->softcap;
-      scale_log2 = 2.f * score->softcap * kLog2e;
+      scale_log2 = 2.f * score->softcap * gqa::kLog2e;
     } else {
       gqa::set_wide_cap(m, cap);
     }

@@ -176,9 +176,10 @@ struct ScoreMod {
   // nullptr: one document.  Contiguous K/V with Sq <= Skv only.
   const int* span_lo;
   const int* span_hi;
-  // Wide cap: tanh(x) = x (1 + u P(u)), u = x^2 = (s / cap)^2: P's coefficients for
-  // |s| up to lim3, their powers of 1 / cap folded in (set_wide_cap).
-  float wide_exp, lim3, p3[3];
+  // Wide cap: tanh(x) = x (1 + u P(u)), u = x^2 = (s / cap)^2: 1 / cap, and P's
+  // coefficients (kTanhP) for |s| up to lim3, their powers of 1 / cap folded in
+  // (set_wide_cap).
+  float inv_cap, lim3, p3[3];
 };
 
 // Packed query rows per single-pass workgroup (8 waves x 32 rows).
@@ -195,7 +196,7 @@ constexpr int kFwdPartFloats(int D) { return kFwdThreads * (D / 2 + 2); }
 constexpr int kFwdSchedCounters = 32;
 constexpr int kFwdDynMinItemsPerWg = 8;
 // ln(2): converts a log2-domain log-sum-exp to the natural-log LSE.
-constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kLn2 = 0.693147180559945309f, kLog2e = 1.44269504088896340736f;
 // Keys per single-pass LDS tile, and per split-KV LDS tile.
 constexpr int kFwdTileKeys = 64;
 constexpr int kSplitTileKeys = 128;
@@ -235,16 +236,18 @@ struct CacheWriteParams {
 // Softcaps up to this are usual ones: their form is off by 2^-22 of the softcap.
 constexpr float kUsualCap = 128.f;
 
-// A wide cap (in raw units) and its polynomial (a least-squares fit iterated to
-// equal ripple, of relative error 7e-8 on |x| <= 0.375).  The widest: up to where
-// the folded coefficients are normal numbers.
+// tanh(x) = x (1 + u P(u)), u = x^2, up to |x| = kTanhEnd (a least-squares fit
+// iterated to equal ripple, of relative error 7e-8).
+constexpr float kTanhEnd = 0.375f, kTanhP[3] = {-0.33332332968711853f, 0.1328972578048706f, -0.04848729446530342f};
+
+// A wide cap (in raw units).  The widest: lim3 up to where the folded coefficients
+// are normal numbers.
 inline void set_wide_cap(ScoreMod& m, float cap) {
-  constexpr double kP3[3] = {-0.33332332968711853, 0.1328972578048706, -0.04848729446530342};
   m.cap = cap;
-  m.wide_exp = 2.0f * 1.44269504088896340736f / cap;
-  m.lim3 = cap > 262144.f ? cap / 64.f : 0.375f * cap;
+  m.inv_cap = 1.0f / cap;
+  m.lim3 = cap > 262144.f ? cap / 64.f : kTanhEnd * cap;
   double f = 1.0;
-  for (int i = 0; i < 3; ++i) m.p3[i] = (float)(kP3[i] * (f /= (double)cap * cap));
+  for (int i = 0; i < 3; ++i) m.p3[i] = (float)(kTanhP[i] * (f /= (double)cap * cap));
 }
 
 struct FwdModParams : FwdParams {

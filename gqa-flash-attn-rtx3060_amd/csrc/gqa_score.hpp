@@ -52,8 +52,12 @@ __device__ __forceinline__ float vmax3_abs(float a, float b, float c) {
 // The scores of one tile are in W-wide register vectors (N * W a multiple of 8).
 //
 // s <- cap tanh(s / cap) for wide caps, where a rounding of the other form, 2^-22
-// of the cap, would be lost to scores far below it.  By the largest |s| of the
-// wave's tile: s (1 + u P(u)), u = s^2, or cap - 2 cap / (1 + exp(2 s / cap)).
+// of the cap, would be lost to scores far below it: s (1 + u P(u)), u = s^2, with the
+// cap's powers in P, if all of the wave's tile are within lim3; else score by
+// score that polynomial of s / cap up to its end, and cap - 2 cap / (1 + exp(2 s /
+// cap)) past it, where 2^-22 of the cap is 2^-20 of the value.  (By the tile's
+// largest score alone the second form would take that error to the ordinary rows
+// beside a row of large scores: 0.2 at softcap 8e6.)
 template <int W, typename V, int N>
 __device__ __forceinline__ void wide_cap_scores(V (&s)[N], const ScoreMod& m) {
   constexpr int E = N * W;
@@ -73,8 +77,11 @@ __device__ __forceinline__ void wide_cap_scores(V (&s)[N], const ScoreMod& m) {
   } else {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float x = fast_exp2(s[e / W][e % W] * m.wide_exp);
-      s[e / W][e % W] = __builtin_fmaf(-2.f * m.cap, __builtin_amdgcn_rcpf(1.f + x), m.cap);
+      const float x = s[e / W][e % W], y = x * m.inv_cap, u = y * y;
+      const float in = __builtin_fmaf(x * u, __builtin_fmaf(__builtin_fmaf(kTanhP[2], u, kTanhP[1]), u, kTanhP[0]), x);
+      const float ex = fast_exp2(y * (2.f * kLog2e));
+      const float out = __builtin_fmaf(-2.f * m.cap, __builtin_amdgcn_rcpf(1.f + ex), m.cap);
+      s[e / W][e % W] = __builtin_fabsf(y) <= kTanhEnd ? in : out;
     }
   }
 }
