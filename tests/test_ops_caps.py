@@ -98,8 +98,19 @@ def test_ordinary_rows_beside_rows_of_large_scores(cap, D):
     assert ((o[0].double() - o64).abs() <= tol)[:, rows].all() and ((lse[0].double() - l64).abs() <= ltol)[:, rows].all()
 
 
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("cap", [0.5, 5.0, 50.0, 128.0])
+def test_usual_caps_far_past_their_bend(shape, cap):
+    """Scores up to a thousand caps: tanh is 1 to the last bit."""
+    dtype = FP if cap == 50.0 else BF
+    q, k, v = whole_numbers(*shape, dtype, [cap / 128.0 * 2.0 ** e for e in (-1, 2, 4, 10)] if cap == 128.0 else [2.0 ** e for e in (-3, 0, 4, 9)],
+                            seed=5)
+    o, lse = gqa_flash_attn(q, k, v, return_lse=True, softcap=cap)
+    check(o, lse, q, k, v, cap)
+
+
 @pytest.mark.parametrize("route", ["split", "single", "chunks", "short", None])
-@pytest.mark.parametrize("cap", [2000.0, 1e6])
+@pytest.mark.parametrize("cap", [5.0, 2000.0, 1e6])
 def test_caps_over_pages(route, cap):
     lens, bs, D = [400, 37], 16, 128
     q, k, v = whole_numbers(2, 8, 2, 20, 400, D, BF, factors_of(max(cap, 200.0), D, BF), seed=7)
