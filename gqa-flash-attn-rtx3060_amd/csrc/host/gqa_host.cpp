@@ -395,7 +395,10 @@ py::object flash_attn(const py::handle& hq, const py::handle& hk, const py::hand
   const auto found = g_plans.find(Key{ch.any ? 2 : 0, B, Hq, Hkv, Sq, Skv, D, causal, dev, ch.spans});
   if (found == g_plans.end() || !rows_ready(q) || !rows_ready(k) || !rows_ready(v)) return py::none();
   const Plan p = found->second;
-  if (p.kind != kSingle && (Skv + 192) * std::max(k.stride(2), v.stride(2)) >= ((int64_t)1 << 30)) return py::none();
+  // (Rows too far apart for 32-bit byte offsets: not the shape's route, whatever it
+  // is.  Without changes the single pass is refused by its entry point.)
+  if ((ch.any || p.kind != kSingle) && (Skv + 192) * std::max(k.stride(2), v.stride(2)) >= ((int64_t)1 << 30))
+    return py::none();
   hipStream_t stream = c10::hip::getCurrentHIPStream(dev).stream();
 
   void *ws = nullptr, *cnt = nullptr;
