@@ -61,6 +61,13 @@ bool rows_fit_32bit(int seq_kv, const int64_t st[4]) {
   return ((int64_t)seq_kv + 192) * st[2] * 2 < ((int64_t)1 << 31);
 }
 
+// The single pass over pages: a descriptor's rows (64 of a tile, a wave's 16, an
+// instruction's 512 / D: issue_fwd_tile) at 32-bit byte offsets.
+bool page_rows_fit_32bit(int block_size, int head_dim, const int64_t st[4]) {
+  const int rows = block_size >= 64 ? 64 : block_size >= 16 ? 16 : 512 / head_dim;
+  return st[1] >= 0 && (int64_t)(rows - 1) * st[1] * 2 + 2 * head_dim < ((int64_t)1 << 32);
+}
+
 TensorRef ref(const void* ptr, const int64_t st[4]) { return TensorRef{ptr, st[0], st[1], st[2]}; }
 
 // A paged cache (num_blocks, block_size, heads, D) as the kernels address it:
@@ -83,8 +90,8 @@ const char* gqa_strerror(int code) {
     case GQA_E_HEAD_DIM: return "unsupported head_dim (supported: 64, 128)";
     case GQA_E_DTYPE: return "unsupported dtype (supported: bf16, fp16)";
     case GQA_E_STRIDE:
-      return "unsupported layout: last dim must be contiguous, rows 16-byte aligned, and one head's K/V rows "
-             "within 2 GiB";
+      return "unsupported layout: last dim must be contiguous, rows 16-byte aligned, one head's K/V rows within 2 GiB "
+             "and, in the single pass over pages, a page's rows of up to 64 keys within 4 GiB";
     case GQA_E_SPLITS:
       return "splits out of range [1, GQA_MAX_SPLITS], or a paged chunk spans more than "
              "GQA_PAGED_CHUNK_PAGES pages of under 64 keys";
@@ -869,6 +876,9 @@ int paged_fwd_impl(const void* q, const int64_t q_stride[4], const void* k_cache
     if (block_table == nullptr) return GQA_E_NULL;
     if ((reinterpret_cast<uintptr_t>(block_table) & 3u) != 0) return GQA_E_STRIDE;
     if ((rc = check_tensor(k_cache, k_cache_stride)) || (rc = check_tensor(v_cache, v_cache_stride))) return rc;
+    if (!page_rows_fit_32bit(block_size, head_dim, k_cache_stride) ||
+        !page_rows_fit_32bit(block_size, head_dim, v_cache_stride))
+      return GQA_E_STRIDE;
   }
 
   gqa::FwdParams p{};

@@ -438,7 +438,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
             paged_kv_chunks finds few query blocks against long sequences, and
             "short", the short form of the single pass, where paged_short
             finds it faster; all but "split" need block_size >= 512 /
-            head_dim).
+            head_dim, and up to 64 slots of a page within 4 GiB).
         query_start, query_lens, max_query_len: variable query lengths.  q
             is then token-major (num_tokens, num_heads, head_dim); sequence
             b's queries are tokens query_start[b] .. + query_lens[b] - 1

@@ -393,7 +393,9 @@ int gqa_paged_split_first_launch(const void* q, const int64_t q_stride[4],
  * the rows of one LDS-DMA instruction).  Caches, block_table, seq_lens,
  * max_seq_len and the causal alignment as gqa_paged_split_first_launch;
  * q and o are (batch, num_heads, seq_q, head_dim); lse may be NULL (no side
- * output) or as in gqa_fwd_lse_launch. */
+ * output) or as in gqa_fwd_lse_launch.  The slots that one load descriptor spans
+ * (64 of a page; 16 of pages of 16 or 32; 512 / head_dim of smaller ones) must lie
+ * within 4 GiB, else GQA_E_STRIDE, here and in its chunk, split and short forms. */
 int gqa_paged_fwd_launch(const void* q, const int64_t q_stride[4],
                          const void* k_cache, const int64_t k_cache_stride[4],
                          const void* v_cache, const int64_t v_cache_stride[4],

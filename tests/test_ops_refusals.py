@@ -1,0 +1,34 @@
+"""Calls around the attention that are refused before any HIP call (no GPU here)."""
+import ctypes
+
+import pytest
+
+from gqa_kernels import _lib
+
+SHAPE, STRIDE = -1, -4
+P = 0x10000  # an aligned address that is never read
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load()
+
+
+@pytest.mark.parametrize("scored", [False, True])
+@pytest.mark.parametrize("block,D,rows", [(64, 128, 64), (4096, 64, 64), (16, 128, 16), (32, 64, 16), (4, 128, 4), (8, 64, 8)])
+def test_slots_of_a_page_past_32_bit_offsets(lib, block, D, rows, scored):
+    """A descriptor's rows end past 4 GiB: the offsets would wrap and other keys be read."""
+    q_st = _lib._i64x4(8 * 64 * D, 64 * D, D, 1)
+    step = ((1 << 32) - 2 * D) // (2 * (rows - 1)) // 8 * 8 + 8
+    for k_step, v_step in ((step, D), (D, step), (1 << 40, D)):
+        kst, vst = (_lib._i64x4(1 << 20, s, D, 1) for s in (k_step, v_step))
+        common = (1, 8, 2, 4, D, 0.1, 1, 0)
+        head = (P, q_st, P, kst, P, vst, P, 8, P, None, None, block, 64 if block > 4 else 32, P, q_st, None)
+        if scored:
+            s = _lib.Score(softcap=10.0)
+            for form, parts, ws in ((1, 0, None), (2, 2, P), (4, 0, None)):
+                assert lib.gqa_paged_scored_launch(form, *head, ws, parts, *common, ctypes.byref(s), None) == STRIDE
+        else:
+            assert lib.gqa_paged_fwd_launch(*head, *common, None) == STRIDE
+            assert lib.gqa_paged_fwd_short_launch(*head, *common, None) == STRIDE
+            assert lib.gqa_paged_fwd_chunks_launch(*head, P, 2, *common, None) == STRIDE

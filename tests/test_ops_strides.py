@@ -3,7 +3,9 @@ import pytest
 import torch
 
 from gqa_kernels import gqa_flash_attn
+from gqa_kernels._lib import GQAError
 from gqa_kernels.dispatch import _scored_route
+from gqa_kernels.paged import paged_attention
 from ops_reference import attend64, check_attention
 
 pytestmark = pytest.mark.gpu
@@ -35,3 +37,33 @@ def test_a_call_does_not_depend_on_the_one_before(Hq, Hkv, Sq, Skv, D):
         if far:
             assert first is None or torch.equal(o, first)
             first = o
+
+
+@pytest.mark.parametrize("softcap", [None, 20.0])
+@pytest.mark.parametrize("route", ["single", "chunks"])
+def test_slots_far_apart_over_pages(route, softcap):
+    """64 slots of a page as far apart as 32-bit offsets reach; one step more is refused there, and taken by the split pass."""
+    bs, D, Hkv, Sq, lens = 64, 128, 2, 40, [130, 64]
+    most = ((1 << 32) - 2 * D - 2) // (63 * 2) // 8 * 8
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn(2, 8, Sq, D, generator=g).to(BF).cuda()
+    near = torch.randn(2, 5, bs, Hkv, D, generator=g).to(BF).cuda()
+    table = torch.tensor([[4, 0, 2], [1, 0, 0]], dtype=torch.int32).cuda()
+    sl = torch.tensor(lens, dtype=torch.int32).cuda()
+    call = lambda k, v, r: paged_attention(q, k, v, table, sl, True, softcap=softcap, route=r)  # noqa: E731
+    want = call(near[0], near[1], route)
+    for step in (most, most + 8):
+        far = [torch.empty(63 * step + 5 * Hkv * D, dtype=BF, device="cuda").as_strided((5, bs, Hkv, D), (Hkv * D, step, D, 1)) for _ in range(2)]
+        for f, x in zip(far, near):
+            f.copy_(x)
+        if step == most:
+            assert torch.equal(call(*far, route), want)
+        else:
+            with pytest.raises(GQAError, match="4 GiB"):
+                call(*far, route)
+        o = call(*far, "split")
+        for b, n in enumerate(lens):
+            k, v = (x[table[b].long()].reshape(-1, Hkv, D)[:n].transpose(0, 1) for x in near)
+            check_attention(o[b], None, attend64(q[b], k, v, softcap=softcap or 0.0))
+        del far, f
+
