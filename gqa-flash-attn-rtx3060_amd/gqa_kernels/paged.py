@@ -115,6 +115,7 @@ _LDS_WG_PER_CU = 1
 _LDS_WG_PER_CU_INTERLEAVED = 4
 _MIN_CHUNK = 256
 SCORED_SLOT_TILES = 32  # 64-key tiles a slot, scored_split
+SCORED_THREE_FILL = 0.7  # scored_paged_plan
 # Tile steps a piece of the flat split keeps, and steps that its ranges are
 # shorter than the fixed count's chunks (paged_flat_slots): head_dim 64,
 # head_dim 128 up to 16 packed rows, 17-32 rows.
@@ -284,6 +285,28 @@ def scored_split(batch: int, num_heads: int, num_kv_heads: int, seq_q: int, max_
             and batch * max_seq_len >= 64 * SCORED_SLOT_TILES * slots):
         slots *= 2
     return slots, splits
+
+
+@functools.lru_cache(maxsize=4096)
+def scored_paged_plan(batch: int, num_heads: int, num_kv_heads: int, seq_q: int, max_seq_len: int, cu_count: int,
+                      causal: bool = True, head_dim: int = 128) -> tuple:
+    """(route, key chunks or 0) of a paged single-pass call with changed scores.
+
+    scored_plan's, which counts chunks in powers of two and takes every sequence
+    for as long as the longest.  Where it says two, a batch takes three if they
+    still fit one round of workgroups, nearly (two fill up to SCORED_THREE_FILL of
+    the slots), or at head_dim 64.  Measured on MI355X (bf16, 464 batches drawn at
+    random, three chunks' time over two's in the mean and at the ends, equal /
+    unequal lengths): head_dim 128 up to there 0.90 (0.81-1.12) / 0.89 (0.75-1.16),
+    past it 1.10 (0.94-1.29) / 1.00 (0.74-1.29); head_dim 64 0.95 (0.79-1.07) /
+    0.94 (0.76-1.13)."""
+    planned = scored_plan(batch, num_heads, num_kv_heads, seq_q, max_seq_len, cu_count, causal, head_dim)
+    if planned.kind != "chunks":
+        return planned.kind, 0
+    if batch > 1 and planned.splits == 2 and (
+            head_dim == 64 or planned.workgroups <= SCORED_THREE_FILL * 2 * cu_count):
+        return "chunks", 3
+    return "chunks", planned.splits
 
 
 def _paged_host():
@@ -549,15 +572,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
         if short and max(k_cache.stride(1), v_cache.stride(1)) >= 1 << 24:
             short, plan_key = False, None
         if changed and route == "single":
-            planned = scored_plan(batch, num_heads, num_kv_heads, seq_q, max_seq_len, _cu_count(dev), bool(causal),
-                                  head_dim)
-            route, kv_chunks = planned.kind, planned.splits if planned.kind == "chunks" else 0
-            # Two chunks of the longest sequence, whose halves outlast what the
-            # others have: three (ten batches 0.80-1.25, 0.96 in the mean; 4 x 256
-            # tokens over 2000-9000 keys 161 -> 130 us, 8 x 256 over 2619-7659 140 ->
-            # 174).
-            if batch > 1 and kv_chunks == 2:
-                kv_chunks = 3
+            route, kv_chunks = scored_paged_plan(batch, num_heads, num_kv_heads, seq_q, max_seq_len, _cu_count(dev),
+                                                 bool(causal), head_dim)
             if route == "short" and max(k_cache.stride(1), v_cache.stride(1)) >= 1 << 24:
                 route, plan_key = "single", None
         elif short:
