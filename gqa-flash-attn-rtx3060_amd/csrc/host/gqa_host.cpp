@@ -316,13 +316,23 @@ void check_rc(int rc, const char* what) {
   if (rc != GQA_OK) raise_rc(rc, what);
 }
 
+// A tensor that carries a tangent of forward-mode differentiation.
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
+bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
+  const bool backward = at::GradMode::is_enabled();
+  for (const at::Tensor* t : ts)
+    if (t != nullptr && ((backward && t->requires_grad()) || has_tangent(*t))) return true;
+  return false;
+}
+
 // A contiguous 1-d tensor of n values (or 2-d, rows x n), or false; None gives
 // nullptr.
 bool optional_values(const py::handle& h, at::ScalarType type, int64_t rows, int64_t n, int64_t dev, const void*& out) {
   out = nullptr;
   if (h.is_none()) return true;
   const at::Tensor* t = plain(h);
-  if (t == nullptr || t->scalar_type() != type || !t->is_contiguous() || t->get_device() != dev || t->requires_grad())
+  if (t == nullptr || t->scalar_type() != type || !t->is_contiguous() || t->get_device() != dev || t->requires_grad() ||
+      has_tangent(*t))
     return false;
   if (rows < 0 ? t->dim() != 1 || t->size(0) != n : t->dim() != 2 || t->size(0) != rows || t->size(1) != n)
     return false;
@@ -353,13 +363,6 @@ bool read_changes(double softcap, const py::handle& slopes, const py::handle& pr
   c.score.span_hi = static_cast<const int*>(hi);
   return true;
 }
-bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const at::Tensor* t : ts)
-    if (t != nullptr && t->requires_grad()) return true;
-  return false;
-}
-
 // The workspace of a call with changed scores: the stream's, or (none large
 // enough, or a capture) one of its own.
 float* call_workspace(const py::dict& buffers, int64_t dev, hipStream_t stream, size_t bytes, const at::Tensor& like,

@@ -13,6 +13,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .gqa_split import _decode_host, stream_handle
@@ -20,11 +21,16 @@ from .gqa_split import _decode_host, stream_handle
 __all__ = ["DocumentSpans", "document_spans"]
 
 
+def _has_tangent(t) -> bool:
+    return forward_ad.unpack_dual(t).tangent is not None
+
+
 def refuse_grad(name: str, *tensors) -> None:
-    """There is no backward pass: better an error than outputs that silently
-    carry no gradient."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NotImplementedError(f"{name} has no backward pass: call it under torch.no_grad()")
+    """There is no backward pass, and none of forward mode: better an error than
+    outputs that silently carry no gradient or tangent."""
+    backward = torch.is_grad_enabled()
+    if any(t is not None and ((backward and t.requires_grad) or _has_tangent(t)) for t in tensors):
+        raise NotImplementedError(f"{name} has no derivative: call it under torch.no_grad(), on tensors without tangents")
 
 
 class DocumentSpans(NamedTuple):
