@@ -331,8 +331,7 @@ bool optional_values(const py::handle& h, at::ScalarType type, int64_t rows, int
   out = nullptr;
   if (h.is_none()) return true;
   const at::Tensor* t = plain(h);
-  if (t == nullptr || t->scalar_type() != type || !t->is_contiguous() || t->get_device() != dev || t->requires_grad() ||
-      has_tangent(*t))
+  if (t == nullptr || t->scalar_type() != type || !t->is_contiguous() || t->get_device() != dev || wants_grad({t}))
     return false;
   if (rows < 0 ? t->dim() != 1 || t->size(0) != n : t->dim() != 2 || t->size(0) != rows || t->size(1) != n)
     return false;

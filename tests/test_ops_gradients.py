@@ -56,3 +56,19 @@ def test_what_would_lose_a_derivative_is_refused(name, mode):
                     call(y)
             call(x)
     call(x)
+
+
+@pytest.mark.parametrize("name", ["flash", "paged"])
+def test_learned_slopes_take_the_native_calls_under_no_grad(name, monkeypatch):
+    _, call = calls()[name]
+    x = inputs()
+    x["slopes"].requires_grad_()
+    with torch.no_grad():
+        want = call(x)  # (plans the shape)
+
+        def never(*a, **k):
+            raise RuntimeError("the call went through Python's checks")
+
+        monkeypatch.setattr("gqa_kernels.dispatch.check_score", never)
+        monkeypatch.setattr("gqa_kernels.paged.check_score", never)
+        assert torch.equal(call(x), want)
