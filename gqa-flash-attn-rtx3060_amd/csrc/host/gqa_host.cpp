@@ -674,6 +674,7 @@ py::object norm_rope(const py::handle& hq, const py::handle& hk, const py::handl
     const py::tuple tt = py::reinterpret_borrow<py::tuple>(table);
     const at::Tensor& data = THPVariable_Unpack(tt[0].ptr());
     r = *reinterpret_cast<const gqa_rope*>(tt[1].cast<intptr_t>());
+    r.table = data.data_ptr<float>();
     const int64_t axes = tt[2].cast<int64_t>();  // (0: positions without an axis dimension)
     const at::Tensor* pos = plain(hpos);
     if (data.get_device() != dev || tt[3].cast<int64_t>() != D || pos == nullptr || pos->get_device() != dev ||

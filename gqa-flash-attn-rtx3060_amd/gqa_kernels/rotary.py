@@ -46,7 +46,8 @@ class RotaryTable:
             instead of base.
 
     ``table`` is float32 (max_positions, rotary_dim / 2, 2), pairs of (cos, sin)
-    rounded from float64.
+    rounded from float64.  The attributes are fixed; copies and pickles hold a table
+    of their own.
     """
 
     def __init__(self, head_dim: int, max_positions: int, base: float = 10000.0, rotary_dim: Optional[int] = None,
@@ -61,9 +62,6 @@ class RotaryTable:
             axes = [int(a) for a in axes]
             assert len(axes) == half, f"axes has {len(axes)} entries for {half} pairs"
             assert all(0 <= a < _MAX_AXES for a in axes), f"axes must be in [0, {_MAX_AXES})"
-        self.head_dim, self.rotary_dim, self.max_positions = head_dim, rotary_dim, int(max_positions)
-        self.interleaved, self.axes = bool(interleaved), axes
-        self.num_axes = 1 if axes is None else max(axes) + 1
         if inv_freq is None:
             assert base > 0
             inv = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
@@ -71,22 +69,35 @@ class RotaryTable:
             inv = torch.as_tensor(inv_freq, dtype=torch.float64).cpu()
             assert tuple(inv.shape) == (half,), f"inv_freq must hold {half} frequencies"
         inv = inv.to(device)
-        self.table = torch.empty(self.max_positions, half, 2, dtype=torch.float32, device=device)
-        for at in range(0, self.max_positions, 1 << 16):  # (bounds the float64 temporaries)
-            end = min(at + (1 << 16), self.max_positions)
+        max_positions = int(max_positions)
+        table = torch.empty(max_positions, half, 2, dtype=torch.float32, device=device)
+        for at in range(0, max_positions, 1 << 16):  # (bounds the float64 temporaries)
+            end = min(at + (1 << 16), max_positions)
             ang = torch.arange(at, end, dtype=torch.float64, device=device)[:, None] * inv
-            self.table[at:end, :, 0] = ang.cos()
-            self.table[at:end, :, 1] = ang.sin()
+            table[at:end, :, 0] = ang.cos()
+            table[at:end, :, 1] = ang.sin()
+        self.__setstate__(dict(table=table, head_dim=head_dim, interleaved=bool(interleaved), axes=axes))
+
+    def __setstate__(self, state):
+        table, axes = state["table"], state["axes"]
         words = [0, 0, 0, 0]
         for i, a in enumerate(axes or ()):
             words[i >> 4] |= a << (2 * (i & 15))
-        self._pair_axis = (ctypes.c_uint32 * 4)(*words)
         # For the native calls: the table, its gqa_rope, axes (0: positions
         # without an axis dimension), head_dim.
-        r = self._rope = _lib.Rope()
-        r.table, r.max_positions, r.rotary_dim = self.table.data_ptr(), self.max_positions, self.rotary_dim
-        r.interleaved, r.axes, r.pair_axis = int(self.interleaved), self.num_axes, self._pair_axis
-        self._native = (self.table, ctypes.addressof(r), 0 if axes is None else self.num_axes, head_dim)
+        r = _lib.Rope()
+        r.table, r.max_positions, r.rotary_dim = table.data_ptr(), table.shape[0], 2 * table.shape[1]
+        r.interleaved, r.axes = int(state["interleaved"]), 1 if axes is None else max(axes) + 1
+        r.pair_axis = (ctypes.c_uint32 * 4)(*words)
+        self.__dict__.update(state, max_positions=r.max_positions, rotary_dim=r.rotary_dim, num_axes=r.axes, _rope=r,
+                             _native=(table, ctypes.addressof(r), 0 if axes is None else r.axes, state["head_dim"]))
+
+    def __getstate__(self):
+        # (Copies and pickles: the gqa_rope is made anew, of the copy's own table.)
+        return {n: self.__dict__[n] for n in ("table", "head_dim", "interleaved", "axes")}
+
+    def __setattr__(self, name, value):
+        raise AttributeError("a RotaryTable's attributes are fixed: make another one, or write into its table")
 
     @staticmethod
     def sections(sizes: Sequence[int]) -> list:
@@ -133,7 +144,7 @@ def _rope(q, positions, table: Optional[RotaryTable], q_weight, k_weight, eps: f
         positions = positions.contiguous()
         keep.append(positions)
         r.table, r.max_positions, r.rotary_dim = table.table.data_ptr(), table.max_positions, table.rotary_dim
-        r.interleaved, r.axes, r.pair_axis = int(table.interleaved), table.num_axes, table._pair_axis
+        r.interleaved, r.axes, r.pair_axis = int(table.interleaved), table.num_axes, table._rope.pair_axis
         r.positions, r.positions64 = positions.data_ptr(), int(positions.dtype == torch.int64)
     assert (q_weight is None and k_weight is None) or eps >= 0
     w32 = None
