@@ -35,12 +35,17 @@ __device__ inline int64_t block_scan(int64_t x, int64_t* tmp, int64_t& total) {
 
 }  // namespace
 
-// A workgroup a row's kSpanChunk tokens, kSpanPer a thread.  The run that
-// reaches into them starts at the last change before them, the one that leaves
-// them ends at the first change behind; both are looked for a chunk at a time
-// (the chunk beside it holds them unless a document is longer than that).  2 x 8192
-// ids: 8 us, of barriers and dependent reads (bytes: 0.03 us).
-constexpr int kSpanPer = 4, kSpanChunk = kPlanThreads * kSpanPer;
+// A workgroup a row's kSpanChunk tokens, kSpanPer a thread.  The run that reaches
+// into them starts at the last change before them, the one that leaves them ends at
+// the first change behind.  In rows of up to kSpanWalk tokens both are looked for a
+// thread's width at a time (the chunk beside it holds them unless a document is
+// longer than that); in longer ones, where that would grow with the square of a
+// document, those ends are left open (kOpen) for a second launch.  Measured, us, one
+// launch / two, documents of 100 tokens and one of the whole row: 2 x 8192 ids 6.9,
+// 7.9 / 9.1, 9.8; 16384 7.3, 10.8 / 10.5, 11.8; 32768 7.4, 16.8 / 11.0, 11.9; 131072 7.5,
+// 52 / 11.8, 12.1; 2^20 9.3, 384 / 16.9, 14.4.  Bound by barriers and dependent reads
+// (bytes: 0.03 us for the first).
+constexpr int kSpanPer = 4, kSpanChunk = kPlanThreads * kSpanPer, kSpanWalk = 32768, kOpen = -1;
 
 // Inclusive running maximum over the workgroup; kPlanThreads / 64 ints.
 __device__ inline int block_max_scan(int x, int* tmp) {
@@ -60,7 +65,7 @@ __device__ inline int block_max_scan(int x, int* tmp) {
   return x;
 }
 
-__global__ __launch_bounds__(kPlanThreads) void gqa_spans_kernel(SpanParams p) {
+template <bool WALK> __global__ __launch_bounds__(kPlanThreads) void gqa_spans_kernel(SpanParams p) {
   __shared__ int s_id[kSpanChunk + 2], s_scan[kPlanThreads], tmp[kPlanThreads / 64], s_found;
   const int t = threadIdx.x;
   const int* ids = p.ids + blockIdx.y * p.stride;
@@ -73,33 +78,38 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_spans_kernel(SpanParams p) {
     s_id[i] = at >= 0 && at < p.S ? ids[at] : 0;
   }
   // The first change at or behind c1 (S: none), the last one at or before c0.
-  int behind = p.S, before = 0;
-  for (int a = c1; a < p.S; a += kPlanThreads) {
-    const int at = a + t;
-    if (t == 0) s_found = p.S;
-    __syncthreads();
-    if (at < p.S && ids[at] != ids[at - 1]) atomicMin(&s_found, at);
-    __syncthreads();
-    behind = s_found;
-    __syncthreads();
-    if (behind < p.S) break;
-  }
-  for (int a = c0; a > 0; a -= kPlanThreads) {
-    const int at = a - t;
-    if (t == 0) s_found = 0;
-    __syncthreads();
-    if (at > 0 && ids[at] != ids[at - 1]) atomicMax(&s_found, at);
-    __syncthreads();
-    before = s_found;
-    __syncthreads();
-    if (before > 0) break;
+  constexpr int kFar = 0x7fffffff;
+  int behind = p.S, before = kOpen;
+  if constexpr (WALK) {
+    for (int a = c1; a < p.S; a += kPlanThreads) {
+      const int at = a + t;
+      if (t == 0) s_found = p.S;
+      __syncthreads();
+      if (at < p.S && ids[at] != ids[at - 1]) atomicMin(&s_found, at);
+      __syncthreads();
+      behind = s_found;
+      __syncthreads();
+      if (behind < p.S) break;
+    }
+    before = 0;
+    for (int a = c0; a > 0; a -= kPlanThreads) {
+      const int at = a - t;
+      if (t == 0) s_found = 0;
+      __syncthreads();
+      if (at > 0 && ids[at] != ids[at - 1]) atomicMax(&s_found, at);
+      __syncthreads();
+      before = s_found;
+      __syncthreads();
+      if (before > 0) break;
+    }
   }
   __syncthreads();  // s_id
+  if constexpr (!WALK) behind = c1 == p.S || s_id[c1 - c0 + 1] != s_id[c1 - c0] ? c1 : kFar;
   // This thread's tokens a .. a + 3, and the changes among them.
   const int a = t * kSpanPer;
   int id[kSpanPer];
   bool change[kSpanPer];
-  int last = -1, first = 0x7fffffff;
+  int last = kOpen, first = kFar;
 #pragma unroll
   for (int i = 0; i < kSpanPer; ++i) {
     id[i] = a + i < c1 - c0 ? s_id[a + i + 1] : 0;
@@ -113,7 +123,7 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_spans_kernel(SpanParams p) {
   // round) of the negated first ones from the right.
   s_scan[t] = block_max_scan(last, tmp);
   __syncthreads();
-  int start = max(t > 0 ? s_scan[t - 1] : -1, before);
+  int start = max(t > 0 ? s_scan[t - 1] : kOpen, before);
   __syncthreads();
   s_scan[kPlanThreads - 1 - t] = -first;
   __syncthreads();
@@ -130,7 +140,7 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_spans_kernel(SpanParams p) {
   }
 #pragma unroll
   for (int i = kSpanPer - 1; i >= 0; --i) {
-    en[i] = id[i] < 0 ? 0 : end;
+    en[i] = id[i] < 0 ? 0 : end == kFar ? kOpen : end;
     if (change[i]) end = c0 + a + i;
   }
 #pragma unroll
@@ -141,6 +151,53 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_spans_kernel(SpanParams p) {
     }
 }
 
+// The open ends.  A run that enters a chunk starts where the run of the last token
+// of the nearest chunk before it does whose start is known: the chunks between are
+// that run from end to end (1024 of them looked at a round).  Other workgroups may
+// be filling theirs: what is read is open or right.
+__global__ __launch_bounds__(kPlanThreads) void gqa_spans_join_kernel(SpanParams p) {
+  __shared__ int s_near;
+  const int t = threadIdx.x, chunk = blockIdx.x, chunks = gridDim.x;
+  const int c0 = chunk * kSpanChunk, c1 = min(c0 + kSpanChunk, p.S);
+  int* lo = p.lo + (int64_t)blockIdx.y * p.S;
+  int* hi = p.hi + (int64_t)blockIdx.y * p.S;
+  const auto load = [](int* x) { return __hip_atomic_load(x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  const auto fill = [](int* x, int v) {
+    if (*x == kOpen) __hip_atomic_store(x, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  const bool open_lo = load(lo + c0) == kOpen, open_hi = load(hi + c1 - 1) == kOpen;
+  if (!open_lo && !open_hi) return;
+  int start = 0, end = 0;
+  for (int k0 = chunk - 1; open_lo && k0 >= 0; k0 -= kPlanThreads) {
+    const int k = k0 - t;
+    if (t == 0) s_near = -1;
+    __syncthreads();
+    if (k >= 0 && load(lo + (k + 1) * kSpanChunk - 1) != kOpen) atomicMax(&s_near, k);
+    __syncthreads();
+    const int near = s_near;
+    __syncthreads();
+    if (near < 0) continue;
+    start = load(lo + (near + 1) * kSpanChunk - 1);
+    break;
+  }
+  for (int k0 = chunk + 1; open_hi && k0 < chunks; k0 += kPlanThreads) {
+    const int k = k0 + t;
+    if (t == 0) s_near = chunks;
+    __syncthreads();
+    if (k < chunks && load(hi + k * kSpanChunk) != kOpen) atomicMin(&s_near, k);
+    __syncthreads();
+    const int near = s_near;
+    __syncthreads();
+    if (near == chunks) continue;
+    end = load(hi + near * kSpanChunk);
+    break;
+  }
+  for (int i = c0 + t; i < c1; i += kPlanThreads) {
+    if (open_lo) fill(lo + i, start);
+    if (open_hi) fill(hi + i, end);
+  }
+}
+
 hipError_t launch_spans(const SpanParams& p, hipStream_t stream) {
   if (p.B <= 0 || p.S <= 0) return hipSuccess;
   // (Rows in the grid's second dimension, at most 65535 a launch.)
@@ -149,8 +206,13 @@ hipError_t launch_spans(const SpanParams& p, hipStream_t stream) {
     q.ids += b * p.stride;
     q.lo += (int64_t)b * p.S;
     q.hi += (int64_t)b * p.S;
-    hipLaunchKernelGGL(gqa_spans_kernel, dim3((p.S + kSpanChunk - 1) / kSpanChunk, std::min(p.B - b, 65535)),
-                       dim3(kPlanThreads), 0, stream, q);
+    const dim3 grid((p.S + kSpanChunk - 1) / kSpanChunk, std::min(p.B - b, 65535));
+    if (p.S <= kSpanWalk) {
+      hipLaunchKernelGGL(gqa_spans_kernel<true>, grid, dim3(kPlanThreads), 0, stream, q);
+    } else {
+      hipLaunchKernelGGL(gqa_spans_kernel<false>, grid, dim3(kPlanThreads), 0, stream, q);
+      hipLaunchKernelGGL(gqa_spans_join_kernel, grid, dim3(kPlanThreads), 0, stream, q);
+    }
   }
   return hipGetLastError();
 }
