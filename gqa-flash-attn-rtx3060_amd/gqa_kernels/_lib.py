@@ -178,6 +178,12 @@ SIGNATURES = {
     ),
 }
 
+# Two launches over one workspace in a call, by default the stream's shared one:
+# they keep the interpreter's lock, so that a call of another thread on that stream
+# (native calls keep it too) cannot come in between and write over the partials.
+TWO_LAUNCHES = ("gqa_split_launch", "gqa_split_flat_launch", "gqa_fwd_chunks_launch", "gqa_paged_split_flat_launch",
+                "gqa_paged_fwd_chunks_launch")
+
 _lock = threading.Lock()
 _lib = None
 
@@ -199,7 +205,9 @@ def load() -> ctypes.CDLL:
                 f"{LIB_PATH} not found: build it with "
                 "`python gqa-flash-attn-rtx3060_amd/build.py` (or __graft_entry__.build())"
             )
-        lib = ctypes.CDLL(str(LIB_PATH))
+        lib, locked = ctypes.CDLL(str(LIB_PATH)), ctypes.PyDLL(str(LIB_PATH))
+        for name in TWO_LAUNCHES:
+            setattr(lib, name, getattr(locked, name))
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(lib, name)  # AttributeError if a symbol is missing
             fn.restype = res

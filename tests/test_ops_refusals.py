@@ -1,4 +1,4 @@
-"""Calls around the attention that are refused before any HIP call (no GPU here)."""
+"""What the C entry points refuse before any HIP call, and which of them keep the interpreter's lock (no GPU here)."""
 import ctypes
 
 import pytest
@@ -32,3 +32,12 @@ def test_slots_of_a_page_past_32_bit_offsets(lib, block, D, rows, scored):
             assert lib.gqa_paged_fwd_launch(*head, *common, None) == STRIDE
             assert lib.gqa_paged_fwd_short_launch(*head, *common, None) == STRIDE
             assert lib.gqa_paged_fwd_chunks_launch(*head, P, 2, *common, None) == STRIDE
+
+
+def test_two_launches_over_a_shared_workspace_keep_the_lock(lib):
+    """Another thread's call on the stream would write over the partials between the first pass and its combine."""
+    for name in ("gqa_fwd_chunks_launch", "gqa_split_launch", "gqa_split_flat_launch", "gqa_paged_fwd_chunks_launch",
+                 "gqa_paged_split_flat_launch"):
+        fn = getattr(lib, name)
+        assert fn._flags_ & ctypes._FUNCFLAG_PYTHONAPI and fn.argtypes == _lib.SIGNATURES[name][1], name
+    assert not lib.gqa_fwd_split_launch._flags_ & ctypes._FUNCFLAG_PYTHONAPI  # (one launch: others run)
