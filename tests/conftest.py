@@ -9,6 +9,8 @@ root (for ``oracle``) are put on sys.path so the tests import the drop-in as
 import sys
 from pathlib import Path
 
+import pytest
+
 REPO = Path(__file__).resolve().parent.parent
 PKG_DIR = REPO / "gqa-flash-attn-rtx3060_amd"
 for p in (str(PKG_DIR), str(REPO)):
@@ -18,3 +20,17 @@ for p in (str(PKG_DIR), str(REPO)):
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs an AMD GPU (MI355X) and the built HIP library")
+
+
+@pytest.fixture(autouse=True)
+def _streams_without_workspaces(request):
+    """A GPU test starts with no stream's workspace: torch hands out 32 streams in
+    turn, so a test's new stream may be one that a test before it has used."""
+    if request.node.get_closest_marker("gpu") is not None:
+        import torch
+        from gqa_kernels import gqa_split
+
+        if torch.cuda.is_available():
+            torch.cuda.synchronize()
+            gqa_split._workspaces.clear()
+    yield
