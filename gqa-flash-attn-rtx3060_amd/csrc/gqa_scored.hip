@@ -12,8 +12,9 @@
 // Measured, us, gqa_fwd.hip's form with the same changes / this one: 8192 causal
 // tokens with a cap, head_dim 128 607 / 594, head_dim 64 500 / 406; with a distance
 // bias, head_dim 64 380 / 309; documents in 2 x 8192 tokens 208 / 170 (580 TFLOP/s
-// of visible pairs); 4 x 777 with a cap and a prefix 42.7 / 39.9; 500 tokens over
-// 6001 keys in 4 chunks 56.2 / 54.8.  Wave priorities by phase or by slot, a
+// of visible pairs); 4 x 777 with a cap and a prefix 42.7 / 39.9; 2 x 500 tokens over
+// 6001 keys in 4 chunks at head_dim 64, joined by gqa_split_reduce_kernel, 56.2 / 54.8
+// (41-46 with the combine below).  Wave priorities by phase or by slot, a
 // workgroup started half a tile late and Q loaded ahead of the spans: all within
 // the noise of 2 %, or slower.
 //
@@ -33,8 +34,10 @@ namespace gqa {
 
 constexpr int kScoredThreads = 256;
 
-// KC: key chunks (FwdParams::kv_splits > 0), whose partials the split combine
-// joins.
+// KC: key chunks (FwdParams::kv_splits > 0), whose partials the combine below
+// joins.  Scores, sums and accumulators are fp32; P is rounded to the inputs' type for
+// its matrix product with V (half a step of each probability: outputs of bf16
+// prompts off by 2.2e-3 of their size against float64, with fp32 probabilities 1.66e-3).
 template <int DT, int D, int PG, bool KC>
 __global__ __launch_bounds__(kScoredThreads) __attribute__((amdgpu_waves_per_eu(2))) void gqa_scored_kernel(
     FwdModParams p) {

@@ -799,9 +799,11 @@ def gqa_flash_attn(q, k, v, causal=True, *, return_lse=False, softcap=None, alib
                 document only (needs seq_q <= seq_kv).
 
         With one of them a row that sees no key gives zeros and LSE -inf
-        (without: NaN, as the reference), and inputs that need a gradient are
-        refused.  V must be finite at hidden keys that share a 64-key tile with
-        a visible one.
+        (without: NaN, as the reference), and inputs that need a gradient or
+        carry a tangent are refused.  V must be finite at hidden keys that are
+        multiplied with a probability of zero: in the 64-key tiles of which a
+        query of the same block (up to 128 rows of queries and the group's
+        heads) sees a key, up to the last key that the block sees.
 
     Returns:
         (batch, num_heads, seq_q, head_dim), same dtype as q; with

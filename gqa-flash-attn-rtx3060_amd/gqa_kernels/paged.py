@@ -965,7 +965,9 @@ class GQAPagedAttention(torch.nn.Module):
     ``RotaryTable``), q_norm_weight, k_norm_weight, norm_eps: queries and keys are
     normed per head and rotated in the pass that stores K and V
     (``qk_norm_rope_write``, at ``attn_metadata.positions``); the caller's query
-    is not changed.
+    is not changed.  Slopes, weights given as plain tensors and the table are
+    kept as they are: ``.to()`` and ``state_dict`` pass them by (parameters
+    register as a module's).
     """
 
     def __init__(self, num_heads: int, head_size: int, scale: Optional[float] = None,

@@ -3,8 +3,10 @@ document masks (include/gqa_attn.h, gqa_scored_launch).
 
 The reference's attention has one score and one mask (reference
 gqa_kernels/dispatch.py:14-27).  Here ``gqa_flash_attn`` and
-``paged_attention`` take the changes of other models as keyword arguments; the
-kernels are the ones that run without them, in instances of their own.
+``paged_attention`` take the changes of other models as keyword arguments.  The
+split passes and the short form run in second instances of their kernels; the
+single pass, its key chunks and their combine are kernels of their own
+(csrc/gqa_scored.hip).
 """
 from __future__ import annotations
 

@@ -2,8 +2,8 @@
 
 ``PagedKVCache`` (paged.py) allocates blocks on the host and copies slots and
 tables to the device each step.  Here the pool itself — tables, lengths and the
-list of free blocks — lives on the device: a step is two small kernels, no copy
-and no wait, and can be captured in a HIP graph, whose replays then serve one
+list of free blocks — lives on the device: a step is one small kernel, or two (more
+than 32 requests), no copy and no wait, and can be captured in a HIP graph, whose replays then serve one
 token after another.  (No counterpart in the reference, whose README.md:140-146
 names a paged cache as its next step.)
 """

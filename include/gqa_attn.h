@@ -464,7 +464,9 @@ int gqa_paged_fwd_split_launch(const void* q, const int64_t q_stride[4],
  * span_hi[b, p].  A row without visible keys gives zeros and LSE -inf.
  * softcap 0 and NULL pointers leave a change out; the pointers are device
  * arrays, 4-byte aligned, contiguous.  V rows of hidden keys must be finite
- * (they are multiplied with a probability of zero), K rows may hold anything.
+ * (those in 64-key tiles of which a row of the same block sees a key, up to the
+ * block's last visible one, are multiplied with a probability of zero), K rows may
+ * hold anything.
  * GQA_E_SCORE: softcap / scale outside its range, scale_log2 not positive,
  * prefix_lens without causal, spans with paged caches, with seq_q > seq_kv or
  * with the split and flat forms, or an unknown form. */
