@@ -378,9 +378,21 @@ __device__ inline int block_sum_scan(int x, int* tmp, int& total) {
   return before + x;
 }
 
+// block_sum_scan of counts from 0 to 2^31 - 1, which may pass 32 bits together: a
+// wave that has one over 2^17 says -2^27 in place of its sum (the others' are 2^23 at
+// most), which makes the total negative, and the sums are made in 64.
+__device__ inline int64_t block_count_scan(int n, int* tmp, int64_t* tmp64, int64_t& total) {
+  const bool large = __builtin_amdgcn_ballot_w64(n > (1 << 17)) != 0;
+  int sum;
+  const int upto = block_sum_scan(large ? ((threadIdx.x & 63) == 0 ? -(1 << 27) : 0) : n, tmp, sum);
+  total = sum;
+  return __builtin_expect(sum < 0, 0) ? block_scan(n, tmp64, total) : upto;
+}
+
 __global__ __launch_bounds__(kPlanThreads) void gqa_tables_step_kernel(TablesParams p) {
   extern __shared__ int lds[];
   __shared__ int tmp[kPlanThreads / 64], s_refused, s_taken;
+  __shared__ int64_t tmp64[kPlanThreads / 64];
   int* s_start = lds;           // (B) first token
   int* s_old = s_start + p.B;   // (B) keys before
   int* s_new = s_old + p.B;     // (B) new tokens, 0 if refused
@@ -399,20 +411,22 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_tables_step_kernel(TablesPar
     }
   }
   __syncthreads();
-  int tokens = 0, blocks = 0;
+  int64_t tokens = 0;
+  int blocks = 0;
   for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
     const int b = b0 + t;
     int r = -1, fresh = 0, old = 0;
     bool fits = false;
     if (b < p.B) {
       r = p.rows != nullptr ? p.rows[b] : b;
-      fresh = min(max(p.new_lens[b], 0), p.n_tokens + 1);  // (more than there is room for is as good as one more)
+      fresh = max(p.new_lens[b], 0);
       fits = r >= 0 && r < p.n_rows && (p.rows == nullptr || owner[r] == b);
       old = fits ? min(max(p.lens[r], 0), p.width << p.block_shift) : 0;
     }
     int total;
-    const int upto = block_sum_scan(fresh, tmp, total) + tokens;
-    tokens = min(tokens + total, 1 << 30);
+    int64_t asked;
+    const int64_t upto = block_count_scan(fresh, tmp, tmp64, asked) + tokens;
+    tokens += asked;
     const int64_t len = (int64_t)old + fresh;
     fits = fits && len <= ((int64_t)p.width << p.block_shift) && upto <= p.n_tokens;
     const int pages = (old + mask) >> p.block_shift;
@@ -421,7 +435,7 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_tables_step_kernel(TablesPar
     blocks += total;
     const bool ok = fits && (need == 0 || bl <= have_free);
     if (b < p.B) {
-      s_start[b] = upto - fresh;
+      s_start[b] = (int)min(upto - fresh, (int64_t)0x7fffffff);
       s_old[b] = old;
       s_new[b] = ok ? fresh : 0;
       s_base[b] = bl - need;

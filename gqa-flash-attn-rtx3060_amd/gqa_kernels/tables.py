@@ -24,7 +24,8 @@ class StepTables(NamedTuple):
     for slot_mapping (int64).
 
     seq_lens (batch,): keys of each request, its new tokens included.
-    query_start, query_lens (batch,): its tokens (query_lens 0 if refused).
+    query_start, query_lens (batch,): its tokens, behind those of the requests
+        before it, refused ones included (query_lens 0 if refused).
     slot_mapping, positions (num_tokens,): each token's cache slot (-1: none)
         and position.
     block_tables (batch, width): the requests' pages in key order, 0 behind

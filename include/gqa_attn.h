@@ -607,7 +607,8 @@ int gqa_document_spans_launch(const int* ids, int64_t row_stride, int* lo, int* 
  * (rows table_stride apart, table_width entries).  New pages come from the top
  * of the free list (free_blocks[0 .. *free_count)), request by request, and are
  * entered in block_tables; with update != 0, pool_lens and *free_count move on
- * too.  Outputs: seq_lens (batch) keys after the step; query_start (batch);
+ * too.  Outputs: seq_lens (batch) keys after the step; query_start (batch), the sum
+ * of the counts before it, refused ones too (at most 2^31 - 1);
  * query_lens_out (batch), 0 for a refused request; slot_mapping and positions
  * (num_tokens): the tokens in request order, slot -1 and position 0 for tokens of
  * refused requests and behind the last; batch_tables (batch, table_width), 0
