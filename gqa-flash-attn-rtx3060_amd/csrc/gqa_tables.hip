@@ -43,8 +43,8 @@ __device__ inline int64_t block_scan(int64_t x, int64_t* tmp, int64_t& total) {
 // document, those ends are left open (kOpen) for a second launch.  Measured, us, one
 // launch / two, documents of 100 tokens and one of the whole row: 2 x 8192 ids 6.9,
 // 7.9 / 9.1, 9.8; 16384 7.3, 10.8 / 10.5, 11.8; 32768 7.4, 16.8 / 11.0, 11.9; 131072 7.5,
-// 52 / 11.8, 12.1; 2^20 9.3, 384 / 16.9, 14.4.  Bound by barriers and dependent reads
-// (bytes: 0.03 us for the first).
+// 52 / 11.8, 12.1; 2^20 9.3, 384 / 16.9, 14.4 (2^30 in one document 0.3 s).  Bound by
+// barriers and dependent reads (bytes: 0.03 us for the first).
 constexpr int kSpanPer = 4, kSpanChunk = kPlanThreads * kSpanPer, kSpanWalk = 32768, kOpen = -1;
 
 // Inclusive running maximum over the workgroup; kPlanThreads / 64 ints.
@@ -352,8 +352,8 @@ __global__ __launch_bounds__(256) void gqa_tables_expand_kernel(TablesParams p) 
 // workgroup's plan reads is written (the pool's lengths and the free count move
 // on in a launch behind, gqa_tables_update_kernel; with one workgroup at its end).
 // Bound by that chain of reads, not by its bytes: 256 requests of up to 8000 keys
-// as a plan 5.9 us (plan and expansion in a launch each: 15.3), 256 of 4000 keys with
-// the launch behind 6.7, 41663 tokens of 48 prompts as a plan 7.1.
+// as a plan 6.1 us (plan and expansion in a launch each: 15.3), 256 of 4000 keys with
+// the launch behind 6.9, 41663 tokens of 48 prompts as a plan 7.3.
 constexpr int kStepMaxBatch = 2048, kStepMaxRows = 4096, kStepMaxTokens = 1 << 18;  // (48 KiB of LDS)
 
 __device__ inline int block_sum_scan(int x, int* tmp, int& total) {
