@@ -34,7 +34,8 @@ using gqa::TensorRef;
 // short calls).
 // 16: changed scores (gqa_scored_launch, gqa_paged_scored_launch), norms and
 // rotation, document spans, block tables (gqa_abi_ops.hip).
-constexpr int kAbiVersion = 16;
+// 17: the paged cache in 8 bits (gqa_abi_cache8.hip).
+constexpr int kAbiVersion = 17;
 
 int check_dims(int B, int Hq, int Hkv, int Sq, int Skv, int D, int dtype) {
   if (B < 0 || Hq <= 0 || Hkv <= 0 || Sq < 0 || Skv < 0) return GQA_E_SHAPE;
@@ -114,6 +115,9 @@ const char* gqa_strerror(int code) {
     case GQA_E_ROPE:
       return "rotation: rotary_dim must be a multiple of 16 up to head_dim, axes in [1, 4] and every pair's below it, "
              "max_positions positive, eps not negative";
+    case GQA_E_CACHE8:
+      return "paged cache in 8 bits: block_size must be a power of two from 16 on, page rows 16-byte aligned and 16 of "
+             "them within 2 GiB, the scale positive and finite, the form one of those that gqa_paged8_plan gives";
     default: break;
   }
   if (code > 0) return hipGetErrorString(static_cast<hipError_t>(code));
@@ -997,28 +1001,26 @@ int gqa_split_noalloc_launch(const void* q, const int64_t q_stride[4], const voi
 // ---------------------------------------------------------------------------
 // Changed scores
 // ---------------------------------------------------------------------------
-namespace {
+namespace gqa {
 
-// The kernels' parameters of `score`; scale = scale_log2 / log2(e).
-// scale_log2 becomes the kernel's Dims::c.
-int score_mod(const gqa_score* score, float& scale_log2, int causal, bool paged, int seq_q, int seq_kv,
-              gqa::ScoreMod& m) {
+// scale = scale_log2 / log2(e).
+int score_mod(const gqa_score* score, float& scale_log2, int causal, bool paged, int seq_q, int seq_kv, ScoreMod& m) {
   if (score == nullptr) return GQA_E_NULL;
-  m = gqa::ScoreMod{};
-  const float scale = scale_log2 / gqa::kLog2e;
+  m = ScoreMod{};
+  const float scale = scale_log2 / kLog2e;
   if (!(scale > 0.f) || !std::isfinite(scale)) return GQA_E_SCORE;
   m.unit = 1.f / scale;
   if (score->softcap != 0.f) {
     if (!(score->softcap > 0.f)) return GQA_E_SCORE;
     const float cap = score->softcap / scale;
     if (!(cap >= GQA_MIN_RAW_SOFTCAP && cap <= GQA_MAX_RAW_SOFTCAP)) return GQA_E_SCORE;
-    if (score->softcap <= gqa::kUsualCap) {
-      m.cap_exp = 2.f * gqa::kLog2e / cap;
-      m.shift2 = score->softcap * gqa::kLog2e;
+    if (score->softcap <= kUsualCap) {
+      m.cap_exp = 2.f * kLog2e / cap;
+      m.shift2 = score->softcap * kLog2e;
       m.unit = 0.5f / score->softcap;
-      scale_log2 = 2.f * score->softcap * gqa::kLog2e;
+      scale_log2 = 2.f * score->softcap * kLog2e;
     } else {
-      gqa::set_wide_cap(m, cap);
+      set_wide_cap(m, cap);
     }
   }
   if (((reinterpret_cast<uintptr_t>(score->alibi_slopes) | reinterpret_cast<uintptr_t>(score->prefix_lens) |
@@ -1035,7 +1037,7 @@ int score_mod(const gqa_score* score, float& scale_log2, int causal, bool paged,
   return GQA_OK;
 }
 
-}  // namespace
+}  // namespace gqa
 
 extern "C" {
 
@@ -1045,7 +1047,7 @@ int gqa_scored_launch(int form, const void* q, const int64_t q_stride[4], const 
                       int seq_q, int seq_kv, int head_dim, float scale_log2, int causal, int dtype,
                       const gqa_score* score, void* stream) {
   gqa::ScoreMod m;
-  int rc = score_mod(score, scale_log2, causal, false, seq_q, seq_kv, m);
+  int rc = gqa::score_mod(score, scale_log2, causal, false, seq_q, seq_kv, m);
   if (rc) return rc;
   if ((reinterpret_cast<uintptr_t>(lse) & 3u) != 0) return GQA_E_STRIDE;
   if (m.span_lo != nullptr && (form == GQA_FORM_SPLIT || form == GQA_FORM_FLAT)) return GQA_E_SCORE;
@@ -1079,7 +1081,7 @@ int gqa_paged_scored_launch(int form, const void* q, const int64_t q_stride[4], 
                             int num_kv_heads, int seq_q, int head_dim, float scale_log2, int causal, int dtype,
                             const gqa_score* score, void* stream) {
   gqa::ScoreMod m;
-  int rc = score_mod(score, scale_log2, causal, true, seq_q, max_seq_len, m);
+  int rc = gqa::score_mod(score, scale_log2, causal, true, seq_q, max_seq_len, m);
   if (rc) return rc;
   if ((reinterpret_cast<uintptr_t>(lse) & 3u) != 0) return GQA_E_STRIDE;
   switch (form) {

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+struct gqa_score;
+
 namespace gqa {
 
 // Strides are in elements; the head_dim stride is 1 (checked by the ABI).
@@ -250,11 +252,31 @@ inline void set_wide_cap(ScoreMod& m, float cap) {
   for (int i = 0; i < 3; ++i) m.p3[i] = (float)(kTanhP[i] * (f /= (double)cap * cap));
 }
 
+// The kernels' parameters of `score`, checked; scale_log2 becomes the kernel's
+// Dims::c (gqa_abi.hip).
+int score_mod(const gqa_score* score, float& scale_log2, int causal, bool paged, int seq_q, int seq_kv, ScoreMod& m);
+
 struct FwdModParams : FwdParams {
   ScoreMod mod;
 };
 struct SplitModParams : SplitParams {
   ScoreMod mod;
+};
+
+// A paged cache in 8 bits (gqa_cache8.hpp): k and v of the base are its e4m3 codes,
+// strides in bytes; a page and kv head's codes stand for their value times 2^e, e
+// of ke or ve at page * sb + head * sh.
+struct Exponents {
+  int* e;
+  int64_t sb, sh;
+};
+struct Split8Params : SplitParams {
+  ScoreMod mod;
+  Exponents ke, ve;
+};
+struct Fwd8Params : FwdParams {
+  ScoreMod mod;
+  Exponents ke, ve;
 };
 
 // Per-head norm and rotation of queries and keys (gqa_rope.hip); with kc.ptr
@@ -276,6 +298,25 @@ struct RopeParams {
   // by S.
   int parts;
   FastDiv div_parts, div_s;
+};
+
+// The same into a paged cache in 8 bits, whose strides are in bytes
+// (gqa_cache8.hip); q may have no pointer.
+struct Store8Params : RopeParams {
+  Exponents ke, ve;
+  float limit;    // stored values are kept within it
+  // Set by the launcher: tokens and workgroups of a key or value task, heads of a
+  // workgroup (a power of two), head groups; workgroups of keys and values.
+  int chunk, n_chunks, head_shift, n_groups, n_kv;
+};
+
+// Rows of a paged cache in 8 bits back to 16 (gqa_cache8.hip).
+struct Read8Params {
+  TensorRef kc, vc;  // as CacheWriteParams, strides in bytes
+  Exponents ke, ve;
+  TensorRef k, v;    // (token, head) rows: ss, sh
+  const int64_t* slots;
+  int n_tokens, Hkv, D, block_shift;
 };
 
 // The spans of documents, runs of equal ids (gqa_tables.hip).
@@ -349,6 +390,16 @@ hipError_t launch_paged_split_first(const SplitParams& p, int dtype, hipStream_t
 hipError_t launch_paged_cache_write(const CacheWriteParams& p, hipStream_t stream);
 hipError_t launch_split_reduce(const ReduceParams& p, int dtype, hipStream_t stream);
 hipError_t launch_rope(const RopeParams& p, int dtype, hipStream_t stream);
+// The paged cache in 8 bits: attention of up to kDecode8Rows packed rows a kv head
+// (a flat split of p.slots, partials and plan in the split workspace), of any number
+// (single pass, or p.kv_splits key chunks), and its writes and reads.
+constexpr int kDecode8Rows = 16;
+// Keys of the flat split's unit.
+constexpr int decode8_unit(int head_dim) { return 16384 / head_dim; }
+hipError_t launch_decode8(const Split8Params& p, int dtype, hipStream_t stream);
+hipError_t launch_chunk8(const Fwd8Params& p, int dtype, hipStream_t stream);
+hipError_t launch_store8(const Store8Params& p, int dtype, hipStream_t stream);
+hipError_t launch_read8(const Read8Params& p, int dtype, hipStream_t stream);
 hipError_t launch_spans(const SpanParams& p, hipStream_t stream);
 hipError_t launch_tables(const TablesParams& p, hipStream_t stream);
 hipError_t launch_release(const ReleaseParams& p, hipStream_t stream);

@@ -24,60 +24,9 @@
 
 #include "gqa_common.hpp"
 #include "gqa_params.hpp"
+#include "gqa_rope_rows.hpp"
 
 namespace gqa {
-
-namespace {
-
-template <int DT> __device__ inline void unpack8(u32x4 x, float (&y)[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t w = x[i];  // (a value: the builtin reads a vector's element from the vector's start)
-    if constexpr (DT == 0) {
-      y[2 * i] = __uint_as_float(w << 16);
-      y[2 * i + 1] = __uint_as_float(w & 0xFFFF0000u);
-    } else {
-      typedef _Float16 f16x2 __attribute__((__vector_size__(2 * sizeof(_Float16))));
-      const f16x2 h = __builtin_bit_cast(f16x2, w);
-      y[2 * i] = (float)h[0];
-      y[2 * i + 1] = (float)h[1];
-    }
-  }
-}
-template <int DT> __device__ inline u32x4 pack8(const float (&y)[8]) {
-  u32x4 x;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = Elem<DT>::pack2(y[2 * i], y[2 * i + 1]);
-  return x;
-}
-
-// Sum over the LPR lanes (4 or 8, aligned) that hold a row.
-template <int LPR> __device__ inline float row_sum(float x) {
-  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0xB1, 0xF, 0xF, true));  // lane ^ 1
-  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x4E, 0xF, 0xF, true));  // lane ^ 2
-  if constexpr (LPR == 8)
-    x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x141, 0xF, 0xF, true));  // 7 - lane
-  return x;
-}
-
-// Norm weights of this lane's two chunks.
-template <int DT>
-__device__ inline void load_weights(const void* w, int w32, int ca, int cb, float (&wa)[8], float (&wb)[8]) {
-  if (w32) {
-    const float* f = static_cast<const float*>(w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      wa[i] = f[8 * ca + i];
-      wb[i] = f[8 * cb + i];
-    }
-  } else {
-    const u32x4* x = static_cast<const u32x4*>(w);
-    unpack8<DT>(x[ca], wa);
-    unpack8<DT>(x[cb], wb);
-  }
-}
-
-}  // namespace
 
 // Wave: token, and units part, part + parts, ... of its rows; a unit is RPW
 // heads of q, of k or of v.  The next unit's rows are loaded while one is worked
@@ -93,12 +42,8 @@ __global__ __launch_bounds__(256) void gqa_rope_kernel(RopeParams p) {
   const int part = wid - tok * p.parts;
   const int b = fast_div(tok, p.div_s.mul, p.div_s.shift), s = tok - b * p.S;
   const int j = lane % LPR, row = lane / LPR;
-  // This lane's chunks (8 values each): a rotated pair of them, or two behind
-  // the rotated dimensions.
-  const int rl = p.table != nullptr ? p.R / 16 : 0;  // lanes with rotated chunks
-  const bool rot = j < rl;
-  const bool apart = rot && !p.interleaved;
-  const int ca = apart ? j : 2 * j, cb = apart ? p.R / 16 + j : 2 * j + 1;
+  const RowLane at = row_lane(p, j);
+  const int ca = at.ca, cb = at.cb;
 
   const int nq = (p.Hq + RPW - 1) / RPW, nk = p.k.ptr != nullptr ? (p.Hkv + RPW - 1) / RPW : 0;
   const int units = nq + nk + (p.kc.ptr != nullptr ? nk : 0);
@@ -118,50 +63,10 @@ __global__ __launch_bounds__(256) void gqa_rope_kernel(RopeParams p) {
   };
   fetch(part);
 
-  // cos and sin of this lane's 8 pairs: of the half form, or 4 of each chunk
-  // (interleaved chunks 2 j and 2 j + 1 hold pairs 8 j .. 8 j + 7).
   float cs[8], sn[8];
   int64_t slot = -1;
   if (p.kc.ptr != nullptr) slot = p.slots[tok];
-  const auto position = [&](int axis) -> int64_t {
-    const int64_t at = (int64_t)axis * p.n_tokens + tok;
-    return p.pos64 ? static_cast<const int64_t*>(p.pos)[at] : (int64_t)static_cast<const int*>(p.pos)[at];
-  };
-  const auto line = [&](int64_t ps) {  // the table's row of a position, in it
-    return p.table + (ps < 0 ? 0 : ps < p.max_pos ? ps : p.max_pos - 1) * p.R;
-  };
-  if (rl > 0) {
-    if (p.axes == 1) {
-      const int64_t ps = position(0);
-      const f32x4* e = reinterpret_cast<const f32x4*>(line(ps)) + 4 * (rot ? j : 0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 x = e[i];
-        cs[2 * i] = x[0], sn[2 * i] = x[1], cs[2 * i + 1] = x[2], sn[2 * i + 1] = x[3];
-      }
-      if (ps >= p.max_pos)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) cs[i] = sn[i] = __builtin_nanf("");
-    } else {
-      const int64_t p0 = position(0), p1 = position(1), p2 = p.axes > 2 ? position(2) : 0,
-                    p3 = p.axes > 3 ? position(3) : 0;
-      typedef float f32x2 __attribute__((__vector_size__(8)));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int pair = 8 * (rot ? j : 0) + i;
-        const int w = pair >> 4;
-        const uint32_t word = w == 0   ? p.pair_axis[0]
-                              : w == 1 ? p.pair_axis[1]
-                              : w == 2 ? p.pair_axis[2]
-                                       : p.pair_axis[3];
-        const uint32_t axis = (word >> (2 * (pair & 15))) & 3;
-        const int64_t ps = axis == 0 ? p0 : axis == 1 ? p1 : axis == 2 ? p2 : p3;
-        const f32x2 x = reinterpret_cast<const f32x2*>(line(ps))[pair];
-        cs[i] = ps < p.max_pos ? x[0] : __builtin_nanf("");
-        sn[i] = ps < p.max_pos ? x[1] : __builtin_nanf("");
-      }
-    }
-  }
+  if (at.rl > 0) row_angles(p, at, tok, cs, sn);
   const int64_t blk = slot >> p.block_shift, off = slot & ((1 << p.block_shift) - 1);
 
   for (int u = part; u < units; u += p.parts) {
@@ -186,7 +91,7 @@ __global__ __launch_bounds__(256) void gqa_rope_kernel(RopeParams p) {
           yb[i] = yb[i] * inv * wb[i];
         }
       }
-      if (rot) {
+      if (at.rot) {
         if (!p.interleaved) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {

@@ -636,6 +636,190 @@ bool write_kv(const py::handle& hk, const py::handle& hv, const py::handle& hkc,
 }
 
 // ---------------------------------------------------------------------------
+// A paged cache in 8 bits.  As above: None, or false (nothing launched) unless every
+// check passes.
+// ---------------------------------------------------------------------------
+bool cache8_of(const py::handle& hc, const py::handle& he, int64_t dev, gqa_cache8& out) {
+  const at::Tensor *c = plain(hc), *e = plain(he);
+  if (c == nullptr || e == nullptr || c->scalar_type() != at::kFloat8_e4m3fn || c->dim() != 4 || c->stride(3) != 1 ||
+      c->get_device() != dev || e->scalar_type() != at::kInt || e->dim() != 2 || e->size(0) != c->size(0) ||
+      e->size(1) != c->size(2) || e->get_device() != dev)
+    return false;
+  out.codes = c->data_ptr();
+  uint64_t bits = reinterpret_cast<uintptr_t>(out.codes);
+  for (int i = 0; i < 4; ++i) {
+    out.stride[i] = c->stride(i);
+    if (i < 3) bits |= static_cast<uint64_t>(out.stride[i]);
+  }
+  out.exponents = static_cast<int*>(e->data_ptr());
+  out.exp_stride[0] = e->stride(0);
+  out.exp_stride[1] = e->stride(1);
+  const int64_t bs = c->size(1);
+  return (bits & 15) == 0 && bs >= 16 && bs <= GQA_MAX_BLOCK_SIZE && (bs & (bs - 1)) == 0;
+}
+bool caches8_ready(const py::handle& hkc, const py::handle& hvc, const py::handle& hke, const py::handle& hve,
+                   int64_t dev, gqa_cache8 (&c)[2]) {
+  return cache8_of(hkc, hke, dev, c[0]) && cache8_of(hvc, hve, dev, c[1]) &&
+         THPVariable_Unpack(hkc.ptr()).sizes() == THPVariable_Unpack(hvc.ptr()).sizes();
+}
+int cu_count(int64_t dev) {  // (guarded by the GIL)
+  static std::array<int, 64> counts{};
+  if (dev < 0 || dev >= 64) return gqa_device_cu_count(static_cast<int>(dev));
+  if (counts[dev] <= 0) counts[dev] = gqa_device_cu_count(static_cast<int>(dev));
+  return counts[dev];
+}
+
+// paged_attention on the route that gqa_paged8_plan chooses.
+py::object paged_attn8(const py::handle& hq, const py::handle& hkc, const py::handle& hvc, const py::handle& hke,
+                       const py::handle& hve, const py::handle& htab, const py::handle& hlens, bool causal,
+                       int64_t max_seq_len, double scale_log2, bool return_lse, const py::handle& hout,
+                       const py::handle& hqs, const py::handle& hql, int64_t max_query_len, double softcap,
+                       const py::handle& slopes, const py::handle& prefix) {
+  const at::Tensor *pq = plain(hq), *ptab = plain(htab), *plens = plain(hlens);
+  if (pq == nullptr || ptab == nullptr || plens == nullptr || modes_active()) return py::none();
+  const at::Tensor &q = *pq, &tab = *ptab, &lens = *plens;
+  const bool varlen = !hqs.is_none();
+  if (!half_type(q) || q.dim() != (varlen ? 3 : 4) || !rows_ready(q) || wants_grad({pq})) return py::none();
+  const int64_t dev = q.get_device(), H = q.size(1), D = q.size(-1);
+  gqa_cache8 c[2];
+  if (c10::hip::current_device() != dev || !caches8_ready(hkc, hvc, hke, hve, dev, c)) return py::none();
+  const at::Tensor& kc = THPVariable_Unpack(hkc.ptr());
+  const int64_t Hkv = kc.size(2), bs = kc.size(1);
+  const int64_t B = varlen ? (lens.dim() == 1 ? lens.size(0) : -1) : q.size(0);
+  const int64_t Sq = varlen ? max_query_len : q.size(2);
+  const at::Tensor *qst = nullptr, *qln = nullptr;
+  if (varlen) {
+    qst = plain(hqs);
+    qln = plain(hql);
+    if (Sq < 0 || !int_rows(qst, B, dev) || !int_rows(qln, B, dev)) return py::none();
+  }
+  if (kc.size(3) != D || (D != 64 && D != 128) || Hkv < 1 || H % Hkv != 0 || H > 128 * Hkv ||
+      !int_rows(&lens, B, dev) || tab.scalar_type() != at::kInt || tab.dim() != 2 || tab.size(0) != B ||
+      tab.get_device() != dev || tab.stride(1) != 1 || (B > 1 && tab.stride(0) < tab.size(1)))
+    return py::none();
+  const int64_t capacity = tab.size(1) * bs, limit = (int64_t)1 << 31;
+  if (max_seq_len == -1) max_seq_len = capacity;
+  if (max_seq_len < 0 || max_seq_len > capacity || max_seq_len >= limit || B >= limit || Sq >= limit ||
+      tab.stride(0) >= limit || !(scale_log2 > 0.0) || !std::isfinite(scale_log2))
+    return py::none();
+  Changes ch;
+  if (!read_changes(softcap, slopes, prefix, py::none(), py::none(), B, H, Sq, max_seq_len, causal, dev, ch))
+    return py::none();
+  const int b = B, h = H, hkv = Hkv, sq = Sq, d = D, ms = max_seq_len;
+  int form = 0, parts = 0;
+  if (gqa_paged8_plan(b, h, hkv, sq, ms, d, cu_count(dev), &form, &parts) != GQA_OK) return py::none();
+  at::Tensor out, lse, ws;
+  if (hout.is_none()) {
+    out = at::empty(q.sizes(), q.options());
+  } else {
+    const at::Tensor* po = plain(hout);
+    if (po == nullptr || po->sizes() != q.sizes() || po->scalar_type() != q.scalar_type() || po->get_device() != dev ||
+        !rows_ready(*po))
+      return py::none();
+    out = *po;
+  }
+  const auto f32 = q.options().dtype(at::kFloat);
+  if (return_lse) lse = varlen ? at::empty({q.size(0), H}, f32) : at::empty({B, H, Sq}, f32);
+  // (A workspace of the call's own: it launches twice without the GIL.)
+  const size_t need = gqa_paged8_workspace_bytes(form, parts, b, h, sq, d);
+  if (need > 0) ws = at::empty({static_cast<int64_t>((need + 3) / 4)}, f32);
+  int64_t qs[4], os[4];
+  if (varlen) {
+    const int64_t qv[4] = {0, q.stride(1), q.stride(0), 1}, ov[4] = {0, out.stride(1), out.stride(0), 1};
+    std::copy(qv, qv + 4, qs);
+    std::copy(ov, ov + 4, os);
+  } else {
+    strides_of(q, qs);
+    strides_of(out, os);
+  }
+  hipStream_t stream = c10::hip::getCurrentHIPStream(dev).stream();
+  int rc;
+  {
+    py::gil_scoped_release others;
+    rc = gqa_paged8_launch(form, q.data_ptr(), qs, &c[0], &c[1], tab.data_ptr<int>(),
+                           static_cast<int>(B > 1 ? tab.stride(0) : tab.size(1)), lens.data_ptr<int>(),
+                           varlen ? qst->data_ptr<int>() : nullptr, varlen ? qln->data_ptr<int>() : nullptr,
+                           static_cast<int>(bs), ms, out.data_ptr(), os, return_lse ? lse.data_ptr<float>() : nullptr,
+                           need > 0 ? ws.data_ptr<float>() : nullptr, parts, b, h, hkv, sq, d,
+                           static_cast<float>(scale_log2), causal ? 1 : 0, dtype_code(q), ch.any ? &ch.score : nullptr,
+                           stream);
+  }
+  if (rc == GQA_E_SCORE) return py::none();  // (Python names the argument)
+  check_rc(rc, "gqa_paged8_launch");
+  if (return_lse) return py::make_tuple(out, lse);
+  return py::cast(out);
+}
+
+bool slots_ready(const at::Tensor* t, int64_t n, int64_t dev) {
+  return t != nullptr && t->scalar_type() == at::kLong && t->dim() == 1 && (n < 0 || t->size(0) == n) &&
+         t->get_device() == dev && t->is_contiguous();
+}
+
+bool write_kv8(const py::handle& hk, const py::handle& hv, const py::handle& hkc, const py::handle& hvc,
+               const py::handle& hslots, const py::handle& hke, const py::handle& hve) {
+  const at::Tensor *k = plain(hk), *v = plain(hv), *sl = plain(hslots);
+  if (k == nullptr || v == nullptr || modes_active() || !half_type(*k) || k->dim() != 3 || v->sizes() != k->sizes() ||
+      v->scalar_type() != k->scalar_type() || !rows_ready(*k) || !rows_ready(*v) || wants_grad({k, v}))
+    return false;
+  const int64_t dev = k->get_device(), T = k->size(0), D = k->size(2);
+  gqa_cache8 c[2];
+  if (c10::hip::current_device() != dev || v->get_device() != dev || (D != 64 && D != 128) ||
+      T >= GQA_MAX_ROPE_TOKENS || !slots_ready(sl, T, dev) || !caches8_ready(hkc, hvc, hke, hve, dev, c))
+    return false;
+  const at::Tensor& kc = THPVariable_Unpack(hkc.ptr());
+  if (kc.size(2) != k->size(1) || kc.size(3) != D) return false;
+  hipStream_t stream = c10::hip::getCurrentHIPStream(dev).stream();
+  int rc;
+  {
+    py::gil_scoped_release others;
+    rc = gqa_cache8_write_launch(nullptr, nullptr, k->data_ptr(), k->strides().data(), v->data_ptr(),
+                                 v->strides().data(), nullptr, nullptr, &c[0], &c[1], sl->data_ptr<int64_t>(), nullptr,
+                                 static_cast<int>(T), 0, static_cast<int>(k->size(1)), static_cast<int>(D),
+                                 static_cast<int>(kc.size(1)), dtype_code(*k), stream);
+  }
+  check_rc(rc, "gqa_cache8_write_launch");
+  return true;
+}
+
+// bf16: whether the rows are bf16 (else fp16; None: neither).
+py::object read_kv8(const py::handle& hkc, const py::handle& hvc, const py::handle& hslots, const py::handle& hke,
+                    const py::handle& hve, const py::handle& bf16, const py::handle& hk, const py::handle& hv) {
+  const at::Tensor *kc = plain(hkc), *sl = plain(hslots);
+  if (kc == nullptr || modes_active() || bf16.is_none() || hk.is_none() != hv.is_none()) return py::none();
+  const int64_t dev = kc->get_device();
+  gqa_cache8 c[2];
+  if (c10::hip::current_device() != dev || !slots_ready(sl, -1, dev) || sl->size(0) >= (int64_t)1 << 31 ||
+      !caches8_ready(hkc, hvc, hke, hve, dev, c) || (kc->size(3) != 64 && kc->size(3) != 128))
+    return py::none();
+  const at::ScalarType type = bf16.cast<bool>() ? at::kBFloat16 : at::kHalf;
+  const int64_t shape[3] = {sl->size(0), kc->size(2), kc->size(3)};
+  at::Tensor rows[2];
+  const py::handle* given[2] = {&hk, &hv};
+  for (int i = 0; i < 2; ++i) {
+    if (given[i]->is_none()) {
+      rows[i] = at::empty(shape, kc->options().dtype(type));
+      continue;
+    }
+    const at::Tensor* t = plain(*given[i]);
+    if (t == nullptr || t->sizes() != at::IntArrayRef(shape) || t->scalar_type() != type || t->get_device() != dev ||
+        !rows_ready(*t) || wants_grad({t}))
+      return py::none();
+    rows[i] = *t;
+  }
+  hipStream_t stream = c10::hip::getCurrentHIPStream(dev).stream();
+  int rc;
+  {
+    py::gil_scoped_release others;
+    rc = gqa_cache8_read_launch(&c[0], &c[1], sl->data_ptr<int64_t>(), rows[0].data_ptr(), rows[0].strides().data(),
+                                rows[1].data_ptr(), rows[1].strides().data(), static_cast<int>(shape[0]),
+                                static_cast<int>(shape[1]), static_cast<int>(shape[2]), static_cast<int>(kc->size(1)),
+                                type == at::kBFloat16 ? GQA_DTYPE_BF16 : GQA_DTYPE_FP16, stream);
+  }
+  check_rc(rc, "gqa_cache8_read_launch");
+  return py::make_tuple(rows[0], rows[1]);
+}
+
+// ---------------------------------------------------------------------------
 // Around the attention: norms and rotation, document spans, block tables.  As
 // above: None (nothing launched) unless every check passes.
 // ---------------------------------------------------------------------------
@@ -653,8 +837,8 @@ at::Tensor part_of(const at::Tensor& t, int64_t offset, at::IntArrayRef sizes) {
 py::object norm_rope(const py::handle& hq, const py::handle& hk, const py::handle& hv, const py::handle& hpos,
                      const py::handle& table, const py::handle& hkc, const py::handle& hvc, const py::handle& hslots,
                      const py::handle& hwq, const py::handle& hwk, double eps, const py::handle& hqo,
-                     const py::handle& hko) {
-  const bool write = !hkc.is_none();
+                     const py::handle& hko, const py::handle& hke, const py::handle& hve) {
+  const bool write = !hkc.is_none(), bits8 = !hke.is_none() || !hve.is_none();
   const at::Tensor *q = plain(hq), *k = hk.is_none() ? nullptr : plain(hk);
   if (q == nullptr || modes_active() || (!hk.is_none() && k == nullptr) || !half_type(*q)) return py::none();
   const int64_t nd = q->dim(), dev = q->get_device();
@@ -704,11 +888,16 @@ py::object norm_rope(const py::handle& hq, const py::handle& hk, const py::handl
   r.weights32 = wq != nullptr ? wq->scalar_type() == at::kFloat : wk != nullptr && wk->scalar_type() == at::kFloat;
   r.eps = static_cast<float>(eps);
   const at::Tensor *v = nullptr, *kc = nullptr, *vc = nullptr, *sl = nullptr;
+  gqa_cache8 c8[2] = {};
   if (write) {
     v = plain(hv), kc = plain(hkc), vc = plain(hvc), sl = plain(hslots);
     if (v == nullptr || kc == nullptr || vc == nullptr || sl == nullptr || v->sizes() != k->sizes() ||
-        v->scalar_type() != k->scalar_type() || v->get_device() != dev || !rows_ready(*v) || !caches_ready(*kc, *vc) ||
-        kc->get_device() != dev || kc->scalar_type() != k->scalar_type() || kc->size(2) != k->size(1) ||
+        v->scalar_type() != k->scalar_type() || v->get_device() != dev || !rows_ready(*v))
+      return py::none();
+    if (bits8 ? !caches8_ready(hkc, hvc, hke, hve, dev, c8) || v->get_device() != k->get_device()
+              : !caches_ready(*kc, *vc) || kc->scalar_type() != k->scalar_type())
+      return py::none();
+    if (kc->get_device() != dev || kc->size(2) != k->size(1) ||
         kc->size(3) != D || sl->scalar_type() != at::kLong || sl->dim() != 1 || sl->size(0) != S ||
         sl->get_device() != dev || !sl->is_contiguous())
       return py::none();
@@ -733,7 +922,13 @@ py::object norm_rope(const py::handle& hq, const py::handle& hk, const py::handl
   int rc;
   {
     py::gil_scoped_release others;  // (one launch, as above)
-    if (write) {
+    if (bits8) {
+      rc = gqa_cache8_write_launch(q->data_ptr(), q->strides().data(), k->data_ptr(), k->strides().data(),
+                                   v->data_ptr(), v->strides().data(), outs[0].data_ptr(), outs[0].strides().data(),
+                                   &c8[0], &c8[1], sl->data_ptr<int64_t>(), &r, static_cast<int>(S),
+                                   static_cast<int>(Hq), static_cast<int>(k->size(1)), static_cast<int>(D),
+                                   static_cast<int>(kc->size(1)), dtype_code(*q), stream);
+    } else if (write) {
       int64_t kcs[4], vcs[4];
       strides_of(*kc, kcs);
       strides_of(*vc, vcs);
@@ -761,7 +956,9 @@ py::object norm_rope(const py::handle& hq, const py::handle& hk, const py::handl
                                    static_cast<int>(D), dtype_code(*q), stream);
     }
   }
-  check_rc(rc, write ? "gqa_qk_norm_rope_write_launch" : "gqa_qk_norm_rope_launch");
+  check_rc(rc, bits8   ? "gqa_cache8_write_launch"
+               : write ? "gqa_qk_norm_rope_write_launch"
+                       : "gqa_qk_norm_rope_launch");
   if (write) return py::cast(outs[0]);
   return py::make_tuple(outs[0], k == nullptr ? py::none() : py::cast(outs[1]));
 }
@@ -935,6 +1132,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("query_lens"), py::arg("max_query_len"), py::arg("workspaces"), py::arg("counters"),
         py::arg("softcap") = 0.0, py::arg("slopes") = none, py::arg("prefix") = none);
   m.def("write_kv", &write_kv, "write_kv with its checks, or False");
+  m.def("paged_attn8", &paged_attn8, "paged_attention over a cache in 8 bits, or None");
+  m.def("write_kv8", &write_kv8, "write_kv into a cache in 8 bits with its checks, or False");
+  m.def("read_kv8", &read_kv8, "read_kv with its checks, or None");
   m.def("norm_rope", &norm_rope, "qk_norm_rope or qk_norm_rope_write with its checks, or None");
   m.def("document_spans", &document_spans, "document_spans with its checks, or None");
   m.def("extend_tables", &extend_tables, "extend_block_tables with its checks, or None");

@@ -24,9 +24,13 @@ GQA_E_SCRATCH = -9
 GQA_E_FLAT = -10
 GQA_E_SCORE = -11
 GQA_E_ROPE = -12
+GQA_E_CACHE8 = -13
+GQA_MIN_EXPONENT = -126
+GQA_MAX_EXPONENT = 126
+FORM_SINGLE, FORM_CHUNKS, FORM_FLAT = 1, 2, 3  # GQA_FORM_*
 GQA_MIN_RAW_SOFTCAP = 1e-2
 GQA_MAX_RAW_SOFTCAP = 1e8
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 _i64x4 = ctypes.c_int64 * 4
 _i64x3 = ctypes.c_int64 * 3
@@ -47,6 +51,12 @@ class Rope(ctypes.Structure):
     _fields_ = [("table", _p), ("max_positions", _i), ("rotary_dim", _i), ("interleaved", _i), ("positions", _p),
                 ("positions64", _i), ("axes", _i), ("pair_axis", ctypes.c_uint32 * 4), ("q_weight", _p),
                 ("k_weight", _p), ("weights32", _i), ("eps", _f)]
+
+
+class Cache8(ctypes.Structure):
+    """gqa_cache8 of include/gqa_attn.h: K or V of a paged cache in 8 bits."""
+
+    _fields_ = [("codes", _p), ("stride", ctypes.c_int64 * 4), ("exponents", _p), ("exp_stride", ctypes.c_int64 * 2)]
 
 
 # (name, restype, argtypes) for every entry point of include/gqa_attn.h.
@@ -160,6 +170,22 @@ SIGNATURES = {
         _i,
         [_p, _i64x3, _p, _i64x3, _p, _i64x3, _p, _i64x3, _p, _i64x4, _p, _i64x4, _p, ctypes.POINTER(Rope),
          _i, _i, _i, _i, _i, _i, _p],
+    ),
+    "gqa_paged8_plan": (_i, [_i] * 7 + [ctypes.POINTER(_i)] * 2),
+    "gqa_paged8_workspace_bytes": (ctypes.c_size_t, [_i] * 6),
+    "gqa_paged8_launch": (
+        _i,
+        [_i, _p, _i64x4, ctypes.POINTER(Cache8), ctypes.POINTER(Cache8), _p, _i, _p, _p, _p, _i, _i, _p, _i64x4, _p, _p,
+         _i, _i, _i, _i, _i, _i, _f, _i, _i, ctypes.POINTER(Score), _p],
+    ),
+    "gqa_cache8_write_launch": (
+        _i,
+        [_p, _i64x3, _p, _i64x3, _p, _i64x3, _p, _i64x3, ctypes.POINTER(Cache8), ctypes.POINTER(Cache8), _p,
+         ctypes.POINTER(Rope), _i, _i, _i, _i, _i, _i, _p],
+    ),
+    "gqa_cache8_read_launch": (
+        _i,
+        [ctypes.POINTER(Cache8), ctypes.POINTER(Cache8), _p, _p, _i64x3, _p, _i64x3, _i, _i, _i, _i, _i, _p],
     ),
     "gqa_document_spans_launch": (_i, [_p, ctypes.c_int64, _p, _p, _i, _i, _p]),
     "gqa_extend_tables_scratch_bytes": (ctypes.c_size_t, [_i, _i]),

@@ -40,7 +40,8 @@ from typing import Dict, Hashable, List, Optional, Sequence
 
 import torch
 
-from . import _lib
+from . import _lib, cache8
+from .cache8 import read_kv
 from .dispatch import (_KIND_IDS, FWD_ROWS, SCORED_CHUNK_TILES, SPLIT_MIN_KV, _fwd_block_tiles, choose_fwd_split,
                        choose_kv_chunks, flat_max_rows, flat_piece_steps, flat_steps, fwd_split_makespan,
                        scored_fine_split, scored_plan, use_short)
@@ -54,6 +55,7 @@ from .tables import BlockPool, StepTables, extend_block_tables, release_blocks
 __all__ = [
     "paged_attention",
     "write_kv",
+    "read_kv",
     "paged_chunk",
     "paged_splits",
     "paged_flat_slots",
@@ -426,7 +428,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
                     out: Optional[torch.Tensor] = None, route: Optional[str] = None,
                     query_start: Optional[torch.Tensor] = None, query_lens: Optional[torch.Tensor] = None,
                     max_query_len: Optional[int] = None, softcap: Optional[float] = None,
-                    alibi_slopes: Optional[torch.Tensor] = None, prefix_lens: Optional[torch.Tensor] = None):
+                    alibi_slopes: Optional[torch.Tensor] = None, prefix_lens: Optional[torch.Tensor] = None,
+                    k_exponents: Optional[torch.Tensor] = None, v_exponents: Optional[torch.Tensor] = None):
     """GQA attention of q over K/V held in a paged cache.
 
     Args:
@@ -472,10 +475,22 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
         softcap, alibi_slopes, prefix_lens: changed scores, as
             ``gqa_flash_attn`` takes them (p = i + seq_lens[b] - the sequence's
             query length).
+        k_exponents, v_exponents: int32 (num_blocks, num_kv_heads); the caches then
+            hold ``torch.float8_e4m3fn`` codes (blocks of 16 keys or more), each
+            its value times 2 ** the exponent of its page and head (in [-126,
+            126]), and enter the products as those values in q's dtype.  Groups of
+            at most 128 query heads, a positive scale, routes "split" (up to 16
+            packed rows a kv head), "chunks" and "single"; a row that sees no key
+            gives zeros and LSE -inf; V finite at hidden keys in the 64-key tiles
+            of which the row's block sees a key.
 
     Returns:
         o (batch, num_heads, seq_q, head_dim), or (o, lse).
     """
+    if k_exponents is not None or v_exponents is not None or k_cache.dtype is cache8.CODES:
+        return cache8.attention(q, k_cache, v_cache, block_table, seq_lens, causal, max_seq_len, scale, splits,
+                                return_lse, out, route, query_start, query_lens, max_query_len, softcap, alibi_slopes,
+                                prefix_lens, k_exponents, v_exponents)
     varlen = query_start is not None
     changed = bool(softcap) or alibi_slopes is not None or prefix_lens is not None
     default_route = route is None and splits is None and (not varlen or query_lens is not None)
@@ -729,14 +744,26 @@ def _paged_scored(kind, parts, q, k_cache, v_cache, block_table, table_stride, s
     return out if lse is None else (out, lse)
 
 
-def write_kv(key, value, k_cache, v_cache, slot_mapping):
+def write_kv(key, value, k_cache, v_cache, slot_mapping, *, k_exponents=None, v_exponents=None):
     """Store K/V of new tokens at their cache slots (in place).
 
     key, value: (num_tokens, num_kv_heads, head_dim) in the caches' dtype;
     slot_mapping: int64 (num_tokens,), slot = block * block_size + offset,
     negative = skip (padding).  Every non-negative slot must lie inside the
     caches.
+
+    k_exponents, v_exponents (int32 (num_blocks, num_kv_heads), in place): the
+    caches hold ``torch.float8_e4m3fn`` codes, key and value are fp16 or bf16.  A
+    page's exponent becomes the least that brings its new values within 448 times
+    2 ** it, not below what it was, unless the call stores the page's first slot,
+    which begins the page anew; the tokens in front of the new ones are brought to
+    it.  A page's tokens stand next to one another in the call (no padding in
+    between), no slot twice.  fp16 values past 61440 (bf16: past 1.875 * 2 ** 127)
+    are stored as that, NaN as NaN.
     """
+    if k_exponents is not None or v_exponents is not None or k_cache.dtype is cache8.CODES:
+        cache8.write(key, value, k_cache, v_cache, slot_mapping, k_exponents, v_exponents)
+        return
     if _lib._host is not None and _lib._host.write_kv(key, value, k_cache, v_cache, slot_mapping):
         return
     block_size = _check_cache(k_cache, v_cache)
@@ -789,6 +816,10 @@ class PagedKVCache:
     about 8% faster on MI355X at 131072 keys) or "NHD" (slots outer, vLLM's
     FlashAttention layout).  Both are strided views the kernels take as they
     are.
+
+    dtype ``torch.float8_e4m3fn``: a cache in 8 bits (``write_kv``), whose
+    ``exponents``, int32 (2, num_blocks, num_kv_heads), go with it; ``append`` takes
+    keys and values of 16 bits, ``read`` gives them back.
     """
 
     def __init__(self, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
@@ -803,6 +834,10 @@ class PagedKVCache:
                                   device=device).transpose(2, 3)
         else:
             self.kv = torch.zeros(2, num_blocks, block_size, num_kv_heads, head_dim, dtype=dtype, device=device)
+        self.exponents = None
+        if dtype is cache8.CODES:
+            assert block_size >= cache8.MIN_BLOCK, f"a cache in 8 bits has blocks of {cache8.MIN_BLOCK} tokens or more"
+            self.exponents = cache8.new_exponents(num_blocks, num_kv_heads, device)
         self._free: List[int] = list(range(num_blocks - 1, -1, -1))
         self._refs: List[int] = [0] * num_blocks
         self._seqs: Dict[Hashable, _Seq] = {}
@@ -867,6 +902,8 @@ class PagedKVCache:
             old = s.blocks[-1]
             new = self._alloc()
             self.kv[:, new].copy_(self.kv[:, old])
+            if self.exponents is not None:
+                self.exponents[:, new].copy_(self.exponents[:, old])
             self._refs[old] -= 1
             s.blocks[-1] = new
         for _ in range(need):
@@ -889,8 +926,23 @@ class PagedKVCache:
         for sid, n in zip(seq_ids, num_new):
             slots += self.reserve(sid, n)
         slot_mapping = torch.tensor(slots, dtype=torch.int64).to(self.kv.device)
-        write_kv(key, value, self.k_cache, self.v_cache, slot_mapping)
+        write_kv(key, value, self.k_cache, self.v_cache, slot_mapping, **self._exponents())
         return slot_mapping
+
+    def _exponents(self) -> dict:
+        e = self.exponents
+        return {} if e is None else dict(k_exponents=e[0], v_exponents=e[1])
+
+    # -- reading -------------------------------------------------------------
+    def read(self, seq_id, dtype=torch.bfloat16):
+        """K and V of seq_id's tokens, (length, num_kv_heads, head_dim) each: of a
+        cache in 8 bits in dtype (``read_kv``), else in the cache's own."""
+        s, bs = self._seqs[seq_id], self.block_size
+        slots = [s.blocks[j // bs] * bs + j % bs for j in range(s.length)]
+        slots = torch.tensor(slots, dtype=torch.int64).to(self.kv.device)
+        if self.exponents is not None:
+            return read_kv(self.k_cache, self.v_cache, slots, *self.exponents, dtype=dtype)
+        return tuple(c[slots // bs, slots % bs] for c in self.kv)
 
     # -- attention -----------------------------------------------------------
     def block_table(self, seq_ids: Sequence) -> torch.Tensor:
@@ -912,7 +964,7 @@ class PagedKVCache:
         over these sequences (their new tokens already appended)."""
         max_len = max(self._seqs[s].length for s in seq_ids)
         return paged_attention(q, self.k_cache, self.v_cache, self.block_table(seq_ids), self.seq_lens(seq_ids),
-                               causal, max_seq_len=max_len, return_lse=return_lse)
+                               causal, max_seq_len=max_len, return_lse=return_lse, **self._exponents())
 
 
 # ---------------------------------------------------------------------------
@@ -968,6 +1020,9 @@ class GQAPagedAttention(torch.nn.Module):
     is not changed.  Slopes, weights given as plain tensors and the table are
     kept as they are: ``.to()`` and ``state_dict`` pass them by (parameters
     register as a module's).
+
+    A cache in 8 bits (kv_cache of ``torch.float8_e4m3fn``) comes with
+    ``kv_exponents``, int32 (2, num_blocks, num_kv_heads).
     """
 
     def __init__(self, num_heads: int, head_size: int, scale: Optional[float] = None,
@@ -990,22 +1045,27 @@ class GQAPagedAttention(torch.nn.Module):
     def _normed(self) -> bool:
         return self.rotary is not None or self.q_norm_weight is not None or self.k_norm_weight is not None
 
-    def forward(self, query, key, value, kv_cache, attn_metadata: PagedAttentionMetadata, output=None):
+    def forward(self, query, key, value, kv_cache, attn_metadata: PagedAttentionMetadata, output=None,
+                kv_exponents=None):
         md = attn_metadata
         num_tokens = query.shape[0]
         H, Hkv, D = self.num_heads, self.num_kv_heads, self.head_size
         batch = md.block_tables.shape[0]
         assert kv_cache.dim() == 5 and kv_cache.shape[0] == 2 and kv_cache.shape[3] == Hkv and kv_cache.shape[4] == D
         k_cache, v_cache = kv_cache[0], kv_cache[1]
+        exps = {}
+        if kv_exponents is not None:
+            assert kv_exponents.dim() == 3 and kv_exponents.shape[0] == 2
+            exps = dict(k_exponents=kv_exponents[0], v_exponents=kv_exponents[1])
         if md.query_lens is None:
             assert num_tokens == batch * md.query_len, "num_tokens must equal num_seqs * query_len"
         else:
             assert len(md.query_lens) == batch and sum(md.query_lens) == num_tokens
         if self._normed():
-            query = self._norm_rope(query, key, value, k_cache, v_cache, md)
+            query = self._norm_rope(query, key, value, k_cache, v_cache, md, exps)
         elif key is not None:
             write_kv(key.view(num_tokens, Hkv, D), value.view(num_tokens, Hkv, D), k_cache, v_cache,
-                     md.slot_mapping)
+                     md.slot_mapping, **exps)
         if output is None:
             output = torch.empty(num_tokens, H * D, dtype=query.dtype, device=query.device)
         if md.query_lens is None:
@@ -1014,7 +1074,7 @@ class GQAPagedAttention(torch.nn.Module):
             o4 = output.view(batch, sq, H, D).permute(0, 2, 1, 3)
             paged_attention(q4, k_cache, v_cache, md.block_tables, md.seq_lens, self.causal,
                             max_seq_len=md.max_seq_len, scale=self.scale, out=o4, softcap=self.softcap,
-                            alibi_slopes=self.alibi_slopes, prefix_lens=md.prefix_lens)
+                            alibi_slopes=self.alibi_slopes, prefix_lens=md.prefix_lens, **exps)
             return output
         # Mixed batch: token-major views, one launch per kernel route over
         # that route's sequences only (a launch spreads its sequences' work
@@ -1027,7 +1087,8 @@ class GQAPagedAttention(torch.nn.Module):
         # device in one asynchronous copy from pinned memory.
         q3, o3 = query.view(num_tokens, H, D), output.view(num_tokens, H, D)
         block_size = k_cache.shape[1]
-        routes = [paged_route(H, Hkv, ql, block_size, D) if ql > 0 else None for ql in md.query_lens]
+        route_of = functools.partial(paged_route, block_size=block_size, head_dim=D) if not exps else cache8.route
+        routes = [route_of(H, Hkv, ql) if ql > 0 else None for ql in md.query_lens]
         starts, t = [], 0
         for ql in md.query_lens:
             starts.append(t)
@@ -1058,10 +1119,10 @@ class GQAPagedAttention(torch.nn.Module):
             # (paged_attention routes the longest query block as `kind`.)
             paged_attention(q3, k_cache, v_cache, tables, lens, self.causal, max_seq_len=max_seq_len,
                             scale=self.scale, out=o3, query_start=qs, query_lens=ql, max_query_len=max_q,
-                            softcap=self.softcap, alibi_slopes=self.alibi_slopes, prefix_lens=prefix)
+                            softcap=self.softcap, alibi_slopes=self.alibi_slopes, prefix_lens=prefix, **exps)
         return output
 
-    def _norm_rope(self, query, key, value, k_cache, v_cache, md):
+    def _norm_rope(self, query, key, value, k_cache, v_cache, md, exps):
         """Normed and rotated queries (a new tensor); keys and values, if given,
         go to the cache."""
         T, H, Hkv, D = query.shape[0], self.num_heads, self.num_kv_heads, self.head_size
@@ -1073,5 +1134,5 @@ class GQAPagedAttention(torch.nn.Module):
         else:
             out = qk_norm_rope_write(q, key.view(T, Hkv, D), value.view(T, Hkv, D), md.positions, self.rotary, k_cache,
                                      v_cache, md.slot_mapping, q_weight=self.q_norm_weight,
-                                     k_weight=self.k_norm_weight, eps=self.norm_eps)
+                                     k_weight=self.k_norm_weight, eps=self.norm_eps, **exps)
         return out.reshape(T, H * D)

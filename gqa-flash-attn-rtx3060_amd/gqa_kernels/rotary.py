@@ -195,7 +195,7 @@ def qk_norm_rope(q, k, positions, table: Optional[RotaryTable] = None, *, q_weig
     if _lib._host is not None:
         # Every check passed, natively; else None.
         res = _lib._host.norm_rope(q, k, None, positions, None if table is None else table._native, None, None, None,
-                                   q_weight, k_weight, eps, q_out, k_out)
+                                   q_weight, k_weight, eps, q_out, k_out, None, None)
         if res is not None:
             return res
     refuse_grad("qk_norm_rope", q, k, q_weight, k_weight)
@@ -236,21 +236,28 @@ def qk_norm_rope(q, k, positions, table: Optional[RotaryTable] = None, *, q_weig
 
 
 def qk_norm_rope_write(q, k, v, positions, table: Optional[RotaryTable], k_cache, v_cache, slot_mapping, *,
-                       q_weight=None, k_weight=None, eps: float = 1e-6, q_out=None):
+                       q_weight=None, k_weight=None, eps: float = 1e-6, q_out=None, k_exponents=None,
+                       v_exponents=None):
     """``qk_norm_rope`` of token-major q (num_tokens, num_heads, head_dim) and k
     (num_tokens, num_kv_heads, head_dim), and ``write_kv`` of the rotated k and of
     v, in one pass; returns q.
 
     Caches and slot_mapping as ``write_kv`` (negative slots are not stored,
-    every other one lies inside the caches, no slot twice)."""
+    every other one lies inside the caches, no slot twice).  k_exponents, v_exponents:
+    a cache in 8 bits, as ``write_kv`` fills it, with k's codes made of the fp32 results
+    (rounded once)."""
+    from . import cache8
     from .paged import _check_cache
 
     if _lib._host is not None:
         # Every check passed, natively; else None.
         res = _lib._host.norm_rope(q, k, v, positions, None if table is None else table._native, k_cache, v_cache,
-                                   slot_mapping, q_weight, k_weight, eps, q_out, None)
+                                   slot_mapping, q_weight, k_weight, eps, q_out, None, k_exponents, v_exponents)
         if res is not None:
             return res
+    if cache8.takes(k_cache, k_exponents, v_exponents):
+        return cache8.norm_rope_write(q, k, v, positions, table, k_cache, v_cache, slot_mapping, q_weight, k_weight,
+                                      eps, q_out, k_exponents, v_exponents)
     refuse_grad("qk_norm_rope_write", q, k, v, q_weight, k_weight)
     _check_qk(q, k, 3)
     assert v is not None and tuple(v.shape) == tuple(k.shape) and v.dtype == k.dtype and v.device == k.device

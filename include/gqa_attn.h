@@ -56,6 +56,7 @@ extern "C" {
                                  the LDS-DMA first pass does not take (see gqa_split_flat_launch) */
 #define GQA_E_SCORE (-11)     /* changed scores: see gqa_scored_launch */
 #define GQA_E_ROPE (-12)      /* rotation: see gqa_rope */
+#define GQA_E_CACHE8 (-13)    /* paged cache in 8 bits: see gqa_cache8 */
 
 #define GQA_MAX_SPLITS 1024
 #define GQA_MAX_BLOCK_SIZE 65536
@@ -594,6 +595,72 @@ int gqa_qk_norm_rope_write_launch(const void* q, const int64_t q_stride[3],
                                   int num_tokens, int num_heads, int num_kv_heads,
                                   int head_dim, int block_size, int dtype,
                                   void* stream);
+
+/* K or V of a paged cache in 8 bits (no counterpart in the reference): e4m3 codes
+ * (1 sign bit, 4 of exponent, 3 of mantissa, no infinities), (num_blocks,
+ * block_size, num_kv_heads, head_dim) with byte strides (last 1, rows 16-byte
+ * aligned, 16 rows of a page within 2 GiB), block_size a power of two in [16,
+ * GQA_MAX_BLOCK_SIZE]; a code of page b and head h stands for its value times
+ * 2^exponents[b * exp_stride[0] + h * exp_stride[1]], exponents clamped to
+ * [GQA_MIN_EXPONENT, GQA_MAX_EXPONENT]. */
+#define GQA_MIN_EXPONENT (-126)
+#define GQA_MAX_EXPONENT 126
+typedef struct gqa_cache8 {
+  void* codes;
+  int64_t stride[4];
+  int* exponents;
+  int64_t exp_stride[2];
+} gqa_cache8;
+
+/* Attention over it.  q, o, lse, block_table, seq_lens, q_start, q_len, max_seq_len
+ * as gqa_paged_fwd_launch; dtype is q's and o's, and K and V enter the products as
+ * the cache's values in it.  score: as gqa_paged_scored_launch, or NULL.  A row
+ * that sees no key gives zeros and LSE -inf.  Groups of at most 128 query heads.
+ * gqa_paged8_plan: the form that a call of these sizes takes on a device of
+ * cu_count compute units, GQA_FORM_FLAT (`parts` slots, up to 16 packed rows a kv
+ * head), GQA_FORM_CHUNKS (`parts` key chunks) or GQA_FORM_SINGLE (0).  Others may
+ * be given, within those limits and GQA_MAX_SPLITS.  workspace: 16-byte aligned,
+ * gqa_paged8_workspace_bytes bytes (0: NULL). */
+int gqa_paged8_plan(int batch, int num_heads, int num_kv_heads, int seq_q,
+                    int max_seq_len, int head_dim, int cu_count, int* form,
+                    int* parts);
+size_t gqa_paged8_workspace_bytes(int form, int parts, int batch, int num_heads,
+                                  int seq_q, int head_dim);
+int gqa_paged8_launch(int form, const void* q, const int64_t q_stride[4],
+                      const gqa_cache8* k_cache, const gqa_cache8* v_cache,
+                      const int* block_table, int table_stride, const int* seq_lens,
+                      const int* q_start, const int* q_len, int block_size,
+                      int max_seq_len, void* o, const int64_t o_stride[4], float* lse,
+                      float* workspace, int parts, int batch, int num_heads,
+                      int num_kv_heads, int seq_q, int head_dim, float scale_log2,
+                      int causal, int dtype, const gqa_score* score, void* stream);
+
+/* gqa_qk_norm_rope_write_launch into it; rope NULL: k is stored as it is (and q and
+ * q_out are NULL); q and q_out NULL: k and v alone.  A page's exponent becomes the
+ * least that brings its new values within 448 times it, not below what it was
+ * unless the call stores the page's first slot, which begins the page anew; the
+ * codes of the slots in front of the new ones are brought to it (to the nearest).
+ * Codes behind them stay, and so mean something else under another exponent.
+ * Values outside what dtype holds are stored as the largest e4m3 multiple of a
+ * power of two within it (fp16 61440); NaN as NaN, without a say in the exponent.
+ * A page's tokens stand next to one another in the call, no slot twice; every
+ * non-negative slot must lie inside the cache. */
+int gqa_cache8_write_launch(const void* q, const int64_t q_stride[3],
+                            const void* k, const int64_t k_stride[3],
+                            const void* v, const int64_t v_stride[3],
+                            void* q_out, const int64_t q_out_stride[3],
+                            const gqa_cache8* k_cache, const gqa_cache8* v_cache,
+                            const int64_t* slot_mapping, const gqa_rope* rope,
+                            int num_tokens, int num_heads, int num_kv_heads,
+                            int head_dim, int block_size, int dtype, void* stream);
+
+/* k, v (num_tokens, num_kv_heads, head_dim; element strides) <- the cache's values at
+ * slot_mapping in dtype; zeros for negative slots. */
+int gqa_cache8_read_launch(const gqa_cache8* k_cache, const gqa_cache8* v_cache,
+                           const int64_t* slot_mapping, void* k, const int64_t k_stride[3],
+                           void* v, const int64_t v_stride[3], int num_tokens,
+                           int num_kv_heads, int head_dim, int block_size, int dtype,
+                           void* stream);
 
 /* lo, hi (batch, seq) <- the first token, and the first behind the last, of each
  * token's document: a run of equal ids in its row of ids (batch, seq; int32, rows
