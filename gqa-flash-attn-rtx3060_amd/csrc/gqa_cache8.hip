@@ -14,15 +14,21 @@
 //
 // A page's new tokens follow one another in the call (sequence-major, as batches
 // are), so the workgroup that meets the first of them does the page: a task is (run
-// of tokens of one page, K or V, 2^head_shift heads).  Two passes over the run, one
-// for the largest value and one for the codes; the second reads from L2.  Nothing is
-// ordered by chance: results do not depend on the schedule.
+// of tokens of one page, K or V, 2^head_shift heads).  One pass over the run finds its
+// largest value, one makes the codes: of values still in registers if the run is one
+// step (32 (token, head) rows at head_dim 128, 64 at 64), else from L2.
+// Nothing is ordered by chance: results do not depend on the schedule.
 //
-// Bound by memory where tokens are many (rows read once from HBM, codes written),
-// by the chain of dependent reads (slot, position, table row, exponent) where few.
+// Measured, bf16, 32/8 heads of 128, 16-token pages: norms, rotation and store of 8192
+// tokens 51 us, 189 MB at 3.7 TB/s (a large copy 5.1; registers for four waves a
+// SIMD are what keeps it from more: the rotation of 16-bit caches alone, at six, 49.5
+// us for 206 MB); K and V alone 13.8 us, 51 MB.  64 tokens, one a page: 4.4 and 3.7
+// us, a chain of dependent reads (slot; exponent, table row) after a launch of 2.6.
+// Rows and angles of a small call's tokens are loaded before their slots are known.
 #include <algorithm>
 
 #include "gqa_cache8.hpp"
+#include "gqa_lds.hpp"
 #include "gqa_rope_rows.hpp"
 #include "gqa_score.hpp"
 
@@ -53,28 +59,41 @@ __device__ inline int64_t load_uniform64(const int64_t* p) {
 }  // namespace
 
 // Workgroups [0, n_kv): keys and values; the others: queries, a wave for part of a
-// token's heads, as gqa_rope_kernel.
-template <int DT, int D> __global__ __launch_bounds__(256) void gqa_store8_kernel(Store8Params p) {
+// token's heads, as gqa_rope_kernel.  ROPE: keys are normed or rotated, and there may
+// be queries; without, half the registers.
+template <int DT, int D, bool ROPE> __global__ __launch_bounds__(256) void gqa_store8_kernel(Store8Params p) {
   using T = typename Elem<DT>::T;
   constexpr int LPR = D / 16, RPW = 64 / LPR;
   const int lane = threadIdx.x & 63;
+  constexpr int waves = 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const RowLane at = row_lane(p, lane % LPR);
 
-  if ((int)blockIdx.x >= p.n_kv) {
-    const int wid = ((int)blockIdx.x - p.n_kv) * 4 + wave;
+  if (ROPE && (int)blockIdx.x >= p.n_kv) {
+    const int wid = ((int)blockIdx.x - p.n_kv) * waves + wave;
     const int tok = fast_div(wid, p.div_parts.mul, p.div_parts.shift);
     if (tok >= p.n_tokens) return;
-    float cs[8], sn[8];
-    if (at.rl > 0) row_angles(p, at, tok, cs, sn);
     const T* qr = static_cast<const T*>(p.q.ptr) + tok * p.q.ss;
     T* qo = static_cast<T*>(const_cast<void*>(p.qo.ptr)) + tok * p.qo.ss;
-    for (int h = (wid - tok * p.parts) * RPW + lane / LPR; h - lane / LPR < p.Hq; h += p.parts * RPW) {
-      float ya[8] = {}, yb[8] = {};
+    // The next heads' rows are loaded while these are worked on.
+    const int turn = p.parts * RPW, h0 = (wid - tok * p.parts) * RPW, row = lane / LPR;
+    u32x4 xa, xb;
+    const auto fetch = [&](int h) {
+      xa = xb = u32x4{0u, 0u, 0u, 0u};
       if (h < p.Hq) {
-        unpack8<DT>(*reinterpret_cast<const u32x4*>(qr + h * p.q.sh + 8 * at.ca), ya);
-        unpack8<DT>(*reinterpret_cast<const u32x4*>(qr + h * p.q.sh + 8 * at.cb), yb);
+        xa = *reinterpret_cast<const u32x4*>(qr + h * p.q.sh + 8 * at.ca);
+        xb = *reinterpret_cast<const u32x4*>(qr + h * p.q.sh + 8 * at.cb);
       }
+    };
+    fetch(h0 + row);
+    float cs[8], sn[8];
+    if (at.rl > 0) row_angles(p, at, tok, cs, sn);
+    for (int hw = h0; hw < p.Hq; hw += turn) {
+      const int h = hw + row;
+      float ya[8], yb[8];
+      unpack8<DT>(xa, ya);
+      unpack8<DT>(xb, yb);
+      fetch(h + turn);
       row_norm_rotate<DT, D>(p, at, p.wq, cs, sn, ya, yb);
       if (h < p.Hq) {
         *reinterpret_cast<u32x4*>(qo + h * p.qo.sh + 8 * at.ca) = pack8<DT>(ya);
@@ -85,12 +104,14 @@ template <int DT, int D> __global__ __launch_bounds__(256) void gqa_store8_kerne
   }
 
   __shared__ int most[64];  // largest |y| of each head, by its bits
-  int rest = blockIdx.x;
+  // (Tasks with work may be every block_size-th of them: dealt as the hardware deals
+  // workgroups, they would all be on one or two XCDs.)
+  int rest = xcd_remap(blockIdx.x, p.n_kv);
   const bool is_k = (rest & 1) == 0;
   rest >>= 1;
   const int group = rest % p.n_groups;
   const int t0 = (rest / p.n_groups) * p.chunk, t1 = min(t0 + p.chunk, p.n_tokens);
-  const int hg = 1 << p.head_shift, step = (4 * RPW) >> p.head_shift;  // heads; tokens a step
+  const int hg = 1 << p.head_shift, step = (waves * RPW) >> p.head_shift;  // heads; tokens a step
   const int row = wave * RPW + lane / LPR;
   const int h = group * hg + (row & (hg - 1)), first = row >> p.head_shift;
   const bool mine = h < p.Hkv;
@@ -98,70 +119,99 @@ template <int DT, int D> __global__ __launch_bounds__(256) void gqa_store8_kerne
   const TensorRef& dst = is_k ? p.kc : p.vc;
   const Exponents& ex = is_k ? p.ke : p.ve;
   const T* rows = static_cast<const T*>(src.ptr) + (mine ? h : 0) * src.sh;
+  const int bs = 1 << p.block_shift;
 
-  for (int tok = t0; tok < t1; ++tok) {
-    const int64_t slot = load_uniform64(p.slots + tok);
-    if (slot < 0) continue;
-    const int64_t page = slot >> p.block_shift;
-    if (tok > 0) {
-      const int64_t before = load_uniform64(p.slots + tok - 1);
-      if (before >= 0 && before >> p.block_shift == page) continue;  // not the page's first token
+  // y of the lane's two chunks of token tok (`on`: it has one).
+  const auto fetch = [&](int tok, bool on, u32x4& xa, u32x4& xb) __attribute__((always_inline)) {
+    xa = xb = u32x4{0u, 0u, 0u, 0u};
+    if (on) {
+      const T* x = rows + (int64_t)tok * src.ss;
+      xa = *reinterpret_cast<const u32x4*>(x + 8 * at.ca);
+      xb = *reinterpret_cast<const u32x4*>(x + 8 * at.cb);
     }
-    // The page's tokens from here on, at most a page of them, and their first slot.
-    const int bs = 1 << p.block_shift, end = min(p.n_tokens - tok, bs);
-    int n = 0, low = bs;
-    for (int at0 = 0; at0 < end; at0 += 64) {
-      const int64_t s = at0 + lane < end ? p.slots[tok + at0 + lane] : -1;
-      const uint64_t other = __builtin_amdgcn_ballot_w64(s < 0 || s >> p.block_shift != page);
+  };
+  const auto angles = [&](int tok, float (&cs)[8], float (&sn)[8]) __attribute__((always_inline)) {
+    if constexpr (ROPE) {
+      if (is_k && at.rl > 0) row_angles(p, at, tok, cs, sn);
+    }
+  };
+  const auto finish = [&](const u32x4& xa, const u32x4& xb, const float (&cs)[8], const float (&sn)[8], float (&ya)[8],
+                          float (&yb)[8]) __attribute__((always_inline)) {
+    unpack8<DT>(xa, ya);
+    unpack8<DT>(xb, yb);
+    if constexpr (ROPE) {
+      if (is_k) row_norm_rotate<DT, D>(p, at, p.wk, cs, sn, ya, yb);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      ya[e] = within(ya[e], p.limit);
+      yb[e] = within(yb[e], p.limit);
+    }
+  };
+
+  // Lane l: token t0 + l, its page (none: -1) and the slot in it.
+  const int left = min(64, p.n_tokens - t0);
+  const int64_t slot = lane < left ? p.slots[t0 + lane] : -1;
+  const int64_t before = t0 > 0 ? load_uniform64(p.slots + t0 - 1) : -1;
+  // (The first token's rows and angles, which a decode step's task is about, with
+  // them.)
+  u32x4 xa, xb;
+  float cs[8] = {}, sn[8] = {};
+  if (p.chunk == 1) {
+    fetch(t0 + first, mine && first < left, xa, xb);
+    angles(t0 + min(first, left - 1), cs, sn);
+  }
+  if (threadIdx.x < 64) most[threadIdx.x] = 0;
+  const int page_of = slot < 0 ? -1 : (int)(slot >> p.block_shift), off_of = (int)(slot & (bs - 1));
+  const int front = __shfl_up(page_of, 1);
+  const int prev = lane > 0 ? front : before < 0 ? -1 : (int)(before >> p.block_shift);
+  uint64_t owners = __builtin_amdgcn_ballot_w64(lane < t1 - t0 && page_of >= 0 && page_of != prev);
+  while (owners != 0) {
+    const int j = __builtin_ctzll(owners), tok = t0 + j;
+    owners &= owners - 1;
+    const int page = __builtin_amdgcn_readlane(page_of, j);
+    // The page's tokens from here on, n of them, and their first slot.
+    const uint64_t same = __builtin_amdgcn_ballot_w64(page_of == page) >> j;
+    int n = same == ~0ull ? 64 : __builtin_ctzll(~same);
+    int low = wave_min(lane >= j && lane < j + n ? off_of : bs);
+    for (int more = 64; j + n == more && t0 + more < p.n_tokens; more += 64) {
+      const int64_t s = t0 + more + lane < p.n_tokens ? p.slots[t0 + more + lane] : -1;
+      const uint64_t other = __builtin_amdgcn_ballot_w64(s < 0 || (int)(s >> p.block_shift) != page);
       const int here = other == 0 ? 64 : __builtin_ctzll(other);
       low = min(low, wave_min(lane < here ? (int)(s & (bs - 1)) : bs));
-      n = at0 + here;
+      n += here;
       if (here < 64) break;
     }
+    n = min(n, bs);
 
-    // y of the lane's two chunks of the run's token i.
-    const auto values = [&](int i, float (&ya)[8], float (&yb)[8]) __attribute__((always_inline)) {
-      const T* x = rows + (int64_t)(tok + i) * src.ss;
-      u32x4 xa = {0u, 0u, 0u, 0u}, xb = {0u, 0u, 0u, 0u};
-      const bool on = mine && i < n;
-      if (on) {
-        xa = *reinterpret_cast<const u32x4*>(x + 8 * at.ca);
-        xb = *reinterpret_cast<const u32x4*>(x + 8 * at.cb);
-      }
-      unpack8<DT>(xa, ya);
-      unpack8<DT>(xb, yb);
-      if (is_k) {
-        float cs[8] = {}, sn[8] = {};
-        if (at.rl > 0) row_angles(p, at, tok + min(i, n - 1), cs, sn);
-        row_norm_rotate<DT, D>(p, at, p.wk, cs, sn, ya, yb);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        ya[e] = within(ya[e], p.limit);
-        yb[e] = within(yb[e], p.limit);
-      }
-    };
-
-    __syncthreads();  // (most is free)
-    if (threadIdx.x < 64) most[threadIdx.x] = 0;
-    __syncthreads();
-    float big = 0.f;
+    char* base = static_cast<char*>(const_cast<void*>(dst.ptr)) + page * dst.sb + (mine ? h : 0) * dst.sh;
+    int* ep = ex.e + page * ex.sb + (mine ? h : 0) * ex.sh;
+    int was = clamp_exp(*ep);
+    float big = 0.f, ya[8], yb[8];
     for (int i0 = 0; i0 < n; i0 += step) {
-      float ya[8], yb[8];
-      values(i0 + first, ya, yb);
+      if (p.chunk > 1 || i0 > 0) {
+        const int i = i0 + first;
+        fetch(tok + i, mine && i < n, xa, xb);
+        angles(tok + min(i, n - 1), cs, sn);
+      } else if (first >= n) {
+        xa = xb = u32x4{0u, 0u, 0u, 0u};
+      }
+      finish(xa, xb, cs, sn, ya, yb);
 #pragma unroll
       for (int e = 0; e < 8; ++e) big = fmaxf(big, fmaxf(__builtin_fabsf(ya[e]), __builtin_fabsf(yb[e])));
     }
     big = row_max<LPR>(big);
+    pin(was);
+    // (Barriers of LDS alone: loads and stores stay in flight.)
+    phase_barrier();  // most is zero, and all have read the exponent
     if (lane % LPR == 0) atomicMax(&most[row & (hg - 1)], __float_as_int(big));
-    __syncthreads();
-
-    char* base = static_cast<char*>(const_cast<void*>(dst.ptr)) + page * dst.sb + (mine ? h : 0) * dst.sh;
-    int* ep = ex.e + page * ex.sb + (mine ? h : 0) * ex.sh;
-    const int was = clamp_exp(*ep);
+    phase_barrier();
     int e = exponent_of(__int_as_float(most[row & (hg - 1)]));
+    if (owners != 0) {  // (for the next page)
+      phase_barrier();
+      if (threadIdx.x < 64) most[threadIdx.x] = 0;
+    }
     if (low > 0) e = max(e, was);
-    __syncthreads();  // (all have read the exponent)
     if (mine && first == 0 && lane % LPR == 0) *ep = e;
     if (mine && low > 0 && e > was) {
       // The tokens in front, brought to the new exponent: 16 codes a lane.
@@ -182,11 +232,15 @@ template <int DT, int D> __global__ __launch_bounds__(256) void gqa_store8_kerne
     const float scale = exp_scale(-e);
     for (int i0 = 0; i0 < n; i0 += step) {
       const int i = i0 + first;
-      float ya[8], yb[8];
-      values(i, ya, yb);
+      if (n > step) {  // (else y is there)
+        fetch(tok + i, mine && i < n, xa, xb);
+        angles(tok + min(i, n - 1), cs, sn);
+        finish(xa, xb, cs, sn, ya, yb);
+      }
+      int o = __shfl(off_of, (j + i) & 63);
       if (!mine || i >= n) continue;
-      const int64_t o = p.slots[tok + i] & (bs - 1);
-      char* c = base + o * dst.ss;
+      if (j + i >= 64) o = (int)(p.slots[tok + i] & (bs - 1));
+      char* c = base + (int64_t)o * dst.ss;
       u32x2 a, b;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -196,8 +250,15 @@ template <int DT, int D> __global__ __launch_bounds__(256) void gqa_store8_kerne
       *reinterpret_cast<u32x2*>(c + 8 * at.ca) = a;
       *reinterpret_cast<u32x2*>(c + 8 * at.cb) = b;
     }
-    tok += n - 1;
   }
+}
+
+template <int DT, int D> static void launch_store8_t(const Store8Params& p, int64_t total, hipStream_t stream) {
+  const dim3 grid((unsigned)total), block(256);
+  if (p.q.ptr != nullptr || p.table != nullptr || p.wk != nullptr)
+    hipLaunchKernelGGL((gqa_store8_kernel<DT, D, true>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((gqa_store8_kernel<DT, D, false>), grid, block, 0, stream, p);
 }
 
 hipError_t launch_store8(const Store8Params& in, int dtype, hipStream_t stream) {
@@ -207,8 +268,23 @@ hipError_t launch_store8(const Store8Params& in, int dtype, hipStream_t stream) 
   // Keys and values.
   p.head_shift = 0;
   while ((1 << p.head_shift) < p.Hkv && (1 << p.head_shift) < rpw) ++p.head_shift;
-  p.n_groups = (p.Hkv + (1 << p.head_shift) - 1) >> p.head_shift;
-  p.chunk = 1;
+  // A wave's worth of heads a workgroup, fewer where a page's tokens then go in one
+  // step: a prompt's pages (us, K and V alone, 8 kv heads of 128, a wave's heads / fewer,
+  // pages of 16, 64, 256: 400 tokens 10.8 / 4.0, 18 / 5.4, 65 / 12; 8192 tokens 15.4 /
+  // 13.8, 38 / 15.5, 141 / 25).  Not in small calls of more than a few tokens, which
+  // may be a token of each of many pages: more workgroups for the same rows (64 with
+  // norms and queries 4.4 / 5.0, 256 in pages of 64 4.0 / 7.5; a prompt of 100 pays
+  // 6.8 for 4.9).
+  const int bs = 1 << p.block_shift;
+  const auto groups = [&] { return (p.Hkv + (1 << p.head_shift) - 1) >> p.head_shift; };
+  while (p.head_shift > 0 && ((4 * rpw) >> p.head_shift) < bs &&
+         (p.n_tokens > 256 || p.n_tokens * groups() <= 32))
+    --p.head_shift;
+  p.n_groups = groups();
+  // Tokens that a workgroup looks at, up to a page of 16-64: a workgroup that finds no
+  // page's first token costs as much as one that does (8192 tokens in pages of 16, 4 a
+  // workgroup 20 us, 16 15), while 512 still fill the device.
+  p.chunk = std::max(1, std::min(std::min(std::max(bs, 16), 64), (int)(2ll * p.n_groups * p.n_tokens / 512)));
   p.n_chunks = (p.n_tokens + p.chunk - 1) / p.chunk;
   const int64_t n_kv = 2ll * p.n_groups * p.n_chunks;
   // Queries: as launch_rope.
@@ -220,13 +296,12 @@ hipError_t launch_store8(const Store8Params& in, int dtype, hipStream_t stream) 
   const int64_t total = n_kv + (waves + 3) / 4;
   if (total >= (int64_t)1 << 31) return hipErrorInvalidValue;
   p.n_kv = (int)n_kv;
-  const dim3 grid((unsigned)total), block(256);
   if (dtype == 0) {
-    if (p.D == 128) hipLaunchKernelGGL((gqa_store8_kernel<0, 128>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((gqa_store8_kernel<0, 64>), grid, block, 0, stream, p);
+    if (p.D == 128) launch_store8_t<0, 128>(p, total, stream);
+    else launch_store8_t<0, 64>(p, total, stream);
   } else {
-    if (p.D == 128) hipLaunchKernelGGL((gqa_store8_kernel<1, 128>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((gqa_store8_kernel<1, 64>), grid, block, 0, stream, p);
+    if (p.D == 128) launch_store8_t<1, 128>(p, total, stream);
+    else launch_store8_t<1, 64>(p, total, stream);
   }
   return hipGetLastError();
 }

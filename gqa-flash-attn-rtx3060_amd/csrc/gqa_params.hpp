@@ -305,8 +305,9 @@ struct RopeParams {
 struct Store8Params : RopeParams {
   Exponents ke, ve;
   float limit;    // stored values are kept within it
-  // Set by the launcher: tokens and workgroups of a key or value task, heads of a
-  // workgroup (a power of two), head groups; workgroups of keys and values.
+  // Set by the launcher: tokens that a key or value task looks at and their number,
+  // heads of a workgroup (a power of two), head groups; workgroups of keys and
+  // values.
   int chunk, n_chunks, head_shift, n_groups, n_kv;
 };
 
