@@ -163,7 +163,8 @@ int gqa_paged8_launch(int form, const void* q, const int64_t q_stride[4], const 
     r.ws_m = p.ws_m;
     r.ws_l = p.ws_l;
     r.plan = p.plan;
-    return gqa::to_code(gqa::launch_split_reduce(r, dtype, st));
+    r.slots = parts;
+    return gqa::to_code(gqa::launch_decode8_join(r, G, dtype, st));
   }
   gqa::Fwd8Params p{};
   p.q = ref4(q, q_stride);

@@ -1,6 +1,6 @@
 // gqa_decode8.hip — attention over a paged cache in 8 bits (gqa_cache8.hpp) for few
-// query rows: single tokens, and as many as give 16 packed rows per kv head (row r ->
-// position r / G, head r % G).
+// query rows: single tokens, and as many as give 32 packed rows per kv head (row r ->
+// position r / G, head r % G), NR blocks of 16: codes are widened once for both.
 //
 //   s_j = scale q . (kc_j 2^ke(page of j)),  o = sum_j p_j (vc_j 2^ve(page of j)) / l
 //
@@ -56,7 +56,7 @@ __device__ inline u32x2 ld_tr8(const char* p) {
 // keys 4 lg + e and 16 + 4 lg + (e - 4), the lane's own probabilities; V^T is read
 // transposed, 8 rows of one dim a read.  The chunks of a row are swizzled so that the
 // 16 lanes of a K read, and the 32 of a V read, cover all banks once: fk, fv below.
-template <int DT, int D, bool MOD>
+template <int DT, int D, int NR, bool MOD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void gqa_decode8_kernel(Split8Params p) {
   using E = Elem<DT>;
   constexpr int TW = 4096 / D;     // keys of a wave's tile
@@ -68,6 +68,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   constexpr int NDB = D / 16;      // 16-dim blocks of O^T
   constexpr int NLD = 2 * NB * IPB;  // loads of a tile
   constexpr int UNIT = 4 * TW;
+  // The running reference follows a row's maximum only once it lags by 2^kLag: until then
+  // probabilities exceed 1, which no type here minds (fp16 holds 2^15), and the
+  // accumulators need no scaling (16 x 8 queries of 8000 keys 71.0 -> 69.7 us).
+  constexpr float kLag = 8.f;
   static_assert(UNIT == decode8_unit(D), "unit of the flat split");
   // An array a stage, so that the compiler can tell the load's target from the stage
   // being read; a wave's 8 KiB of each: K, then V.
@@ -75,9 +79,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ __attribute__((aligned(1024))) char lds_b[4 * 8192];
   // Where the waves' states meet: kMeet rows of each (two workgroups a CU have 80 KiB
   // each).
-  constexpr int kMeet = 768 / D;
+  constexpr int kMeet = 768 / D, kEnd = (int)sizeof(lds_a) / (16 * D);
   __shared__ __attribute__((aligned(16))) float meet[4 * kMeet * D];
-  __shared__ float st_m[4][16], st_l[4][16];
+  __shared__ float st_m[4][16 * NR], st_l[4][16 * NR];
 
   const Dims& dm = p.dm;
   const int t = threadIdx.x, lane = t & 63;
@@ -90,11 +94,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     return;
   }
   const int w = xcd_remap(blockIdx.x, total);
-  const int kvh = fast_div(w, p.div_splits.mul, p.div_splits.shift), s = w - kvh * p.slots;
+  // Heads whose rows share a 128-byte line of the cache, PAIR of them, are neighbours in
+  // the launch, so that the line comes to an XCD's L2 once (head_dim 64, 16 x 8 queries of
+  // 8000 keys 51.0 -> 40.2 us).
+  constexpr int PAIR = 128 / D;
+  const int wp = dm.Hkv % PAIR == 0 ? w / PAIR : w;
+  const int kp = fast_div(wp, p.div_splits.mul, p.div_splits.shift), s = wp - kp * p.slots;
+  const int kvh = dm.Hkv % PAIR == 0 ? kp * PAIR + w % PAIR : kp;
   const bool varlen = p.q_len != nullptr;
-  const int pos = fast_div(i16, p.div_g.mul, p.div_g.shift), g = i16 - pos * dm.G;
-  const int head = kvh * dm.G + min(g, dm.G - 1);
-  [[maybe_unused]] const float slope = MOD ? row_slope(p.mod, head) : 0.f;
+  // This lane's query rows, i16 of each 16-row block.
+  int pos[NR], head[NR];
+  [[maybe_unused]] float slope[NR];
+#pragma unroll
+  for (int rb = 0; rb < NR; ++rb) {
+    const int r = 16 * rb + i16;
+    pos[rb] = fast_div(r, p.div_g.mul, p.div_g.shift);
+    head[rb] = kvh * dm.G + r - pos[rb] * dm.G;
+    slope[rb] = MOD ? row_slope(p.mod, head[rb]) : 0.f;
+  }
   const float c = dm.c;
 
   const uint32_t kss = (uint32_t)p.k.ss, vss = (uint32_t)p.v.ss;
@@ -131,9 +148,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   Piece cur, nxt;
   int n = 0;  // this wave's tiles: wave, wave + 4, ...
-  int qpos = 0, qpos_lo = 0, seen = 0, seen_lo = 0;
-  bool valid = false;
-  u32x4 qreg[NKS];
+  int qpos[NR], seen[NR], qpos_lo = 0, seen_lo = 0;
+  bool valid[NR];
+  u32x4 qreg[NR][NKS];
   // Pages and scales of this wave's 64 16-key blocks from its tile `base` on, a block a
   // lane (page -1: behind the piece): read together, handed out by lane, so that the
   // stream of tiles waits for no scalar load.
@@ -211,18 +228,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int sq = varlen ? min(max(load_uniform(p.q_len + cur.b), 0), dm.Sq) : dm.Sq;
     const int64_t tok0 = varlen ? (int64_t)load_uniform(p.q_start + cur.b) : 0;
     const int prefix = MOD ? seq_prefix(p.mod, cur.b, cur.skv) : 0;
-    valid = pos < sq;
-    qpos = pos + (cur.skv - sq);
     qpos_lo = cur.skv - sq;
-    seen = max(qpos, prefix - 1);
     seen_lo = max(qpos_lo, prefix - 1);
     n = ((cur.c1 - cur.c0 + TW - 1) / TW - wave + 3) >> 2;
-    const char* qrow = static_cast<const char*>(p.q.ptr) +
-                       2 * ((varlen ? (tok0 + pos) * p.q.ss : (int64_t)cur.b * p.q.sb + (int64_t)pos * p.q.ss) +
-                            (int64_t)head * p.q.sh + (D / 4) * lg);
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks)
-      qreg[ks] = valid ? *reinterpret_cast<const u32x4*>(qrow + 16 * ks) : u32x4{0u, 0u, 0u, 0u};
+    for (int rb = 0; rb < NR; ++rb) {
+      valid[rb] = pos[rb] < sq;
+      qpos[rb] = pos[rb] + (cur.skv - sq);
+      seen[rb] = max(qpos[rb], prefix - 1);
+      const char* qrow = static_cast<const char*>(p.q.ptr) +
+                         2 * ((varlen ? (tok0 + pos[rb]) * p.q.ss : (int64_t)cur.b * p.q.sb + (int64_t)pos[rb] * p.q.ss) +
+                              (int64_t)head[rb] * p.q.sh + (D / 4) * lg);
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks)
+        qreg[rb][ks] = valid[rb] ? *reinterpret_cast<const u32x4*>(qrow + 16 * ks) : u32x4{0u, 0u, 0u, 0u};
+    }
     look();
     // (Always both, so that the compiler counts on them and waits for the first alone:
     // tiles behind the piece load nothing.)
@@ -230,8 +250,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     issue(1, lb);
   };
 
-  f32x4 acc[NDB];
-  float m_run, l_run;
+  f32x4 acc[NR][NDB];
+  float m_run[NR], l_run[NR];
   // Tile `it` out of its stage, then its stage's next one.
   const auto step = [&](auto issue_c, auto last_c, int it, char* stage) __attribute__((always_inline)) {
     constexpr bool ISSUE = decltype(issue_c)::value;
@@ -244,62 +264,119 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     const char* ck = stage;
     const char* cv = stage + 4096;
-    f32x4 sx[NB];
-#pragma unroll
-    for (int kb = 0; kb < NB; ++kb) {
-      sx[kb] = f32x4{};
-#pragma unroll
-      for (int x = 0; x < NKS / 2; ++x) {
-        const u32x4 raw = *reinterpret_cast<const u32x4*>(ck + kb * 16 * D + ka[x]);
-        sx[kb] = E::mfma16(widen8<DT>(raw[0], sk[kb], raw[1], sk[kb]), qreg[2 * x], sx[kb]);
-        sx[kb] = E::mfma16(widen8<DT>(raw[2], sk[kb], raw[3], sk[kb]), qreg[2 * x + 1], sx[kb]);
-      }
-    }
-    const int key0 = cur.c0 + (4 * it + wave) * TW;
-    float row_t = 0.f;  // added to every score of the lane
-    if constexpr (MOD) {
-      cap_scores<4>(sx, p.mod);
-      if (p.mod.slopes != nullptr)
-        row_t = bias_scores<4>(sx, slope, key0 + 4 * lg - qpos, key0 + TW - 1 <= qpos_lo,
-                               [](int e) { return 16 * (e >> 2) + (e & 3); });
-    }
-    if (key0 + TW > cur.c1 || (dm.causal && key0 + TW - 1 > seen_lo)) {
+    // One row block: all reads of the tile first (32 sequences of up to 8000 keys 34.1 ->
+    // 33.0 us).  Two: where they are used (all first, for the registers they hold, 42.7 ->
+    // 44.1 us in 16 x 8 queries of up to 8000 keys).
+    u32x4 rawk[NB][NKS / 2];
+    u32x2 rawv[NB / 2][NDB];
+    if constexpr (NR == 1) {
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int key = key0 + 16 * kb + 4 * lg + v;
-          const bool off = key >= cur.c1 || (dm.causal && key > seen);
-          sx[kb][v] = off ? -__builtin_inff() : sx[kb][v];
-        }
-    }
-    float mx = fmaxf(fmaxf(sx[0][0], sx[0][1]), fmaxf(sx[0][2], sx[0][3]));
+        for (int x = 0; x < NKS / 2; ++x) rawk[kb][x] = *reinterpret_cast<const u32x4*>(ck + kb * 16 * D + ka[x]);
 #pragma unroll
-    for (int kb = 1; kb < NB; ++kb) mx = fmaxf(vmax3(mx, sx[kb][0], sx[kb][1]), fmaxf(sx[kb][2], sx[kb][3]));
-    mx = xhalf_max(xquad_max(mx + row_t));
-    const float m_new = fmaxf(m_run, mx);
-    const float m_use = (m_new == -__builtin_inff()) ? 0.f : m_new;
-    const float alpha = fast_exp2((m_run - m_use) * c), nmc = (row_t - m_use) * c;
-    float pv[NB][4], rs = 0.f;
+      for (int jj = 0; jj < NB / 2; ++jj)
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) rawv[jj][db] = ld_tr8(cv + 32 * jj * D + (va ^ (uint32_t)(16 * db)));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    f32x4 sx[NR][NB];
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v) pv[kb][v] = fast_exp2(__builtin_fmaf(sx[kb][v], c, nmc));
-      rs += (pv[kb][0] + pv[kb][1]) + (pv[kb][2] + pv[kb][3]);
-    }
-    l_run = l_run * alpha + rs;
-    m_run = m_new;
+      for (int rb = 0; rb < NR; ++rb) sx[rb][kb] = f32x4{};
 #pragma unroll
-    for (int db = 0; db < NDB; ++db) acc[db] *= alpha;
+      for (int x = 0; x < NKS / 2; ++x) {
+        const u32x4 raw = NR == 1 ? rawk[kb][x] : *reinterpret_cast<const u32x4*>(ck + kb * 16 * D + ka[x]);
+        const u32x4 lo = widen8<DT>(raw[0], sk[kb], raw[1], sk[kb]), hi = widen8<DT>(raw[2], sk[kb], raw[3], sk[kb]);
+#pragma unroll
+        for (int rb = 0; rb < NR; ++rb) {
+          sx[rb][kb] = E::mfma16(lo, qreg[rb][2 * x], sx[rb][kb]);
+          sx[rb][kb] = E::mfma16(hi, qreg[rb][2 * x + 1], sx[rb][kb]);
+        }
+      }
+    }
+    const int key0 = cur.c0 + (4 * it + wave) * TW;
+    u32x4 pk[NR][NB / 2];
+    float row_t[NR], mx[NR], nmc[NR], pv[NR][NB][4];
+#pragma unroll
+    for (int rb = 0; rb < NR; ++rb) {
+      row_t[rb] = 0.f;  // added to every score of the lane
+      if constexpr (MOD) {
+        cap_scores<4>(sx[rb], p.mod);
+        if (p.mod.slopes != nullptr)
+          row_t[rb] = bias_scores<4>(sx[rb], slope[rb], key0 + 4 * lg - qpos[rb], key0 + TW - 1 <= qpos_lo,
+                                     [](int e) { return 16 * (e >> 2) + (e & 3); });
+      }
+    }
+    if (key0 + TW > cur.c1 || (dm.causal && key0 + TW - 1 > seen_lo)) {
+#pragma unroll
+      for (int rb = 0; rb < NR; ++rb)
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int key = key0 + 16 * kb + 4 * lg + v;
+            const bool off = key >= cur.c1 || (dm.causal && key > seen[rb]);
+            sx[rb][kb][v] = off ? -__builtin_inff() : sx[rb][kb][v];
+          }
+    }
+    bool lags = false;
+#pragma unroll
+    for (int rb = 0; rb < NR; ++rb) mx[rb] = fmaxf(fmaxf(sx[rb][0][0], sx[rb][0][1]), fmaxf(sx[rb][0][2], sx[rb][0][3]));
+#pragma unroll
+    for (int kb = 1; kb < NB; ++kb)
+#pragma unroll
+      for (int rb = 0; rb < NR; ++rb)
+        mx[rb] = fmaxf(vmax3(mx[rb], sx[rb][kb][0], sx[rb][kb][1]), fmaxf(sx[rb][kb][2], sx[rb][kb][3]));
+#pragma unroll
+    for (int rb = 0; rb < NR; ++rb) mx[rb] = xquad_max(mx[rb] + row_t[rb]);
+#pragma unroll
+    for (int rb = 0; rb < NR; ++rb) mx[rb] = xhalf_max(mx[rb]);
+#pragma unroll
+    for (int rb = 0; rb < NR; ++rb) lags |= (mx[rb] - m_run[rb]) * c > kLag || m_run[rb] == -__builtin_inff();
+    if (__any(lags)) {
+#pragma unroll
+      for (int rb = 0; rb < NR; ++rb) {
+        const float m_new = fmaxf(m_run[rb], mx[rb]);
+        const float alpha = m_new == -__builtin_inff() ? 1.f : fast_exp2((m_run[rb] - m_new) * c);
+        m_run[rb] = m_new;
+        l_run[rb] *= alpha;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) acc[rb][db] *= alpha;
+      }
+    }
+#pragma unroll
+    for (int rb = 0; rb < NR; ++rb) nmc[rb] = (row_t[rb] - (m_run[rb] == -__builtin_inff() ? 0.f : m_run[rb])) * c;
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+      for (int rb = 0; rb < NR; ++rb) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) pv[rb][kb][v] = fast_exp2(__builtin_fmaf(sx[rb][kb][v], c, nmc[rb]));
+      }
+#pragma unroll
+    for (int jj = 0; jj < NB / 2; ++jj)
+#pragma unroll
+      for (int rb = 0; rb < NR; ++rb)
+        pk[rb][jj] = u32x4{E::pack2(pv[rb][2 * jj][0], pv[rb][2 * jj][1]), E::pack2(pv[rb][2 * jj][2], pv[rb][2 * jj][3]),
+                           E::pack2(pv[rb][2 * jj + 1][0], pv[rb][2 * jj + 1][1]),
+                           E::pack2(pv[rb][2 * jj + 1][2], pv[rb][2 * jj + 1][3])};
+#pragma unroll
+    for (int rb = 0; rb < NR; ++rb) {
+      float rs = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) rs += (pv[rb][kb][0] + pv[rb][kb][1]) + (pv[rb][kb][2] + pv[rb][kb][3]);
+      l_run[rb] += rs;
+    }
 #pragma unroll
     for (int jj = 0; jj < NB / 2; ++jj) {
-      const u32x4 pk =
-          u32x4{E::pack2(pv[2 * jj][0], pv[2 * jj][1]), E::pack2(pv[2 * jj][2], pv[2 * jj][3]),
-                E::pack2(pv[2 * jj + 1][0], pv[2 * jj + 1][1]), E::pack2(pv[2 * jj + 1][2], pv[2 * jj + 1][3])};
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
-        const u32x2 raw = ld_tr8(cv + 32 * jj * D + (va ^ (uint32_t)(16 * db)));
-        acc[db] = E::mfma16(widen8<DT>(raw[0], sv[2 * jj], raw[1], sv[2 * jj + 1]), pk, acc[db]);
+        const u32x2 raw = NR == 1 ? rawv[jj][db] : ld_tr8(cv + 32 * jj * D + (va ^ (uint32_t)(16 * db)));
+        const u32x4 w = widen8<DT>(raw[0], sv[2 * jj], raw[1], sv[2 * jj + 1]);
+#pragma unroll
+        for (int rb = 0; rb < NR; ++rb) acc[rb][db] = E::mfma16(w, pk[rb][jj], acc[rb][db]);
       }
     }
     if constexpr (ISSUE) {
@@ -317,68 +394,90 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
   const int rows = dm.G * dm.Sq;
   int done_b = -1;  // the piece whose state the waves hold
-  bool done_valid = false;
+  bool done_valid[NR] = {};
+  // The four waves' states meet and leave as the slot's partials, as many query rows at
+  // a time as the place has room for: kMeet while the next piece's loads are on their
+  // way into the stages, at the slot's end (last) kEnd, in the first stage.  16-byte
+  // chunks of a row are swizzled, so that the lanes of a write cover the banks.
+  const auto join = [&](auto last) __attribute__((always_inline)) {
+    constexpr bool LAST = decltype(last)::value;
+    constexpr int kRows = LAST ? kEnd : kMeet;
+    float* const place = LAST ? reinterpret_cast<float*>(lds_a) : meet;
+    const auto at = [&](int wv, int rl, int chunk) {
+      return place + (wv * kRows + rl) * D + 4 * (chunk ^ (rl & 15));
+    };
+#pragma unroll
+    for (int rb = 0; rb < NR; ++rb) {
+      const float l_tot = xhalf_sum(xquad_sum(l_run[rb]));
+      if (lg == 0) {
+        st_m[wave][16 * rb + i16] = m_run[rb];
+        st_l[wave][16 * rb + i16] = done_valid[rb] ? l_tot : -1.f;
+      }
+    }
+    if constexpr (LAST) {
+      wave_wait<vmcnt_imm(0)>();
+      phase_barrier();
+    }
+    for (int r0 = 0; r0 < rows; r0 += kRows) {
+#pragma unroll
+      for (int rb = 0; rb < NR; ++rb) {
+        const int rl = 16 * rb + i16 - r0;
+        if (rl >= 0 && rl < kRows) {
+#pragma unroll
+          for (int db = 0; db < NDB; ++db) *reinterpret_cast<f32x4*>(at(wave, rl, 4 * db + lg)) = acc[rb][db];
+        }
+      }
+      phase_barrier();
+      for (int f = t; f < min(kRows, rows - r0) * (D / 4); f += 256) {
+        const int rl = f / (D / 4), d4 = f - rl * (D / 4), r = r0 + rl;
+        if (st_l[0][r] < 0.f) continue;
+        float ms = st_m[0][r];
+#pragma unroll
+        for (int x = 1; x < 4; ++x) ms = fmaxf(ms, st_m[x][r]);
+        const float mu = ms == -__builtin_inff() ? 0.f : ms;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float a = fast_exp2((st_m[x][r] - mu) * c);
+          l += a * st_l[x][r];
+          o += a * *reinterpret_cast<const f32x4*>(at(x, rl, d4));
+        }
+        const int ps = fast_div(r, p.div_g.mul, p.div_g.shift);
+        const int64_t row = partial_row(p, true, done_b, kvh * dm.G + r - ps * dm.G, ps, s);
+        *reinterpret_cast<f32x4*>(p.ws_acc + row * D + 4 * d4) = o;
+        if (d4 == 0) {
+          p.ws_m[row] = ms == -__builtin_inff() ? kEmptyRef : __builtin_fmaf(ms, c, MOD ? p.mod.shift2 : 0.f);
+          p.ws_l[row] = l;
+        }
+      }
+      phase_barrier();
+    }
+  };
+  using BT = std::true_type;
+  using BF = std::false_type;
   look();
   if (!nxt.some) return;
   for (;;) {
-    const bool more = nxt.some;
-    if (more) begin();
-    if (done_b >= 0) {
-      // With the next piece's loads on their way the four waves' states meet, kMeet query
-      // rows at a time.
-      const float l_tot = xhalf_sum(xquad_sum(l_run));
-      if (lg == 0) {
-        st_m[wave][i16] = m_run;
-        st_l[wave][i16] = done_valid ? l_tot : -1.f;
-      }
-      for (int r0 = 0; r0 < rows; r0 += kMeet) {
-        if (i16 >= r0 && i16 < r0 + kMeet) {
-          float* to = meet + ((wave * kMeet + i16 - r0) * D + 4 * lg);
+    if (!nxt.some) break;
+    begin();
+    if (done_b >= 0) join(BF{});
 #pragma unroll
-          for (int db = 0; db < NDB; ++db) *reinterpret_cast<f32x4*>(to + 16 * db) = acc[db];
-        }
-        phase_barrier();
+    for (int rb = 0; rb < NR; ++rb) {
 #pragma unroll
-        for (int f = t; f < kMeet * (D / 4); f += 256) {
-          const int rl = f / (D / 4), d4 = f - rl * (D / 4), r = r0 + rl;
-          if (r >= rows || st_l[0][r] < 0.f) continue;
-          float ms = st_m[0][r];
-#pragma unroll
-          for (int x = 1; x < 4; ++x) ms = fmaxf(ms, st_m[x][r]);
-          const float mu = ms == -__builtin_inff() ? 0.f : ms;
-          f32x4 o = {0.f, 0.f, 0.f, 0.f};
-          float l = 0.f;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float a = fast_exp2((st_m[x][r] - mu) * c);
-            l += a * st_l[x][r];
-            o += a * *reinterpret_cast<const f32x4*>(meet + (x * kMeet + rl) * D + 4 * d4);
-          }
-          const int ps = fast_div(r, p.div_g.mul, p.div_g.shift);
-          const int64_t row = partial_row(p, true, done_b, kvh * dm.G + r - ps * dm.G, ps, s);
-          *reinterpret_cast<f32x4*>(p.ws_acc + row * D + 4 * d4) = o;
-          if (d4 == 0) {
-            p.ws_m[row] = ms == -__builtin_inff() ? kEmptyRef : __builtin_fmaf(ms, c, MOD ? p.mod.shift2 : 0.f);
-            p.ws_l[row] = l;
-          }
-        }
-        phase_barrier();
-      }
+      for (int db = 0; db < NDB; ++db) acc[rb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m_run[rb] = -__builtin_inff();
+      l_run[rb] = 0.f;
+      done_valid[rb] = valid[rb];
     }
-    if (!more) break;
-#pragma unroll
-    for (int db = 0; db < NDB; ++db) acc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m_run = -__builtin_inff();
-    l_run = 0.f;
     done_b = cur.b;
-    done_valid = valid;
     wave_wait<vmcnt_imm(2 * NLD)>();  // what came before the first tile's loads
     finish_scales();
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) pin(qreg[ks]);
+    for (int rb = 0; rb < NR; ++rb)
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) pin(qreg[rb][ks]);
     // Tiles in pairs; the last one or two refill nothing.
-    using BT = std::true_type;
-    using BF = std::false_type;
     int it = 0;
     for (; it + 4 <= ((n + 1) & ~1); it += 2) {
       step(BT{}, BF{}, it, la);
@@ -391,7 +490,69 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       step(BF{}, BT{}, it + 1, lb);
     }
   }
-  wave_wait<vmcnt_imm(0)>();  // (no load may be on its way into LDS when the workgroup ends)
+  join(BT{});
+}
+
+// Joins the slots' partials of each row, as gqa_split_reduce_kernel does with a workgroup
+// a row, for sequences that lie in few slots: a row's D / 4 lanes take all of its
+// partials, 1024 / D rows a workgroup.  Rows in the order of the slots' walk, (kv head,
+// sequence, head, query), so that a row is joined on the XCD that wrote its partials.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void gqa_decode8_join_kernel(ReduceParams p, FastDiv div_g, int G) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  constexpr int ND4 = D / 4, R = 256 / ND4, BATCH = 4;
+  const int t = threadIdx.x, d4 = t % ND4, bg = p.B * G;
+  const int x = xcd_remap(blockIdx.x, gridDim.x) * R + t / ND4;
+  const int xh = fast_div(x, p.div_sq.mul, p.div_sq.shift), pos = x - xh * p.Sq;
+  const int kvh = fast_div(xh, p.div_total.mul, p.div_total.shift), xb = xh - kvh * bg;
+  const int b = fast_div(xb, div_g.mul, div_g.shift), h = kvh * G + xb - b * G;
+  if (h >= p.Hq) return;
+  const bool varlen = p.q_len != nullptr;
+  if (varlen && pos >= p.q_len[b]) return;
+  const int64_t step = (int64_t)p.Hq * p.Sq;
+  const int S = p.plan[2 * b + 1];
+  const int64_t row0 = p.plan[2 * b] * step + (int64_t)h * p.Sq + pos;
+  const float *wm = p.ws_m + row0, *wl = p.ws_l + row0, *wa = p.ws_acc + row0 * D + 4 * d4;
+  float m = kEmptyRef, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < S; s0 += BATCH) {
+    float mv[BATCH], lv[BATCH];
+    f32x4 av[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int s = s0 + k;
+      mv[k] = kEmptyRef;
+      lv[k] = 0.f;
+      av[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (s < S) {
+        mv[k] = wm[s * step];
+        lv[k] = wl[s * step];
+        av[k] = *reinterpret_cast<const f32x4*>(wa + s * step * D);
+      }
+    }
+    const float mb = fmaxf(fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])), m);
+    const float keep = fast_exp2(m - mb);
+    l *= keep;
+    o *= keep;
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const float a = fast_exp2(mv[k] - mb);
+      l += a * lv[k];
+      o += a * av[k];
+    }
+    m = mb;
+  }
+  const int64_t tok = varlen ? (int64_t)p.q_start[b] + pos : 0;
+  if (p.lse != nullptr && d4 == 0)
+    p.lse[varlen ? tok * p.Hq + h : ((int64_t)b * p.Hq + h) * p.Sq + pos] = (m + __log2f(l)) * kLn2;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;  // (a row that sees no key: zeros)
+  T* orow = static_cast<T*>(const_cast<void*>(p.o.ptr)) + (int64_t)h * p.o.sh +
+            (varlen ? tok * p.o.ss : (int64_t)b * p.o.sb + (int64_t)pos * p.o.ss);
+  u32x2 y;
+  y[0] = E::pack2(o[0] * inv, o[1] * inv);
+  y[1] = E::pack2(o[2] * inv, o[3] * inv);
+  *reinterpret_cast<u32x2*>(orow + 4 * d4) = y;
 }
 
 template <int DT, int D> static hipError_t launch_decode8_t(Split8Params p, hipStream_t stream) {
@@ -406,8 +567,13 @@ template <int DT, int D> static hipError_t launch_decode8_t(Split8Params p, hipS
   const ScoreMod& m = p.mod;
   const bool changed = m.cap_exp != 0.f || m.cap != 0.f || m.slopes != nullptr || m.prefix != nullptr;
   const dim3 grid((unsigned)(total + 1)), block(256);
-  if (changed) hipLaunchKernelGGL((gqa_decode8_kernel<DT, D, true>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((gqa_decode8_kernel<DT, D, false>), grid, block, 0, stream, p);
+  if (p.dm.G * p.dm.Sq <= 16) {
+    if (changed) hipLaunchKernelGGL((gqa_decode8_kernel<DT, D, 1, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((gqa_decode8_kernel<DT, D, 1, false>), grid, block, 0, stream, p);
+  } else {
+    if (changed) hipLaunchKernelGGL((gqa_decode8_kernel<DT, D, 2, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((gqa_decode8_kernel<DT, D, 2, false>), grid, block, 0, stream, p);
+  }
   return hipGetLastError();
 }
 
@@ -415,6 +581,29 @@ hipError_t launch_decode8(const Split8Params& p, int dtype, hipStream_t stream) 
   if (p.dm.G * p.dm.Sq > kDecode8Rows || p.block_shift < 4) return hipErrorInvalidValue;
   if (dtype == 0) return p.dm.D == 128 ? launch_decode8_t<0, 128>(p, stream) : launch_decode8_t<0, 64>(p, stream);
   return p.dm.D == 128 ? launch_decode8_t<1, 128>(p, stream) : launch_decode8_t<1, 64>(p, stream);
+}
+
+template <int DT, int D> static hipError_t launch_join_t(ReduceParams p, int G, hipStream_t stream) {
+  const int64_t rows = (int64_t)p.B * p.Hq * p.Sq, wgs = (rows * (D / 4) + 255) / 256;
+  if (rows <= 0 || rows >= (int64_t)1 << 30) return hipErrorInvalidValue;
+  p.div_sq = make_fast_div((uint32_t)p.Sq);
+  p.div_total = make_fast_div((uint32_t)(p.B * G));
+  hipLaunchKernelGGL((gqa_decode8_join_kernel<DT, D>), dim3((unsigned)wgs), dim3(256), 0, stream, p,
+                     make_fast_div((uint32_t)G), G);
+  return hipGetLastError();
+}
+
+// Slots a sequence, on average, up to which its rows share a workgroup.  A workgroup a row
+// / this, us a call, head_dim 128 of 32 heads over 8: 256 sequences of up to 300 keys (0.25
+// slots each) 48.6 / 37.6, 64 of 1000 (1) 29.1 / 26.5, 16 of 4000 (4) 26.6 / 25.8, with 8
+// queries each 48.5 / 43.0; 8 of 4000 (8) 18.0 / 18.0 and 33.1 / 30.3; 4 of 8000 (16) 17.1
+// / 18.6; 2 of 16000 (32) 17.9 / 22.5.
+constexpr int kFewSlots = 8;
+
+hipError_t launch_decode8_join(const ReduceParams& p, int G, int dtype, hipStream_t stream) {
+  if (p.slots > kFewSlots * p.B) return launch_split_reduce(p, dtype, stream);
+  if (dtype == 0) return p.D == 128 ? launch_join_t<0, 128>(p, G, stream) : launch_join_t<0, 64>(p, G, stream);
+  return p.D == 128 ? launch_join_t<1, 128>(p, G, stream) : launch_join_t<1, 64>(p, G, stream);
 }
 
 }  // namespace gqa

@@ -32,7 +32,7 @@ __all__ = ["CODES", "MIN_EXPONENT", "MAX_EXPONENT", "read_kv"]
 CODES = torch.float8_e4m3fn
 MIN_EXPONENT, MAX_EXPONENT = _lib.GQA_MIN_EXPONENT, _lib.GQA_MAX_EXPONENT
 MIN_BLOCK = 16
-FEW_ROWS = 16  # packed rows per kv head up to which a call takes the flat split
+FEW_ROWS = 32  # packed rows per kv head up to which a call takes the flat split
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 _ROUTES = {"split": _lib.FORM_FLAT, "chunks": _lib.FORM_CHUNKS, "single": _lib.FORM_SINGLE}
 _LOG2E = math.log2(math.e)

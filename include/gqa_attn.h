@@ -617,7 +617,7 @@ typedef struct gqa_cache8 {
  * the cache's values in it.  score: as gqa_paged_scored_launch, or NULL.  A row
  * that sees no key gives zeros and LSE -inf.  Groups of at most 128 query heads.
  * gqa_paged8_plan: the form that a call of these sizes takes on a device of
- * cu_count compute units, GQA_FORM_FLAT (`parts` slots, up to 16 packed rows a kv
+ * cu_count compute units, GQA_FORM_FLAT (`parts` slots, up to 32 packed rows a kv
  * head), GQA_FORM_CHUNKS (`parts` key chunks) or GQA_FORM_SINGLE (0).  Others may
  * be given, within those limits and GQA_MAX_SPLITS.  workspace: 16-byte aligned,
  * gqa_paged8_workspace_bytes bytes (0: NULL). */

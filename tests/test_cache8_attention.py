@@ -63,9 +63,9 @@ MANY = [("chunks", 1), ("chunks", 2), ("chunks", 5), ("single", None), None]
 @pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("bs", [16, 32, 64, 256])
-@pytest.mark.parametrize("Hq,Hkv,Sq", [(32, 8, 1), (8, 8, 1), (7, 1, 2), (16, 1, 1), (6, 2, 5), (4, 4, 16)])
+@pytest.mark.parametrize("Hq,Hkv,Sq", [(32, 8, 1), (8, 8, 1), (7, 1, 2), (16, 1, 1), (6, 2, 5), (4, 4, 16), (32, 8, 8), (23, 1, 1), (6, 2, 7), (2, 2, 32)])
 def test_few_rows(Hq, Hkv, Sq, bs, D, dtype):
-    """Up to 16 packed rows; lengths from none over one, a tile's ends and a unit's to many; every route."""
+    """Up to 16 and up to 32 packed rows; lengths from none over one, a tile's ends and a unit's to many; every route."""
     lens = [0, 1, Sq, 15, 16, 17, 31, 33, 127, 128, 129, 255, 300, 1000]
     Batch(lens, Hq, Hkv, Sq, D, bs, dtype, seed=Sq).check(FEW)
 
@@ -81,21 +81,21 @@ def test_many_rows(Hq, Hkv, Sq, lens, D, dtype):
     Batch(lens, Hq, Hkv, Sq, D, 16 if Sq % 2 else 64, dtype, seed=Sq, layout="HND" if Sq % 3 else "NHD").check(MANY)
 
 
-@pytest.mark.parametrize("Hq,Hkv,Sq", [(8, 2, 1), (8, 2, 4), (8, 2, 40)])
+@pytest.mark.parametrize("Hq,Hkv,Sq", [(8, 2, 1), (8, 2, 4), (8, 2, 6), (8, 2, 40)])
 @pytest.mark.parametrize("D", [64, 128])
 def test_without_a_mask(Hq, Hkv, Sq, D):
     Batch([1, 50, 3 * 64, 700], Hq, Hkv, Sq, D, 16).check((None, ("single", None), ("chunks", 3)), causal=False)
 
 
 @pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp16"])
-@pytest.mark.parametrize("Hq,Hkv,Sq", [(16, 4, 1), (16, 4, 4), (16, 4, 50)])
+@pytest.mark.parametrize("Hq,Hkv,Sq", [(16, 4, 1), (16, 4, 4), (16, 4, 7), (16, 4, 50)])
 @pytest.mark.parametrize("D", [64, 128])
 def test_changed_scores(Hq, Hkv, Sq, D, dtype):
     lens = [1, 70, 129, 640, 0, 333]
     b = Batch(lens, Hq, Hkv, Sq, D, 32, dtype, seed=3, scale=2.0)
     slopes = torch.tensor([2.0 ** (-8 * (h + 1) / Hq) for h in range(Hq)]).cuda()
     prefix = ints([0, 50, 200, 640, 5, -3])
-    routes = (None, ("single", None), ("chunks", 4)) + ((("split", 5),) if Hq // Hkv * Sq <= 16 else ())
+    routes = (None, ("single", None), ("chunks", 4)) + ((("split", 5),) if Hq // Hkv * Sq <= 32 else ())
     for kw in (dict(softcap=20.0), dict(softcap=500.0), dict(slopes=slopes), dict(prefix=prefix), dict(softcap=30.0, slopes=slopes, prefix=prefix)):
         b.check(routes, **kw)
 
@@ -286,7 +286,7 @@ def test_refusals():
         with pytest.raises(_lib.GQAError):
             paged_attention(**{**a, **kw})
     with pytest.raises(_lib.GQAError):  # more rows than the flat split takes
-        paged_attention(**{**a, "q": rand(2, 8, 5, 64), "route": "split"})
+        paged_attention(**{**a, "q": rand(2, 8, 9, 64), "route": "split"})
     with pytest.raises(NotImplementedError):
         paged_attention(**{**a, "q": b.q.clone().requires_grad_()})
     wide = Batch([40], 2 * 129, 2, 1, 64, 16)

@@ -40,7 +40,7 @@ def test_attention_refusals(lib):
     for kw, code in BAD_CACHES:
         assert attend(lib, k=cache(**kw)) == code and attend(lib, v=cache(**kw)) == code, kw
     for kw in (dict(block=8), dict(block=0), dict(block=24), dict(block=1 << 17), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
-               dict(scale=float("inf")), dict(form=0), dict(form=4), dict(form=7), dict(form=3, parts=1, seq_q=5), dict(form=3, parts=1, max_len=0)):
+               dict(scale=float("inf")), dict(form=0), dict(form=4), dict(form=7), dict(form=3, parts=1, seq_q=9), dict(form=3, parts=1, max_len=0)):
         assert attend(lib, **kw) == E8, kw
     for kw in (dict(form=2, parts=0), dict(form=2, parts=1025), dict(form=3, parts=0), dict(form=3, parts=1025)):
         assert attend(lib, **kw) == SPLITS, kw
@@ -91,10 +91,10 @@ def test_write_and_read_refusals(lib):
 
 def test_plans_keep_their_limits(lib):
     for D in (64, 128):
-        for batch, heads, kv, sq, n in ((1, 32, 8, 1, 1), (1, 32, 8, 1, 131072), (256, 32, 8, 1, 4000), (3, 8, 8, 16, 77), (1, 128, 1, 1, 500), (7, 28, 4, 9, 8192),
+        for batch, heads, kv, sq, n in ((1, 32, 8, 1, 1), (1, 32, 8, 1, 131072), (256, 32, 8, 1, 4000), (3, 8, 8, 16, 77), (1, 128, 1, 1, 500), (7, 28, 4, 9, 8192), (16, 32, 8, 8, 4000), (2, 31, 1, 1, 3000), (2, 11, 1, 3, 900),
                                         (4, 32, 8, 256, 9000), (1, 32, 8, 4096, 4096), (2, 64, 1, 2, 1 << 20), (1 << 16, 8, 8, 1, 1 << 20)):
             form, parts = cache8.plan(batch, heads, kv, sq, n, D, 256)
-            few = heads // kv * sq <= 16
+            few = heads // kv * sq <= 32
             assert form == (_lib.FORM_FLAT if few else form) and 0 <= parts <= 1024
             assert (form == _lib.FORM_SINGLE) == (parts == 0)
             if form == _lib.FORM_FLAT:
@@ -106,7 +106,7 @@ def test_plans_keep_their_limits(lib):
     for bad in ((1, 7, 2, 1, 64, 128, 256), (1, 8, 2, 1, 64, 96, 256), (-1, 8, 2, 1, 64, 128, 256), (1, 258, 2, 1, 64, 128, 256), (1, 8, 2, 1, 64, 128, 0)):
         with pytest.raises(_lib.GQAError):
             cache8.plan(*bad)
-    assert cache8.route(32, 8, 4) == "split" and cache8.route(32, 8, 5) == "single"
+    assert cache8.route(32, 8, 8) == "split" and cache8.route(32, 8, 9) == "single"
 
 
 def test_python_refusals():
