@@ -44,6 +44,11 @@ bool flat_fits(int batch, int max_seq_len, int head_dim, int slots) {
   return (units * batch + 1) * (slots + 1) < ((int64_t)1 << 31);
 }
 
+// Tiles of all sequences that the cut into key pieces can add up in 32 bits.
+bool pieces_fit(int batch, int max_seq_len) {
+  return ((int64_t)max_seq_len + kTile - 1) / kTile * batch < ((int64_t)1 << 31) - GQA_MAX_SPLITS;
+}
+
 }  // namespace
 
 extern "C" {
@@ -70,21 +75,20 @@ int gqa_paged8_plan(int batch, int num_heads, int num_kv_heads, int seq_q, int m
       return GQA_OK;
     }
   }
-  const int block_m = gqa::kShortRows / G;
-  const int64_t items = ((int64_t)seq_q + block_m - 1) / block_m * num_kv_heads * batch;
-  const int tiles = (max_seq_len + kTile - 1) / kTile;
-  const int64_t chunks = std::min<int64_t>({2 * cu_count / items, tiles / 4, GQA_MAX_SPLITS});
-  if (chunks >= 2) {
+  const int rows = gqa::chunk8_rows((int64_t)G * seq_q), block_m = rows / G;
+  const int64_t blocks = ((int64_t)seq_q + block_m - 1) / block_m * num_kv_heads;
+  const int64_t tiles = (max_seq_len + kTile - 1) / kTile;
+  const int64_t pieces = std::min<int64_t>({(rows > gqa::kShortRows ? 1 : 2) * cu_count / blocks, batch * (tiles / 4), GQA_MAX_SPLITS});
+  if (2 * pieces >= 3 * (int64_t)batch && pieces_fit(batch, max_seq_len)) {
     *form = GQA_FORM_CHUNKS;
-    *parts = (int)chunks;
+    *parts = (int)pieces;
   }
   return GQA_OK;
 }
 
 size_t gqa_paged8_workspace_bytes(int form, int parts, int batch, int num_heads, int seq_q, int head_dim) {
-  if (form == GQA_FORM_FLAT) return gqa_split_flat_workspace_bytes(batch, num_heads, seq_q, head_dim, parts);
-  if (form == GQA_FORM_CHUNKS) return gqa_split_workspace_bytes(batch, num_heads, seq_q, head_dim, parts);
-  return 0;
+  if (form != GQA_FORM_FLAT && form != GQA_FORM_CHUNKS) return 0;
+  return gqa_split_flat_workspace_bytes(batch, num_heads, seq_q, head_dim, parts);
 }
 
 int gqa_paged8_launch(int form, const void* q, const int64_t q_stride[4], const gqa_cache8* k_cache,
@@ -103,6 +107,7 @@ int gqa_paged8_launch(int form, const void* q, const int64_t q_stride[4], const 
   if (form == GQA_FORM_FLAT && ((int64_t)G * seq_q > gqa::kDecode8Rows || max_seq_len < 1)) return GQA_E_CACHE8;
   if (form != GQA_FORM_SINGLE && (parts < 1 || parts > GQA_MAX_SPLITS)) return GQA_E_SPLITS;
   if (form == GQA_FORM_FLAT && !flat_fits(batch, max_seq_len, head_dim, parts)) return GQA_E_CACHE8;
+  if (form == GQA_FORM_CHUNKS && (parts < batch || !pieces_fit(batch, max_seq_len))) return GQA_E_SPLITS;
   gqa::ScoreMod mod{};
   if (score != nullptr) {
     if ((rc = gqa::score_mod(score, scale_log2, causal, true, seq_q, max_seq_len, mod))) return rc;
@@ -172,7 +177,7 @@ int gqa_paged8_launch(int form, const void* q, const int64_t q_stride[4], const 
   p.v = cache_ref(vc);
   p.o = r.o;
   p.dm = dm;
-  p.block_m = gqa::kShortRows / G;
+  p.block_m = gqa::chunk8_rows((int64_t)G * seq_q) / G;
   p.n_mblk = (seq_q + p.block_m - 1) / p.block_m;
   p.block_table = block_table;
   p.seq_lens = seq_lens;
@@ -188,16 +193,18 @@ int gqa_paged8_launch(int form, const void* q, const int64_t q_stride[4], const 
     return gqa::to_code(gqa::launch_chunk8(p, dtype, st));
   }
   p.kv_splits = parts;
-  p.kv_chunk_tiles = std::max(((max_seq_len + kTile - 1) / kTile + parts - 1) / parts, 1);
-  const size_t rows = (size_t)batch * num_heads * seq_q * parts;
+  const size_t rows = ((size_t)parts + batch) * num_heads * seq_q;
   p.ws_acc = workspace;
   p.ws_m = workspace + rows * head_dim;
   p.ws_l = p.ws_m + rows;
+  p.plan = reinterpret_cast<int*>(p.ws_l + rows);
   if ((rc = gqa::to_code(gqa::launch_chunk8(p, dtype, st)))) return rc;
   r.ws_acc = p.ws_acc;
   r.ws_m = p.ws_m;
   r.ws_l = p.ws_l;
-  return gqa::to_code(gqa::launch_scored_combine(r, dtype, st));
+  r.plan = p.plan;
+  r.slots = parts;
+  return gqa::to_code(gqa::launch_decode8_join(r, G, dtype, st));
 }
 
 int gqa_cache8_write_launch(const void* q, const int64_t q_stride[3], const void* k, const int64_t k_stride[3],

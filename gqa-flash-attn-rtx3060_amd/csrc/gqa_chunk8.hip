@@ -2,32 +2,102 @@
 // query rows than gqa_decode8.hip takes: verification of drafts, chunks of prompts,
 // whole prompts.
 //
-// Rows, products, softmax, changed scores and the key chunks' partials are those of
-// gqa_scored.hip: 128 packed rows in four waves, S^T = K Q^T and O^T += V^T P^T by
-// 32x32x16 MFMAs over 64-key tiles, lazily rescaled online softmax.  What differs is
-// the way of a tile into LDS: its codes are loaded into registers a phase ahead,
-// widened there to the queries' type with their page's power of two (exact), and
-// stored in the swizzled layout of the 16-bit tiles.  A workgroup widens a code once,
-// for all four waves: an instruction per two codes, 32 a lane and tile beside the
-// softmax of 32 scores.  (Each wave widening what it reads from LDS would take four
-// times as many.)  Registers are the second stage, so K and V have one each in LDS.
+// Rows, products, softmax and changed scores are those of gqa_scored.hip: 128 packed
+// rows in four waves, S^T = K Q^T and O^T += V^T P^T by 32x32x16 MFMAs over 64-key
+// tiles, lazily rescaled online softmax.  What differs is the way of a tile into LDS:
+// its codes are loaded into registers a phase ahead, widened there to the queries' type
+// with their page's power of two (exact), and stored in the swizzled layout of the
+// 16-bit tiles.  A workgroup widens a code once, for all of its waves: an instruction
+// per two codes.  (Each wave widening what it reads from LDS would take as many times
+// that as there are waves.)
 //
-// Tile j: MFMA phase (P V of the tile before, S of this one), barrier, softmax
-// phase, which first stores K(j + 1) and V(j) where K(j) and V(j - 1) were, then
-// loads K(j + 2) and V(j + 1); barrier.
+// One group of four waves, tile j: MFMA phase (P V of the tile before, S of this one),
+// which first loads the codes of K(j + 1) and V(j), barrier, softmax phase, which ends by
+// storing them where K(j) and V(j - 1) were; barrier.  K and V have one stage each.  Two
+// groups, for more than 256 packed rows: group 1 is a phase behind group 0, so that one's
+// MFMAs run beside the other's softmax on each SIMD; group 0 fills K's stages, group 1
+// V's, two of each.  That halves what a row pays for loads, widening and LDS writes, which
+// are most of what the cache in 8 bits costs over one in 16: 2048 queries over 16384
+// keys, 32 heads over 8, 550 us for one group and 503 for two (390 without loads and
+// stores, 443 the 16-bit kernel).  Up to 256 rows the finer blocks win (8 x 64 queries over
+// 1000-4000 keys 44.6 us / 49.8).  Loading in the softmax phase took 4 % more, pages and
+// exponents by scalar loads instead of by lane 1 %, and storing first there another 5 %.
 #include <algorithm>
 #include <type_traits>
 
 #include "gqa_cache8.hpp"
+#include "gqa_decode_kernel.hpp"
 #include "gqa_fwd_parts.hpp"
 #include "gqa_lds.hpp"
 #include "gqa_score.hpp"
 
 namespace gqa {
 
-// KC: key chunks (p.kv_splits > 0), whose partials launch_scored_combine joins.
-template <int DT, int D, bool KC>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void gqa_chunk8_kernel(Fwd8Params p) {
+namespace {
+
+constexpr int kTileKeys = FwdStage<64>::kKeys;
+static_assert(kTileKeys == FwdStage<128>::kKeys, "tiles of both head dimensions");
+
+// How a call over key pieces (p.kv_splits of them, at least one a sequence) cuts its
+// sequences: into pieces of `tiles` tiles, the fewest of which there are not more than
+// p.kv_splits, counted from the lengths by every wave for itself (gqa_flat.hpp cuts at
+// equal shares, through the middle of what many query blocks read).  The shares of equal
+// chunks of the longest sequence, most of them empty or short, cost 4 x 256 queries over
+// 2000-9000 keys 143 us for 2 chunks, 120 for 3 and 154 for 4, and these pieces 111.
+struct Pieces {
+  const Fwd8Params& p;
+  int lane, tiles;
+
+  // Tiles of sequence g0 + lane (none without queries).
+  __device__ int tiles_of(int g0) const {
+    const int s = g0 + lane;
+    if (s >= p.dm.B || (p.q_len != nullptr && p.q_len[s] <= 0)) return 0;
+    return (min(max(p.seq_lens[s], 0), p.dm.Skv) + kTileKeys - 1) / kTileKeys;
+  }
+  __device__ static int last(int x) { return __builtin_amdgcn_readlane(x, 63); }
+
+  __device__ Pieces(const Fwd8Params& p, int lane) : p(p), lane(lane) {
+    int total = 0, longest = 1;
+    for (int g0 = 0; g0 < p.dm.B; g0 += 64) {
+      const int t = tiles_of(g0);
+      total += last(wave_scan(t));
+      longest = max(longest, wave_max(t));
+    }
+    // A candidate a lane, from the equal share up in steps of a sixteenth; the last one
+    // always does.
+    const int share = max((total + p.kv_splits - 1) / p.kv_splits, 1);
+    const int mine = lane == 63 ? longest : share + lane * ((share + 15) / 16);
+    const float inv = 1.0f / (float)mine;
+    int count = 0;
+    for (int g0 = 0; g0 < p.dm.B; g0 += 64) {
+      const int t = tiles_of(g0), n = min(p.dm.B - g0, 64);
+      for (int l = 0; l < n; ++l) {
+        const int x = __builtin_amdgcn_readlane(t, l), q = (int)((float)x * inv), r = x - q * mine;
+        count += q + (r > 0) + (r > mine) - (r <= -mine);  // ceil(x / mine): q is off by at most one
+      }
+    }
+    const uint64_t fits = __builtin_amdgcn_ballot_w64(count <= p.kv_splits || lane == 63);
+    tiles = __builtin_amdgcn_readlane(mine, __builtin_ffsll((long long)fits) - 1);
+  }
+
+  // f(sequence of the lane, its first piece, its pieces), by 64 sequences, until it
+  // returns true.
+  template <class F> __device__ void each(F f) const {
+    int before = 0;
+    for (int g0 = 0; g0 < p.dm.B; g0 += 64) {
+      const int n = (tiles_of(g0) + tiles - 1) / tiles, upto = wave_scan(n);
+      if (f(g0, before + upto - n, n)) return;
+      before += last(upto);
+    }
+  }
+};
+
+}  // namespace
+
+// NG: groups of four waves, 128 rows each.  KC: over key pieces, whose partials
+// launch_decode8_join joins by the plan that one workgroup past the others writes.
+template <int DT, int D, int NG, bool KC>
+__global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) void gqa_chunk8_kernel(Fwd8Params p) {
   using E = Elem<DT>;
   using T = typename E::T;
   using ST = FwdStage<D>;
@@ -38,27 +108,58 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g
   constexpr int CPR8 = D / 16;  // 16-code chunks per row
   constexpr int RPL = 64 / CPR8;  // rows per load of a wave: 8 or 16
   constexpr int NL = 16 / RPL;    // loads of a wave's 16 rows
-  __shared__ __attribute__((aligned(1024))) char lds0_v[TB];
-  __shared__ __attribute__((aligned(1024))) char lds1_k[TB];
+  __shared__ __attribute__((aligned(1024))) char lds[2 * NG * TB];  // NG stages of K, then of V
 
   const Dims& dm = p.dm;
   const int t = threadIdx.x, lane = t & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6) & 3;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6) & (4 * NG - 1);
+  const int group = NG == 2 ? wave >> 2 : 0, gw = wave & 3;
   const int i = lane & 31, hh = lane >> 5;
   const bool varlen = p.q_len != nullptr;
 
-  // Work item: as gqa_scored.hip.
-  const int n_items = KC ? p.n_mblk * p.kv_splits : p.n_mblk;
-  const int w = xcd_remap(blockIdx.x, n_items * dm.Hkv * dm.B);
-  int bh, mrank, chunk = 0;
-  item_of(p, w, n_items, bh, mrank);
-  if (p.xcd_heads > 1) bh = turned_pair(p, bh, mrank);
+  // Work item: as gqa_scored.hip, or (kv head, piece, query block), so that the blocks
+  // that read a piece are neighbours on an XCD.
+  int b, kvh, mrank, piece = 0, tb = 0, piece_tiles = 0;
   if constexpr (KC) {
-    chunk = fast_div(mrank, p.div_mblk.mul, p.div_mblk.shift);
-    mrank -= chunk * p.n_mblk;
+    const int total = dm.Hkv * p.kv_splits * p.n_mblk;
+    const Pieces pieces(p, lane);
+    if (blockIdx.x == (unsigned)total) {
+      if (wave == 0) {
+        pieces.each([&](int g0, int first, int n) {
+          if (g0 + lane < dm.B) {  // (within the partials whatever the lengths did meanwhile)
+            p.plan[2 * (g0 + lane)] = min(first, p.kv_splits);
+            p.plan[2 * (g0 + lane) + 1] = min(n, p.kv_splits - min(first, p.kv_splits));
+          }
+          return false;
+        });
+      }
+      return;
+    }
+    const int w = xcd_remap(blockIdx.x, total);
+    const int rest = fast_div(w, p.div_mblk.mul, p.div_mblk.shift);
+    mrank = w - rest * p.n_mblk;
+    kvh = fast_div(rest, p.div_items.mul, p.div_items.shift);
+    piece = rest - kvh * p.kv_splits;
+    b = -1;
+    pieces.each([&](int g0, int first, int n) {
+      const uint64_t at = __builtin_amdgcn_ballot_w64(first <= piece && piece < first + n);
+      if (at == 0) return false;
+      const int l = __builtin_ffsll((long long)at) - 1;
+      b = g0 + l;
+      tb = (piece - __builtin_amdgcn_readlane(first, l)) * pieces.tiles;
+      return true;
+    });
+    if (b < 0) return;  // (fewer pieces)
+    piece_tiles = pieces.tiles;
+  } else {
+    const int w = xcd_remap(blockIdx.x, p.n_mblk * dm.Hkv * dm.B);
+    int bh;
+    item_of(p, w, p.n_mblk, bh, mrank);
+    if (p.xcd_heads > 1) bh = turned_pair(p, bh, mrank);
+    b = fast_div(bh, p.div_hkv.mul, p.div_hkv.shift);
+    kvh = bh - b * dm.Hkv;
   }
   const int pid_m = dm.causal ? p.n_mblk - 1 - mrank : mrank;
-  const int b = fast_div(bh, p.div_hkv.mul, p.div_hkv.shift), kvh = bh - b * dm.Hkv;
   const int skv = min(max(load_uniform(p.seq_lens + b), 0), dm.Skv);
   const int sq = varlen ? min(max(load_uniform(p.q_len + b), 0), dm.Sq) : dm.Sq;
   const int64_t tok0 = varlen ? (int64_t)load_uniform(p.q_start + b) : 0;
@@ -76,69 +177,102 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g
   const RowSpan span = row_span(p.mod, dm, b, skv, sq, pos_lo, pos_hi, pos, valid, lane, hh);
   float slope = row_slope(p.mod, head);
   // Tiles [tb, tb + n) of this item.
-  int tb = 0, n = (span.end + ST::kKeys - 1) / ST::kKeys;
-  if constexpr (KC) {
-    tb = chunk * p.kv_chunk_tiles;
-    n = max(min(n - tb, p.kv_chunk_tiles), 0);
-  }
-  // The chunk's partial of this lane's row, in the split workspace's layout.
-  const int64_t part = (((int64_t)b * dm.Hq + head) * dm.Sq + pos) * p.kv_splits + chunk;
-  if (KC && n == 0) {  // (no sum: the combine reads nothing else of it)
-    if (valid && hh == 0) {
-      p.ws_m[part] = kEmptyRef;
-      p.ws_l[part] = 0.f;
+  int n = (span.end + ST::kKeys - 1) / ST::kKeys;
+  if constexpr (KC) n = max(min(n - tb, piece_tiles), 0);
+  // The piece's partial of this lane's row, in the flat split's layout.
+  const int64_t part = ((int64_t)piece * dm.Hq + head) * dm.Sq + pos;
+  if (KC && n == 0) {  // (behind the last key that the block sees)
+    if (valid) {
+      for (int d = 4 * hh; d < D; d += 8) *reinterpret_cast<f32x4*>(p.ws_acc + part * D + d) = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (hh == 0) {
+        p.ws_m[part] = kEmptyRef;
+        p.ws_l[part] = 0.f;
+      }
     }
     return;
   }
   const bool back = p.mod.slopes != nullptr && dm.causal;
   const auto tile_of = [&](int j) __attribute__((always_inline)) { return tile_at(tb, n, j, back); };
 
-  // This wave's rows of a tile: 16 wave + 0..15, which lie in one page.  Rows past the
-  // item's last key, or the last that the block sees, load as zeros.
+  // This wave's rows of a tile: 16 gw + 0..15, which lie in one page.  Rows past the
+  // item's last key, or the last that the block sees, load as zeros.  One group: of K
+  // and of V; two: group 0's are K's, group 1's V's.
+  constexpr int NOP = NG == 1 ? 2 : 1;
   const int rows_ld = KC ? min(span.end, (tb + n) * ST::kKeys) : span.end;
-  const uint32_t kss = (uint32_t)p.k.ss, vss = (uint32_t)p.v.ss;
+  const bool of_v = NG == 2 && group == 1;
   const char* kbh = static_cast<const char*>(p.k.ptr) + (int64_t)kvh * p.k.sh;
   const char* vbh = static_cast<const char*>(p.v.ptr) + (int64_t)kvh * p.v.sh;
   const int* keb = p.ke.e + kvh * p.ke.sh;
   const int* veb = p.ve.e + kvh * p.ve.sh;
+  const char* const op_base[2] = {of_v ? vbh : kbh, vbh};
+  const int64_t op_sb[2] = {of_v ? p.v.sb : p.k.sb, p.v.sb};
+  const uint32_t op_ss[2] = {(uint32_t)(of_v ? p.v.ss : p.k.ss), (uint32_t)p.v.ss};
+  const int* const op_e[2] = {of_v ? veb : keb, veb};
+  const int64_t op_eb[2] = {of_v ? p.ve.sb : p.ke.sb, p.ve.sb};
   const int* table_row = p.block_table + (int64_t)b * p.table_stride;
-  const auto page_of = [&](int j) __attribute__((always_inline)) {  // (-1: no rows)
-    const int key = tile_of(j) * ST::kKeys + 16 * wave;
-    return key < rows_ld ? load_uniform(table_row + (key >> p.block_shift)) : -1;
+  // Pages (-1: no rows) and scales of this wave's rows of tiles base .. base + 63, a tile
+  // a lane.
+  int base = 0, page_l;
+  float scale_l[NOP];
+  const auto look = [&](int from) __attribute__((always_inline)) {
+    base = from;
+    const int key = tile_of(from + lane) * ST::kKeys + 16 * gw;
+    page_l = key < rows_ld ? table_row[key >> p.block_shift] : -1;
+#pragma unroll
+    for (int o = 0; o < NOP; ++o)
+      scale_l[o] = exp_scale(clamp_exp(page_l >= 0 ? op_e[o][(int64_t)page_l * op_eb[o]] : 0));
+    pin(page_l);
+#pragma unroll
+    for (int o = 0; o < NOP; ++o) pin(scale_l[o]);
   };
-  const auto scale_of = [&](const int* e, int64_t sb, int page) __attribute__((always_inline)) {
-    return page < 0 ? 1.f : exp_scale(clamp_exp(load_uniform(e + (int64_t)page * sb)));
+  const auto page_of = [&](int j) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(page_l, j - base); };
+  const auto scale_of = [&](int o, int j) __attribute__((always_inline)) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scale_l[o]), j - base));
   };
   const int lrow = lane / CPR8, lch = lane % CPR8;
-  const auto load = [&](u32x4 (&x)[NL], const char* head_ptr, int64_t sb, uint32_t ss, int j, int page)
-                        __attribute__((always_inline)) {
-    const int key = tile_of(j) * ST::kKeys + 16 * wave, rows = rows_ld - key;
-    __amdgpu_buffer_rsrc_t rt = make_rsrc(head_ptr, 0u);
+  u32x4 rx[NOP][NL];
+  float rs[NOP];
+  uint32_t off[NOP];
+#pragma unroll
+  for (int o = 0; o < NOP; ++o) off[o] = (uint32_t)lrow * op_ss[o] + 16u * lch;
+  // Operand o's rows of tile j from `page`.
+  const auto load = [&](int o, int j, int page) __attribute__((always_inline)) {
+    const int key = tile_of(j) * ST::kKeys + 16 * gw, rows = rows_ld - key;
+    __amdgpu_buffer_rsrc_t rt = make_rsrc(op_base[o], 0u);
     if (rows > 0) {
       const int64_t slot = key & ((1 << p.block_shift) - 1);
-      rt = make_rsrc(head_ptr + (int64_t)page * sb + slot * ss, (uint32_t)(min(rows, 16) - 1) * ss + D);
+      rt = make_rsrc(op_base[o] + (int64_t)page * op_sb[o] + slot * op_ss[o],
+                     (uint32_t)(min(rows, 16) - 1) * op_ss[o] + D);
     }
-    const uint32_t off = (uint32_t)lrow * ss + 16u * lch;
 #pragma unroll
     for (int u = 0; u < NL; ++u)
-      x[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rt, off, (uint32_t)(u * RPL) * ss, 0));
+      rx[o][u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rt, off[o], (uint32_t)(u * RPL) * op_ss[o], 0));
   };
   // Sixteen codes a lane and load into two 16-byte chunks of the 16-bit tile.
-  const auto store = [&](char* tile, const u32x4 (&x)[NL], float scale, bool is_k) __attribute__((always_inline)) {
+  uint32_t so[NOP][NL];
+#pragma unroll
+  for (int o = 0; o < NOP; ++o)
 #pragma unroll
     for (int u = 0; u < NL; ++u) {
-      const int row = 16 * wave + RPL * u + lrow;
-      const int sw = is_k ? ST::gk(row & 15) : ST::sv(row);
-      char* to = tile + row * (2 * D);
-      *reinterpret_cast<u32x4*>(to + 16 * ((2 * lch) ^ sw)) = widen8<DT>(x[u][0], scale, x[u][1], scale);
-      *reinterpret_cast<u32x4*>(to + 16 * ((2 * lch + 1) ^ sw)) = widen8<DT>(x[u][2], scale, x[u][3], scale);
+      const int row = 16 * gw + RPL * u + lrow;
+      const int sw = of_v || o == 1 ? ST::sv(row) : ST::gk(row & 15);
+      so[o][u] = (uint32_t)(row * (2 * D) + 16 * ((2 * lch) ^ sw)) + (of_v || o == 1 ? (uint32_t)(NG * TB) : 0u);
+    }
+  const auto store = [&](int o, int stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NL; ++u) {
+      char* to = lds + stage * TB;
+      *reinterpret_cast<u32x4*>(to + so[o][u]) = widen8<DT>(rx[o][u][0], rs[o], rx[o][u][1], rs[o]);
+      *reinterpret_cast<u32x4*>(to + (so[o][u] ^ 16u)) = widen8<DT>(rx[o][u][2], rs[o], rx[o][u][3], rs[o]);
     }
   };
 
-  u32x4 rk[NL], rv[NL];
-  int id_v = page_of(0), id_k = page_of(1);
-  load(rk, kbh, p.k.sb, kss, 0, id_v);
-  float sk = scale_of(keb, p.ke.sb, id_v), sv = scale_of(veb, p.ve.sb, id_v);
+  // The stages of tile 0: K's, and with two groups V's.
+  look(0);
+  int page_v = page_of(0);  // one group: the tile at hand's, for V
+  float scale_v = NG == 1 ? scale_of(NOP - 1, 0) : 1.f;
+  load(0, 0, page_v);
+  rs[0] = scale_of(0, 0);
   u32x4 qreg[NKS];
   {
     const int ps = valid ? pos : pos_lo;  // (an invalid row's are zeroed)
@@ -147,12 +281,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) qreg[ks] = *reinterpret_cast<const u32x4*>(qrow + 16 * ks + 8 * hh);
   }
-  store(lds1_k, rk, sk, true);
-  load(rv, vbh, p.v.sb, vss, 0, id_v);
-  load(rk, kbh, p.k.sb, kss, 1, id_k);
-  sk = scale_of(keb, p.ke.sb, id_k);
-  id_v = id_k;
-  id_k = page_of(2);
+  store(0, 0);
   if (!valid) {
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) qreg[ks] = u32x4{0u, 0u, 0u, 0u};
@@ -186,14 +315,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g
   using BT = std::true_type;
   using BF = std::false_type;
 
-  // MFMA phase of tile j: P*V of the tile before and S^T of this one.
-  const auto mphase = [&](auto pvc, auto sc_) __attribute__((always_inline)) {
+  // MFMA phase of tile j: P*V of the tile before and S^T of this one.  par: j's parity.
+  const auto mphase = [&](int mj, auto pvc, auto sc_, auto par) __attribute__((always_inline)) {
     constexpr bool DO_PV = decltype(pvc)::value;
     constexpr bool DO_S = decltype(sc_)::value;
     constexpr int NPV = DO_PV ? 4 * NDB : 0;
     constexpr int NS = DO_S ? 2 * NKS : 0;
-    const char* ck = lds1_k;
-    const char* cv = lds0_v;
+    constexpr int PAR = decltype(par)::value ? 1 : 0;
+    if constexpr (DO_S) {  // the codes that the softmax phase stores
+      if (mj + 1 - base >= 64) look(mj + 1);
+      if constexpr (NG == 1) {
+        load(1, mj, page_v);
+        rs[1] = scale_v;
+        page_v = page_of(mj + 1);
+        scale_v = scale_of(1, mj + 1);
+        load(0, mj + 1, page_v);
+      } else {
+        load(0, mj + 1, page_of(mj + 1));
+      }
+      rs[0] = scale_of(0, mj + 1);
+    }
+    const char* ck = lds + (NG == 2 ? PAR * TB : 0);
+    const char* cv = lds + NG * TB + (NG == 2 ? (1 - PAR) * TB : 0);
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(3);
     __builtin_amdgcn_sched_barrier(0);
@@ -239,17 +382,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g
     phase_barrier();
   };
 
-  // Softmax phase of tile j.
-  const auto vphase = [&](int j, auto first_c) __attribute__((always_inline)) {
+  // Softmax phase of tile j, which stores the next tile's codes and loads ahead.
+  const auto vphase = [&](int j, auto first_c, auto par) __attribute__((always_inline)) {
     constexpr bool FIRST = decltype(first_c)::value;
-    store(lds1_k, rk, sk, true);
-    store(lds0_v, rv, sv, false);
-    load(rk, kbh, p.k.sb, kss, j + 2, id_k);
-    load(rv, vbh, p.v.sb, vss, j + 1, id_v);
-    sk = scale_of(keb, p.ke.sb, id_k);
-    sv = scale_of(veb, p.ve.sb, id_v);
-    id_v = id_k;
-    id_k = page_of(j + 3);
     const int key0 = tile_of(j) * ST::kKeys;
     float row_t = 0.f;  // added to every score of the lane
     cap_scores<16>(sc, p.mod);
@@ -277,6 +412,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g
       rs0 = softmax_exp<DT>(sc[0], nmc, c, pk[0]);
       rs1 = softmax_exp<DT>(sc[1], nmc, c, pk[1]);
     }
+    store(0, NG == 1 || decltype(par)::value ? 0 : 1);
+    if constexpr (NG == 1) store(1, 0);
     l_run += rs0 + rs1;
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
@@ -286,15 +423,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g
   };
 
   phase_barrier();
+  if (group == 1) phase_barrier();  // (a phase behind group 0)
   if (n > 0) {
-    mphase(BF{}, BT{});
-    vphase(0, BT{});
-    for (int j = 1; j < n; ++j) {
-      mphase(BT{}, BT{});
-      vphase(j, BF{});
+    mphase(0, BF{}, BT{}, BF{});
+    vphase(0, BT{}, BF{});
+    int j = 1;
+    for (; j + 1 < n; j += 2) {
+      mphase(j, BT{}, BT{}, BT{});
+      vphase(j, BF{}, BT{});
+      mphase(j + 1, BT{}, BT{}, BF{});
+      vphase(j + 1, BF{}, BF{});
     }
-    mphase(BT{}, BF{});
+    if (j < n) {
+      mphase(j, BT{}, BT{}, BT{});
+      vphase(j, BF{}, BT{});
+      mphase(n, BT{}, BF{}, BF{});
+    } else {
+      mphase(n, BT{}, BF{}, BT{});
+    }
   }
+  if (NG == 2 && group == 0) phase_barrier();
   __syncthreads();
 
   const float l_tot = xhalf_sum(l_run);
@@ -320,10 +468,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g
     p.lse[li] = (__builtin_fmaf(m_run, c, p.mod.shift2) + __log2f(l_tot)) * kLn2;
   }
   // The wave's 32 x D output goes through LDS (row-major, 16-byte chunks
-  // XOR-swizzled by row; two waves a former stage), so that it leaves as whole
+  // XOR-swizzled by row; in the former stages), so that it leaves as whole
   // rows.
   constexpr int CPR16 = 2 * D / 16, RPI = 64 / CPR16;
-  char* ot = (wave < 2 ? lds1_k : lds0_v) + (wave & 1) * (32 * 2 * D);
+  char* ot = lds + wave * (32 * 2 * D);
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -350,22 +498,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void g
 }
 
 template <int DT, int D> static hipError_t launch_chunk8_t(Fwd8Params p, hipStream_t stream) {
-  const int per_bh = p.kv_splits > 0 ? p.n_mblk * p.kv_splits : p.n_mblk;
-  const int64_t total = (int64_t)per_bh * p.dm.Hkv * p.dm.B;
+  const int64_t total = (int64_t)p.n_mblk * p.dm.Hkv * (p.kv_splits > 0 ? p.kv_splits : p.dm.B);
   if (total <= 0) return hipSuccess;
-  if (total >= (int64_t)1 << 31) return hipErrorInvalidValue;
-  set_item_order(p, per_bh, true, kDealPairs(D));
+  if (total >= ((int64_t)1 << 31) - 1) return hipErrorInvalidValue;
+  set_item_order(p, p.n_mblk, true, kDealPairs(D));
+  if (p.kv_splits > 0) p.div_items = make_fast_div((uint32_t)p.kv_splits);
   p.div_mblk = make_fast_div((uint32_t)p.n_mblk);
   p.div_hkv = make_fast_div((uint32_t)p.dm.Hkv);
   p.bm_mul = (65536u + (uint32_t)p.block_m - 1) / (uint32_t)p.block_m;
-  if (p.kv_splits > 0)
-    hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, true>), dim3((unsigned)total), dim3(256), 0, stream, p);
-  else
-    hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, false>), dim3((unsigned)total), dim3(256), 0, stream, p);
+  const dim3 grid((unsigned)(total + (p.kv_splits > 0 ? 1 : 0)));
+  if (p.block_m * p.dm.G > kShortRows) {
+    if (p.kv_splits > 0) hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 2, true>), grid, dim3(512), 0, stream, p);
+    else hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 2, false>), grid, dim3(512), 0, stream, p);
+  } else {
+    if (p.kv_splits > 0) hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 1, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 1, false>), grid, dim3(256), 0, stream, p);
+  }
   return hipGetLastError();
 }
 
-// p.block_m = kShortRows / G, p.n_mblk accordingly.
+// p.block_m = chunk8_rows(G, Sq) / G, p.n_mblk accordingly.
 hipError_t launch_chunk8(const Fwd8Params& p, int dtype, hipStream_t stream) {
   if (p.block_shift < 4 || p.block_table == nullptr) return hipErrorInvalidValue;
   if (dtype == 0) return p.dm.D == 128 ? launch_chunk8_t<0, 128>(p, stream) : launch_chunk8_t<0, 64>(p, stream);

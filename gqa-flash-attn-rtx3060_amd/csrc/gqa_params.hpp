@@ -276,6 +276,7 @@ struct Split8Params : SplitParams {
 };
 struct Fwd8Params : FwdParams {
   ScoreMod mod;
+  int* plan;  // over key pieces (kv_splits of them): as SplitParams::plan
   Exponents ke, ve;
 };
 
@@ -393,13 +394,16 @@ hipError_t launch_split_reduce(const ReduceParams& p, int dtype, hipStream_t str
 hipError_t launch_rope(const RopeParams& p, int dtype, hipStream_t stream);
 // The paged cache in 8 bits: attention of up to kDecode8Rows packed rows a kv head
 // (a flat split of p.slots, partials and plan in the split workspace), of any number
-// (single pass, or p.kv_splits key chunks), and its writes and reads.
+// (single pass, or p.kv_splits key pieces of all sequences, partials and plan likewise),
+// and its writes and reads.
 constexpr int kDecode8Rows = 32;
 // Keys of the flat split's unit.
 constexpr int decode8_unit(int head_dim) { return 16384 / head_dim; }
 hipError_t launch_decode8(const Split8Params& p, int dtype, hipStream_t stream);
-// Joins the partials of launch_decode8's slots (p.slots of them).
+// Joins the partials of the two by the plan, p.slots of them at most.
 hipError_t launch_decode8_join(const ReduceParams& p, int G, int dtype, hipStream_t stream);
+// Packed rows of a workgroup of launch_chunk8.
+constexpr int chunk8_rows(int64_t packed) { return packed > 2 * kShortRows ? 2 * kShortRows : kShortRows; }
 hipError_t launch_chunk8(const Fwd8Params& p, int dtype, hipStream_t stream);
 hipError_t launch_store8(const Store8Params& p, int dtype, hipStream_t stream);
 hipError_t launch_read8(const Read8Params& p, int dtype, hipStream_t stream);

@@ -163,10 +163,10 @@ def attention(q, k_cache, v_cache, block_table, seq_lens, causal, max_seq_len, s
     if route is not None:
         assert route in _ROUTES, f"a cache in 8 bits has the routes {', '.join(_ROUTES)}"
         if _ROUTES[route] != form:
-            form, parts = _ROUTES[route], {"split": 1, "chunks": 2, "single": 0}[route]
+            form, parts = _ROUTES[route], {"split": 1, "chunks": 2 * batch, "single": 0}[route]
     if splits is not None:
         assert form != _lib.FORM_SINGLE, "the single pass has no parts"
-        parts = int(splits)
+        parts = int(splits) * (batch if form == _lib.FORM_CHUNKS else 1)
     lse = None
     if return_lse:
         lse = torch.empty((q.shape[0], num_heads) if varlen else (batch, num_heads, seq_q), dtype=torch.float32,

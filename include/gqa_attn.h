@@ -618,7 +618,8 @@ typedef struct gqa_cache8 {
  * that sees no key gives zeros and LSE -inf.  Groups of at most 128 query heads.
  * gqa_paged8_plan: the form that a call of these sizes takes on a device of
  * cu_count compute units, GQA_FORM_FLAT (`parts` slots, up to 32 packed rows a kv
- * head), GQA_FORM_CHUNKS (`parts` key chunks) or GQA_FORM_SINGLE (0).  Others may
+ * head), GQA_FORM_CHUNKS (`parts` key pieces in all, at least `batch`, shared out over
+ * the sequences by their lengths, on the device) or GQA_FORM_SINGLE (0).  Others may
  * be given, within those limits and GQA_MAX_SPLITS.  workspace: 16-byte aligned,
  * gqa_paged8_workspace_bytes bytes (0: NULL). */
 int gqa_paged8_plan(int batch, int num_heads, int num_kv_heads, int seq_q,
