@@ -16,12 +16,15 @@
 // storing them where K(j) and V(j - 1) were; barrier.  K and V have one stage each.  Two
 // groups, for more than 256 packed rows: group 1 is a phase behind group 0, so that one's
 // MFMAs run beside the other's softmax on each SIMD; group 0 fills K's stages, group 1
-// V's, two of each.  That halves what a row pays for loads, widening and LDS writes, which
+// V's, two of each, in their MFMA phases, from what their softmax phases load: group 0
+// K(j + 1) in the phase of its S(j), group 1 V(j) in that of its, before group 0's next
+// phase takes it; what they write over was read a phase before or earlier.  That halves what a row pays for loads, widening and LDS writes, which
 // are most of what the cache in 8 bits costs over one in 16: 2048 queries over 16384
-// keys, 32 heads over 8, 550 us for one group and 503 for two (390 without loads and
-// stores, 443 the 16-bit kernel).  Up to 256 rows the finer blocks win (8 x 64 queries over
-// 1000-4000 keys 44.6 us / 49.8).  Loading in the softmax phase took 4 % more, pages and
-// exponents by scalar loads instead of by lane 1 %, and storing first there another 5 %.
+// keys, 32 heads over 8, 550 us for one group and 486 for two (470 the kernel over a cache
+// in 16 bits; 390 without loads and stores).  Up to 256 rows the finer blocks win (8 x 64
+// queries over 1000-4000 keys 44.6 us / 49.8).  Widening in the softmax phase, whose
+// instructions then outlast the other group's MFMAs, took 2.5 % more, pages and exponents
+// by scalar loads instead of by lane 1 %.
 #include <algorithm>
 #include <type_traits>
 
@@ -103,10 +106,10 @@ __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) v
   using ST = FwdStage<D>;
   constexpr int NDB = D / 32;   // 32-wide d blocks of O^T
   constexpr int NKS = D / 16;   // k-steps of S^T
-  constexpr int PF = 6;         // MFMA slots of LDS-read lookahead
+  constexpr int PF = 4;         // MFMA slots of LDS-read lookahead
   constexpr int TB = ST::kTileBytes;
-  constexpr int CPR8 = D / 16;  // 16-code chunks per row
-  constexpr int RPL = 64 / CPR8;  // rows per load of a wave: 8 or 16
+  constexpr int CPR8 = D / 8;   // 8-code chunks per row, 16 bytes of the widened tile
+  constexpr int RPL = 64 / CPR8;  // rows per load of a wave: 4 or 8
   constexpr int NL = 16 / RPL;    // loads of a wave's 16 rows
   __shared__ __attribute__((aligned(1024))) char lds[2 * NG * TB];  // NG stages of K, then of V
 
@@ -230,11 +233,11 @@ __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) v
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scale_l[o]), j - base));
   };
   const int lrow = lane / CPR8, lch = lane % CPR8;
-  u32x4 rx[NOP][NL];
+  u32x2 rx[NOP][NL];
   float rs[NOP];
   uint32_t off[NOP];
 #pragma unroll
-  for (int o = 0; o < NOP; ++o) off[o] = (uint32_t)lrow * op_ss[o] + 16u * lch;
+  for (int o = 0; o < NOP; ++o) off[o] = (uint32_t)lrow * op_ss[o] + 8u * lch;
   // Operand o's rows of tile j from `page`.
   const auto load = [&](int o, int j, int page) __attribute__((always_inline)) {
     const int key = tile_of(j) * ST::kKeys + 16 * gw, rows = rows_ld - key;
@@ -246,9 +249,11 @@ __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) v
     }
 #pragma unroll
     for (int u = 0; u < NL; ++u)
-      rx[o][u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rt, off[o], (uint32_t)(u * RPL) * op_ss[o], 0));
+      rx[o][u] = __builtin_bit_cast(
+          u32x2, __builtin_amdgcn_raw_buffer_load_b64(rt, off[o], (uint32_t)(u * RPL) * op_ss[o], 0));
   };
-  // Sixteen codes a lane and load into two 16-byte chunks of the 16-bit tile.
+  // Eight codes a lane and load into 16 bytes of the widened tile: 16 lanes write a whole
+  // row, or two (sixteen codes a lane would put the lanes of a V write on half the banks).
   uint32_t so[NOP][NL];
 #pragma unroll
   for (int o = 0; o < NOP; ++o)
@@ -256,14 +261,13 @@ __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) v
     for (int u = 0; u < NL; ++u) {
       const int row = 16 * gw + RPL * u + lrow;
       const int sw = of_v || o == 1 ? ST::sv(row) : ST::gk(row & 15);
-      so[o][u] = (uint32_t)(row * (2 * D) + 16 * ((2 * lch) ^ sw)) + (of_v || o == 1 ? (uint32_t)(NG * TB) : 0u);
+      so[o][u] = (uint32_t)(row * (2 * D) + 16 * (lch ^ sw)) + (of_v || o == 1 ? (uint32_t)(NG * TB) : 0u);
     }
   const auto store = [&](int o, int stage) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < NL; ++u) {
       char* to = lds + stage * TB;
       *reinterpret_cast<u32x4*>(to + so[o][u]) = widen8<DT>(rx[o][u][0], rs[o], rx[o][u][1], rs[o]);
-      *reinterpret_cast<u32x4*>(to + (so[o][u] ^ 16u)) = widen8<DT>(rx[o][u][2], rs[o], rx[o][u][3], rs[o]);
     }
   };
 
@@ -271,8 +275,10 @@ __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) v
   look(0);
   int page_v = page_of(0);  // one group: the tile at hand's, for V
   float scale_v = NG == 1 ? scale_of(NOP - 1, 0) : 1.f;
-  load(0, 0, page_v);
-  rs[0] = scale_of(0, 0);
+  if (NG == 1 || group == 0) {
+    load(0, 0, page_v);
+    rs[0] = scale_of(0, 0);
+  }
   u32x4 qreg[NKS];
   {
     const int ps = valid ? pos : pos_lo;  // (an invalid row's are zeroed)
@@ -281,7 +287,14 @@ __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) qreg[ks] = *reinterpret_cast<const u32x4*>(qrow + 16 * ks + 8 * hh);
   }
-  store(0, 0);
+  if (NG == 1 || group == 0) store(0, 0);
+  const int lead = NG == 2 ? 1 - group : 0;
+  if constexpr (NG == 2) {
+    load(0, lead, page_of(lead));
+    rs[0] = scale_of(0, lead);
+#pragma unroll
+    for (int u = 0; u < NL; ++u) so[0][u] += lead * TB;
+  }
   if (!valid) {
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) qreg[ks] = u32x4{0u, 0u, 0u, 0u};
@@ -322,17 +335,13 @@ __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) v
     constexpr int NPV = DO_PV ? 4 * NDB : 0;
     constexpr int NS = DO_S ? 2 * NKS : 0;
     constexpr int PAR = decltype(par)::value ? 1 : 0;
-    if constexpr (DO_S) {  // the codes that the softmax phase stores
+    if constexpr (NG == 1 && DO_S) {  // the codes that the softmax phase stores
       if (mj + 1 - base >= 64) look(mj + 1);
-      if constexpr (NG == 1) {
-        load(1, mj, page_v);
-        rs[1] = scale_v;
-        page_v = page_of(mj + 1);
-        scale_v = scale_of(1, mj + 1);
-        load(0, mj + 1, page_v);
-      } else {
-        load(0, mj + 1, page_of(mj + 1));
-      }
+      load(1, mj, page_v);
+      rs[1] = scale_v;
+      page_v = page_of(mj + 1);
+      scale_v = scale_of(1, mj + 1);
+      load(0, mj + 1, page_v);
       rs[0] = scale_of(0, mj + 1);
     }
     const char* ck = lds + (NG == 2 ? PAR * TB : 0);
@@ -369,6 +378,12 @@ __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
       for (int j = 0; j < NS; ++j) sc[j & 1] = E::mfma(opk[j], qreg[j >> 1], sc[j & 1]);
     }
+    if constexpr (NG == 2 && DO_S) {
+#pragma unroll
+      for (int u = 0; u < NL; ++u)
+        *reinterpret_cast<u32x4*>(lds + (so[0][u] ^ (uint32_t)(PAR * TB))) =
+            widen8<DT>(rx[0][u][0], rs[0], rx[0][u][1], rs[0]);
+    }
     mphase_prefetch<NPV, NPV + NS, PF, 0>();
     mphase_pipe<NPV, NPV + NS, PF, 0>();
     if constexpr (DO_S) {
@@ -385,6 +400,11 @@ __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) v
   // Softmax phase of tile j, which stores the next tile's codes and loads ahead.
   const auto vphase = [&](int j, auto first_c, auto par) __attribute__((always_inline)) {
     constexpr bool FIRST = decltype(first_c)::value;
+    if constexpr (NG == 2) {
+      if (j + 1 + lead - base >= 64) look(j + 1 + lead);
+      load(0, j + 1 + lead, page_of(j + 1 + lead));
+      rs[0] = scale_of(0, j + 1 + lead);
+    }
     const int key0 = tile_of(j) * ST::kKeys;
     float row_t = 0.f;  // added to every score of the lane
     cap_scores<16>(sc, p.mod);
@@ -412,8 +432,10 @@ __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) v
       rs0 = softmax_exp<DT>(sc[0], nmc, c, pk[0]);
       rs1 = softmax_exp<DT>(sc[1], nmc, c, pk[1]);
     }
-    store(0, NG == 1 || decltype(par)::value ? 0 : 1);
-    if constexpr (NG == 1) store(1, 0);
+    if constexpr (NG == 1) {
+      store(0, 0);
+      store(1, 0);
+    }
     l_run += rs0 + rs1;
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
