@@ -140,7 +140,7 @@ template <int DT, int D, bool ROPE> __global__ __launch_bounds__(256) void gqa_s
     unpack8<DT>(xa, ya);
     unpack8<DT>(xb, yb);
     if constexpr (ROPE) {
-      if (is_k) row_norm_rotate<DT, D>(p, at, p.wk, cs, sn, ya, yb);
+      if (is_k) row_norm_rotate_closely<DT, D>(p, at, p.wk, cs, sn, ya, yb);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {

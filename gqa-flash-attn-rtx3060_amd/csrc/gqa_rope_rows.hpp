@@ -1,7 +1,9 @@
 // gqa_rope_rows.hpp — a (token, head) row of queries or keys as gqa_rope.hip and the
-// 8-bit cache's writes (gqa_store8.hip) hold it: D / 16 lanes, 16 values each, as the
+// 8-bit cache's writes (gqa_cache8.hip) hold it: D / 16 lanes, 16 values each, as the
 // two 8-value chunks whose pairs they rotate; norm and rotation in fp32.
 #pragma once
+
+#include <type_traits>
 
 #include "gqa_common.hpp"
 #include "gqa_params.hpp"
@@ -154,6 +156,75 @@ __device__ __forceinline__ void row_norm_rotate(const RopeParams& p, const RowLa
         yb[2 * i] = d * cs[4 + i] - e * sn[4 + i];
         yb[2 * i + 1] = e * cs[4 + i] + d * sn[4 + i];
       }
+    }
+  }
+}
+
+// The same for a row that becomes e4m3 codes, closer to its exact value than fp32's
+// roundings one after another: a value that they move across the middle of two codes is
+// off by a whole step, an eighth of it.  1 / rms in 64 bits, as two floats; weighted
+// values of 16-bit types are exact; the product that a rotation subtracts keeps its
+// rounding error (p + e = c sin).
+template <int LPR> __device__ inline double row_sum(double x) {
+  const auto from = [&](auto ctrl) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)b, decltype(ctrl)::value, 0xF, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(b >> 32), decltype(ctrl)::value, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  };
+  x += from(std::integral_constant<int, 0xB1>{});
+  x += from(std::integral_constant<int, 0x4E>{});
+  if constexpr (LPR == 8) x += from(std::integral_constant<int, 0x141>{});
+  return x;
+}
+template <int DT, int D>
+__device__ __forceinline__ void row_norm_rotate_closely(const RopeParams& p, const RowLane& at, const void* w,
+                                                        const float (&cs)[8], const float (&sn)[8], float (&ya)[8],
+                                                        float (&yb)[8]) {
+  float hi = 1.f, lo = 0.f;
+  if (w != nullptr) {
+    float wa[8], wb[8];
+    double ss = 0.0;
+    load_weights<DT>(w, p.w32, at.ca, at.cb, wa, wb);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      ss = __builtin_fma((double)ya[i], (double)ya[i], __builtin_fma((double)yb[i], (double)yb[i], ss));
+    const double x = row_sum<D / 16>(ss) * (1.0 / D) + (double)p.eps;
+    const double r = 1.0f / __builtin_sqrtf((float)x), inv = r * (1.5 - 0.5 * x * r * r);  // (a step of Newton's)
+    hi = (float)inv;
+    lo = (float)(inv - (double)hi);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ya[i] *= wa[i];
+      yb[i] *= wb[i];
+    }
+  }
+  const auto minus = [](float a, float co, float c, float si) __attribute__((always_inline)) {  // a co - c si
+    const float q = c * si, e = __builtin_fmaf(c, si, -q);
+    return __builtin_fmaf(a, co, -q) - (e == e ? e : 0.f);  // (infinite products have no error term)
+  };
+  const auto turn = [&](float& a, float& c, float co, float si) __attribute__((always_inline)) {
+    const float x = minus(a, co, c, si);
+    c = minus(c, co, a, -si);
+    a = x;
+  };
+  if (at.rot) {
+    if (!p.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) turn(ya[i], yb[i], cs[i], sn[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        turn(ya[2 * i], ya[2 * i + 1], cs[i], sn[i]);
+        turn(yb[2 * i], yb[2 * i + 1], cs[4 + i], sn[4 + i]);
+      }
+    }
+  }
+  if (w != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ya[i] = __builtin_fmaf(ya[i], hi, ya[i] * lo);
+      yb[i] = __builtin_fmaf(yb[i], hi, yb[i] * lo);
     }
   }
 }

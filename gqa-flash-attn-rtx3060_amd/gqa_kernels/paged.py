@@ -1122,7 +1122,7 @@ class GQAPagedAttention(torch.nn.Module):
                             softcap=self.softcap, alibi_slopes=self.alibi_slopes, prefix_lens=prefix, **exps)
         return output
 
-    def _norm_rope(self, query, key, value, k_cache, v_cache, md, exps):
+    def _norm_rope(self, query, key, value, k_cache, v_cache, md, exps=None):
         """Normed and rotated queries (a new tensor); keys and values, if given,
         go to the cache."""
         T, H, Hkv, D = query.shape[0], self.num_heads, self.num_kv_heads, self.head_size
@@ -1134,5 +1134,5 @@ class GQAPagedAttention(torch.nn.Module):
         else:
             out = qk_norm_rope_write(q, key.view(T, Hkv, D), value.view(T, Hkv, D), md.positions, self.rotary, k_cache,
                                      v_cache, md.slot_mapping, q_weight=self.q_norm_weight,
-                                     k_weight=self.k_norm_weight, eps=self.norm_eps, **exps)
+                                     k_weight=self.k_norm_weight, eps=self.norm_eps, **(exps or {}))
         return out.reshape(T, H * D)
