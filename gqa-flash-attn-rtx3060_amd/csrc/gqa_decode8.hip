@@ -151,19 +151,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   int qpos[NR], seen[NR], qpos_lo = 0, seen_lo = 0;
   bool valid[NR];
   u32x4 qreg[NR][NKS];
-  // Pages and scales of this wave's 64 16-key blocks from its tile `base` on, a block a
+  // Addresses and scales of this wave's 64 16-key blocks from its tile `base` on, a block a
   // lane (page -1: behind the piece): read together, handed out by lane, so that the
-  // stream of tiles waits for no scalar load.
+  // stream of tiles waits for no scalar load and multiplies no strides (from L2, 16 x 4
+  // queries of 8000 keys 26.3 -> 24.5 us).
   constexpr int W = 64 / NB;
   int base = 0, page_l = -1, page_n = -1;
+  uint32_t klo = 0, khi = 0, vlo = 0, vhi = 0;
   float sk_l = 1.f, sv_l = 1.f;
 
   const auto pages_of = [&](const Piece& x, int it) __attribute__((always_inline)) {
     const int key = x.c0 + (4 * (it + lane / NB) + wave) * TW + 16 * (lane % NB);
     return x.some && key < x.c1 ? p.block_table[(int64_t)x.b * p.table_stride + (key >> p.block_shift)] : -1;
   };
-  const auto scales = [&]() __attribute__((always_inline)) {  // of page_l: exponents, loaded
+  const auto scales = [&]() __attribute__((always_inline)) {  // of page_l: addresses; exponents, loaded
     const int64_t id = max(page_l, 0);
+    const int key = cur.c0 + (4 * (base + lane / NB) + wave) * TW + 16 * (lane % NB);
+    const int64_t slot = key & ((1 << p.block_shift) - 1);
+    const uint64_t ko = (uint64_t)kbase + id * p.k.sb + slot * p.k.ss, vo = (uint64_t)vbase + id * p.v.sb + slot * p.v.ss;
+    klo = (uint32_t)ko, khi = (uint32_t)(ko >> 32), vlo = (uint32_t)vo, vhi = (uint32_t)(vo >> 32);
     sk_l = __int_as_float(page_l >= 0 ? keb[id * p.ke.sb] : 0);
     sv_l = __int_as_float(page_l >= 0 ? veb[id * p.ve.sb] : 0);
   };
@@ -181,14 +187,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
     for (int bl = 0; bl < NB; ++bl) {
       const int key = cur.c0 + (4 * it + wave) * TW + 16 * bl, rows = cur.c1 - key;
-      const int page = __builtin_amdgcn_readlane(page_l, (it - base) * NB + bl);
-      __amdgpu_buffer_rsrc_t tk = make_rsrc(kbase, 0u), tv = make_rsrc(vbase, 0u);
-      if (rows > 0) {
-        const int64_t slot = key & ((1 << p.block_shift) - 1);
-        const uint32_t last = (uint32_t)(min(rows, 16) - 1);
-        tk = make_rsrc(kbase + (int64_t)page * p.k.sb + slot * p.k.ss, last * kss + D);
-        tv = make_rsrc(vbase + (int64_t)page * p.v.sb + slot * p.v.ss, last * vss + D);
-      }
+      const int from = (it - base) * NB + bl;
+      const auto at = [&](uint32_t lo, uint32_t hi) {
+        return reinterpret_cast<const char*>((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32 |
+                                             (uint32_t)__builtin_amdgcn_readlane(lo, from));
+      };
+      const uint32_t last = (uint32_t)(min(rows, 16) - 1);
+      const __amdgpu_buffer_rsrc_t tk = make_rsrc(at(klo, khi), rows > 0 ? last * kss + D : 0u);
+      const __amdgpu_buffer_rsrc_t tv = make_rsrc(at(vlo, vhi), rows > 0 ? last * vss + D : 0u);
 #pragma unroll
       for (int i = 0; i < IPB; ++i) {
         const int row = 16 * bl + RPI * i + lrow;

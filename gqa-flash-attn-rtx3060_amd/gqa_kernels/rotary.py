@@ -246,7 +246,6 @@ def qk_norm_rope_write(q, k, v, positions, table: Optional[RotaryTable], k_cache
     every other one lies inside the caches, no slot twice).  k_exponents, v_exponents:
     a cache in 8 bits, as ``write_kv`` fills it, with k's codes made of the fp32 results
     (rounded once)."""
-    from . import cache8
     from .paged import _check_cache
 
     if _lib._host is not None:
@@ -255,6 +254,8 @@ def qk_norm_rope_write(q, k, v, positions, table: Optional[RotaryTable], k_cache
                                    slot_mapping, q_weight, k_weight, eps, q_out, None, k_exponents, v_exponents)
         if res is not None:
             return res
+    from . import cache8
+
     if cache8.takes(k_cache, k_exponents, v_exponents):
         return cache8.norm_rope_write(q, k, v, positions, table, k_cache, v_cache, slot_mapping, q_weight, k_weight,
                                       eps, q_out, k_exponents, v_exponents)
