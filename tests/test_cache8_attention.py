@@ -81,14 +81,14 @@ def test_many_rows(Hq, Hkv, Sq, lens, D, dtype):
     Batch(lens, Hq, Hkv, Sq, D, 16 if Sq % 2 else 64, dtype, seed=Sq, layout="HND" if Sq % 3 else "NHD").check(MANY)
 
 
-@pytest.mark.parametrize("Hq,Hkv,Sq", [(8, 2, 1), (8, 2, 4), (8, 2, 6), (8, 2, 40)])
+@pytest.mark.parametrize("Hq,Hkv,Sq", [(8, 2, 1), (8, 2, 4), (8, 2, 6), (8, 2, 40), (8, 2, 100)])
 @pytest.mark.parametrize("D", [64, 128])
 def test_without_a_mask(Hq, Hkv, Sq, D):
     Batch([1, 50, 3 * 64, 700], Hq, Hkv, Sq, D, 16).check((None, ("single", None), ("chunks", 3)), causal=False)
 
 
 @pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp16"])
-@pytest.mark.parametrize("Hq,Hkv,Sq", [(16, 4, 1), (16, 4, 4), (16, 4, 7), (16, 4, 50)])
+@pytest.mark.parametrize("Hq,Hkv,Sq", [(16, 4, 1), (16, 4, 4), (16, 4, 7), (16, 4, 50), (16, 4, 90)])
 @pytest.mark.parametrize("D", [64, 128])
 def test_changed_scores(Hq, Hkv, Sq, D, dtype):
     lens = [1, 70, 129, 640, 0, 333]
@@ -206,7 +206,7 @@ def test_results_repeat_and_two_calls_at_once():
         assert len(got[i]) == 20 and all(torch.equal(x, want[i]) for x in got[i])
 
 
-@pytest.mark.parametrize("Sq", [1, 60])
+@pytest.mark.parametrize("Sq", [1, 6, 60, 100])
 def test_captured_and_replayed(Sq):
     """Two graphs over one cache, replayed in turn and at once with eager calls in between; lengths and queries that change under them."""
     b = Batch([900, 33, 512, 129], 8, 2, Sq, 128, 16, seed=4)
@@ -234,6 +234,23 @@ def test_captured_and_replayed(Sq):
             assert torch.equal(outs[i][0], eager) and torch.equal(outs[i][1], lse)
             for s in range(4):
                 check_attention(outs[i][0][s], outs[i][1][s], b.want(s, qs[i][s]))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq", [1, 7, 30, 100])
+def test_one_sequence_in_many_parts(Sq, D):
+    """Joined by a workgroup a row; pieces beyond the query block's last key."""
+    Batch([4999], 8, 2, Sq, D, 16, seed=Sq).check((None, ("split", 39) if Sq <= 8 else ("chunks", 70), ("chunks", 9)))
+
+
+def test_pieces_of_very_unequal_sequences():
+    """One long sequence among those of a tile or none: it takes what they leave, down to a piece each."""
+    for lens, splits in (([1] * 40 + [0, 4000] + [64] * 30, 2), ([0] * 65 + [1300, 3], 1), ([700, 100, 0, 1], 256), ([129] * 9, 3)):
+        b = Batch(lens, 8, 2, 40, 64, 16, seed=len(lens))
+        o, lse = b.run(return_lse=True, route="chunks", splits=splits)
+        for i in range(len(lens)):
+            if lens[i] != 1 or i < 3:
+                check_attention(o[i], lse[i], b.want(i))
 
 
 def test_many_sequences():

@@ -42,7 +42,7 @@ def test_attention_refusals(lib):
     for kw in (dict(block=8), dict(block=0), dict(block=24), dict(block=1 << 17), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
                dict(scale=float("inf")), dict(form=0), dict(form=4), dict(form=7), dict(form=3, parts=1, seq_q=9), dict(form=3, parts=1, max_len=0)):
         assert attend(lib, **kw) == E8, kw
-    for kw in (dict(form=2, parts=0), dict(form=2, parts=1025), dict(form=3, parts=0), dict(form=3, parts=1025)):
+    for kw in (dict(form=2, parts=0), dict(form=2, parts=1025), dict(form=2, parts=2, batch=3), dict(form=3, parts=0), dict(form=3, parts=1025)):
         assert attend(lib, **kw) == SPLITS, kw
     for kw in (dict(q=None), dict(o=None), dict(table=None), dict(lens=None), dict(qs=P), dict(ql=P), dict(form=2, parts=2), dict(form=3, parts=2)):
         assert attend(lib, **kw) == NULL, kw
