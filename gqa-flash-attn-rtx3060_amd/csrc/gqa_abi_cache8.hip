@@ -62,6 +62,7 @@ int gqa_paged8_plan(int batch, int num_heads, int num_kv_heads, int seq_q, int m
   if (head_dim != 64 && head_dim != 128) return GQA_E_HEAD_DIM;
   const int G = num_heads / num_kv_heads;
   if (G > gqa::kShortRows) return GQA_E_GROUP;
+  if (max_seq_len > GQA_MAX_CACHE8_KEYS) return GQA_E_CACHE8;
   *form = GQA_FORM_SINGLE;
   *parts = 0;
   if (batch == 0 || seq_q == 0 || max_seq_len == 0) return GQA_OK;
@@ -103,6 +104,7 @@ int gqa_paged8_launch(int form, const void* q, const int64_t q_stride[4], const 
   const int G = num_heads / num_kv_heads;
   if (G > gqa::kShortRows) return GQA_E_GROUP;
   if (table_stride < 0 || (int64_t)table_stride * block_size < (int64_t)max_seq_len) return GQA_E_BLOCK;
+  if (max_seq_len > GQA_MAX_CACHE8_KEYS) return GQA_E_CACHE8;
   if (form != GQA_FORM_FLAT && form != GQA_FORM_CHUNKS && form != GQA_FORM_SINGLE) return GQA_E_CACHE8;
   if (form == GQA_FORM_FLAT && ((int64_t)G * seq_q > gqa::kDecode8Rows || max_seq_len < 1)) return GQA_E_CACHE8;
   if (form != GQA_FORM_SINGLE && (parts < 1 || parts > GQA_MAX_SPLITS)) return GQA_E_SPLITS;

@@ -27,6 +27,7 @@ GQA_E_ROPE = -12
 GQA_E_CACHE8 = -13
 GQA_MIN_EXPONENT = -126
 GQA_MAX_EXPONENT = 126
+GQA_MAX_CACHE8_KEYS = 0x7FFFC000
 FORM_SINGLE, FORM_CHUNKS, FORM_FLAT = 1, 2, 3  # GQA_FORM_*
 GQA_MIN_RAW_SOFTCAP = 1e-2
 GQA_MAX_RAW_SOFTCAP = 1e8

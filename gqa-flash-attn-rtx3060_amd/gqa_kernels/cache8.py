@@ -145,6 +145,7 @@ def attention(q, k_cache, v_cache, block_table, seq_lens, causal, max_seq_len, s
     capacity = block_table.shape[1] * block_size
     max_seq_len = capacity if max_seq_len is None else int(max_seq_len)
     assert 0 <= max_seq_len <= capacity, "max_seq_len exceeds the block table's capacity"
+    assert max_seq_len <= _lib.GQA_MAX_CACHE8_KEYS, f"max_seq_len of at most {_lib.GQA_MAX_CACHE8_KEYS}"
     scale = head_dim ** -0.5 if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"a cache in 8 bits needs a positive scale, not {scale}")

@@ -605,6 +605,7 @@ int gqa_qk_norm_rope_write_launch(const void* q, const int64_t q_stride[3],
  * [GQA_MIN_EXPONENT, GQA_MAX_EXPONENT]. */
 #define GQA_MIN_EXPONENT (-126)
 #define GQA_MAX_EXPONENT 126
+#define GQA_MAX_CACHE8_KEYS 0x7FFFC000 /* max_seq_len: key indices past a sequence's end stay below 2^31 */
 typedef struct gqa_cache8 {
   void* codes;
   int64_t stride[4];
@@ -615,7 +616,8 @@ typedef struct gqa_cache8 {
 /* Attention over it.  q, o, lse, block_table, seq_lens, q_start, q_len, max_seq_len
  * as gqa_paged_fwd_launch; dtype is q's and o's, and K and V enter the products as
  * the cache's values in it.  score: as gqa_paged_scored_launch, or NULL.  A row
- * that sees no key gives zeros and LSE -inf.  Groups of at most 128 query heads.
+ * that sees no key gives zeros and LSE -inf.  Groups of at most 128 query heads,
+ * max_seq_len of at most GQA_MAX_CACHE8_KEYS.
  * gqa_paged8_plan: the form that a call of these sizes takes on a device of
  * cu_count compute units, GQA_FORM_FLAT (`parts` slots, up to 32 packed rows a kv
  * head), GQA_FORM_CHUNKS (`parts` key pieces in all, at least `batch`, shared out over

@@ -51,6 +51,8 @@ def test_attention_refusals(lib):
         assert attend(lib, **kw) == STRIDE, kw
     assert attend(lib, head_dim=96) == HEAD and attend(lib, dtype=2) == DTYPE and attend(lib, heads=7) == SHAPE and attend(lib, batch=-1) == SHAPE
     assert attend(lib, max_len=129) == BLOCK and attend(lib, table_stride=-1) == BLOCK
+    for form, parts in ((1, 0), (2, 4), (3, 4)):  # keys whose tiles' ends would pass 32 bits
+        assert attend(lib, form=form, parts=parts, ws=P, max_len=0x7FFFC001, table_stride=1 << 28) == E8
     assert attend(lib, heads=2 * 129, kv=2) == GROUP
     assert attend(lib, batch=0) == 0 and attend(lib, seq_q=0) == 0
     # More units and slots than the flat split's walk multiplies in 32 bits.
@@ -103,7 +105,8 @@ def test_plans_keep_their_limits(lib):
             need = lib.gqa_paged8_workspace_bytes(form, parts, batch, heads, sq, D)
             assert (need == 0) == (parts == 0)
     assert cache8.plan(0, 8, 2, 1, 100, 128, 256) == cache8.plan(1, 8, 2, 0, 100, 128, 256) == cache8.plan(1, 8, 2, 1, 0, 128, 256) == (_lib.FORM_SINGLE, 0)
-    for bad in ((1, 7, 2, 1, 64, 128, 256), (1, 8, 2, 1, 64, 96, 256), (-1, 8, 2, 1, 64, 128, 256), (1, 258, 2, 1, 64, 128, 256), (1, 8, 2, 1, 64, 128, 0)):
+    assert cache8.plan(1, 8, 2, 1, 0x7FFFC000, 128, 256)[0] == _lib.FORM_FLAT
+    for bad in ((1, 8, 2, 1, 0x7FFFC001, 128, 256), (1, 8, 2, 100, 2 ** 31 - 1, 128, 256), (1, 7, 2, 1, 64, 128, 256), (1, 8, 2, 1, 64, 96, 256), (-1, 8, 2, 1, 64, 128, 256), (1, 258, 2, 1, 64, 128, 256), (1, 8, 2, 1, 64, 128, 0)):
         with pytest.raises(_lib.GQAError):
             cache8.plan(*bad)
     assert cache8.route(32, 8, 8) == "split" and cache8.route(32, 8, 9) == "single"
