@@ -77,10 +77,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // being read; a wave's 8 KiB of each: K, then V.
   __shared__ __attribute__((aligned(1024))) char lds_a[4 * 8192];
   __shared__ __attribute__((aligned(1024))) char lds_b[4 * 8192];
-  // Where the waves' states meet: kMeet rows of each (two workgroups a CU have 80 KiB
-  // each).
-  constexpr int kMeet = 768 / D, kEnd = (int)sizeof(lds_a) / (16 * D);
-  __shared__ __attribute__((aligned(16))) float meet[4 * kMeet * D];
+  constexpr int kJoin = (int)sizeof(lds_b) / (16 * D);  // query rows whose four states a stage holds
   __shared__ float st_m[4][16 * NR], st_l[4][16 * NR];
 
   const Dims& dm = p.dm;
@@ -250,10 +247,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         qreg[rb][ks] = valid[rb] ? *reinterpret_cast<const u32x4*>(qrow + 16 * ks) : u32x4{0u, 0u, 0u, 0u};
     }
     look();
-    // (Always both, so that the compiler counts on them and waits for the first alone:
-    // tiles behind the piece load nothing.)
     issue(0, la);
-    issue(1, lb);
   };
 
   f32x4 acc[NR][NDB];
@@ -401,16 +395,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int rows = dm.G * dm.Sq;
   int done_b = -1;  // the piece whose state the waves hold
   bool done_valid[NR] = {};
-  // The four waves' states meet and leave as the slot's partials, as many query rows at
-  // a time as the place has room for: kMeet while the next piece's loads are on their
-  // way into the stages, at the slot's end (last) kEnd, in the first stage.  16-byte
-  // chunks of a row are swizzled, so that the lanes of a write cover the banks.
-  const auto join = [&](auto last) __attribute__((always_inline)) {
-    constexpr bool LAST = decltype(last)::value;
-    constexpr int kRows = LAST ? kEnd : kMeet;
-    float* const place = LAST ? reinterpret_cast<float*>(lds_a) : meet;
+  // The four waves' states meet and leave as the slot's partials, kJoin query rows at a
+  // time, in the second stage (the next piece's first tile is on its way into the first; a
+  // place of its own, and both tiles on their way, took three times the rounds: 16 x 8
+  // queries of up to 8000 keys 43.3 us, this 40.2, 32 tokens of up to 8000 33.5 / 32.4).
+  // 16-byte chunks of a row are swizzled, so that the lanes of a write cover the banks.
+  const auto join = [&]() __attribute__((always_inline)) {
     const auto at = [&](int wv, int rl, int chunk) {
-      return place + (wv * kRows + rl) * D + 4 * (chunk ^ (rl & 15));
+      return reinterpret_cast<float*>(lds_b) + (wv * kJoin + rl) * D + 4 * (chunk ^ (rl & 15));
     };
 #pragma unroll
     for (int rb = 0; rb < NR; ++rb) {
@@ -420,21 +412,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         st_l[wave][16 * rb + i16] = done_valid[rb] ? l_tot : -1.f;
       }
     }
-    if constexpr (LAST) {
-      wave_wait<vmcnt_imm(0)>();
-      phase_barrier();
-    }
-    for (int r0 = 0; r0 < rows; r0 += kRows) {
+    phase_barrier();  // (the stage has been read)
+    for (int r0 = 0; r0 < rows; r0 += kJoin) {
 #pragma unroll
       for (int rb = 0; rb < NR; ++rb) {
         const int rl = 16 * rb + i16 - r0;
-        if (rl >= 0 && rl < kRows) {
+        if (rl >= 0 && rl < kJoin) {
 #pragma unroll
           for (int db = 0; db < NDB; ++db) *reinterpret_cast<f32x4*>(at(wave, rl, 4 * db + lg)) = acc[rb][db];
         }
       }
       phase_barrier();
-      for (int f = t; f < min(kRows, rows - r0) * (D / 4); f += 256) {
+      for (int f = t; f < min(kJoin, rows - r0) * (D / 4); f += 256) {
         const int rl = f / (D / 4), d4 = f - rl * (D / 4), r = r0 + rl;
         if (st_l[0][r] < 0.f) continue;
         float ms = st_m[0][r];
@@ -465,9 +454,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   look();
   if (!nxt.some) return;
   for (;;) {
-    if (!nxt.some) break;
-    begin();
-    if (done_b >= 0) join(BF{});
+    if (done_b >= 0) wave_wait<vmcnt_imm(0)>();  // (loads of tiles behind the last piece)
+    const bool more = nxt.some;
+    if (more) begin();
+    if (done_b >= 0) join();
+    if (!more) return;
+    // (Always both tiles, so that the compiler counts on them and waits for the first
+    // alone: tiles behind the piece load nothing.)
+    issue(1, lb);
 #pragma unroll
     for (int rb = 0; rb < NR; ++rb) {
 #pragma unroll
@@ -496,7 +490,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       step(BF{}, BT{}, it + 1, lb);
     }
   }
-  join(BT{});
 }
 
 // Joins the slots' partials of each row, as gqa_split_reduce_kernel does with a workgroup
@@ -604,6 +597,8 @@ template <int DT, int D> static hipError_t launch_join_t(ReduceParams p, int G, 
 // slots each) 48.6 / 37.6, 64 of 1000 (1) 29.1 / 26.5, 16 of 4000 (4) 26.6 / 25.8, with 8
 // queries each 48.5 / 43.0; 8 of 4000 (8) 18.0 / 18.0 and 33.1 / 30.3; 4 of 8000 (16) 17.1
 // / 18.6; 2 of 16000 (32) 17.9 / 22.5.
+// (A slot that writes the sequences that lie in it alone itself, us: 500 of 1000 keys 161.6
+// -> 154.6, 64 of 1500 33.5 -> 34.3, one token of 700 8.1 -> 8.7: left.)
 constexpr int kFewSlots = 8;
 
 hipError_t launch_decode8_join(const ReduceParams& p, int G, int dtype, hipStream_t stream) {
