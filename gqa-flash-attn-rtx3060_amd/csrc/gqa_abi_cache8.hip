@@ -67,7 +67,7 @@ int gqa_paged8_plan(int batch, int num_heads, int num_kv_heads, int seq_q, int m
   *parts = 0;
   if (batch == 0 || seq_q == 0 || max_seq_len == 0) return GQA_OK;
   if ((int64_t)G * seq_q <= gqa::kDecode8Rows) {
-    const int64_t units = ((int64_t)max_seq_len + gqa::decode8_unit(head_dim) - 1) / gqa::decode8_unit(head_dim) * batch;
+    const int64_t unit = gqa::decode8_unit(head_dim), units = (max_seq_len + unit - 1) / unit * batch;
     int64_t slots = std::min<int64_t>({std::max(2 * cu_count / num_kv_heads, 1), units, GQA_MAX_SPLITS});
     while (slots > 1 && !flat_fits(batch, max_seq_len, head_dim, (int)slots)) slots /= 2;
     if (flat_fits(batch, max_seq_len, head_dim, (int)slots)) {
@@ -79,8 +79,14 @@ int gqa_paged8_plan(int batch, int num_heads, int num_kv_heads, int seq_q, int m
   const int rows = gqa::chunk8_rows((int64_t)G * seq_q), block_m = rows / G;
   const int64_t blocks = ((int64_t)seq_q + block_m - 1) / block_m * num_kv_heads;
   const int64_t tiles = (max_seq_len + kTile - 1) / kTile;
-  const int64_t pieces = std::min<int64_t>({(rows > gqa::kShortRows ? 1 : 2) * cu_count / blocks, batch * (tiles / 4), GQA_MAX_SPLITS});
-  if (2 * pieces >= 3 * (int64_t)batch && pieces_fit(batch, max_seq_len)) {
+  const int64_t slots = (rows > gqa::kShortRows ? 1 : 2) * cu_count;
+  const int64_t pieces = std::min<int64_t>({slots / blocks, batch * (tiles / 4), GQA_MAX_SPLITS});
+  // Pieces that fill the device once, where there are five for four sequences or more.  The
+  // single pass / these, us, 32/8 heads of 128, lengths 2000-9000 and all 5000: 8 x 160
+  // queries (9 pieces) 217 / 201 and 136 / 149, 4 x 384 (5) 221 / 165 and 136 / 151, 4 x 320
+  // (6) 220 / 140 and 135 / 150, 4 x 256 (8) 218 / 107 and 134 / 100.  Twice as many, for two
+  // rounds, take 232 / 209 and 164 / 196 (8 x 256 queries, 16).
+  if (4 * pieces >= 5 * (int64_t)batch && pieces_fit(batch, max_seq_len)) {
     *form = GQA_FORM_CHUNKS;
     *parts = (int)pieces;
   }

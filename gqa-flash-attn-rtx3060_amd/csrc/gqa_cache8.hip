@@ -20,9 +20,9 @@
 // Nothing is ordered by chance: results do not depend on the schedule.
 //
 // Measured, bf16, 32/8 heads of 128, 16-token pages: norms, rotation and store of 8192
-// tokens 51 us, 189 MB at 3.7 TB/s (a large copy 5.1; registers for four waves a
+// tokens 52 us, 189 MB at 3.6 TB/s (a large copy 5.1; registers for four waves a
 // SIMD are what keeps it from more: the rotation of 16-bit caches alone, at six, 49.5
-// us for 206 MB); K and V alone 13.8 us, 51 MB.  64 tokens, one a page: 4.4 and 3.7
+// us for 206 MB); K and V alone 14.0 us, 51 MB.  64 tokens, one a page: 4.6 and 3.7
 // us, a chain of dependent reads (slot; exponent, table row) after a launch of 2.6.
 // Rows and angles of a small call's tokens are loaded before their slots are known.
 #include <algorithm>
@@ -322,13 +322,18 @@ template <int DT> __global__ __launch_bounds__(256) void gqa_read8_kernel(Read8P
   float sk = 1.f, sv = 1.f;
   if (slot >= 0) {
     const int64_t page = slot >> p.block_shift, o = slot & ((1 << p.block_shift) - 1);
-    k = *reinterpret_cast<const u32x4*>(static_cast<const char*>(p.kc.ptr) + page * p.kc.sb + o * p.kc.ss + h * p.kc.sh + 16 * c);
-    v = *reinterpret_cast<const u32x4*>(static_cast<const char*>(p.vc.ptr) + page * p.vc.sb + o * p.vc.ss + h * p.vc.sh + 16 * c);
+    const auto codes = [&](const TensorRef& t) {
+      return static_cast<const char*>(t.ptr) + page * t.sb + o * t.ss + h * t.sh + 16 * c;
+    };
+    k = *reinterpret_cast<const u32x4*>(codes(p.kc));
+    v = *reinterpret_cast<const u32x4*>(codes(p.vc));
     sk = exp_scale(clamp_exp(p.ke.e[page * p.ke.sb + h * p.ke.sh]));
     sv = exp_scale(clamp_exp(p.ve.e[page * p.ve.sb + h * p.ve.sh]));
   }
-  u32x4* ko = reinterpret_cast<u32x4*>(static_cast<T*>(const_cast<void*>(p.k.ptr)) + tok * p.k.ss + h * p.k.sh + 16 * c);
-  u32x4* vo = reinterpret_cast<u32x4*>(static_cast<T*>(const_cast<void*>(p.v.ptr)) + tok * p.v.ss + h * p.v.sh + 16 * c);
+  const auto row = [&](const TensorRef& t) {
+    return reinterpret_cast<u32x4*>(static_cast<T*>(const_cast<void*>(t.ptr)) + tok * t.ss + h * t.sh + 16 * c);
+  };
+  u32x4 *ko = row(p.k), *vo = row(p.v);
   ko[0] = widen8<DT>(k[0], sk, k[1], sk);
   ko[1] = widen8<DT>(k[2], sk, k[3], sk);
   vo[0] = widen8<DT>(v[0], sv, v[1], sv);

@@ -18,13 +18,14 @@
 // MFMAs run beside the other's softmax on each SIMD; group 0 fills K's stages, group 1
 // V's, two of each, in their MFMA phases, from what their softmax phases load: group 0
 // K(j + 1) in the phase of its S(j), group 1 V(j) in that of its, before group 0's next
-// phase takes it; what they write over was read a phase before or earlier.  That halves what a row pays for loads, widening and LDS writes, which
-// are most of what the cache in 8 bits costs over one in 16: 2048 queries over 16384
-// keys, 32 heads over 8, 550 us for one group and 486 for two (470 the kernel over a cache
-// in 16 bits; 390 without loads and stores).  Up to 256 rows the finer blocks win (8 x 64
-// queries over 1000-4000 keys 44.6 us / 49.8).  Widening in the softmax phase, whose
-// instructions then outlast the other group's MFMAs, took 2.5 % more, pages and exponents
-// by scalar loads instead of by lane 1 %.
+// phase takes it; what they write over was read a phase before or earlier.  That halves
+// what a row pays for loads, widening and LDS writes, which are most of what the cache in
+// 8 bits costs over one in 16: 2048 queries over 16384 keys, 32 heads over 8, 550 us for
+// one group and 486 for two (470 the kernel over a cache in 16 bits; 390 without loads and
+// stores).  Up to 256 rows the finer blocks win (8 x 64 queries over 1000-4000 keys 44.6
+// us / 49.8).  Widening in the softmax phase, whose instructions then outlast the other
+// group's MFMAs, took 2.5 % more, pages and exponents by scalar loads instead of by lane
+// 1 %.
 #include <algorithm>
 #include <type_traits>
 
@@ -186,7 +187,8 @@ __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) v
   const int64_t part = ((int64_t)piece * dm.Hq + head) * dm.Sq + pos;
   if (KC && n == 0) {  // (behind the last key that the block sees)
     if (valid) {
-      for (int d = 4 * hh; d < D; d += 8) *reinterpret_cast<f32x4*>(p.ws_acc + part * D + d) = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int d = 4 * hh; d < D; d += 8)
+        *reinterpret_cast<f32x4*>(p.ws_acc + part * D + d) = f32x4{0.f, 0.f, 0.f, 0.f};
       if (hh == 0) {
         p.ws_m[part] = kEmptyRef;
         p.ws_l[part] = 0.f;
@@ -228,7 +230,9 @@ __global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
     for (int o = 0; o < NOP; ++o) pin(scale_l[o]);
   };
-  const auto page_of = [&](int j) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(page_l, j - base); };
+  const auto page_of = [&](int j) __attribute__((always_inline)) {
+    return __builtin_amdgcn_readlane(page_l, j - base);
+  };
   const auto scale_of = [&](int o, int j) __attribute__((always_inline)) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scale_l[o]), j - base));
   };

@@ -165,7 +165,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int64_t id = max(page_l, 0);
     const int key = cur.c0 + (4 * (base + lane / NB) + wave) * TW + 16 * (lane % NB);
     const int64_t slot = key & ((1 << p.block_shift) - 1);
-    const uint64_t ko = (uint64_t)kbase + id * p.k.sb + slot * p.k.ss, vo = (uint64_t)vbase + id * p.v.sb + slot * p.v.ss;
+    const uint64_t ko = (uint64_t)kbase + id * p.k.sb + slot * p.k.ss;
+    const uint64_t vo = (uint64_t)vbase + id * p.v.sb + slot * p.v.ss;
     klo = (uint32_t)ko, khi = (uint32_t)(ko >> 32), vlo = (uint32_t)vo, vhi = (uint32_t)(vo >> 32);
     sk_l = __int_as_float(page_l >= 0 ? keb[id * p.ke.sb] : 0);
     sv_l = __int_as_float(page_l >= 0 ? veb[id * p.ve.sb] : 0);
@@ -239,9 +240,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       valid[rb] = pos[rb] < sq;
       qpos[rb] = pos[rb] + (cur.skv - sq);
       seen[rb] = max(qpos[rb], prefix - 1);
-      const char* qrow = static_cast<const char*>(p.q.ptr) +
-                         2 * ((varlen ? (tok0 + pos[rb]) * p.q.ss : (int64_t)cur.b * p.q.sb + (int64_t)pos[rb] * p.q.ss) +
-                              (int64_t)head[rb] * p.q.sh + (D / 4) * lg);
+      const int64_t at = varlen ? (tok0 + pos[rb]) * p.q.ss : (int64_t)cur.b * p.q.sb + (int64_t)pos[rb] * p.q.ss;
+      const char* qrow = static_cast<const char*>(p.q.ptr) + 2 * (at + (int64_t)head[rb] * p.q.sh + (D / 4) * lg);
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks)
         qreg[rb][ks] = valid[rb] ? *reinterpret_cast<const u32x4*>(qrow + 16 * ks) : u32x4{0u, 0u, 0u, 0u};
@@ -323,7 +323,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     bool lags = false;
 #pragma unroll
-    for (int rb = 0; rb < NR; ++rb) mx[rb] = fmaxf(fmaxf(sx[rb][0][0], sx[rb][0][1]), fmaxf(sx[rb][0][2], sx[rb][0][3]));
+    for (int rb = 0; rb < NR; ++rb)
+      mx[rb] = fmaxf(fmaxf(sx[rb][0][0], sx[rb][0][1]), fmaxf(sx[rb][0][2], sx[rb][0][3]));
 #pragma unroll
     for (int kb = 1; kb < NB; ++kb)
 #pragma unroll
@@ -359,7 +360,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     for (int jj = 0; jj < NB / 2; ++jj)
 #pragma unroll
       for (int rb = 0; rb < NR; ++rb)
-        pk[rb][jj] = u32x4{E::pack2(pv[rb][2 * jj][0], pv[rb][2 * jj][1]), E::pack2(pv[rb][2 * jj][2], pv[rb][2 * jj][3]),
+        pk[rb][jj] = u32x4{E::pack2(pv[rb][2 * jj][0], pv[rb][2 * jj][1]),
+                           E::pack2(pv[rb][2 * jj][2], pv[rb][2 * jj][3]),
                            E::pack2(pv[rb][2 * jj + 1][0], pv[rb][2 * jj + 1][1]),
                            E::pack2(pv[rb][2 * jj + 1][2], pv[rb][2 * jj + 1][3])};
 #pragma unroll

@@ -480,7 +480,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
             its value times 2 ** the exponent of its page and head (in [-126,
             126]), and enter the products as those values in q's dtype.  Groups of
             at most 128 query heads, a positive scale, routes "split" (up to 32
-            packed rows a kv head), "chunks" and "single"; a row that sees no key
+            packed rows a kv head), "chunks" (splits pieces a sequence in the mean,
+            shared out by the lengths) and "single"; a row that sees no key
             gives zeros and LSE -inf; V finite at hidden keys in the 64-key tiles
             of which the row's block sees a key.
 
