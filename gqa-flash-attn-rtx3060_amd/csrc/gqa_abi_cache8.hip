@@ -76,7 +76,7 @@ int gqa_paged8_plan(int batch, int num_heads, int num_kv_heads, int seq_q, int m
       return GQA_OK;
     }
   }
-  const int rows = gqa::chunk8_rows((int64_t)G * seq_q), block_m = rows / G;
+  const int rows = gqa::chunk8_rows(G, seq_q, max_seq_len, head_dim), block_m = rows / G;
   const int64_t blocks = ((int64_t)seq_q + block_m - 1) / block_m * num_kv_heads;
   const int64_t tiles = (max_seq_len + kTile - 1) / kTile;
   const int64_t slots = (rows > gqa::kShortRows ? 1 : 2) * cu_count;
@@ -185,7 +185,7 @@ int gqa_paged8_launch(int form, const void* q, const int64_t q_stride[4], const 
   p.v = cache_ref(vc);
   p.o = r.o;
   p.dm = dm;
-  p.block_m = gqa::chunk8_rows((int64_t)G * seq_q) / G;
+  p.block_m = gqa::chunk8_rows(G, seq_q, max_seq_len, head_dim) / G;
   p.n_mblk = (seq_q + p.block_m - 1) / p.block_m;
   p.block_table = block_table;
   p.seq_lens = seq_lens;

@@ -13,19 +13,19 @@
 //
 // One group of four waves, tile j: MFMA phase (P V of the tile before, S of this one),
 // which first loads the codes of K(j + 1) and V(j), barrier, softmax phase, which ends by
-// storing them where K(j) and V(j - 1) were; barrier.  K and V have one stage each.  Two
-// groups, for more than 256 packed rows: group 1 is a phase behind group 0, so that one's
-// MFMAs run beside the other's softmax on each SIMD; group 0 fills K's stages, group 1
-// V's, two of each, in their MFMA phases, from what their softmax phases load: group 0
-// K(j + 1) in the phase of its S(j), group 1 V(j) in that of its, before group 0's next
-// phase takes it; what they write over was read a phase before or earlier.  That halves
-// what a row pays for loads, widening and LDS writes, which are most of what the cache in
-// 8 bits costs over one in 16: 2048 queries over 16384 keys, 32 heads over 8, 550 us for
-// one group and 486 for two (470 the kernel over a cache in 16 bits; 390 without loads and
-// stores).  Up to 256 rows the finer blocks win (8 x 64 queries over 1000-4000 keys 44.6
-// us / 49.8).  Widening in the softmax phase, whose instructions then outlast the other
-// group's MFMAs, took 2.5 % more, pages and exponents by scalar loads instead of by lane
-// 1 %.
+// storing them where K(j) and V(j - 1) were; barrier.  K and V have one stage each.
+//
+// Two groups, for more rows of long sequences (chunk8_rows): group 1 is a phase behind
+// group 0, so that one's MFMAs run beside the other's softmax on each SIMD; group 0 fills
+// K's stages, group 1 V's, two of each, in their MFMA phases, from what their softmax
+// phases load: group 0 K(j + 1) in the phase of its S(j), group 1 V(j) in that of its,
+// before group 0's next phase takes it; what they write over was read a phase before or
+// earlier.  That halves what a row pays for loads, widening and LDS writes, which are most
+// of what the cache in 8 bits costs over one in 16: 2048 queries over 16384 keys, 32 heads
+// over 8, 550 us for one group and 486 for two (470 the kernel over a cache in 16 bits;
+// 390 without loads and stores).  Widening in the softmax phase, whose instructions then
+// outlast the other group's MFMAs, took 2.5 % more, pages and exponents by scalar loads
+// instead of by lane 1 %.
 #include <algorithm>
 #include <type_traits>
 
@@ -543,7 +543,7 @@ template <int DT, int D> static hipError_t launch_chunk8_t(Fwd8Params p, hipStre
   return hipGetLastError();
 }
 
-// p.block_m = chunk8_rows(G, Sq) / G, p.n_mblk accordingly.
+// p.block_m = chunk8_rows(..) / G, p.n_mblk accordingly.
 hipError_t launch_chunk8(const Fwd8Params& p, int dtype, hipStream_t stream) {
   if (p.block_shift < 4 || p.block_table == nullptr) return hipErrorInvalidValue;
   if (dtype == 0) return p.dm.D == 128 ? launch_chunk8_t<0, 128>(p, stream) : launch_chunk8_t<0, 64>(p, stream);

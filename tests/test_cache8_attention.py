@@ -57,6 +57,7 @@ class Batch:
 
 
 FEW = [("split", n) for n in (1, 3, 16)] + [("chunks", 1), ("chunks", 3), ("single", None), None]
+WIDE = 8192  # keys
 MANY = [("chunks", 1), ("chunks", 2), ("chunks", 5), ("single", None), None]
 
 
@@ -76,15 +77,18 @@ def test_few_rows(Hq, Hkv, Sq, bs, D, dtype):
     (32, 8, 8, [8, 100, 513, 64]), (28, 4, 3, [3, 0, 700, 65]), (8, 8, 17, [17, 500, 129]), (4, 1, 130, [130, 131, 1000]), (128, 1, 1, [1, 63, 900]),
     (5, 1, 77, [77, 300]), (12, 4, 200, [200, 264, 1111]), (8, 2, 333, [333, 64]),
 ])
-def test_many_rows(Hq, Hkv, Sq, lens, D, dtype):
-    """Up to several blocks of 128 packed rows; a sequence shorter than its queries leaves rows empty: zeros and LSE -inf."""
-    Batch(lens, Hq, Hkv, Sq, D, 16 if Sq % 2 else 64, dtype, seed=Sq, layout="HND" if Sq % 3 else "NHD").check(MANY)
+@pytest.mark.parametrize("wide", [False, True], ids=["", "wide"])
+def test_many_rows(Hq, Hkv, Sq, lens, D, dtype, wide):
+    """Up to several blocks of 128 packed rows, or (under a large bound on the lengths) of 256; a sequence shorter than its queries leaves rows
+    empty: zeros and LSE -inf."""
+    bs = 16 if Sq % 2 else 64
+    Batch(lens, Hq, Hkv, Sq, D, bs, dtype, seed=Sq, layout="HND" if Sq % 3 else "NHD", width=(WIDE // bs if wide else None)).check(MANY)
 
 
 @pytest.mark.parametrize("Hq,Hkv,Sq", [(8, 2, 1), (8, 2, 4), (8, 2, 6), (8, 2, 40), (8, 2, 100)])
 @pytest.mark.parametrize("D", [64, 128])
 def test_without_a_mask(Hq, Hkv, Sq, D):
-    Batch([1, 50, 3 * 64, 700], Hq, Hkv, Sq, D, 16).check((None, ("single", None), ("chunks", 3)), causal=False)
+    Batch([1, 50, 3 * 64, 700], Hq, Hkv, Sq, D, 16, width=WIDE // 16 if Sq > 64 else None).check((None, ("single", None), ("chunks", 3)), causal=False)
 
 
 @pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp16"])
@@ -92,7 +96,7 @@ def test_without_a_mask(Hq, Hkv, Sq, D):
 @pytest.mark.parametrize("D", [64, 128])
 def test_changed_scores(Hq, Hkv, Sq, D, dtype):
     lens = [1, 70, 129, 640, 0, 333]
-    b = Batch(lens, Hq, Hkv, Sq, D, 32, dtype, seed=3, scale=2.0)
+    b = Batch(lens, Hq, Hkv, Sq, D, 32, dtype, seed=3, scale=2.0, width=WIDE // 32 if Sq > 64 else None)
     slopes = torch.tensor([2.0 ** (-8 * (h + 1) / Hq) for h in range(Hq)]).cuda()
     prefix = ints([0, 50, 200, 640, 5, -3])
     routes = (None, ("single", None), ("chunks", 4)) + ((("split", 5),) if Hq // Hkv * Sq <= 32 else ())
@@ -116,7 +120,7 @@ def test_exponents_near_the_types_ends():
     assert ((o[0, :, 0].double() - v).abs() <= 2.0 ** -8 * v.abs() + 2.0 ** -8 * gather(b.vc, b.ve, b.table[0], 40, BF).double().abs().mean(1).repeat_interleave(4, 0)).all()
 
 
-@pytest.mark.parametrize("Hq,Hkv,lens,ql", [(8, 2, [40, 9, 300, 0, 64], [1, 2, 4, 0, 3]), (8, 2, [140, 9, 300, 512], [100, 1, 0, 37]), (4, 1, [30] * 70, [1, 0, 2] * 23 + [4])])
+@pytest.mark.parametrize("Hq,Hkv,lens,ql", [(8, 2, [40, 9, 300, 0, 64], [1, 2, 4, 0, 3]), (8, 2, [140, 9, 300, 512], [100, 1, 0, 37]), (8, 2, [5000, 90, 400], [150, 70, 1]), (4, 1, [30] * 70, [1, 0, 2] * 23 + [4])])
 def test_variable_query_lengths(Hq, Hkv, lens, ql):
     """Token-major queries; sequences without any, tokens that belong to none (left as they were)."""
     D, start, at = 64, [], 2
@@ -167,8 +171,8 @@ def test_layouts_and_strides():
 
 def test_what_lies_past_a_sequence_is_not_read():
     """NaN codes in pages' ends and other pages, and exponents of pages that belong to nobody: no output changes."""
-    for Sq, Hq in ((1, 8), (40, 8)):
-        b = Batch([35, 100, 17], Hq, 2, Sq, 128, 16, seed=2)
+    for Sq, Hq in ((1, 8), (40, 8), (100, 8)):
+        b = Batch([35, 100, 17], Hq, 2, Sq, 128, 16, seed=2, width=WIDE // 16 if Sq > 64 else None)
         o = b.run()
         used = torch.zeros(b.kc.shape[0], 16, dtype=torch.bool, device="cuda")
         for i, n in enumerate(b.n):
@@ -209,7 +213,7 @@ def test_results_repeat_and_two_calls_at_once():
 @pytest.mark.parametrize("Sq", [1, 6, 60, 100])
 def test_captured_and_replayed(Sq):
     """Two graphs over one cache, replayed in turn and at once with eager calls in between; lengths and queries that change under them."""
-    b = Batch([900, 33, 512, 129], 8, 2, Sq, 128, 16, seed=4)
+    b = Batch([900, 33, 512, 129], 8, 2, Sq, 128, 16, seed=4, width=WIDE // 16 if Sq > 64 else None)
     b.run()
     graphs, outs, qs = [], [], []
     for i in range(2):
