@@ -85,8 +85,11 @@ int gqa_paged8_plan(int batch, int num_heads, int num_kv_heads, int seq_q, int m
   // single pass / these, us, 32/8 heads of 128, lengths 2000-9000 and all 5000: 8 x 160
   // queries (9 pieces) 217 / 201 and 136 / 149, 4 x 384 (5) 221 / 165 and 136 / 151, 4 x 320
   // (6) 220 / 140 and 135 / 150, 4 x 256 (8) 218 / 107 and 134 / 100.  Twice as many, for two
-  // rounds, take 232 / 209 and 164 / 196 (8 x 256 queries, 16).
-  if (4 * pieces >= 5 * (int64_t)batch && pieces_fit(batch, max_seq_len)) {
+  // rounds, take 232 / 209 and 164 / 196 (8 x 256 queries, 16).  Not where the queries are
+  // more than half of the keys: causal blocks then see few keys of most pieces (1024 tokens
+  // over themselves 32.9 / 36.7, 512 18.5 / 21.6; 512 over 1024 30.8 / 27.4, 1024 over 2048
+  // 56.7 / 56.9).
+  if (4 * pieces >= 5 * (int64_t)batch && max_seq_len / 2 >= seq_q && pieces_fit(batch, max_seq_len)) {
     *form = GQA_FORM_CHUNKS;
     *parts = (int)pieces;
   }
