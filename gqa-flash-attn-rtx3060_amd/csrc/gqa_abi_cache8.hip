@@ -79,7 +79,7 @@ int gqa_paged8_plan(int batch, int num_heads, int num_kv_heads, int seq_q, int m
   const int rows = gqa::chunk8_rows(G, seq_q, max_seq_len, head_dim), block_m = rows / G;
   const int64_t blocks = ((int64_t)seq_q + block_m - 1) / block_m * num_kv_heads;
   const int64_t tiles = (max_seq_len + kTile - 1) / kTile;
-  const int64_t slots = (rows > gqa::kShortRows ? 1 : 2) * cu_count;
+  const int64_t slots = (rows > gqa::kShortRows ? 1 : head_dim == 64 ? 3 : 2) * cu_count;
   const int64_t pieces = std::min<int64_t>({slots / blocks, batch * (tiles / 4), GQA_MAX_SPLITS});
   // Pieces that fill the device once, where there are five for four sequences or more.  The
   // single pass / these, us, 32/8 heads of 128, lengths 2000-9000 and all 5000: 8 x 160

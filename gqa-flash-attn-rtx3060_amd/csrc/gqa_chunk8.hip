@@ -25,7 +25,11 @@
 // over 8, 550 us for one group and 486 for two (470 the kernel over a cache in 16 bits;
 // 390 without loads and stores).  Widening in the softmax phase, whose instructions then
 // outlast the other group's MFMAs, took 2.5 % more, pages and exponents by scalar loads
-// instead of by lane 1 %.
+// instead of by lane 1 %.  At head_dim 64 the softmax takes twice as long as the matrix
+// instructions, so that three workgroups of one group a CU, each for itself, do more than
+// groups in step (8192 tokens over themselves 330 us / 375, 4 x 256 queries over 2000-9000
+// keys 79 / 86, but 2048 queries over 16384 keys, two workgroups a CU, 339 / 318), and more
+// than two (8 x 512 queries over 512-4096 keys 118 / 128).
 #include <algorithm>
 #include <type_traits>
 
@@ -101,7 +105,7 @@ struct Pieces {
 // NG: groups of four waves, 128 rows each.  KC: over key pieces, whose partials
 // launch_decode8_join joins by the plan that one workgroup past the others writes.
 template <int DT, int D, int NG, bool KC>
-__global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(2))) void gqa_chunk8_kernel(Fwd8Params p) {
+__global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void gqa_chunk8_kernel(Fwd8Params p) {
   using E = Elem<DT>;
   using T = typename E::T;
   using ST = FwdStage<D>;
@@ -534,8 +538,12 @@ template <int DT, int D> static hipError_t launch_chunk8_t(Fwd8Params p, hipStre
   p.bm_mul = (65536u + (uint32_t)p.block_m - 1) / (uint32_t)p.block_m;
   const dim3 grid((unsigned)(total + (p.kv_splits > 0 ? 1 : 0)));
   if (p.block_m * p.dm.G > kShortRows) {
-    if (p.kv_splits > 0) hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 2, true>), grid, dim3(512), 0, stream, p);
-    else hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 2, false>), grid, dim3(512), 0, stream, p);
+    if constexpr (D == 128) {
+      if (p.kv_splits > 0) hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 2, true>), grid, dim3(512), 0, stream, p);
+      else hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 2, false>), grid, dim3(512), 0, stream, p);
+    } else {
+      return hipErrorInvalidValue;
+    }
   } else {
     if (p.kv_splits > 0) hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 1, true>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 1, false>), grid, dim3(256), 0, stream, p);

@@ -402,17 +402,16 @@ constexpr int decode8_unit(int head_dim) { return 16384 / head_dim; }
 hipError_t launch_decode8(const Split8Params& p, int dtype, hipStream_t stream);
 // Joins the partials of the two by the plan, p.slots of them at most.
 hipError_t launch_decode8_join(const ReduceParams& p, int G, int dtype, hipStream_t stream);
-// Packed rows of a workgroup of launch_chunk8: 256 where that adds at most a quarter to the
-// rows of whole blocks and a sequence's codes of a head are long enough that what a tile
-// costs counts for more than filling the device with twice the workgroups.  128 / 256 rows,
-// us, 32/8 heads, at head_dim 128 and 64: prompts of 512 tokens 21.4 / 25.4 and 16.0 /
-// 19.2, 2048 59.6 / 65.5 and 43.8 / 53.9, 4096 165 / 145 and 115 / 112; 8 x 512 queries
-// over 512-4096 keys 179 / 176 and 129 / 145; 512 over 16384 160 / 143 and 109 / 104; 320
-// rows (4 x 80 queries) over 2000-6000 47.0 / 50.8 and 34.4 / 39.6.
+// Packed rows of a workgroup of launch_chunk8: at head_dim 128 (gqa_chunk8.hip) 256 where
+// that adds at most a quarter to the rows of whole blocks and the sequences are long, so
+// that what a tile costs counts for more than filling the device with twice the workgroups.
+// 128 / 256 rows, us, 32/8 heads: prompts of 512 tokens 21.4 / 25.4, 2048 59.6 / 65.5, 3000
+// 93.2 / 92.4, 4096 165 / 145; 8 x 512 queries over 512-4096 keys 179 / 176; 512 over 16384
+// 160 / 143; 320 rows (4 x 80 queries) over 2000-6000 47.0 / 50.8.
 constexpr int chunk8_rows(int G, int64_t seq_q, int64_t seq_kv, int head_dim) {
   const int64_t one = (seq_q + kShortRows / G - 1) / (kShortRows / G);
   const int64_t two = (seq_q + 2 * kShortRows / G - 1) / (2 * kShortRows / G);
-  return one > 2 && 8 * two <= 5 * one && seq_kv * head_dim >= 1 << 19 ? 2 * kShortRows : kShortRows;
+  return head_dim == 128 && one > 2 && 8 * two <= 5 * one && seq_kv >= 4096 ? 2 * kShortRows : kShortRows;
 }
 hipError_t launch_chunk8(const Fwd8Params& p, int dtype, hipStream_t stream);
 hipError_t launch_store8(const Store8Params& p, int dtype, hipStream_t stream);

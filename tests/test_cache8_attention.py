@@ -57,7 +57,7 @@ class Batch:
 
 
 FEW = [("split", n) for n in (1, 3, 16)] + [("chunks", 1), ("chunks", 3), ("single", None), None]
-WIDE = 8192  # keys
+WIDE = 4096  # keys
 MANY = [("chunks", 1), ("chunks", 2), ("chunks", 5), ("single", None), None]
 
 
