@@ -105,7 +105,8 @@ struct Pieces {
 // NG: groups of four waves, 128 rows each.  KC: over key pieces, whose partials
 // launch_decode8_join joins by the plan that one workgroup past the others writes.
 template <int DT, int D, int NG, bool KC>
-__global__ __launch_bounds__(256 * NG) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void gqa_chunk8_kernel(Fwd8Params p) {
+__global__ __launch_bounds__(256 * NG)
+__attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void gqa_chunk8_kernel(Fwd8Params p) {
   using E = Elem<DT>;
   using T = typename E::T;
   using ST = FwdStage<D>;
@@ -537,17 +538,15 @@ template <int DT, int D> static hipError_t launch_chunk8_t(Fwd8Params p, hipStre
   p.div_hkv = make_fast_div((uint32_t)p.dm.Hkv);
   p.bm_mul = (65536u + (uint32_t)p.block_m - 1) / (uint32_t)p.block_m;
   const dim3 grid((unsigned)(total + (p.kv_splits > 0 ? 1 : 0)));
-  if (p.block_m * p.dm.G > kShortRows) {
-    if constexpr (D == 128) {
+  if constexpr (D == 128) {
+    if (p.block_m * p.dm.G > kShortRows) {
       if (p.kv_splits > 0) hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 2, true>), grid, dim3(512), 0, stream, p);
       else hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 2, false>), grid, dim3(512), 0, stream, p);
-    } else {
-      return hipErrorInvalidValue;
+      return hipGetLastError();
     }
-  } else {
-    if (p.kv_splits > 0) hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 1, true>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 1, false>), grid, dim3(256), 0, stream, p);
   }
+  if (p.kv_splits > 0) hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 1, true>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((gqa_chunk8_kernel<DT, D, 1, false>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
