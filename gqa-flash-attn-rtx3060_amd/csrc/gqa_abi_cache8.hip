@@ -39,8 +39,8 @@ TensorRef ref4(const void* ptr, const int64_t* st) { return TensorRef{ptr, st[0]
 TensorRef token_ref(const void* ptr, const int64_t* st) { return TensorRef{ptr, 0, st[1], st[0]}; }
 
 // Units of the flat split and slots that its walk can multiply in 32 bits.
-bool flat_fits(int batch, int max_seq_len, int head_dim, int slots) {
-  const int64_t units = ((int64_t)max_seq_len + gqa::decode8_unit(head_dim) - 1) / gqa::decode8_unit(head_dim);
+bool flat_fits(int batch, int max_seq_len, int slots) {
+  const int64_t units = ((int64_t)max_seq_len + gqa::kDecode8Unit - 1) / gqa::kDecode8Unit;
   return (units * batch + 1) * (slots + 1) < ((int64_t)1 << 31);
 }
 
@@ -67,10 +67,10 @@ int gqa_paged8_plan(int batch, int num_heads, int num_kv_heads, int seq_q, int m
   *parts = 0;
   if (batch == 0 || seq_q == 0 || max_seq_len == 0) return GQA_OK;
   if ((int64_t)G * seq_q <= gqa::kDecode8Rows) {
-    const int64_t unit = gqa::decode8_unit(head_dim), units = (max_seq_len + unit - 1) / unit * batch;
+    const int64_t unit = gqa::kDecode8Unit, units = (max_seq_len + unit - 1) / unit * batch;
     int64_t slots = std::min<int64_t>({std::max(2 * cu_count / num_kv_heads, 1), units, GQA_MAX_SPLITS});
-    while (slots > 1 && !flat_fits(batch, max_seq_len, head_dim, (int)slots)) slots /= 2;
-    if (flat_fits(batch, max_seq_len, head_dim, (int)slots)) {
+    while (slots > 1 && !flat_fits(batch, max_seq_len, (int)slots)) slots /= 2;
+    if (flat_fits(batch, max_seq_len, (int)slots)) {
       *form = GQA_FORM_FLAT;
       *parts = (int)slots;
       return GQA_OK;
@@ -117,7 +117,7 @@ int gqa_paged8_launch(int form, const void* q, const int64_t q_stride[4], const 
   if (form != GQA_FORM_FLAT && form != GQA_FORM_CHUNKS && form != GQA_FORM_SINGLE) return GQA_E_CACHE8;
   if (form == GQA_FORM_FLAT && ((int64_t)G * seq_q > gqa::kDecode8Rows || max_seq_len < 1)) return GQA_E_CACHE8;
   if (form != GQA_FORM_SINGLE && (parts < 1 || parts > GQA_MAX_SPLITS)) return GQA_E_SPLITS;
-  if (form == GQA_FORM_FLAT && !flat_fits(batch, max_seq_len, head_dim, parts)) return GQA_E_CACHE8;
+  if (form == GQA_FORM_FLAT && !flat_fits(batch, max_seq_len, parts)) return GQA_E_CACHE8;
   if (form == GQA_FORM_CHUNKS && (parts < batch || !pieces_fit(batch, max_seq_len))) return GQA_E_SPLITS;
   gqa::ScoreMod mod{};
   if (score != nullptr) {

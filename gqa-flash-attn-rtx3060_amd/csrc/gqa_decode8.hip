@@ -12,10 +12,10 @@
 // What bounds it is the read of the cache, half the bytes of 16 bits, so each byte
 // has twice the arithmetic of the 16-bit pass.  There the four waves of a workgroup
 // share a tile, wait for each other twice a tile, and each computes all scores of it;
-// here a wave is on its own: it takes every fourth tile of TW keys (4 KiB of K and
-// of V), all of its scores and all head dimensions, loads tiles into LDS of its own
-// two ahead, and meets the others once a piece, in LDS.  No barrier within the
-// stream, no score computed twice.
+// here a wave is on its own: it takes every fourth tile of 32 keys (4 KiB of K and of V, 2
+// at head_dim 64), all of its scores and all head dimensions, loads tiles into LDS of its
+// own two ahead, and meets the others once a piece, in LDS.  No barrier within the stream,
+// no score computed twice.
 //
 // The keys of all sequences are cut into equal ranges, one a workgroup, on the
 // device (gqa_flat.hpp), in units of four tiles.
@@ -59,7 +59,11 @@ __device__ inline u32x2 ld_tr8(const char* p) {
 template <int DT, int D, int NR, bool MOD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void gqa_decode8_kernel(Split8Params p) {
   using E = Elem<DT>;
-  constexpr int TW = 4096 / D;     // keys of a wave's tile
+  // Keys of a wave's tile.  (64 at head_dim 64, as many bytes: 24 tokens of 200-6000 keys
+  // 17.1 us, this 16.0; 256 of up to 300 28.6 / 25.8; 8 queries of 8000 11.0 / 12.7, of
+  // 131072 41.6 / 39.4.)
+  constexpr int TW = 32;
+  constexpr int TBY = TW * D;      // its bytes of K, and of V
   constexpr int NB = TW / 16;      // 16-key blocks
   constexpr int CPR = D / 16;      // 16-byte chunks per row
   constexpr int RPI = 64 / CPR;    // rows per load instruction: 8 or 16, within a block
@@ -72,11 +76,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // probabilities exceed 1, which no type here minds (fp16 holds 2^15), and the
   // accumulators need no scaling (16 x 8 queries of 8000 keys 71.0 -> 69.7 us).
   constexpr float kLag = 8.f;
-  static_assert(UNIT == decode8_unit(D), "unit of the flat split");
+  static_assert(UNIT == kDecode8Unit, "unit of the flat split");
   // An array a stage, so that the compiler can tell the load's target from the stage
-  // being read; a wave's 8 KiB of each: K, then V.
-  __shared__ __attribute__((aligned(1024))) char lds_a[4 * 8192];
-  __shared__ __attribute__((aligned(1024))) char lds_b[4 * 8192];
+  // being read; a wave's part of each: K, then V.
+  __shared__ __attribute__((aligned(1024))) char lds_a[4 * 2 * TBY];
+  __shared__ __attribute__((aligned(1024))) char lds_b[4 * 2 * TBY];
   constexpr int kJoin = (int)sizeof(lds_b) / (16 * D);  // query rows whose four states a stage holds
   __shared__ float st_m[4][16 * NR], st_l[4][16 * NR];
 
@@ -127,8 +131,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     return D == 128 ? ((row >> 1) & 3) | (((row >> 4) & 1) << 2) : ((row >> 2) & 1) | (((row >> 4) & 1) << 1);
   };
   const int lrow = lane / CPR, lch = lane % CPR;
-  char* const la = lds_a + wave * 8192;
-  char* const lb = lds_b + wave * 8192;
+  char* const la = lds_a + wave * 2 * TBY;
+  char* const lb = lds_b + wave * 2 * TBY;
   // LDS read offsets.  K: row i16 of a block (fk does not depend on the block).  V:
   // rows 4 lg + 0..3 and 16 + 4 lg + 0..3 of 32 (fv does not depend on which 32).
   uint32_t ka[NKS / 2];
@@ -201,7 +205,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const int at = (bl * IPB + i) * 1024;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(tk, (lds_void*)(stage + at), 16, ko, (uint32_t)(i * RPI) * kss, 0,
                                                  kDmaStream);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(tv, (lds_void*)(stage + 4096 + at), 16, vo, (uint32_t)(i * RPI) * vss,
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(tv, (lds_void*)(stage + TBY + at), 16, vo, (uint32_t)(i * RPI) * vss,
                                                  0, kDmaStream);
       }
     }
@@ -263,7 +267,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       sv[bl] = scale_at(sv_l, it, bl);
     }
     const char* ck = stage;
-    const char* cv = stage + 4096;
+    const char* cv = stage + TBY;
     // One row block: all reads of the tile first (32 sequences of up to 8000 keys 34.1 ->
     // 33.0 us).  Two: where they are used (all first, for the registers they hold, 42.7 ->
     // 44.1 us in 16 x 8 queries of up to 8000 keys).
@@ -558,7 +562,7 @@ __global__ __launch_bounds__(256) void gqa_decode8_join_kernel(ReduceParams p, F
 
 template <int DT, int D> static hipError_t launch_decode8_t(Split8Params p, hipStream_t stream) {
   const int64_t total = (int64_t)p.dm.Hkv * p.slots;
-  const int64_t units = (p.dm.Skv + decode8_unit(D) - 1) / decode8_unit(D);
+  const int64_t units = (p.dm.Skv + kDecode8Unit - 1) / kDecode8Unit;
   // (32-bit products of units and slots in the walk.)
   if (total <= 0 || total >= (int64_t)1 << 30 || (units * p.dm.B + 1) * (p.slots + 1) >= (int64_t)1 << 31)
     return hipErrorInvalidValue;

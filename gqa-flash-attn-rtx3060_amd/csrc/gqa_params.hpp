@@ -398,7 +398,7 @@ hipError_t launch_rope(const RopeParams& p, int dtype, hipStream_t stream);
 // and its writes and reads.
 constexpr int kDecode8Rows = 32;
 // Keys of the flat split's unit.
-constexpr int decode8_unit(int head_dim) { return 16384 / head_dim; }
+constexpr int kDecode8Unit = 128;
 hipError_t launch_decode8(const Split8Params& p, int dtype, hipStream_t stream);
 // Joins the partials of the two by the plan, p.slots of them at most.
 hipError_t launch_decode8_join(const ReduceParams& p, int G, int dtype, hipStream_t stream);

@@ -100,7 +100,7 @@ def test_plans_keep_their_limits(lib):
             assert form == (_lib.FORM_FLAT if few else form) and 0 <= parts <= 1024
             assert (form == _lib.FORM_SINGLE) == (parts == 0)
             if form == _lib.FORM_FLAT:
-                units = -(-n // (16384 // D)) * batch
+                units = -(-n // 128) * batch
                 assert few and parts <= units and (units + 1) * (parts + 1) < 1 << 31
             need = lib.gqa_paged8_workspace_bytes(form, parts, batch, heads, sq, D)
             assert (need == 0) == (parts == 0)
