@@ -917,17 +917,27 @@ class PagedKVCache:
                num_new: Optional[Sequence[int]] = None) -> torch.Tensor:
         """Append K/V of new tokens, sequence-major: the first num_new[0]
         rows of key/value (num_tokens, num_kv_heads, head_dim) belong to
-        seq_ids[0], and so on (default: an equal share each).  Returns the
-        int64 slot mapping written."""
+        seq_ids[0], and so on (default: an equal share each; a sequence may come
+        more than once).  Returns the int64 slot mapping written."""
         if num_new is None:
             assert key.shape[0] % len(seq_ids) == 0
             num_new = [key.shape[0] // len(seq_ids)] * len(seq_ids)
         assert sum(num_new) == key.shape[0]
         slots: List[int] = []
+        # Over 8 bits a page's tokens stand next to one another in a store: where a
+        # sequence comes back behind others, another one begins.
+        starts, seen, last = [0], set(), None
         for sid, n in zip(seq_ids, num_new):
+            if n > 0 and self.exponents is not None:
+                if sid in seen and sid != last:
+                    starts.append(len(slots))
+                    seen.clear()
+                seen.add(sid)
+                last = sid
             slots += self.reserve(sid, n)
         slot_mapping = torch.tensor(slots, dtype=torch.int64).to(self.kv.device)
-        write_kv(key, value, self.k_cache, self.v_cache, slot_mapping, **self._exponents())
+        for a, b in zip(starts, starts[1:] + [len(slots)]):
+            write_kv(key[a:b], value[a:b], self.k_cache, self.v_cache, slot_mapping[a:b], **self._exponents())
         return slot_mapping
 
     def _exponents(self) -> dict:
