@@ -552,7 +552,7 @@ template <int DT, int D> static hipError_t launch_chunk8_t(Fwd8Params p, hipStre
 
 // p.block_m = chunk8_rows(..) / G, p.n_mblk accordingly.
 hipError_t launch_chunk8(const Fwd8Params& p, int dtype, hipStream_t stream) {
-  if (p.block_shift < 4 || p.block_table == nullptr) return hipErrorInvalidValue;
+  if (p.block_shift < 4 || (p.block_table == nullptr && p.dm.Skv > 0)) return hipErrorInvalidValue;
   if (dtype == 0) return p.dm.D == 128 ? launch_chunk8_t<0, 128>(p, stream) : launch_chunk8_t<0, 64>(p, stream);
   return p.dm.D == 128 ? launch_chunk8_t<1, 128>(p, stream) : launch_chunk8_t<1, 64>(p, stream);
 }

@@ -1,16 +1,28 @@
 """The paged cache in 8 bits at the edges of what its calls allow."""
+import ctypes
+
 import pytest
 import torch
 
-from cache8_reference import CODES
-from gqa_kernels import paged
-from gqa_kernels.paged import PagedKVCache
+from cache8_reference import CODES, new_cache
+from gqa_kernels import _lib, cache8, paged
+from gqa_kernels.paged import PagedKVCache, paged_attention
 
 BF = torch.bfloat16
 
 
 def rand(*shape, dtype=BF, seed=0, scale=1.0):
     return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype).cuda()
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32).cuda()
+
+
+def python_alone(monkeypatch):
+    """Calls go through Python's checks and ctypes."""
+    monkeypatch.setattr(_lib, "_host", None)
+    monkeypatch.setattr(cache8, "_decode_host", lambda: None)
 
 
 # ---------------------------------------------------------------------------
@@ -73,3 +85,38 @@ def test_append_of_a_sequence_that_comes_back(ids, new):
             # Half a step of the value twice (stored, brought to a larger exponent) and half the least step of the page's largest value, once a store.
             unit = x[page].abs().amax((0, 2))[:, None] / 224
             assert ((k[page].double() - x[page]).abs() <= 2 * 2.0 ** -4 * x[page].abs() + 16 * 2.0 ** -10 * unit).all()
+
+
+# ---------------------------------------------------------------------------
+# No keys at all
+# ---------------------------------------------------------------------------
+@pytest.mark.skipif(torch.cuda.is_available(), reason="what follows the checks would launch")
+def test_no_table_is_needed_without_keys():
+    """The checks let the call pass: what fails is the missing device."""
+    P, st = 0x10000, _lib._i64x4(8 * 64 * 128, 64 * 128, 128, 1)
+    none, dead = _lib.Cache8(), 100  # hipErrorNoDevice
+    for form, parts, ws in ((_lib.FORM_SINGLE, 0, None), (_lib.FORM_CHUNKS, 2, P)):
+        assert _lib.load().gqa_paged8_launch(form, P, st, ctypes.byref(none), ctypes.byref(none), None, 0, P, None, None, 16, 0, P, st, P, ws, parts, 1, 8, 2, 4,
+                                             128, 0.1, 1, 0, None, None) == dead
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("binding", ["native", "python"])
+@pytest.mark.parametrize("Sq", [1, 4, 40])
+def test_tables_of_no_pages(Sq, binding, monkeypatch):
+    """Requests that have no page yet, over a cache with blocks and over one without: zeros and LSE -inf."""
+    q = rand(3, 8, Sq, 64)
+    table, lens = torch.empty(3, 0, dtype=torch.int32, device="cuda"), ints([0, 0, 0])
+    for blocks in (4, 0):
+        kc, vc, ke, ve = new_cache(blocks, 16, 2, 64)
+        e = dict(k_exponents=ke, v_exponents=ve)
+        paged_attention(q, kc, vc, table, lens, **e)  # (loads the binding)
+        if binding == "python":
+            python_alone(monkeypatch)
+        for kw in ({}, dict(causal=False), dict(softcap=20.0), dict(out=torch.full_like(q, 7.0))):
+            o, lse = paged_attention(q, kc, vc, table, lens, return_lse=True, **e, **kw)
+            assert o.shape == q.shape and not o.any() and (lse == -float("inf")).all()
+            assert torch.equal(paged_attention(q, kc, vc, table, lens, **e, **kw), o)
+        t = q.transpose(1, 2).flatten(0, 1).contiguous()
+        o = paged_attention(t, kc, vc, table, lens, query_start=ints([0, Sq, 2 * Sq]), query_lens=ints([Sq] * 3), max_query_len=Sq, **e)
+        assert not o.any()
