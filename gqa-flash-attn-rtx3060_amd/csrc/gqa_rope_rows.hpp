@@ -189,14 +189,19 @@ __device__ __forceinline__ void row_norm_rotate_closely(const RopeParams& p, con
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       ss = __builtin_fma((double)ya[i], (double)ya[i], __builtin_fma((double)yb[i], (double)yb[i], ss));
-    const double x = row_sum<D / 16>(ss) * (1.0 / D) + (double)p.eps;
-    const double r = 1.0f / __builtin_sqrtf((float)x), inv = r * (1.5 - 0.5 * x * r * r);  // (a step of Newton's)
+    // Rows are brought to a size about 1 by 2^-h before the weights, whose products then
+    // stay within fp32 whatever the row's size (64 tokens 4.62 -> 4.67 us, 8192 as they were).
+    const double x = row_sum<D / 16>(ss) * (1.0 / D) + (double)p.eps, r = __builtin_amdgcn_rsq(x);
+    const int h = max(min((__builtin_amdgcn_frexp_exp(x) + 1) >> 1, 126), -126);
+    // (The instruction's 2^-23, then a step of Newton's; infinite rows: 0.)
+    const double inv = __builtin_ldexp(x < __builtin_inf() ? r * (1.5 - 0.5 * x * r * r) : r, h);
     hi = (float)inv;
     lo = (float)(inv - (double)hi);
+    const float less = __builtin_ldexpf(1.f, -h);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      ya[i] *= wa[i];
-      yb[i] *= wb[i];
+      ya[i] = ya[i] * less * wa[i];
+      yb[i] = yb[i] * less * wb[i];
     }
   }
   const auto minus = [](float a, float co, float c, float si) __attribute__((always_inline)) {  // a co - c si

@@ -4,9 +4,10 @@ import ctypes
 import pytest
 import torch
 
-from cache8_reference import CODES, new_cache
-from gqa_kernels import _lib, cache8, paged
+from cache8_reference import CODES, new_cache, power, values
+from gqa_kernels import RotaryTable, _lib, cache8, paged, qk_norm_rope_write
 from gqa_kernels.paged import PagedKVCache, paged_attention
+from ops_reference import rope64
 
 BF = torch.bfloat16
 
@@ -120,3 +121,53 @@ def test_tables_of_no_pages(Sq, binding, monkeypatch):
         t = q.transpose(1, 2).flatten(0, 1).contiguous()
         o = paged_attention(t, kc, vc, table, lens, query_start=ints([0, Sq, 2 * Sq]), query_lens=ints([Sq] * 3), max_query_len=Sq, **e)
         assert not o.any()
+
+
+# ---------------------------------------------------------------------------
+# Norms of keys of any size
+# ---------------------------------------------------------------------------
+def stored_keys(k, wk, eps, *, R, inter=False, bs=16, start=3, seed=0):
+    """(keys that the cache then holds, their unit, those of rope64, the row's largest of these)."""
+    T, Hkv, D = k.shape
+    table = None if R == 0 else RotaryTable(D, 9000, rotary_dim=R, interleaved=inter)
+    pos = torch.randint(0, 9000, (T,), generator=torch.Generator().manual_seed(seed)).cuda()
+    kc, vc, ke, ve = new_cache((start + T) // bs + 1, bs, Hkv, D, full=False)
+    slots = (torch.arange(T) + start).cuda()
+    qk_norm_rope_write(k, k, k, pos, table, kc, vc, slots, k_weight=wk, eps=eps, k_exponents=ke, v_exponents=ve)
+    inv = 10000.0 ** (-torch.arange(0, R, 2, dtype=torch.float64) / R) if R else None
+    y, _ = rope64(k, wk, eps, pos[None, :, None] if R else None, rotary_dim=R, interleaved=inter, inv_freq=inv, axes=[0] * (R // 2))
+    page = slots // bs
+    return values(kc, ke)[page, slots % bs], power(ke)[page][..., None], y, y.abs().amax(-1, keepdim=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,R,inter", [(64, 64, False), (128, 64, True), (128, 0, False), (128, 128, False)])
+@pytest.mark.parametrize("w32", [False, True], ids=["w16", "w32"])
+def test_norms_of_keys_of_any_size(D, R, inter, w32):
+    """Rows of bf16 from its smallest numbers to its largest, whose squares and weighted values pass fp32's range (and, below it, vanish): as close as any."""
+    T, Hkv = 40, 2
+    size = torch.exp2(torch.linspace(-122, 125, T * Hkv).round()).view(T, Hkv, 1).cuda()
+    k = (rand(T, Hkv, D).clamp(-3.9, 3.9).float() * size).to(BF)
+    assert torch.isfinite(k).all() and float(k.float().abs().max()) > 1e38
+    for least, most in ((-1, 1), (9, 12), (-12, -9)):
+        w = torch.exp2(torch.empty(D).uniform_(least, most, generator=torch.Generator().manual_seed(1))).cuda()
+        w = w if w32 else w.to(BF)
+        for eps in (1e-6, 0.0):
+            got, unit, y, top = stored_keys(k, w, eps, R=R, inter=inter)
+            assert torch.isfinite(y).all() and (y.abs().amax((0, 2)) > 2.0 ** (least - 1)).all()
+            assert ((got - y).abs() <= 2.0 ** -4 * y.abs() + 2.0 ** -10 * unit + 2.0 ** -18 * top).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, torch.float16], ids=["bf16", "fp16"])
+def test_norms_of_rows_with_infinities_and_nan(dtype):
+    """An infinite key, normed: zeros beside it, as 1 / rms = 0 gives, and NaN where 0 meets it (and in what it turns with); a NaN is the whole row's."""
+    k = rand(6, 2, 128, dtype=dtype)
+    k[1, 0, 3], k[2, 1, 70], k[2, 1, 71], k[4, 0, 5] = float("inf"), -float("inf"), float("inf"), float("nan")
+    w = (rand(128, seed=1) * 0.3 + 1).to(dtype)
+    for R in (0, 128, 64):
+        got, unit, y, top = stored_keys(k, w, 1e-6, R=R, start=0)
+        assert torch.equal(torch.isnan(got), torch.isnan(y)) and torch.isnan(y[4, 0]).all()
+        top = torch.nan_to_num(y, nan=0.0).abs().amax(-1, keepdim=True)
+        ok = ~torch.isnan(y)
+        assert ((got - y).abs() <= 2.0 ** -4 * y.abs() + 2.0 ** -10 * unit + 2.0 ** -18 * top)[ok].all()
