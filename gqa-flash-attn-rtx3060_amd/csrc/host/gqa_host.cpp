@@ -666,8 +666,9 @@ bool cache8_of(const py::handle& hc, const py::handle& he, int64_t dev, gqa_cach
 }
 bool caches8_ready(const py::handle& hkc, const py::handle& hvc, const py::handle& hke, const py::handle& hve,
                    int64_t dev, gqa_cache8 (&c)[2]) {
-  return cache8_of(hkc, hke, dev, c[0]) && cache8_of(hvc, hve, dev, c[1]) &&
-         THPVariable_Unpack(hkc.ptr()).sizes() == THPVariable_Unpack(hvc.ptr()).sizes();
+  if (!cache8_of(hkc, hke, dev, c[0]) || !cache8_of(hvc, hve, dev, c[1])) return false;
+  const at::Tensor &kc = THPVariable_Unpack(hkc.ptr()), &vc = THPVariable_Unpack(hvc.ptr());
+  return kc.sizes() == vc.sizes() && !wants_grad({&kc, &vc});
 }
 int cu_count(int64_t dev) {  // (guarded by the GIL)
   static std::array<int, 64> counts{};
@@ -721,7 +722,7 @@ py::object paged_attn8(const py::handle& hq, const py::handle& hkc, const py::ha
   } else {
     const at::Tensor* po = plain(hout);
     if (po == nullptr || po->sizes() != q.sizes() || po->scalar_type() != q.scalar_type() || po->get_device() != dev ||
-        !rows_ready(*po))
+        !rows_ready(*po) || wants_grad({po}))
       return py::none();
     out = *po;
   }
@@ -918,7 +919,7 @@ py::object norm_rope(const py::handle& hq, const py::handle& hk, const py::handl
     } else {
       const at::Tensor* o = plain(*given[i]);
       if (o == nullptr || o->sizes() != ins[i]->sizes() || o->scalar_type() != ins[i]->scalar_type() ||
-          o->get_device() != dev)
+          o->get_device() != dev || (bits8 && wants_grad({o})))
         return py::none();
       outs[i] = *o;
     }

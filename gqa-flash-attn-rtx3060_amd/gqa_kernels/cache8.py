@@ -111,7 +111,7 @@ def attention(q, k_cache, v_cache, block_table, seq_lens, causal, max_seq_len, s
             return res
     from .paged import _cu_count, _row_strides, _rows_ready
 
-    refuse_grad("paged_attention over a cache in 8 bits", q, alibi_slopes)
+    refuse_grad("paged_attention over a cache in 8 bits", q, k_cache, v_cache, alibi_slopes, out)
     dev = q.device
     varlen = query_start is not None
     assert q.is_cuda and q.dtype in _DTYPES, f"unsupported dtype {q.dtype}"
@@ -218,7 +218,7 @@ def write(key, value, k_cache, v_cache, slot_mapping, k_exponents, v_exponents) 
         return
     from .rotary import _ready
 
-    refuse_grad("write_kv into a cache in 8 bits", key, value)
+    refuse_grad("write_kv into a cache in 8 bits", key, value, k_cache, v_cache)
     block_size = check_caches(k_cache, v_cache, k_exponents, v_exponents)
     _check_tokens(key, value, k_cache, slot_mapping)
     _launch_write(None, _ready(key), _ready(value), None, k_cache, v_cache, k_exponents, v_exponents,
@@ -230,7 +230,7 @@ def norm_rope_write(q, k, v, positions, table, k_cache, v_cache, slot_mapping, q
     """``qk_norm_rope_write`` into a cache in 8 bits."""
     from .rotary import _check_out, _check_qk, _out_like, _ready, _rope
 
-    refuse_grad("qk_norm_rope_write", q, k, v, q_weight, k_weight)
+    refuse_grad("qk_norm_rope_write", q, k, v, q_weight, k_weight, k_cache, v_cache, q_out)
     _check_qk(q, k, 3)
     assert k.shape[0] == q.shape[0], "q and k have different tokens"
     block_size = check_caches(k_cache, v_cache, k_exponents, v_exponents)
@@ -270,6 +270,7 @@ def read_kv(k_cache, v_cache, slot_mapping, k_exponents, v_exponents, *, dtype=t
             return res
     from .rotary import _rows_ready
 
+    refuse_grad("read_kv", k_cache, v_cache, key, value)
     block_size = check_caches(k_cache, v_cache, k_exponents, v_exponents)
     assert dtype in _DTYPES, f"unsupported dtype {dtype}"
     assert slot_mapping.dtype == torch.int64 and slot_mapping.dim() == 1 and slot_mapping.device == k_cache.device

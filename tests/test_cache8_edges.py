@@ -3,10 +3,11 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from cache8_reference import CODES, new_cache, power, values
 from gqa_kernels import RotaryTable, _lib, cache8, paged, qk_norm_rope_write
-from gqa_kernels.paged import PagedKVCache, paged_attention
+from gqa_kernels.paged import PagedKVCache, paged_attention, read_kv, write_kv
 from ops_reference import rope64
 
 BF = torch.bfloat16
@@ -171,3 +172,52 @@ def test_norms_of_rows_with_infinities_and_nan(dtype):
         top = torch.nan_to_num(y, nan=0.0).abs().amax(-1, keepdim=True)
         ok = ~torch.isnan(y)
         assert ((got - y).abs() <= 2.0 ** -4 * y.abs() + 2.0 ** -10 * unit + 2.0 ** -18 * top)[ok].all()
+
+
+# ---------------------------------------------------------------------------
+# What would lose a derivative
+# ---------------------------------------------------------------------------
+def losing_calls():
+    """name: (tensors that may not carry one, the call)."""
+    kc, vc, ke, ve = new_cache(3, 16, 2, 64)
+    x = {"kc": kc, "vc": vc, "q": rand(1, 4, 6, 64), "out": rand(1, 4, 6, 64), "slopes": rand(4).float(), "qt": rand(6, 4, 64), "qo": rand(6, 4, 64),
+         "kt": rand(6, 2, 64), "vt": rand(6, 2, 64), "w": rand(64), "key": rand(6, 2, 64), "value": rand(6, 2, 64)}
+    rot, table, lens, pos, slots = RotaryTable(64, 50), ints([[2, 0, 1]]), ints([40]), ints(range(6)), torch.arange(6).cuda()
+    e = dict(k_exponents=ke, v_exponents=ve)
+    return x, {
+        "attention": (("q", "kc", "vc", "slopes", "out"), lambda x: paged_attention(x["q"], x["kc"], x["vc"], table, lens, softcap=9.0, alibi_slopes=x["slopes"],
+                                                                                   out=x["out"], **e)),
+        "write": (("kt", "vt", "kc", "vc"), lambda x: write_kv(x["kt"], x["vt"], x["kc"], x["vc"], slots, **e)),
+        "rope write": (("qt", "kt", "vt", "w", "kc", "vc", "qo"), lambda x: qk_norm_rope_write(x["qt"], x["kt"], x["vt"], pos, rot, x["kc"], x["vc"], slots,
+                                                                                              q_weight=x["w"], k_weight=x["w"], q_out=x["qo"], **e)),
+        "read": (("kc", "vc", "key", "value"), lambda x: read_kv(x["kc"], x["vc"], slots, key=x["key"], value=x["value"], **e)),
+    }
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("binding", ["native", "python"])
+@pytest.mark.parametrize("mode", ["forward", "forward under no_grad", "backward"])
+@pytest.mark.parametrize("name", ["attention", "write", "rope write", "read"])
+def test_what_would_lose_a_derivative_is_refused(name, mode, binding, monkeypatch):
+    x, calls = losing_calls()
+    names, call = calls[name]
+    call(x)  # (loads the binding)
+    if binding == "python":
+        python_alone(monkeypatch)
+    for n in names:
+        if mode == "backward":
+            y = {**x, n: x[n].detach().clone().requires_grad_()}
+            with pytest.raises(NotImplementedError):
+                call(y)
+            with torch.no_grad():
+                call(y)
+        elif x[n].dtype is not CODES:  # (torch makes no tangents of codes)
+            with forward_ad.dual_level():
+                y = {**x, n: forward_ad.make_dual(x[n].clone(), torch.ones_like(x[n]))}
+                with pytest.raises(NotImplementedError):
+                    if "no_grad" in mode:
+                        with torch.no_grad():
+                            call(y)
+                    else:
+                        call(y)
+    call(x)
