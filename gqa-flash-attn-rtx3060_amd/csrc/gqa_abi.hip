@@ -117,7 +117,8 @@ const char* gqa_strerror(int code) {
              "max_positions positive, eps not negative";
     case GQA_E_CACHE8:
       return "paged cache in 8 bits: block_size must be a power of two from 16 on, page rows 16-byte aligned and 16 of "
-             "them within 2 GiB, the scale positive and finite, the form one of those that gqa_paged8_plan gives";
+             "them within 2 GiB, the scale positive and finite, the form one of those that gqa_paged8_plan gives; in a "
+             "store, pages, heads, keys and values with memory of their own";
     default: break;
   }
   if (code > 0) return hipGetErrorString(static_cast<hipError_t>(code));

@@ -33,6 +33,11 @@ int check_cache(const gqa_cache8* c, int head_dim) {
   return GQA_OK;
 }
 
+// A store's slots and heads have memory of their own.
+bool shares(const gqa_cache8* c, int num_kv_heads) {
+  return c->stride[1] == 0 || (num_kv_heads > 1 && (c->stride[2] == 0 || c->exp_stride[1] == 0));
+}
+
 TensorRef cache_ref(const gqa_cache8* c) { return TensorRef{c->codes, c->stride[0], c->stride[2], c->stride[1]}; }
 gqa::Exponents exp_ref(const gqa_cache8* c) { return gqa::Exponents{c->exponents, c->exp_stride[0], c->exp_stride[1]}; }
 TensorRef ref4(const void* ptr, const int64_t* st) { return TensorRef{ptr, st[0], st[1], st[2]}; }
@@ -240,6 +245,9 @@ int gqa_cache8_write_launch(const void* q, const int64_t q_stride[3], const void
   if ((rc = gqa::check_rows(k, k_stride, 3)) || (rc = gqa::check_rows(v, v_stride, 3)) ||
       (rc = check_cache(k_cache, head_dim)) || (rc = check_cache(v_cache, head_dim)))
     return rc;
+  if (shares(k_cache, num_kv_heads) || shares(v_cache, num_kv_heads) || k_cache->codes == v_cache->codes ||
+      k_cache->exponents == v_cache->exponents)
+    return GQA_E_CACHE8;
   if (q != nullptr) {
     p.q = token_ref(q, q_stride);
     p.qo = token_ref(q_out, q_out_stride);

@@ -670,6 +670,16 @@ bool caches8_ready(const py::handle& hkc, const py::handle& hvc, const py::handl
   const at::Tensor &kc = THPVariable_Unpack(hkc.ptr()), &vc = THPVariable_Unpack(hvc.ptr());
   return kc.sizes() == vc.sizes() && !wants_grad({&kc, &vc});
 }
+// For a store: pages, heads, keys and values have memory of their own.
+bool caches8_apart(const py::handle& hkc, const gqa_cache8 (&c)[2]) {
+  const at::Tensor& kc = THPVariable_Unpack(hkc.ptr());
+  for (const gqa_cache8& x : c) {
+    for (int i = 0; i < 4; ++i)
+      if (x.stride[i] == 0 && kc.size(i) > 1) return false;
+    if ((x.exp_stride[0] == 0 && kc.size(0) > 1) || (x.exp_stride[1] == 0 && kc.size(2) > 1)) return false;
+  }
+  return c[0].codes != c[1].codes && c[0].exponents != c[1].exponents;
+}
 int cu_count(int64_t dev) {  // (guarded by the GIL)
   static std::array<int, 64> counts{};
   if (dev < 0 || dev >= 64) return gqa_device_cu_count(static_cast<int>(dev));
@@ -771,7 +781,8 @@ bool write_kv8(const py::handle& hk, const py::handle& hv, const py::handle& hkc
   const int64_t dev = k->get_device(), T = k->size(0), D = k->size(2);
   gqa_cache8 c[2];
   if (c10::hip::current_device() != dev || v->get_device() != dev || (D != 64 && D != 128) ||
-      T >= GQA_MAX_ROPE_TOKENS || !slots_ready(sl, T, dev) || !caches8_ready(hkc, hvc, hke, hve, dev, c))
+      T >= GQA_MAX_ROPE_TOKENS || !slots_ready(sl, T, dev) || !caches8_ready(hkc, hvc, hke, hve, dev, c) ||
+      !caches8_apart(hkc, c))
     return false;
   const at::Tensor& kc = THPVariable_Unpack(hkc.ptr());
   if (kc.size(2) != k->size(1) || kc.size(3) != D) return false;
@@ -901,7 +912,7 @@ py::object norm_rope(const py::handle& hq, const py::handle& hk, const py::handl
     if (v == nullptr || kc == nullptr || vc == nullptr || sl == nullptr || v->sizes() != k->sizes() ||
         v->scalar_type() != k->scalar_type() || v->get_device() != dev || !rows_ready(*v))
       return py::none();
-    if (bits8 ? !caches8_ready(hkc, hvc, hke, hve, dev, c8) || v->get_device() != k->get_device()
+    if (bits8 ? !caches8_ready(hkc, hvc, hke, hve, dev, c8) || !caches8_apart(hkc, c8)
               : !caches_ready(*kc, *vc) || kc->scalar_type() != k->scalar_type())
       return py::none();
     if (kc->get_device() != dev || kc->size(2) != k->size(1) ||

@@ -54,14 +54,20 @@ def _codes_ready(t: torch.Tensor) -> bool:
     return st[-1] == 1 and (t.data_ptr() | st[0] | st[1] | st[2]) % 16 == 0
 
 
-def check_caches(k_cache, v_cache, k_exponents, v_exponents) -> int:
-    """The block size of a cache in 8 bits, its tensors checked."""
+def check_caches(k_cache, v_cache, k_exponents, v_exponents, write: bool = False) -> int:
+    """The block size of a cache in 8 bits, its tensors checked.  write: they are written, so
+    that pages, heads, keys and values have memory of their own."""
     assert k_exponents is not None and v_exponents is not None, \
         "a cache in 8 bits needs k_exponents and v_exponents"
     assert k_cache.dtype is CODES and v_cache.dtype is CODES, \
         "with exponents, k_cache and v_cache hold torch.float8_e4m3fn codes"
     assert k_cache.dim() == 4 and tuple(k_cache.shape) == tuple(v_cache.shape), \
         "k_cache / v_cache must be (num_blocks, block_size, num_kv_heads, head_dim)"
+    if write:
+        for k, v in ((k_cache, v_cache), (k_exponents, v_exponents)):
+            assert not any(s == 0 and n > 1 for t in (k, v) for s, n in zip(t.stride(), t.shape)) and \
+                (k.numel() == 0 or k.data_ptr() != v.data_ptr()), \
+                "a store needs pages, heads, keys and values with memory of their own (no broadcast codes or exponents)"
     assert k_cache.is_cuda and k_cache.device == v_cache.device
     block_size = k_cache.shape[1]
     assert MIN_BLOCK <= block_size <= _lib.GQA_MAX_BLOCK_SIZE and block_size & (block_size - 1) == 0, \
@@ -219,7 +225,7 @@ def write(key, value, k_cache, v_cache, slot_mapping, k_exponents, v_exponents) 
     from .rotary import _ready
 
     refuse_grad("write_kv into a cache in 8 bits", key, value, k_cache, v_cache)
-    block_size = check_caches(k_cache, v_cache, k_exponents, v_exponents)
+    block_size = check_caches(k_cache, v_cache, k_exponents, v_exponents, write=True)
     _check_tokens(key, value, k_cache, slot_mapping)
     _launch_write(None, _ready(key), _ready(value), None, k_cache, v_cache, k_exponents, v_exponents,
                   slot_mapping.contiguous(), None, block_size)
@@ -233,7 +239,7 @@ def norm_rope_write(q, k, v, positions, table, k_cache, v_cache, slot_mapping, q
     refuse_grad("qk_norm_rope_write", q, k, v, q_weight, k_weight, k_cache, v_cache, q_out)
     _check_qk(q, k, 3)
     assert k.shape[0] == q.shape[0], "q and k have different tokens"
-    block_size = check_caches(k_cache, v_cache, k_exponents, v_exponents)
+    block_size = check_caches(k_cache, v_cache, k_exponents, v_exponents, write=True)
     _check_tokens(k, v, k_cache, slot_mapping)
     slot_mapping = slot_mapping.contiguous()
     qo = _out_like(q) if q_out is None else _check_out(q_out, q, "q_out")

@@ -759,7 +759,8 @@ def write_kv(key, value, k_cache, v_cache, slot_mapping, *, k_exponents=None, v_
     2 ** it, not below what it was, unless the call stores the page's first slot,
     which begins the page anew; the tokens in front of the new ones are brought to
     it.  A page's tokens stand next to one another in the call (no padding in
-    between), no slot twice.  fp16 values past 61440 (bf16: past 1.875 * 2 ** 127)
+    between), no slot twice, and pages, heads, keys and values have exponents of
+    their own (no broadcast ones).  fp16 values past 61440 (bf16: past 1.875 * 2 ** 127)
     are stored as that, NaN as NaN.
     """
     if k_exponents is not None or v_exponents is not None or k_cache.dtype is cache8.CODES:

@@ -647,7 +647,9 @@ int gqa_paged8_launch(int form, const void* q, const int64_t q_stride[4],
  * Values outside what dtype holds are stored as the largest e4m3 multiple of a
  * power of two within it (fp16 61440); NaN as NaN, without a say in the exponent.
  * A page's tokens stand next to one another in the call, no slot twice; every
- * non-negative slot must lie inside the cache. */
+ * non-negative slot must lie inside the cache.  Pages, slots and heads of k_cache
+ * and v_cache have memory of their own, codes and exponents (GQA_E_CACHE8 where
+ * slots, heads or the two caches share it). */
 int gqa_cache8_write_launch(const void* q, const int64_t q_stride[3],
                             const void* k, const int64_t k_stride[3],
                             const void* v, const int64_t v_stride[3],

@@ -221,3 +221,61 @@ def test_what_would_lose_a_derivative_is_refused(name, mode, binding, monkeypatc
                     else:
                         call(y)
     call(x)
+
+
+# ---------------------------------------------------------------------------
+# Stores into memory that pages, heads, keys or values share
+# ---------------------------------------------------------------------------
+def sharing(kv, e):
+    """Codes (2, blocks, bs, Hkv, D) and exponents (2, blocks, Hkv) of which some share memory: a store's workgroups would race for it."""
+    return [(kv, e[:, :, :1].expand_as(e)), (kv, e[:, :1].expand_as(e)), (kv, e[:1].expand_as(e)), (kv, e[0].new_zeros(1).expand_as(e)),
+            (kv[:, :, :, :1].expand_as(kv), e), (kv[:, :1].expand_as(kv), e), (kv[:1].expand_as(kv), e)]
+
+
+@pytest.mark.parametrize("i", range(7))
+def test_stores_into_shared_memory_are_refused(i):
+    """(No GPU here: the check comes before any other of the device.)"""
+    kv, e = sharing(torch.zeros(2, 4, 16, 2, 64, dtype=torch.uint8).view(CODES), cache8.new_exponents(4, 2, "cpu"))[i]
+    rows, slots = torch.zeros(1, 2, 64, dtype=BF), torch.zeros(1, dtype=torch.int64)
+    with pytest.raises(AssertionError, match="memory of their own"):
+        cache8.write(rows, rows, kv[0], kv[1], slots, e[0], e[1])
+    with pytest.raises(AssertionError, match="memory of their own"):
+        cache8.check_caches(kv[0], kv[1], e[0], e[1], write=True)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="what passes the checks would launch")
+def test_stores_into_shared_memory_are_refused_by_the_entry_point():
+    P, t3 = 0x10000, _lib._i64x3(1024, 128, 1)
+
+    def write(heads=2, vc=2 * P, ve=2 * P, stride=(4096, 256, 128, 1), exp_stride=(2, 1)):
+        k, v = (_lib.Cache8(c, (ctypes.c_int64 * 4)(*stride), x, (ctypes.c_int64 * 2)(*exp_stride)) for c, x in ((P, P), (vc, ve)))
+        return _lib.load().gqa_cache8_write_launch(None, t3, P, t3, P, t3, None, t3, ctypes.byref(k), ctypes.byref(v), P, None, 4, 0, heads, 128, 16, 0, None)
+
+    for kw in (dict(vc=P), dict(ve=P), dict(stride=(4096, 256, 0, 1)), dict(stride=(4096, 0, 128, 1)), dict(exp_stride=(2, 0))):
+        assert write(**kw) == _lib.GQA_E_CACHE8, kw
+    for kw in ({}, dict(heads=1, stride=(4096, 128, 0, 1), exp_stride=(1, 0))):
+        assert write(**kw) == 100, kw  # hipErrorNoDevice
+
+
+@pytest.mark.gpu
+def test_broadcast_exponents_are_read_and_not_written():
+    kc, vc, ke, ve = new_cache(3, 16, 2, 64)
+    e = torch.full((1, 1), -7, dtype=torch.int32, device="cuda")
+    one, all_ = e.expand(3, 2), e.expand(3, 2).contiguous()
+    slots, k, q = torch.arange(20).cuda(), rand(20, 2, 64), rand(1, 4, 1, 64)
+    for a, b in zip(read_kv(kc, vc, slots, one, one), read_kv(kc, vc, slots, all_, all_.clone())):
+        assert torch.equal(a, b)
+    at = ints([[2, 0, 1]]), ints([40])
+    assert torch.equal(paged_attention(q, kc, vc, *at, k_exponents=one, v_exponents=one), paged_attention(q, kc, vc, *at, k_exponents=all_, v_exponents=all_))
+    w = rand(64)
+    for x, y in ((one, ve), (ke, one), (ke, ke)):
+        for _ in range(2):  # (through Python's checks first, and past the native call's)
+            with pytest.raises(AssertionError, match="memory of their own"):
+                write_kv(k, k, kc, vc, slots, k_exponents=x, v_exponents=y)
+            with pytest.raises(AssertionError, match="memory of their own"):
+                qk_norm_rope_write(rand(20, 4, 64), k, k, None, None, kc, vc, slots, k_weight=w, k_exponents=x, v_exponents=y)
+        read_kv(kc, vc, slots, ke, ve)
+    assert int(e) == -7
+    kc, vc, ke, ve = new_cache(1, 16, 1, 64)  # one page, one head: any stride is their own
+    write_kv(k[:8, :1], k[:8, :1], kc, vc, slots[:8], k_exponents=ke.as_strided((1, 1), (0, 0)), v_exponents=ve.as_strided((1, 1), (0, 0)))
+    assert int(ke) == int(ve)
