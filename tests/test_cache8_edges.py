@@ -5,10 +5,10 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from cache8_reference import CODES, new_cache, power, values
+from cache8_reference import CODES, LEAST, exponents_of, gather, limit_of, new_cache, power, stored, values
 from gqa_kernels import RotaryTable, _lib, cache8, paged, qk_norm_rope_write
 from gqa_kernels.paged import PagedKVCache, paged_attention, read_kv, write_kv
-from ops_reference import rope64
+from ops_reference import attend64, check_attention, rope64
 
 BF = torch.bfloat16
 
@@ -279,3 +279,98 @@ def test_broadcast_exponents_are_read_and_not_written():
     kc, vc, ke, ve = new_cache(1, 16, 1, 64)  # one page, one head: any stride is their own
     write_kv(k[:8, :1], k[:8, :1], kc, vc, slots[:8], k_exponents=ke.as_strided((1, 1), (0, 0)), v_exponents=ve.as_strided((1, 1), (0, 0)))
     assert int(ke) == int(ve)
+
+
+# ---------------------------------------------------------------------------
+# Pages and exponents that a wave holds by lane, and their next 64
+# ---------------------------------------------------------------------------
+def long_batch(lens, Hq, Hkv, Sq, D, dtype, bs=16, seed=0):
+    """(queries, cache, exponents, table, lengths): pages in random order, exponents spread over 2^13."""
+    pages = [-(-n // bs) for n in lens]
+    order, width, rows, at = torch.randperm(sum(pages), generator=torch.Generator().manual_seed(seed)).tolist(), max(pages), [], 0
+    for n in pages:
+        rows.append(order[at:at + n] + [-12345] * (width - n))
+        at += n
+    kc, vc, ke, ve = new_cache(sum(pages), bs, Hkv, D, seed=seed, spread=6)
+    ke -= 4  # (scores of a few units)
+    return rand(len(lens), Hq, Sq, D, dtype=dtype, seed=seed + 1), (kc, vc), dict(k_exponents=ke, v_exponents=ve), ints(rows), ints(lens)
+
+
+def check_long(batch, lens, slopes=None, **kw):
+    q, (kc, vc), e, table, n = batch
+    o, lse = paged_attention(q, kc, vc, table, n, return_lse=True, alibi_slopes=slopes, **e, **kw)
+    for b, m in enumerate(lens):
+        k, v = (gather(c, x, table[b], m, q.dtype) for c, x in ((kc, e["k_exponents"]), (vc, e["v_exponents"])))
+        check_attention(o[b], lse[b], attend64(q[b], k, v, slopes=slopes))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq", [1, 3, 8])
+@pytest.mark.parametrize("lens", [[4096], [4097], [4100, 8192], [4500, 50, 9000], [12345, 4224]])
+def test_few_rows_over_long_pieces(lens, Sq, D, dtype):
+    """One and two 16-row blocks; pieces of more than 32 tiles a wave, once and several times over, ends on a tile's, a unit's and a wave's share."""
+    batch = long_batch(lens, 8, 2, Sq, D, dtype, seed=Sq)
+    slopes = torch.tensor([2.0 ** -(h + 4) for h in range(8)]).cuda()
+    for splits in (1, 2):
+        check_long(batch, lens, route="split", splits=splits)
+    check_long(batch, lens, slopes, route="split", splits=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq", [30, 100])
+@pytest.mark.parametrize("lens", [[4096, 4095], [4097, 100], [4160, 8200], [9000, 4225]])
+def test_many_rows_over_long_pieces(lens, Sq, D, dtype):
+    """Blocks of 128 packed rows, and at head_dim 128 of 256; more than 64 tiles, in order and, with slopes, in reverse."""
+    batch = long_batch(lens, 8, 2, Sq, D, dtype, seed=Sq)
+    slopes = torch.tensor([2.0 ** -(h + 4) for h in range(8)]).cuda()
+    for kw in (dict(route="single"), dict(route="chunks", splits=1)):
+        check_long(batch, lens, **kw)
+        check_long(batch, lens, slopes, **kw)
+
+
+# ---------------------------------------------------------------------------
+# Stores of normed and rotated keys whose pages take more than one step
+# ---------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("T,Hkv,D,bs,R,inter", [(300, 2, 64, 128, 64, False), (300, 8, 128, 256, 64, True), (2500, 2, 128, 256, 128, False), (2500, 4, 64, 128, 32, True),
+                                                (300, 1, 128, 512, 128, False), (40, 3, 128, 64, 128, True)])
+def test_norms_and_rotation_over_pages_of_several_steps(T, Hkv, D, bs, R, inter, dtype):
+    """Two sequences that begin inside a page, most of whose tokens are in later steps and beyond the first 64 of their page."""
+    first, cut = 7, T - T // 3
+    at = torch.cat([torch.arange(first, first + cut), torch.arange(3, T - cut + 3)])
+    pages = -(-(first + cut) // bs)
+    order = torch.randperm(pages + -(-(T - cut + 3) // bs), generator=torch.Generator().manual_seed(T))
+    page = torch.cat([order[at[:cut] // bs], order[pages + at[cut:] // bs]])
+    slots = (page * bs + at % bs).cuda()
+    k, v, q = (rand(T, h, D, dtype=dtype, seed=h, scale=2.0) for h in (Hkv, Hkv + 1, 5))
+    v = v[:, :Hkv]
+    w = (rand(D, seed=2) * 0.3 + 1).to(dtype)
+    pos = torch.randint(0, 9000, (T,), generator=torch.Generator().manual_seed(1)).cuda()
+    table = RotaryTable(D, 9000, rotary_dim=R, interleaved=inter)
+    kc, vc, ke, ve = new_cache(len(order), bs, Hkv, D, seed=2, spread=6)
+    was, codes = ke.clone(), kc.clone()
+    wantv = stored(vc, ve, v.double(), slots, limit_of(dtype))
+    qo = qk_norm_rope_write(q, k, v, pos, table, kc, vc, slots, q_weight=w, k_weight=w, k_exponents=ke, v_exponents=ve)
+    assert torch.equal(vc.view(torch.uint8), wantv[0]) and torch.equal(ve, wantv[1])
+    inv = 10000.0 ** (-torch.arange(0, R, 2, dtype=torch.float64) / R)
+    y, tol = rope64(q, w, 1e-6, pos[None, :, None], rotary_dim=R, interleaved=inter, inv_freq=inv, axes=[0] * (R // 2))
+    assert ((qo.double() - y).abs() <= tol).all()
+    y, _ = rope64(k, w, 1e-6, pos[None, :, None], rotary_dim=R, interleaved=inter, inv_freq=inv, axes=[0] * (R // 2))
+    size, (pg, off) = y.abs().amax(-1, keepdim=True), (slots // bs, slots % bs)
+    got, unit = values(kc, ke)[pg, off], power(ke)[pg][..., None]
+    assert ((got - y).abs() <= 2.0 ** -4 * y.abs() + 2.0 ** -10 * unit + 2.0 ** -18 * size).all()
+    for x in pg.unique().tolist():
+        mine = pg == x
+        most, near = y[mine].abs().amax((0, 2)), 2.0 ** -18 * size[mine].amax((0, 2))
+        old = was[x] if int(off[mine].min()) > 0 else torch.full_like(was[x], LEAST)
+        assert (ke[x] >= torch.maximum(exponents_of(most - near), old)).all() and (ke[x] <= torch.maximum(exponents_of(most + near), old)).all()
+        # The tokens in front as their old codes under the new exponent; what lies behind is left.
+        low, behind = int(off[mine].min()), int(off[mine].max()) + 1
+        want = values(codes[x:x + 1], was[x:x + 1])[0, :low]
+        assert ((values(kc, ke)[x, :low] - want).abs() <= 2.0 ** -10 * power(ke[x])[:, None]).all()
+        assert torch.equal(kc[x, behind:].view(torch.uint8), codes[x, behind:].view(torch.uint8))
