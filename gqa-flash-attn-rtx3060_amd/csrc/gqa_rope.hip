@@ -78,39 +78,7 @@ __global__ __launch_bounds__(256) void gqa_rope_kernel(RopeParams p) {
       float ya[8], yb[8];
       unpack8<DT>(oa, ya);
       unpack8<DT>(ob, yb);
-      const void* w = kind == 0 ? p.wq : p.wk;
-      if (w != nullptr) {
-        float wa[8], wb[8], ss = 0.f;
-        load_weights<DT>(w, p.w32, ca, cb, wa, wb);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(ya[i], ya[i], __builtin_fmaf(yb[i], yb[i], ss));
-        const float inv = 1.0f / __builtin_sqrtf(row_sum<LPR>(ss) * (1.0f / D) + p.eps);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          ya[i] = ya[i] * inv * wa[i];
-          yb[i] = yb[i] * inv * wb[i];
-        }
-      }
-      if (at.rot) {
-        if (!p.interleaved) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float a = ya[i], c = yb[i];
-            ya[i] = a * cs[i] - c * sn[i];
-            yb[i] = c * cs[i] + a * sn[i];
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float a = ya[2 * i], c = ya[2 * i + 1];
-            ya[2 * i] = a * cs[i] - c * sn[i];
-            ya[2 * i + 1] = c * cs[i] + a * sn[i];
-            const float d = yb[2 * i], e = yb[2 * i + 1];
-            yb[2 * i] = d * cs[4 + i] - e * sn[4 + i];
-            yb[2 * i + 1] = e * cs[4 + i] + d * sn[4 + i];
-          }
-        }
-      }
+      row_norm_rotate<DT, D>(p, at, kind == 0 ? p.wq : p.wk, cs, sn, ya, yb);
       oa = pack8<DT>(ya);
       ob = pack8<DT>(yb);
     }

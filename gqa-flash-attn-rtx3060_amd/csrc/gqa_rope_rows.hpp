@@ -122,6 +122,8 @@ __device__ __forceinline__ void row_angles(const RopeParams& p, const RowLane& a
 }
 
 // The row's norm (with weights w, or none) and rotation of the lane's two chunks.
+// (Which product of a rotation is rounded before the sum is written out, so that every
+// kernel gives a row the same bits.)
 template <int DT, int D>
 __device__ __forceinline__ void row_norm_rotate(const RopeParams& p, const RowLane& at, const void* w,
                                                 const float (&cs)[8], const float (&sn)[8], float (&ya)[8],
@@ -143,18 +145,18 @@ __device__ __forceinline__ void row_norm_rotate(const RopeParams& p, const RowLa
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float a = ya[i], c = yb[i];
-        ya[i] = a * cs[i] - c * sn[i];
-        yb[i] = c * cs[i] + a * sn[i];
+        ya[i] = __builtin_fmaf(a, cs[i], -(c * sn[i]));
+        yb[i] = __builtin_fmaf(c, cs[i], a * sn[i]);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float a = ya[2 * i], c = ya[2 * i + 1];
-        ya[2 * i] = a * cs[i] - c * sn[i];
-        ya[2 * i + 1] = c * cs[i] + a * sn[i];
+        ya[2 * i] = __builtin_fmaf(a, cs[i], -(c * sn[i]));
+        ya[2 * i + 1] = __builtin_fmaf(a, sn[i], c * cs[i]);
         const float d = yb[2 * i], e = yb[2 * i + 1];
-        yb[2 * i] = d * cs[4 + i] - e * sn[4 + i];
-        yb[2 * i + 1] = e * cs[4 + i] + d * sn[4 + i];
+        yb[2 * i] = __builtin_fmaf(d, cs[4 + i], -(e * sn[4 + i]));
+        yb[2 * i + 1] = __builtin_fmaf(d, sn[4 + i], e * cs[4 + i]);
       }
     }
   }

@@ -6,7 +6,7 @@ import torch
 from torch.autograd import forward_ad
 
 from cache8_reference import CODES, LEAST, exponents_of, gather, limit_of, new_cache, power, stored, values
-from gqa_kernels import RotaryTable, _lib, cache8, paged, qk_norm_rope_write
+from gqa_kernels import RotaryTable, _lib, cache8, paged, qk_norm_rope, qk_norm_rope_write
 from gqa_kernels.paged import PagedKVCache, paged_attention, read_kv, write_kv
 from ops_reference import attend64, check_attention, rope64
 
@@ -374,3 +374,22 @@ def test_norms_and_rotation_over_pages_of_several_steps(T, Hkv, D, bs, R, inter,
         want = values(codes[x:x + 1], was[x:x + 1])[0, :low]
         assert ((values(kc, ke)[x, :low] - want).abs() <= 2.0 ** -10 * power(ke[x])[:, None]).all()
         assert torch.equal(kc[x, behind:].view(torch.uint8), codes[x, behind:].view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("D,R,inter", [(64, 64, False), (64, 32, True), (128, 128, False), (128, 128, True), (128, 16, False)])
+def test_queries_are_the_same_whatever_stores_the_keys(D, R, inter, dtype):
+    """One form of the norm and rotation: the bits of qk_norm_rope, with keys stored in 8 bits, in 16 or not at all."""
+    T, Hq, Hkv = 257, 6, 2
+    q, k, v = (rand(T, h, D, dtype=dtype, seed=s, scale=3.0) for s, h in ((1, Hq), (2, Hkv), (3, Hkv)))
+    table = RotaryTable(D, 9000, rotary_dim=R, interleaved=inter)
+    pos, slots = torch.randint(0, 9000, (T,), generator=torch.Generator().manual_seed(1)).cuda(), torch.arange(T).cuda()
+    for w in (None, (rand(D, seed=4) * 0.3 + 1).to(dtype), rand(D, seed=4).float() * 0.3 + 1):
+        kw = dict(q_weight=w, k_weight=w)
+        want, keys = qk_norm_rope(q, k, pos, table, **kw)
+        kc, vc, ke, ve = new_cache(17, 16, Hkv, D, full=False)
+        assert torch.equal(qk_norm_rope_write(q, k, v, pos, table, kc, vc, slots, k_exponents=ke, v_exponents=ve, **kw), want)
+        k16, v16 = (torch.zeros(17, 16, Hkv, D, dtype=dtype, device="cuda") for _ in range(2))
+        assert torch.equal(qk_norm_rope_write(q, k, v, pos, table, k16, v16, slots, **kw), want)
+        assert torch.equal(k16.flatten(0, 1)[:T], keys)
