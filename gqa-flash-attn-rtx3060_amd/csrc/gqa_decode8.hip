@@ -29,8 +29,8 @@ namespace gqa {
 
 namespace {
 
-// This wave's memory operations: all but n of its loads into LDS done, and its LDS
-// reads; nothing moves across.
+// This wave's memory operations, as far as the immediate says (vmcnt_imm(n): all but n of
+// its loads, into LDS among them; kLgkm0: its LDS reads); nothing moves across.
 template <int IMM> __device__ inline void wave_wait() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);

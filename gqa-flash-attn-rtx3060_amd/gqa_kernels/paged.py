@@ -488,7 +488,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, causal=True, *,
     Returns:
         o (batch, num_heads, seq_q, head_dim), or (o, lse).
     """
-    if k_exponents is not None or v_exponents is not None or k_cache.dtype is cache8.CODES:
+    if cache8.takes(k_cache, k_exponents, v_exponents):
         return cache8.attention(q, k_cache, v_cache, block_table, seq_lens, causal, max_seq_len, scale, splits,
                                 return_lse, out, route, query_start, query_lens, max_query_len, softcap, alibi_slopes,
                                 prefix_lens, k_exponents, v_exponents)
@@ -763,7 +763,7 @@ def write_kv(key, value, k_cache, v_cache, slot_mapping, *, k_exponents=None, v_
     their own (no broadcast ones).  fp16 values past 61440 (bf16: past 1.875 * 2 ** 127)
     are stored as that, NaN as NaN.
     """
-    if k_exponents is not None or v_exponents is not None or k_cache.dtype is cache8.CODES:
+    if cache8.takes(k_cache, k_exponents, v_exponents):
         cache8.write(key, value, k_cache, v_cache, slot_mapping, k_exponents, v_exponents)
         return
     if _lib._host is not None and _lib._host.write_kv(key, value, k_cache, v_cache, slot_mapping):
