@@ -22,7 +22,7 @@
 // Measured, bf16, 32/8 heads of 128, 16-token pages: norms, rotation and store of 8192
 // tokens 52 us, 189 MB at 3.6 TB/s (a large copy 5.1; registers for four waves a
 // SIMD are what keeps it from more: the rotation of 16-bit caches alone, at six, 49.5
-// us for 206 MB); K and V alone 14.0 us, 51 MB.  64 tokens, one a page: 4.6 and 3.7
+// us for 206 MB); K and V alone 14.0 us, 51 MB.  64 tokens, one a page: 4.7 and 3.7
 // us, a chain of dependent reads (slot; exponent, table row) after a launch of 2.6.
 // Rows and angles of a small call's tokens are loaded before their slots are known.
 #include <algorithm>
